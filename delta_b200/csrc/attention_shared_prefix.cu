@@ -1,0 +1,317 @@
+// Attention of single tokens whose rows share leading pages: each row r of the batch has one query per head and
+// reads kv_len[r] keys through its row of the block table,
+//
+//   out[r, h] = sum_j p_j V[j] / sum_j p_j,   p_j = exp(scale q[r, h] K[j] - m),   j < kv_len[r],
+//
+// and the rows of a group read the same first keys, which are fetched once for all of them (shared_prefix.cuh cuts
+// the work).  A first kernel leaves, for every piece, the outputs relative to the piece's own maximum with that
+// maximum and the sum; a second one merges the pieces of a row, which are few, in the order of their keys:
+//
+//   m = max_i m_i,   out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i      (maxima in units of log2).
+//
+// This file holds the merge and the kernel on the FMA units: 32-bit keys and values, and every head size and page
+// size that the kernel on the tensor cores (attention_shared_prefix_tc.cu) does not take.  A block of 256 threads
+// keeps 32 queries; eight threads share a query.  K and V tiles of 64 keys lie in shared memory as floats, rows of K
+// four floats apart from a multiple of 32 so that eight threads read eight rows without bank conflicts.
+// It is bound by the FMA units and the shared-memory reads that feed them (nine 16-byte reads for 32 FMAs).
+#include "shared_prefix.cuh"
+
+namespace {
+using namespace shared_prefix;
+constexpr int QR = 32;        // queries of a tile
+constexpr int KT = 64;        // keys of a tile
+constexpr int THREADS = 256;
+constexpr int EIGHT = 8;      // threads that share a query
+
+__host__ __device__ constexpr int k_stride(int hd) { return hd + 4; }
+__host__ __device__ constexpr int p_stride() { return KT + 4; }
+static size_t smem_floats(int hd) { return (size_t)QR * hd + (size_t)KT * k_stride(hd) + (size_t)KT * hd + (size_t)QR * p_stride(); }
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <>
+__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&raw.x), b = *reinterpret_cast<const __nv_bfloat162*>(&raw.y);
+  return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
+}
+
+// HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
+template <typename T, int HDM>
+__global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
+  constexpr int OC = HDM / 32;     // groups of four output columns of a thread
+  extern __shared__ __align__(16) float smem[];
+  const int hd = p.hd, ks = k_stride(hd), c4s = hd / 4;
+  float* s_q = smem;                   // [QR][hd]
+  float* s_k = s_q + QR * hd;          // [KT][hd + 4]
+  float* s_v = s_k + KT * ks;          // [KT][hd]
+  float* s_p = s_v + KT * hd;          // [QR][KT + 4]
+  __shared__ int4 list[CAP];
+  __shared__ int s_page[KT];
+  const int tid = threadIdx.x, r = tid / EIGHT, c = tid % EIGHT;
+  const int G = p.H / p.KV, rpt = QR / G;
+  const float sl2 = p.scale * 1.4426950408889634f;
+  auto sync = [] { __syncthreads(); };
+  bool more = true;
+  for (int range = blockIdx.x; more; range += gridDim.x) {
+    const int n_pieces = build<KT, THREADS>(p, rpt, range, list, reinterpret_cast<int*>(smem), tid, sync, range == 0, more);
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
+    for (int i = 0; i < n_pieces; ++i) {
+      const Piece w(list[i]);
+      const int rows = w.n_rows * G;
+      auto row_at = [&](int k) { return w.of_group ? p.members[w.first + k] : w.first; };
+      for (int x = tid; x < QR * c4s; x += THREADS) {
+        const int qr = x / c4s, col = x % c4s * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (qr < rows) {
+          const int row = row_at(qr / G);
+          if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
+        }
+        *reinterpret_cast<float4*>(s_q + qr * hd + col) = v;
+      }
+      const int table_row = row_at(0);
+      const int* table = p.block_table + (size_t)((table_row >= 0 && table_row < p.rows) ? table_row : 0) * p.max_pages;
+      float o[OC][4];
+#pragma unroll
+      for (int k = 0; k < OC; ++k)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[k][d] = 0.f;
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int kb = w.key0; kb < w.limit; kb += KT) {
+        const int n = min(KT, w.limit - kb);
+        __syncthreads();        // the tile before (and what the list was built in) is no longer read
+        if (tid < KT) {
+          int page = -1;
+          if (tid < n) {
+            const int lp = (kb + tid) / p.ps;        // below max_pages: limits are checked when the list is built
+            page = table[lp];
+            if (page < 0 || page >= p.num_pages) {
+              dk_report(p.err, DK_DEV_BAD_PAGE, table_row, lp, page);
+              page = -1;
+            }
+          }
+          s_page[tid] = page;
+        }
+        __syncthreads();
+        for (int x = tid; x < KT * c4s; x += THREADS) {
+          const int key = x / c4s, col = x % c4s * 4, page = s_page[key];
+          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+          if (page >= 0) {
+            const T* src = reinterpret_cast<const T*>(p.kv) + (((size_t)page * 2 * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd + col;
+            k = load4(src);
+            v = load4(src + (size_t)p.KV * p.ps * hd);
+          }
+          *reinterpret_cast<float4*>(s_k + key * ks + col) = k;
+          *reinterpret_cast<float4*>(s_v + key * hd + col) = v;
+        }
+        __syncthreads();
+        float s[KT / EIGHT];
+#pragma unroll
+        for (int j = 0; j < KT / EIGHT; ++j) s[j] = 0.f;
+#pragma unroll 2
+        for (int d = 0; d < hd; d += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(s_q + r * hd + d);
+#pragma unroll
+          for (int j = 0; j < KT / EIGHT; ++j) {
+            const float4 b = *reinterpret_cast<const float4*>(s_k + (j * EIGHT + c) * ks + d);
+            s[j] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[j]))));
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT / EIGHT; ++j) {
+          s[j] = j * EIGHT + c < n ? s[j] * sl2 : -INFINITY;
+          mx = fmaxf(mx, s[j]);
+        }
+#pragma unroll
+        for (int x = 1; x < EIGHT; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        const float m_new = fmaxf(m_run, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = exp2f(m_run - m_use);       // 0 before the first key
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KT / EIGHT; ++j) {
+          const float e = exp2f(s[j] - m_use);
+          sum += e;
+          s_p[r * p_stride() + j * EIGHT + c] = e;
+        }
+        l_run = l_run * keep + sum;
+        m_run = m_new;
+#pragma unroll
+        for (int k = 0; k < OC; ++k)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[k][d] *= keep;
+        __syncwarp();           // a query's eight threads are of one warp
+        for (int key = 0; key < n; ++key) {
+          const float e = s_p[r * p_stride() + key];
+#pragma unroll
+          for (int k = 0; k < OC; ++k) {
+            const int col = k * 32 + c * 4;
+            if (col < hd) {
+              const float4 v = *reinterpret_cast<const float4*>(s_v + key * hd + col);
+              o[k][0] = fmaf(e, v.x, o[k][0]);
+              o[k][1] = fmaf(e, v.y, o[k][1]);
+              o[k][2] = fmaf(e, v.z, o[k][2]);
+              o[k][3] = fmaf(e, v.w, o[k][3]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 1; x < EIGHT; x <<= 1) l_run += __shfl_xor_sync(0xffffffffu, l_run, x);
+      if (r < rows) {
+        const int n = w.of_group ? QR : G;
+        float* part = w.of_group ? group_piece(p, QR, w.id) : row_piece(p, QR, w.id);
+#pragma unroll
+        for (int k = 0; k < OC; ++k)
+          if (k * 32 + c * 4 < hd)
+            *reinterpret_cast<float4*>(part + ((size_t)(k * 8 + c) * n + r) * 4) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
+        if (c == 0) *reinterpret_cast<float2*>(part + (size_t)n * hd + 2 * r) = make_float2(m_run, l_run);
+      }
+      __syncthreads();          // the queries may be overwritten
+    }
+  }
+}
+
+// One block per (key-value head, row): thread (column group, head), heads fastest, as the pieces lie.
+template <typename T>
+__global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p, const int qr) {
+  const int kvh = blockIdx.x, row = blockIdx.y, G = p.H / p.KV;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int4 a = *reinterpret_cast<const int4*>(p.work + row * ROW_INTS), b = *reinterpret_cast<const int4*>(p.work + row * ROW_INTS + 4);
+  const int Q = b.w;
+  // pieces of the shared keys: segment a.x + kvh, tiles [a.y + kvh a.z, + a.z); of the row's own: b.x + kvh, [b.y + kvh b.z, + b.z)
+  const int pf = a.z > 0 ? (a.y + kvh * a.z) / Q : 0, pn = a.z > 0 ? (a.y + kvh * a.z + a.z - 1) / Q - pf + 1 : 0;
+  const int sf = b.z > 0 ? (b.y + kvh * b.z) / Q : 0, sn = b.z > 0 ? (b.y + kvh * b.z + b.z - 1) / Q - sf + 1 : 0;
+  const long long gs = group_piece_floats(qr, p.hd), rs = row_piece_floats(G, p.hd);
+  const float* gp = group_piece(p, qr, a.x + kvh + pf);
+  const float* rp = row_piece(p, qr, b.x + kvh + sf);
+  for (int x = threadIdx.x; x < G * (p.hd / 4); x += blockDim.x) {
+    const int g = x % G, c4 = x / G;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float* part, int n, int r) {
+      const float2 ml = *reinterpret_cast<const float2*>(part + (size_t)n * p.hd + 2 * r);
+      const float4 o = *reinterpret_cast<const float4*>(part + ((size_t)c4 * n + r) * 4);
+      const float m_new = fmaxf(M, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float keep = exp2f(M - m_use), f = exp2f(ml.x - m_use);
+      M = m_new;
+      L = L * keep + ml.y * f;
+      acc.x = acc.x * keep + o.x * f;
+      acc.y = acc.y * keep + o.y * f;
+      acc.z = acc.z * keep + o.z * f;
+      acc.w = acc.w * keep + o.w * f;
+    };
+    for (int i = 0; i < pn; ++i) add(gp + i * gs, qr, a.w + g);
+    for (int i = 0; i < sn; ++i) add(rp + i * rs, G, g);
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
+    T* out = reinterpret_cast<T*>(p.out) + row * p.out_stride + (kvh * G + g) * p.hd + c4 * 4;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+}
+
+template <typename T, int HDM>
+int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
+  const size_t need = smem_floats(p.hd), scratch = scratch_ints(p.rows, p.groups);
+  const size_t smem = 4 * (need > scratch ? need : scratch);
+  static size_t granted_on[DK_MAX_DEVICES] = {0};
+  size_t& granted = granted_on[dk_current_device()];
+  if (smem > granted) {
+    cudaError_t e = cudaFuncSetAttribute(attention_shared_prefix_kernel<T, HDM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+      dk_set_error("attention_shared_prefix: cannot get %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+      return DK_ERR_LAUNCH;
+    }
+    granted = smem;
+  }
+  attention_shared_prefix_kernel<T, HDM><<<p.grid, THREADS, smem, stream>>>(p);
+  return dk_check_launch("attention_shared_prefix");
+}
+
+template <typename T>
+int launch_sized(const DkSharedPrefixParams& p, cudaStream_t stream) {
+  if (p.hd <= 32) return launch<T, 32>(p, stream);
+  if (p.hd <= 64) return launch<T, 64>(p, stream);
+  if (p.hd <= 128) return launch<T, 128>(p, stream);
+  return launch<T, 256>(p, stream);
+}
+
+int fma_grid() { return 2 * dk_sm_count(); }
+
+int merge(const DkSharedPrefixParams& p, int qr, cudaStream_t stream) {
+  const int work = p.H / p.KV * (p.hd / 4);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.KV, p.rows);
+  cfg.blockDim = dim3(work < 32 ? 32 : (work > 512 ? 512 : (work + 31) / 32 * 32));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // its launch overlaps the first kernel's end; it waits for its results
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = p.dtype == DK_F32 ? cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<float>, p, qr)
+                                    : cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<__nv_bfloat16>, p, qr);
+  if (e != cudaSuccess) {
+    dk_set_error("attention_shared_prefix: launch of the merge failed: %s", cudaGetErrorString(e));
+    return DK_ERR_LAUNCH;
+  }
+  return dk_check_launch("attention_shared_prefix_merge");
+}
+}  // namespace
+
+namespace {
+int check_sizes(const DkSharedPrefixParams& p) {
+  DK_REQUIRE(p.dtype == DK_F32 || p.dtype == DK_BF16, "attention_shared_prefix: unknown element type %d", p.dtype);
+  DK_REQUIRE(p.rows >= 0 && p.rows <= MAX_ROWS && p.groups >= 0 && p.groups <= MAX_GROUPS && p.n_members >= 0 && p.n_members <= MAX_ROWS,
+             "attention_shared_prefix: %d rows in %d groups with %d members; at most %d rows and %d groups are taken", p.rows, p.groups,
+             p.n_members, MAX_ROWS, MAX_GROUPS);
+  DK_REQUIRE(p.KV >= 1 && p.KV <= 128 && p.H >= p.KV && p.H % p.KV == 0 && p.H / p.KV <= MAX_G,
+             "attention_shared_prefix: %d query heads and %d key-value heads; 1 to %d to each of at most 128 are taken", p.H, p.KV, MAX_G);
+  DK_REQUIRE(p.hd >= 4 && p.hd <= 256 && p.hd % 4 == 0, "attention_shared_prefix: head size %d is no multiple of 4 up to 256", p.hd);
+  DK_REQUIRE(p.ps >= 1 && p.max_pages >= 1 && p.num_pages >= 1 && (long long)p.max_pages * p.ps < (1ll << 30),
+             "attention_shared_prefix: tables of %d pages of %d tokens", p.max_pages, p.ps);
+  return 0;
+}
+
+int floats_needed(const DkSharedPrefixParams& p, long long* floats) {
+  const Bounds b = bounds(p, QR, KT, fma_grid());
+  DK_REQUIRE(b.tiles < (1ll << 30) && b.group_pieces < 65536 && b.row_pieces < 65536,
+             "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call", p.rows, p.KV, p.max_pages);
+  *floats = b.floats;
+  return 0;
+}
+}  // namespace
+
+// Floats of working memory that a call with these sizes needs.
+extern "C" int dk_attention_shared_prefix_floats(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int dtype, long long* floats) {
+  DkSharedPrefixParams p = {};
+  p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = 1; p.dtype = dtype;
+  if (int rc = check_sizes(p)) return rc;
+  return floats_needed(p, floats);
+}
+
+extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, void* out, long long out_stride, const void* kv, const int* block_table, const int* kv_len,
+                                          const int* members, const int* group_start, const int* group_prefix, void* work, long long work_floats, int rows, int groups,
+                                          int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale, int dtype, int* err, cudaStream_t stream) {
+  DkSharedPrefixParams p = {q, out, kv, block_table, kv_len, members, group_start, group_prefix, (float*)work, err, q_stride, out_stride,
+                            rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype, scale, 0, 0};
+  if (int rc = check_sizes(p)) return rc;
+  if (rows == 0) return 0;
+  long long need = 0;
+  if (int rc = floats_needed(p, &need)) return rc;
+  DK_REQUIRE(q && out && kv && block_table && kv_len && work && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
+  DK_REQUIRE(work_floats >= need, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, need);
+  DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
+  DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
+             "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
+  p.grid = fma_grid();
+  p.prefix_pieces = (int)bounds(p, QR, KT, p.grid).group_pieces;
+  const int rc = dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
+  return rc != 0 ? rc : merge(p, QR, stream);
+}

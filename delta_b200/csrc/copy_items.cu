@@ -1,0 +1,241 @@
+// Copies among the items (pages, slots) of tensors, as if every item were read before any is written: new[dst_i] = old[src_i].
+// An item may be read by several copies and may be the source of one and the target of another (a cache that is compacted
+// moves pages in chains and cycles), so the host puts the copies in an order in which nothing is overwritten that is still to
+// be read: the copy that reads an item comes before the one that writes it.  Every copy has at most one such successor, so
+// the copies form trees and cycles; a cycle is opened by keeping the first overwritten item in a register.
+//
+// A thread owns one unit (16 bytes where sizes and addresses allow it) at one place of an item and carries it through the
+// whole list: units at different places never meet, so nothing has to be synchronised however the copies depend on
+// one another.  It reads eight copies ahead before it writes, which the order allows (a reader stands before the writer or
+// beside it).  Components that do not depend on one another are dealt to lanes (blockIdx.y), as many as fill the device.
+// The kernel is bound by the bytes it moves; a short list travels in the kernel's arguments, so a fork is one launch and no
+// copy from the host.
+#include "common.cuh"
+#include <algorithm>
+#include <new>
+#include <vector>
+
+struct DkCopyTensor {
+  void* base;
+  long long item_stride, layer_stride;     // bytes
+  int layers, item_bytes;
+  int token_bytes, tokens;                 // bytes of one token in a row of tokens, tokens in a row; 0: items are copied whole
+};
+
+namespace {
+constexpr int THREADS = 256;
+constexpr int AHEAD = 8;
+constexpr int MAX_TENSORS = 32;
+constexpr int INLINE = 96;                 // copies that travel in the kernel's arguments
+constexpr int SAVE = 1, TAKE = 2;          // keep the target's old unit; write the kept unit
+
+struct Tensor {
+  char* base;
+  long long item_stride, layer_stride;
+  int layers, units, unit, first_block;
+  int units_per_token, tokens;             // 0: whole items
+};
+struct Args {
+  Tensor t[MAX_TENSORS];
+  int n_tensors, lanes;
+  const int4* list;                        // {source, target, tokens, flags}; null: in ``copies``
+  const int* starts;                       // [lanes + 1]
+  int4 copies[INLINE];
+  short inline_starts[INLINE + 2];
+};
+
+template <typename U>
+__device__ __forceinline__ void carry(const Tensor& t, const int4* list, int begin, int end) {
+  const long long at = ((long long)blockIdx.x - t.first_block) * THREADS + threadIdx.x;
+  if (at >= (long long)t.layers * t.units) return;
+  const int layer = (int)(at / t.units), unit = (int)(at - (long long)layer * t.units);
+  char* place = t.base + layer * t.layer_stride + (long long)unit * sizeof(U);
+  const int token = t.units_per_token > 0 ? unit / t.units_per_token % t.tokens : 0;
+  U kept = U();
+  for (int i = begin; i < end; i += AHEAD) {
+    U v[AHEAD];
+    int to[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      to[j] = -1;
+      if (i + j < end) {
+        const int4 c = list[i + j];
+        if (c.w & SAVE) kept = *reinterpret_cast<const U*>(place + c.y * t.item_stride);
+        if (token < c.z) {
+          to[j] = c.y;
+          if (c.w & TAKE) v[j] = kept;
+          else v[j] = *reinterpret_cast<const U*>(place + c.x * t.item_stride);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (to[j] >= 0) *reinterpret_cast<U*>(place + to[j] * t.item_stride) = v[j];
+  }
+}
+
+__global__ void __launch_bounds__(THREADS) copy_items_kernel(const __grid_constant__ Args a) {
+  int k = 0;
+  while (k + 1 < a.n_tensors && (int)blockIdx.x >= a.t[k + 1].first_block) ++k;
+  const Tensor& t = a.t[k];
+  const int4* list = a.list ? a.list : a.copies;
+  const int begin = a.list ? a.starts[blockIdx.y] : a.inline_starts[blockIdx.y];
+  const int end = a.list ? a.starts[blockIdx.y + 1] : a.inline_starts[blockIdx.y + 1];
+  switch (t.unit) {
+    case 16: carry<uint4>(t, list, begin, end); break;
+    case 8: carry<uint2>(t, list, begin, end); break;
+    case 4: carry<uint32_t>(t, list, begin, end); break;
+    case 2: carry<unsigned short>(t, list, begin, end); break;
+    default: carry<unsigned char>(t, list, begin, end); break;
+  }
+}
+
+// Puts the copies in order.  list: {source, target, tokens, flags} of at most n copies, lane by lane; starts[lanes + 1].  Returns the copies
+// left (a copy of an item to itself is none), or a negative code.
+int order_copies(const int* src, const int* dst, const int* tokens, int n, long long n_items, int whole, int want_lanes, int4* list, int* starts, int* lanes) {
+  DK_REQUIRE(n >= 0, "copy_items: a negative number of copies");
+  std::vector<int> by_target;
+  by_target.reserve(n);
+  for (int i = 0; i < n; ++i) {
+    DK_REQUIRE(src[i] >= 0 && src[i] < n_items && dst[i] >= 0 && dst[i] < n_items, "copy_items: copy %d goes from item %d to item %d of %lld", i, src[i], dst[i], n_items);
+    DK_REQUIRE(tokens == nullptr || (tokens[i] >= 0 && tokens[i] <= whole), "copy_items: copy %d asks for %d tokens of an item of %d", i, tokens ? tokens[i] : 0, whole);
+    by_target.push_back(i);
+  }
+  std::sort(by_target.begin(), by_target.end(), [&](int a, int b) { return dst[a] < dst[b]; });
+  for (int i = 1; i < n; ++i)
+    DK_REQUIRE(dst[by_target[i]] != dst[by_target[i - 1]], "copy_items: item %d is written twice", dst[by_target[i]]);
+  // next[i]: the copy that writes what copy i reads
+  std::vector<int> next(n, -1), readers(n, 0), root(n);
+  auto find = [&](int i) {
+    while (root[i] != i) i = root[i] = root[root[i]];
+    return i;
+  };
+  for (int i = 0; i < n; ++i) root[i] = i;
+  auto moot = [&](int i) { return src[i] == dst[i] || (tokens != nullptr && tokens[i] == 0); };
+  for (int i = 0; i < n; ++i) {
+    if (moot(i)) continue;
+    const auto it = std::lower_bound(by_target.begin(), by_target.end(), src[i], [&](int a, int v) { return dst[a] < v; });
+    if (it == by_target.end() || dst[*it] != src[i] || moot(*it)) continue;
+    next[i] = *it;
+    ++readers[*it];
+    root[find(i)] = find(*it);
+  }
+  std::vector<int> order, flags(n, 0);
+  order.reserve(n);
+  std::vector<char> done(n, 0);
+  for (int i = 0; i < n; ++i)
+    if (!moot(i) && readers[i] == 0) order.push_back(i);
+  for (size_t k = 0; k < order.size(); ++k) {
+    done[order[k]] = 1;
+    const int j = next[order[k]];
+    if (j >= 0 && --readers[j] == 0) order.push_back(j);
+  }
+  for (int i = 0; i < n; ++i) {              // what is left are cycles
+    if (moot(i) || done[i]) continue;
+    int last = i;
+    for (int j = i; !done[j]; j = next[j]) {
+      done[j] = 1;
+      order.push_back(j);
+      last = j;
+    }
+    flags[i] |= SAVE;
+    flags[last] |= TAKE;
+  }
+  // components one after the other, dealt to lanes of about the same length
+  const int left = (int)order.size();
+  std::vector<int> count(n + 1, 0), first(n, -1);
+  for (int i : order) ++count[find(i)];
+  const int target = std::max(1, (left + std::max(1, want_lanes) - 1) / std::max(1, want_lanes));
+  int at = 0, lane = 0;
+  starts[0] = 0;
+  for (int i : order) {
+    const int c = find(i);
+    if (first[c] >= 0) continue;
+    if (at - starts[lane] >= target) starts[++lane] = at;
+    first[c] = at;
+    at += count[c];
+  }
+  starts[lane + 1] = at;
+  *lanes = left > 0 ? lane + 1 : 0;
+  for (int i : order) list[first[find(i)]++] = make_int4(src[i], dst[i], tokens ? tokens[i] : (whole > 0 ? whole : 1), flags[i]);
+  return left;
+}
+
+// Fills a.t; returns the blocks that one lane takes, or a negative code.
+int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a) {
+  DK_REQUIRE(n_tensors >= 1 && n_tensors <= MAX_TENSORS, "copy_items: %d tensors; 1 to %d are taken in one call", n_tensors, MAX_TENSORS);
+  long long blocks = 0;
+  for (int k = 0; k < n_tensors; ++k) {
+    const DkCopyTensor& x = tensors[k];
+    DK_REQUIRE(x.base != nullptr && x.layers >= 0 && x.item_bytes >= 0 && x.token_bytes >= 0 && x.tokens >= 0, "copy_items: tensor %d is missing or has a negative size", k);
+    long long bits = (long long)(uintptr_t)x.base | x.item_stride | x.layer_stride | x.item_bytes | x.token_bytes;
+    int unit = 16;
+    while (unit > 1 && bits % unit != 0) unit /= 2;
+    Tensor& t = a.t[k];
+    t.base = (char*)x.base;
+    t.item_stride = x.item_stride;
+    t.layer_stride = x.layer_stride;
+    t.layers = x.layers;
+    t.unit = unit;
+    t.units = x.item_bytes / unit;
+    t.units_per_token = x.token_bytes / unit;
+    t.tokens = x.tokens > 0 ? x.tokens : 1;
+    t.first_block = (int)blocks;
+    blocks += ((long long)t.layers * t.units + THREADS - 1) / THREADS;
+    DK_REQUIRE(blocks < (1ll << 31) - 1, "copy_items: items of too many bytes");
+  }
+  a.n_tensors = n_tensors;
+  return (int)blocks;
+}
+
+int lanes_for(int blocks, int n) {
+  // four rounds of eight blocks an SM: enough to fill the device and to level the ends
+  const long long want = blocks > 0 ? (32ll * dk_sm_count() + blocks - 1) / blocks : 1;
+  return (int)std::max(1ll, std::min({want, (long long)std::max(1, n), 65535ll}));
+}
+}  // namespace
+
+extern "C" int dk_sizeof_copy_tensor() { return (int)sizeof(DkCopyTensor); }
+extern "C" int dk_copy_items_inline() { return INLINE; }
+
+// Puts n copies in order for a list on the device: list [n][4] ints and starts [n + 1].  Returns the number of lanes (0: nothing to copy) or a negative code.
+extern "C" int dk_copy_items_order(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, int* list, int* starts) {
+  try {
+    Args a = {};
+    const int blocks = lay_out(tensors, n_tensors, a);
+    if (blocks < 0) return blocks;
+    int lanes = 0;
+    const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), reinterpret_cast<int4*>(list), starts, &lanes);
+    return rc < 0 ? rc : lanes;
+  } catch (const std::bad_alloc&) {
+    dk_set_error("copy_items: no memory on the host to order %d copies", n);
+    return DK_ERR_ARG;
+  }
+}
+
+// The copies of src and dst (host) when there are at most INLINE of them, else those of a list on the device that dk_copy_items_order made.
+extern "C" int dk_copy_items(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items,
+                             const int* list, const int* starts, int lanes, cudaStream_t stream) {
+  try {
+    Args a = {};
+    const int blocks = lay_out(tensors, n_tensors, a);
+    if (blocks < 0) return blocks;
+    if (list == nullptr) {
+      DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
+      int s[INLINE + 2];
+      const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), a.copies, s, &lanes);
+      if (rc < 0) return rc;
+      for (int i = 0; i <= lanes; ++i) a.inline_starts[i] = (short)s[i];
+    } else {
+      a.list = reinterpret_cast<const int4*>(list);
+      a.starts = starts;
+    }
+    a.lanes = lanes;
+    if (blocks == 0 || lanes <= 0) return 0;
+    copy_items_kernel<<<dim3(blocks, lanes), THREADS, 0, stream>>>(a);
+    return dk_check_launch("copy_items");
+  } catch (const std::bad_alloc&) {
+    dk_set_error("copy_items: no memory on the host to order %d copies", n);
+    return DK_ERR_ARG;
+  }
+}

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import lib as _l
@@ -81,7 +82,8 @@ def new_error_record(device) -> torch.Tensor:
 _ERR_TEXT = {1: "page id out of range (token {0}, logical page {1}, page id {2})",
              2: "token id out of range (row {0}: id {1}, vocabulary {2})",
              3: "position out of range (token {0}: position {1}, limit {2})",
-             4: "a wait inside a kernel ran out (block {0}, part {1}, {2} steps); its result was not stored"}
+             4: "a wait inside a kernel ran out (block {0}, part {1}, {2} steps); its result was not stored",
+             5: "rows that share a prefix: entry {0} of the groups, their members or the rows' lengths holds {1} (limit {2})"}
 
 
 def error_text(code: int, a: int, b: int, c: int) -> str:
@@ -1411,3 +1413,159 @@ def experts_combine(z, weight, out, shared=None, gate_logit=None, gate_stride=0,
                                           _ptr(choice, "choice", torch.int32), int(first), dtype_code(x.dtype if x is not None else out.dtype),
                                           dtype_code(out.dtype), _stream()), "experts_combine")
     return out
+
+
+# ---------------------------------------------------------------------------
+# requests that share their beginning
+
+def _on_this_device(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.is_cuda and t.get_device() != _device_index():
+            raise KernelError(f"{what}: a tensor is on '{t.device}' and the current device is cuda:{_device_index()}")
+
+
+def _head_rows(t: torch.Tensor, name: str, rows: int, H: int, hd: int, dtype):
+    """Address and row stride of [rows, H, hd] whose rows may lie apart."""
+    if not t.is_cuda:
+        raise KernelError(f"{name} is on '{t.device}': the kernels run on CUDA tensors only and there is no CPU path")
+    if tuple(t.shape) != (rows, H, hd) or t.dtype != dtype:
+        raise KernelError(f"{name} has shape {tuple(t.shape)} / {t.dtype}, expected [{rows}, {H}, {hd}] of {dtype}")
+    if rows and (t.stride(2) != 1 or (H > 1 and t.stride(1) != hd) or (rows > 1 and t.stride(0) < H * hd)):
+        raise KernelError(f"{name}: a row's heads must lie one behind the other, the strides are {t.stride()}")
+    return t.data_ptr(), t.stride(0) if rows > 1 else H * hd
+
+
+_shared_prefix_floats = {}
+
+
+def attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, dtype) -> int:
+    """32-bit words of working memory that ``attention_shared_prefix`` needs for these sizes on the current device."""
+    key = (rows, groups, members, H, KV, hd, ps, max_pages, dtype, _device_index())
+    n = _shared_prefix_floats.get(key)
+    if n is None:
+        out = C.c_longlong()
+        _l.check(_l.load().dk_attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, dtype_code(dtype), C.byref(out)),
+                 "attention_shared_prefix", 0)
+        if len(_shared_prefix_floats) >= 4096:
+            _shared_prefix_floats.clear()
+        n = _shared_prefix_floats[key] = out.value
+    return n
+
+
+def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_start, group_prefix, *, scale, err=None, work=None):
+    """Attention of single tokens, with the keys that rows share read once: row r of ``q`` [rows, H, hd] attends to the first ``kv_len[r]``
+    keys of row r of ``block_table`` [rows, max_pages] in the pages ``kv`` [pages, 2, KV, ps, hd] (its own key among them, appended before).
+
+    ``members`` lists the rows that share something, group by group (group g: places ``group_start[g]`` to ``group_start[g + 1]``); the rows of
+    group g hold the same pages for their first ``group_prefix[g]`` tokens, of which the whole pages are shared and read through the table row
+    of one of them.  A row of no group reads all of its keys alone; one of ``kv_len`` 0 gets zeros.  A request that brings several tokens has a
+    row for each.  All tables are int32 on the device, so a captured call reads them anew at every replay; what does not fit
+    (a row named twice or out of range, a row shorter than its group's prefix, a bad page) is recorded in ``err`` and skipped.
+    Rows of ``q`` and ``out`` may lie apart.  Two products with float sums, the softmax in 32 bits; bfloat16 rounds the weights of the values once
+    and the result once.  ``work``: at least ``attention_shared_prefix_floats`` float32 that no other call uses meanwhile (allocated here when None).
+    """
+    i32 = torch.int32
+    if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or block_table.dim() != 2:
+        raise KernelError(f"attention_shared_prefix: q, pages and table have shapes {tuple(q.shape)}, {tuple(kv.shape)}, {tuple(block_table.shape)}")
+    (rows, H, hd), KV, ps = q.shape, kv.shape[2], kv.shape[3]
+    groups, n = group_prefix.numel(), members.numel()
+    if kv.shape[4] != hd or kv.dtype != q.dtype or block_table.shape[0] != rows or kv_len.numel() != rows or group_start.numel() != groups + 1:
+        raise KernelError(f"attention_shared_prefix: {rows} rows of heads of {hd} ({q.dtype}) do not fit pages {tuple(kv.shape)} of {kv.dtype}, a table of "
+                          f"{block_table.shape[0]} rows, {kv_len.numel()} lengths, {groups} prefixes and {group_start.numel()} starts of groups")
+    _on_this_device("attention_shared_prefix", q, out, kv, block_table, kv_len, members, group_start, group_prefix, err, work)
+    qp, qs = _head_rows(q, "q", rows, H, hd, q.dtype)
+    op, os_ = _head_rows(out, "out", rows, H, hd, q.dtype)
+    need = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, block_table.shape[1], q.dtype)
+    if work is None:
+        work = torch.empty(need, dtype=torch.float32, device=q.device)
+    _l.check(_l.load().dk_attention_shared_prefix(
+        qp, qs, op, os_, _ptr(kv, "kv"), _ptr(block_table, "block_table", i32), _ptr(kv_len, "kv_len", i32), _ptr(members, "members", i32),
+        _ptr(group_start, "group_start", i32), _ptr(group_prefix, "group_prefix", i32), _ptr(work, "work", torch.float32), work.numel(), rows, groups, n,
+        H, KV, hd, ps, block_table.shape[1], kv.shape[0], float(scale), dtype_code(q.dtype), _ptr(err, "err", i32), _stream()),
+        "attention_shared_prefix", 2 if rows else 0)
+    return out
+
+
+def _host_ints(v, name: str) -> np.ndarray:
+    if isinstance(v, torch.Tensor):
+        if v.is_cuda:
+            raise KernelError(f"{name} is on '{v.device}': which items are copied is said on the host")
+        v = v.numpy()
+    a = np.asarray(v)
+    if a.size and (a.dtype.kind not in "iu" or a.ndim != 1 or a.min() < -(1 << 31) or a.max() >= 1 << 31):
+        raise KernelError(f"{name} must be a list of whole numbers, not {a.dtype} of shape {a.shape}")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _copy_items(what: str, records, device, src, dst, tokens, n_items: int) -> None:
+    lib = _l.load()
+    src, dst = _host_ints(src, "src"), _host_ints(dst, "dst")
+    tokens = _host_ints(tokens, "tokens") if tokens is not None else None
+    n = src.size
+    if dst.size != n or (tokens is not None and tokens.size != n):
+        raise KernelError(f"{what}: {n} sources, {dst.size} targets" + (f", {tokens.size} counts of tokens" if tokens is not None else ""))
+    if n == 0:
+        return
+    table = np.array(records, dtype=np.int64)
+    addresses = (src.ctypes.data, dst.ctypes.data, tokens.ctypes.data if tokens is not None else None)
+    if n <= lib.dk_copy_items_inline():
+        _l.check(lib.dk_copy_items(table.ctypes.data, len(records), *addresses, n, n_items, None, None, 0, _stream()), what)
+        return
+    if torch.cuda.is_current_stream_capturing():
+        raise KernelError(f"{what}: {n} copies go through a list that is made on the host; a captured call takes at most {lib.dk_copy_items_inline()}")
+    order = np.empty(5 * n + 2, dtype=np.int32)
+    lanes = lib.dk_copy_items_order(table.ctypes.data, len(records), *addresses, n, n_items, order.ctypes.data, order.ctypes.data + 16 * n)
+    _l.check(min(lanes, 0), what, 0)
+    if lanes > 0:
+        held = torch.from_numpy(order).to(device)
+        _l.check(lib.dk_copy_items(table.ctypes.data, len(records), None, None, None, n, n_items, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what)
+
+
+def _two_ints(lo: int, hi: int) -> int:
+    return int(lo) | int(hi) << 32
+
+
+def copy_pages(pages, src, dst, *, tokens=None, token_axis=None):
+    """Copies pages ``src[i]`` to ``dst[i]`` of ``pages`` [layers, pages, *layout] in every layer, as if all were read before any is written: a page
+    may be read by several copies and may be the source of one and the target of another, so a cache can be permuted in place.  No page is the
+    target of two.  ``tokens[i]``: only the first so many tokens of the page are copied and the others of the target stay; ``token_axis`` says
+    which axis of the layout counts a page's tokens.  Sources, targets and counts are host lists.  One launch."""
+    if pages.dim() < 3:
+        raise KernelError(f"copy_pages: pages have shape {tuple(pages.shape)}, expected [layers, pages, *layout]")
+    _ptr(pages, "pages")
+    _on_this_device("copy_pages", pages)
+    layers, n, layout, size = pages.shape[0], pages.shape[1], pages.shape[2:], pages.element_size()
+    if pages.numel() == 0:
+        raise KernelError(f"copy_pages: there is nothing to copy in pages of shape {tuple(pages.shape)}")
+    item = pages[0, 0].numel() * size
+    if item >= 1 << 31:
+        raise KernelError(f"copy_pages: a page of {item} bytes is too large")
+    token_bytes = per_page = 0
+    if tokens is not None:
+        if token_axis is None or not 0 <= token_axis < len(layout):
+            raise KernelError(f"copy_pages: counts of tokens need the token axis of the layout {tuple(layout)}, got {token_axis}")
+        per_page = layout[token_axis]
+        token_bytes = size
+        for d in layout[token_axis + 1:]:
+            token_bytes *= d
+    _copy_items("copy_pages", [[pages.data_ptr(), item, item * n, _two_ints(layers, item), _two_ints(token_bytes, per_page)]], pages.device, src, dst, tokens, n)
+
+
+def copy_slots(states, src, dst):
+    """Copies slot ``src[i]`` to slot ``dst[i]`` of every tensor [slots, ...] in ``states``, as if all were read before any is written.  Slots are
+    host lists; no slot is the target of two.  One launch for up to 32 tensors."""
+    states = list(states.values()) if isinstance(states, dict) else list(states)
+    records, slots = [], None
+    for s in states:
+        _ptr(s, "a state")
+        _on_this_device("copy_slots", s)
+        if s.dim() < 1 or (slots is not None and s.shape[0] != slots):
+            raise KernelError(f"copy_slots: states have shapes {[tuple(x.shape) for x in states]}; all need the same number of slots")
+        slots = s.shape[0]
+        item = s.numel() // max(1, slots) * s.element_size()
+        if item >= 1 << 31:
+            raise KernelError(f"copy_slots: a slot of {item} bytes is too large")
+        if item:
+            records.append([s.data_ptr(), item, 0, _two_ints(1, item), 0])
+    for i in range(0, len(records), 32):
+        _copy_items("copy_slots", records[i:i + 32], states[0].device, src, dst, None, slots)

@@ -1,0 +1,248 @@
+"""Attention over shared prefixes against the softmax written out in float64.
+
+Queries, keys and values are small whole numbers and the scale is a power of two, so every score is exact in both types.  A few keys (the
+first and last of the prefix and of the row, those at page and tile borders, some at random) score about 8 above the rest and share nearly
+the whole weight: one that is missed or wrongly seen moves the output by its share, about 1 / 30 of a value, while values are -1 or 1.
+
+What rounding can do, to a value of at most 1: the exponent is off by 2^-24 of itself (two products, at most 20 in size) and the
+exponential by 2 units of 2^-23, together below 2^-18; sums of n weights by n 2^-24, in the numerator and in the denominator; bfloat16 rounds the
+weights (2^-8) and the result (2^-8).  A merge rounds a few times more (below 2^-20)."""
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+
+
+def tolerance(dtype, keys):
+    return 2.0 ** -17 + 2 * keys * 2.0 ** -24 + (2 * 2.0 ** -8 if dtype == "bfloat16" else 0.0)
+
+
+def make(dtype, H, KV, hd, ps, groups, loose, own, seed=0, scattered=False, wide=2, q_gap=0):
+    """groups: [(rows, prefix)], own: keys of each row alone (groups' rows first, then the loose ones)."""
+    rnd, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    shared = [p // ps * ps for n, p in groups for _ in range(n)] + [0] * loose
+    lens = [a + b for a, b in zip(shared, own)]
+    rows = len(lens)
+    held = [-(-n // ps) for n in lens]
+    n_pages = sum(p // ps for _, p in groups) + sum(h - s // ps for h, s in zip(held, shared)) + 3
+    ids = list(range(n_pages))
+    if scattered:
+        rnd.shuffle(ids)
+    take = iter(ids).__next__
+    table = torch.full((rows, max(held + [0]) + wide), -1, dtype=torch.int32)
+    row = 0
+    for n, p in groups + [(1, 0)] * loose:
+        first = [take() for _ in range(p // ps)]
+        for _ in range(n):
+            mine = first + [take() for _ in range(held[row] - len(first))]
+            table[row, :len(mine)] = torch.tensor(mine, dtype=torch.int32)
+            row += 1
+    u = torch.randint(0, 2, (KV, hd), generator=gen) * 2 - 1
+    q = u.repeat_interleave(H // KV, 0)[None] + torch.randint(0, 12, (rows, H, hd), generator=gen).eq(0).int() * (torch.randint(0, 2, (rows, H, hd), generator=gen) * 2 - 1)
+    kv = torch.randint(0, 2, (n_pages, 2, KV, ps, hd), generator=gen) * 2 - 1
+    for r in range(rows):
+        special = {0, shared[r] - 1, shared[r], lens[r] - 1} | {rnd.randrange(lens[r]) for _ in range(4) if lens[r]}
+        special |= {x * rnd.randrange(1 + lens[r] // x) - rnd.randrange(2) for x in (ps, 64, 128) if lens[r]}
+        for k in special:
+            if 0 <= k < lens[r]:
+                kv[table[r, k // ps], 0, :, k % ps] = u
+    order = list(range(rows))
+    rnd.shuffle(order)                      # where request i stands in the batch: order.index(i)
+    at = torch.tensor(order, dtype=torch.long)
+    back = torch.argsort(at)
+    starts = [0]
+    for n, _ in groups:
+        starts.append(starts[-1] + n)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    qd = torch.zeros((rows, H * hd + q_gap), dtype=DT[dtype], device="cuda")
+    qd[:, :H * hd] = q[at].reshape(rows, -1).to("cuda", DT[dtype])
+    return dict(q=qd[:, :H * hd].unflatten(1, (H, hd)) if q_gap else qd.view(rows, H, hd), kv=kv.to("cuda", DT[dtype]), block_table=table[at].contiguous().cuda(),
+                kv_len=torch.tensor(lens, dtype=torch.int32)[at].cuda(), members=back[:starts[-1]].to(torch.int32).cuda(),
+                group_start=torch.tensor(starts, **i32), group_prefix=torch.tensor([p for _, p in groups], **i32), scale=8.0 / hd if hd >= 8 else 1.0)
+
+
+def reference(c):
+    out = []
+    q, kv, table = c["q"].double().cpu(), c["kv"].double().cpu(), c["block_table"].cpu()
+    H, hd, KV, ps = q.shape[1], q.shape[2], kv.shape[2], kv.shape[3]
+    for r, n in enumerate(c["kv_len"].tolist()):
+        x = kv[table[r, :-(-n // ps)].long()].permute(1, 2, 0, 3, 4).reshape(2, KV, -1, hd)[:, :, :n]
+        s = torch.einsum("kgd,ksd->kgs", q[r].view(KV, H // KV, hd), x[0]) * c["scale"]
+        out.append(torch.einsum("kgs,ksd->kgd", torch.softmax(s, -1), x[1]).reshape(H, hd) if n else torch.zeros(H, hd, dtype=torch.float64))
+    return torch.stack(out)
+
+
+def call(c, out=None, **more):
+    from delta_b200.kernels import ops
+    out = torch.full_like(c["q"], 7.0) if out is None else out
+    args = {k: v for k, v in c.items() if k not in ("q",)}
+    err = ops.new_error_record("cuda")
+    ops.attention_shared_prefix(c["q"], out, err=err, **{**args, **more})
+    torch.cuda.synchronize()
+    ops.raise_if_error(err)
+    return out
+
+
+def check(dtype, c):
+    got, want = call(c), reference(c)
+    assert torch.isfinite(got.float()).all()
+    off = (got.double().cpu() - want).abs().amax().item()
+    assert off <= tolerance(dtype, int(c["kv_len"].max())), off
+
+
+SHAPES = [  # H, KV, hd, ps
+    (32, 4, 128, 16), (56, 8, 128, 16), (16, 2, 64, 8), (4, 2, 16, 16), (4, 1, 32, 8), (6, 6, 128, 32), (32, 2, 128, 64), (3, 1, 64, 128)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("scattered", [False, True], ids=["runs", "scattered"])
+def test_one_group(dtype, shape, scattered):
+    check(dtype, make(dtype, *shape, [(5, 700)], 0, [1, 40, 128, 129, 300], seed=1, scattered=scattered))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", SHAPES[:5], ids=lambda s: "x".join(map(str, s)))
+def test_groups_and_loose_rows(dtype, shape):
+    groups = [(3, 1000), (1, 333), (20, 129), (2, 5)]
+    own = [random.Random(5).choice([1, 2, 17, 127, 128, 129, 255, 400]) for _ in range(26 + 4)]
+    check(dtype, make(dtype, *shape, groups, 4, own, seed=2, scattered=True))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("case", [([(2, 128)], 0, [0, 1]), ([(2, 128)], 0, [0, 0]), ([], 3, [0, 1, 200]), ([(1, 16)], 0, [1]), ([(2, 0)], 1, [1, 0, 0]),
+                                  ([(40, 16)], 0, [1] * 40), ([(2, 15)], 0, [3, 4])], ids=str)
+def test_small_and_empty(dtype, case):
+    """Rows with no key of their own, rows with no key at all (zeros), prefixes below a page, one row in a group."""
+    check(dtype, make(dtype, 32, 4, 128, 16, *case, seed=3))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_long_prefix_and_many_ranges(dtype):
+    """A line of tiles that blocks walk in several rounds, and a prefix that is cut over most of them."""
+    check(dtype, make(dtype, 8, 8, 64, 16, [(3, 60000)], 2, [5, 700, 1, 9000, 30000], seed=4))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_that_lie_apart(dtype):
+    c = make(dtype, 8, 2, 64, 16, [(4, 300)], 1, [3, 50, 1, 20, 260], seed=5, q_gap=2 * 2 * 64)
+    assert not c["q"].is_contiguous()
+    wide = torch.full((5, 3, 8, 64), 5.0, dtype=DT[dtype], device="cuda")
+    got = call(c, out=wide[:, 1])
+    assert (got.double().cpu() - reference(c)).abs().amax() <= tolerance(dtype, 600)
+    assert (wide[:, 0] == 5).all() and (wide[:, 2] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_no_row_reads_does_not_matter(dtype, bad):
+    """Entries behind a row's last key, and whole pages of others, hold what an earlier request left."""
+    c = make(dtype, 32, 4, 128, 16, [(5, 530)], 1, [1, 40, 128, 129, 300, 77], seed=6)
+    want = reference(c)
+    table, ps = c["block_table"].cpu(), 16
+    used = torch.zeros(c["kv"].shape[0], ps, dtype=torch.bool)
+    for r, n in enumerate(c["kv_len"].tolist()):
+        for k in range(n):
+            used[table[r, k // ps], k % ps] = True
+    hole = (~used).cuda()[:, None, None, :, None].expand_as(c["kv"])
+    c["kv"][hole] = bad
+    assert (call(c).double().cpu() - want).abs().amax() <= tolerance(dtype, 900)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_same_bits_again_and_captured(dtype):
+    """The sums' order is fixed; a captured call reads its tables anew at every replay."""
+    a = make(dtype, 32, 4, 128, 16, [(5, 700), (3, 64)], 2, [1, 40, 128, 129, 300, 5, 6, 7, 90, 91], seed=7)
+    b = make(dtype, 32, 4, 128, 16, [(6, 640), (2, 128)], 2, [1, 4, 12, 200, 300, 50, 60, 7, 0, 19], seed=8, scattered=True)
+    b["block_table"] = torch.nn.functional.pad(b["block_table"], (0, max(0, a["block_table"].shape[1] - b["block_table"].shape[1])), value=-1)
+    a["block_table"] = torch.nn.functional.pad(a["block_table"], (0, max(0, b["block_table"].shape[1] - a["block_table"].shape[1])), value=-1)
+    n = max(a["kv"].shape[0], b["kv"].shape[0])
+    for c in (a, b):
+        c["kv"] = torch.cat([c["kv"], c["kv"][:1].expand(n - c["kv"].shape[0], -1, -1, -1, -1)]) if c["kv"].shape[0] < n else c["kv"]
+        c["block_table"] = c["block_table"].contiguous()
+    first = {id(c): call(c).clone() for c in (a, b)}
+    for c in (a, b):
+        assert torch.equal(call(c), first[id(c)])
+    held = {k: v.clone() for k, v in a.items() if isinstance(v, torch.Tensor)}
+    out = torch.empty_like(a["q"])
+    from delta_b200.kernels import ops
+    run = lambda: ops.attention_shared_prefix(out=out, scale=a["scale"], **held)      # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for c in (b, a, b):
+        for k, v in held.items():
+            v.copy_(c[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first[id(c)])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_two_streams_at_once(dtype):
+    cases = [make(dtype, 32, 4, 128, 16, [(8, 1500)], 1, [3 * i + 1 for i in range(9)], seed=s) for s in (9, 10)]
+    want = [call(c).clone() for c in cases]
+    from delta_b200.kernels import ops
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [torch.empty_like(c["q"]) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, o, st in zip(cases, outs, streams):
+            with torch.cuda.stream(st):
+                ops.attention_shared_prefix(out=o, **c)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_wrong_tables_are_recorded(dtype):
+    """Every index that comes from the device is checked before it is used: a wrong one is an error on the host, not a fault."""
+    from delta_b200.kernels.lib import KernelError
+
+    def broken(key, at, value):
+        c = make(dtype, 32, 4, 128, 16, [(4, 320), (2, 64)], 1, [5, 6, 7, 8, 9, 150, 11], seed=11)
+        c[key] = c[key].clone()
+        c[key][at] = value
+        return c
+    row = make(dtype, 32, 4, 128, 16, [(4, 320), (2, 64)], 1, [5, 6, 7, 8, 9, 150, 11], seed=11)["members"][0].item()
+    for c in (broken("members", 1, row), broken("members", 1, 99), broken("members", 2, -1), broken("group_start", 1, 1 << 20), broken("group_start", 0, -4),
+              broken("group_prefix", 0, 1 << 29), broken("group_prefix", 1, -16), broken("kv_len", row, 100), broken("kv_len", row, 1 << 30)):
+        with pytest.raises(KernelError, match="share a prefix"):
+            call(c)
+    for page in (-1, -7, 1 << 20):
+        with pytest.raises(KernelError, match="page id out of range"):
+            call(broken("block_table", (slice(None), 3), page))
+    check(dtype, make(dtype, 32, 4, 128, 16, [(4, 320), (2, 64)], 1, [5, 6, 7, 8, 9, 150, 11], seed=11))
+
+
+def test_refusals():
+    from delta_b200.kernels import ops
+    from delta_b200.kernels.lib import KernelError
+    c = make("bfloat16", 8, 2, 64, 16, [(2, 64)], 0, [1, 2], seed=12)
+    out = torch.empty_like(c["q"])
+
+    def refused(match, out=out, **change):
+        with pytest.raises(KernelError, match=match):
+            ops.attention_shared_prefix(out=out, **{**c, **change})
+    refused("do not fit", kv=c["kv"].float())
+    refused("do not fit", kv_len=c["kv_len"][:1])
+    refused("do not fit", group_start=c["group_start"][:1])
+    refused("expected", out=out.float())
+    refused("one behind the other", q=c["q"].transpose(1, 2).contiguous().transpose(1, 2))
+    refused("dtype", members=c["members"].long())
+    refused("is on 'cpu'", members=c["members"].cpu())
+    refused("must be positive", scale=-1.0)
+    refused("floats of working memory", work=torch.empty(8, device="cuda"))
+    refused("16-byte", kv=torch.empty(c["kv"].numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view_as(c["kv"]))
+    many = 1025
+    refused("at most", out=torch.empty(many, 8, 64, dtype=torch.bfloat16, device="cuda"), q=torch.empty(many, 8, 64, dtype=torch.bfloat16, device="cuda"),
+            kv_len=torch.zeros(many, dtype=torch.int32, device="cuda"), block_table=torch.zeros(many, 4, dtype=torch.int32, device="cuda"))
+    empty = ops.attention_shared_prefix(c["q"][:0], out[:0], c["kv"], c["block_table"][:0], c["kv_len"][:0], c["members"][:0], c["group_start"][:1] * 0,
+                                        c["group_prefix"][:0], scale=1.0)
+    assert empty.numel() == 0
