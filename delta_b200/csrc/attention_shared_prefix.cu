@@ -16,6 +16,10 @@
 // It is bound by the FMA units and the shared-memory reads that feed them (nine 16-byte reads for 32 FMAs).
 #include "shared_prefix.cuh"
 
+// attention_shared_prefix_tc.cu
+bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
+int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
+
 namespace {
 using namespace shared_prefix;
 constexpr int QR = 32;        // queries of a tile
@@ -279,8 +283,16 @@ int check_sizes(const DkSharedPrefixParams& p) {
   return 0;
 }
 
+// How the kernel that takes these sizes cuts the work: queries and keys of a tile, blocks.
+struct Cut {
+  bool tc;
+  int qr, kt, grid;
+};
+Cut cut_for(const DkSharedPrefixParams& p) { return dk_shared_prefix_tc_takes(p) ? Cut{true, 128, 128, dk_sm_count()} : Cut{false, QR, KT, fma_grid()}; }
+
 int floats_needed(const DkSharedPrefixParams& p, long long* floats) {
-  const Bounds b = bounds(p, QR, KT, fma_grid());
+  const Cut c = cut_for(p);
+  const Bounds b = bounds(p, c.qr, c.kt, c.grid);
   DK_REQUIRE(b.tiles < (1ll << 30) && b.group_pieces < 65536 && b.row_pieces < 65536,
              "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call", p.rows, p.KV, p.max_pages);
   *floats = b.floats;
@@ -289,9 +301,9 @@ int floats_needed(const DkSharedPrefixParams& p, long long* floats) {
 }  // namespace
 
 // Floats of working memory that a call with these sizes needs.
-extern "C" int dk_attention_shared_prefix_floats(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int dtype, long long* floats) {
+extern "C" int dk_attention_shared_prefix_floats(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, int dtype, long long* floats) {
   DkSharedPrefixParams p = {};
-  p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = 1; p.dtype = dtype;
+  p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = num_pages; p.dtype = dtype;
   if (int rc = check_sizes(p)) return rc;
   return floats_needed(p, floats);
 }
@@ -310,8 +322,10 @@ extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, voi
   DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
   DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
              "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
-  p.grid = fma_grid();
-  p.prefix_pieces = (int)bounds(p, QR, KT, p.grid).group_pieces;
-  const int rc = dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
-  return rc != 0 ? rc : merge(p, QR, stream);
+  const Cut c = cut_for(p);
+  DK_REQUIRE(!c.tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
+  p.grid = c.grid;
+  p.prefix_pieces = (int)bounds(p, c.qr, c.kt, c.grid).group_pieces;
+  const int rc = c.tc ? dk_shared_prefix_tc_launch(p, stream) : dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
+  return rc != 0 ? rc : merge(p, c.qr, stream);
 }

@@ -1438,13 +1438,13 @@ def _head_rows(t: torch.Tensor, name: str, rows: int, H: int, hd: int, dtype):
 _shared_prefix_floats = {}
 
 
-def attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, dtype) -> int:
+def attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype) -> int:
     """32-bit words of working memory that ``attention_shared_prefix`` needs for these sizes on the current device."""
-    key = (rows, groups, members, H, KV, hd, ps, max_pages, dtype, _device_index())
+    key = (rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype, _device_index())
     n = _shared_prefix_floats.get(key)
     if n is None:
         out = C.c_longlong()
-        _l.check(_l.load().dk_attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, dtype_code(dtype), C.byref(out)),
+        _l.check(_l.load().dk_attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype_code(dtype), C.byref(out)),
                  "attention_shared_prefix", 0)
         if len(_shared_prefix_floats) >= 4096:
             _shared_prefix_floats.clear()
@@ -1475,7 +1475,7 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
     _on_this_device("attention_shared_prefix", q, out, kv, block_table, kv_len, members, group_start, group_prefix, err, work)
     qp, qs = _head_rows(q, "q", rows, H, hd, q.dtype)
     op, os_ = _head_rows(out, "out", rows, H, hd, q.dtype)
-    need = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, block_table.shape[1], q.dtype)
+    need = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, block_table.shape[1], kv.shape[0], q.dtype)
     if work is None:
         work = torch.empty(need, dtype=torch.float32, device=q.device)
     _l.check(_l.load().dk_attention_shared_prefix(
