@@ -19,6 +19,10 @@
 // attention_shared_prefix_tc.cu
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
 int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
+// attention_shared_prefix_rows.cu
+int dk_shared_prefix_rows_tile();
+int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p);
+int dk_shared_prefix_rows_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
 
 namespace {
 using namespace shared_prefix;
@@ -42,6 +46,62 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
+// The range's pieces; the block of range 0 also writes the rows' records.
+__device__ int make_list(const DkSharedPrefixParams& p, int rpt, int range, int4* list, int* scratch, int tid, bool& more) {
+  const Tables t(scratch, p.rows, p.groups);
+  auto sync = [] { __syncthreads(); };
+  load_tables<true, THREADS>(p, t, tid, sync);
+  // segments of groups come first, those of rows are numbered from zero again: how many there are stands in t.line[67]
+  if (tid == 0) t.line[67] = 0;
+  auto keys_of = [&](int row, bool report) { return row_keys(p, t, row, p.kv_len[row], report); };
+  const Line l = walk_line<THREADS>(
+      p.groups + p.rows, p.grid, range, t.line, tid, sync,
+      [&](int e) {
+        if (e < p.groups) return group_entry<KT>(p, t, e, rpt);
+        const int tiles = cdiv(keys_of(e - p.groups, range == 0) - row_prefix(p, t, e - p.groups), KT);
+        return Entry{tiles > 0 ? p.KV : 0, tiles};
+      },
+      [&](int e, const Entry& x, int tile, int seg) {
+        if (e < p.groups) {
+          t.tile[e] = tile;
+          t.seg[e] = seg;
+          if (e == p.groups - 1) t.line[67] = seg + x.segments;
+        }
+        if (range == 0 && e >= p.groups) {
+          int* rec = row_record(p, e - p.groups);
+          rec[4] = seg;
+          rec[5] = tile;
+          rec[6] = x.tiles;
+        }
+      },
+      [&](int e, const Entry&, int i, int seg, int, int j0, int j1, int place, int) {
+        if (e < p.groups) {
+          list[place] = piece_of_group<KT>(p, t, e, rpt, i, seg + range, j0, j1);
+        } else {
+          const int row = e - p.groups, own = row_prefix(p, t, row);
+          list[place] = make_int4(row, i | (1 << 8) | ((seg - t.line[67] + range) << 16), own + j0 * KT, min(keys_of(row, false), own + j1 * KT));
+        }
+      });
+  if (range == 0)
+    for (int row = tid; row < p.rows; row += THREADS) {
+      const int m = t.member[row], k = row_prefix(p, t, row);
+      int* rec = row_record(p, row);
+      rec[2] = 0;
+      if (k > 0) {
+        const int g = group_of(p, t, m), i = m - t.start[g], pt = cdiv(k, KT);
+        rec[0] = t.seg[g] + i / rpt * p.KV;
+        rec[1] = t.tile[g] + i / rpt * p.KV * pt;
+        rec[2] = pt;
+        rec[3] = i % rpt * (p.H / p.KV);
+      }
+      rec[4] -= t.line[67];
+      rec[7] = l.Q;
+    }
+  more = l.more;
+  __syncthreads();
+  return l.pieces;
+}
+
 // HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
 __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
@@ -57,10 +117,9 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
   const int tid = threadIdx.x, r = tid / EIGHT, c = tid % EIGHT;
   const int G = p.H / p.KV, rpt = QR / G;
   const float sl2 = p.scale * 1.4426950408889634f;
-  auto sync = [] { __syncthreads(); };
   bool more = true;
   for (int range = blockIdx.x; more; range += gridDim.x) {
-    const int n_pieces = build<KT, THREADS>(p, rpt, range, list, reinterpret_cast<int*>(smem), tid, sync, range == 0, more);
+    const int n_pieces = make_list(p, rpt, range, list, reinterpret_cast<int*>(smem), tid, more);
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
     for (int i = 0; i < n_pieces; ++i) {
       const Piece w(list[i]);
@@ -222,7 +281,7 @@ __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams 
 
 template <typename T, int HDM>
 int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
-  const size_t need = smem_floats(p.hd), scratch = scratch_ints(p.rows, p.groups);
+  const size_t need = smem_floats(p.hd), scratch = Tables::ints(p.rows, p.groups);
   const size_t smem = 4 * (need > scratch ? need : scratch);
   static size_t granted_on[DK_MAX_DEVICES] = {0};
   size_t& granted = granted_on[dk_current_device()];
@@ -283,16 +342,19 @@ int check_sizes(const DkSharedPrefixParams& p) {
   return 0;
 }
 
-// How the kernel that takes these sizes cuts the work: queries and keys of a tile, blocks.
+// Whether the tensor cores take these sizes, and how the work is cut then: queries and keys of a tile, blocks; the same for rows.
 struct Cut {
   bool tc;
-  int qr, kt, grid;
+  int qr, kt, grid, rows_kt, rows_grid;
+  Bounds of(const DkSharedPrefixParams& p) const { return bounds(p, qr, kt, grid, rows_kt, rows_grid); }
 };
-Cut cut_for(const DkSharedPrefixParams& p) { return dk_shared_prefix_tc_takes(p) ? Cut{true, 128, 128, dk_sm_count()} : Cut{false, QR, KT, fma_grid()}; }
+Cut cut_for(const DkSharedPrefixParams& p) {
+  if (dk_shared_prefix_tc_takes(p)) return {true, 128, 128, dk_sm_count(), dk_shared_prefix_rows_tile(), dk_shared_prefix_rows_grid(p)};
+  return {false, QR, KT, fma_grid(), KT, fma_grid()};
+}
 
 int floats_needed(const DkSharedPrefixParams& p, long long* floats) {
-  const Cut c = cut_for(p);
-  const Bounds b = bounds(p, c.qr, c.kt, c.grid);
+  const Bounds b = cut_for(p).of(p);
   DK_REQUIRE(b.tiles < (1ll << 30) && b.group_pieces < 65536 && b.row_pieces < 65536,
              "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call", p.rows, p.KV, p.max_pages);
   *floats = b.floats;
@@ -312,11 +374,12 @@ extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, voi
                                           const int* members, const int* group_start, const int* group_prefix, void* work, long long work_floats, int rows, int groups,
                                           int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale, int dtype, int* err, cudaStream_t stream) {
   DkSharedPrefixParams p = {q, out, kv, block_table, kv_len, members, group_start, group_prefix, (float*)work, err, q_stride, out_stride,
-                            rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype, scale, 0, 0};
-  if (int rc = check_sizes(p)) return rc;
+                            rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype, scale, 0, 0, 0, 0};
+  int rc = check_sizes(p);
+  if (rc != 0) return rc;
   if (rows == 0) return 0;
   long long need = 0;
-  if (int rc = floats_needed(p, &need)) return rc;
+  if ((rc = floats_needed(p, &need)) != 0) return rc;
   DK_REQUIRE(q && out && kv && block_table && kv_len && work && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
   DK_REQUIRE(work_floats >= need, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, need);
   DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
@@ -324,8 +387,14 @@ extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, voi
              "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
   const Cut c = cut_for(p);
   DK_REQUIRE(!c.tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
-  p.grid = c.grid;
-  p.prefix_pieces = (int)bounds(p, c.qr, c.kt, c.grid).group_pieces;
-  const int rc = c.tc ? dk_shared_prefix_tc_launch(p, stream) : dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
+  p.grid = c.tc && p.groups == 0 ? 1 : c.grid;
+  p.rows_grid = c.rows_grid;
+  p.group_pieces = (int)c.of(p).group_pieces;
+  p.min_saved = 1;
+  if (c.tc) {
+    rc = dk_shared_prefix_tc_launch(p, stream);
+    return rc != 0 ? rc : dk_shared_prefix_rows_launch(p, stream);
+  }
+  rc = dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
   return rc != 0 ? rc : merge(p, c.qr, stream);
 }

@@ -1,0 +1,479 @@
+// Attention over shared prefixes, bfloat16: the keys that each row holds alone, and the merge with the pieces that the
+// kernel of the groups (attention_shared_prefix_tc.cu) leaves.
+//
+// A row's G <= 16 query heads of one key-value head are the rows of a warp-level MMA tile; the kernel is bound by the bytes of
+// K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM, each over a range of tiles of 64 keys that may
+// begin and end inside a row's segment.  Tiles flow through a ring without a stop between rows:
+//
+//   warp 4     fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
+//              box per page; pages behind the last key are left out), and with a segment's first tile its queries
+//   warps 0-3  S = Q K^T for 16 keys each, the maximum over the tile through shared memory, P in bfloat16 through shared
+//              memory, O += P V for a quarter of the columns each.  So all warps share one maximum, and nothing has to be merged
+//              between them at a segment's end.
+//
+// Behind a segment's last tile its row is finished: the pieces of its group's shared keys are added in their order, then the row's own, and
+// the result is rounded once.  Where a segment is cut between blocks, each leaves its piece in the work buffer and counts itself; the one that comes
+// last adds them all, in their order, so the result does not depend on who that is.  The counters are cleared by the kernel of the groups.
+// This kernel starts while that one runs and waits for its end before it touches what it wrote.
+#include "shared_prefix.cuh"
+#include "tcgen05_helpers.cuh"
+#include "mma_helpers.cuh"
+#include "ring.cuh"
+
+namespace {
+using namespace shared_prefix;
+constexpr int TILE = 64;           // keys of a tile
+constexpr int QR = 128;            // queries of a group's piece
+constexpr int ROWS = 16;           // rows of the MMA tile
+constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
+
+// One block of five stages an SM where two of three do not fit (heads of 128 with more than 8 to a key-value head).
+template <int HD, bool LOW>
+struct Ring {
+  static constexpr int HALVES = HD / 64;
+  static constexpr int KV_BYTES = HALVES * TILE * 128;               // one of K and V
+  static constexpr int Q_BYTES = (LOW ? 8 : ROWS) * HD * 2;
+  static constexpr int STAGE = (2 * KV_BYTES + Q_BYTES + 1023) / 1024 * 1024;
+  static constexpr int STAGES = HD == 128 && LOW ? 3 : 5;
+  static constexpr int BLOCKS = HD == 128 && !LOW ? 1 : 2;            // on an SM
+  static constexpr int TOTAL = STAGES * STAGE + 1024;                // 1024 to start on a swizzle boundary
+  static_assert(4 * Tables::ints(MAX_ROWS, MAX_GROUPS) <= STAGES * STAGE, "the list is made in the ring");
+};
+
+// What a range holds of a row's segment.
+struct RowPiece {
+  int row, kvh, key0, limit;
+  int id, index, pieces;           // number of this piece, its place among its segment's, how many those are
+  int group_id, group_n, r0;       // the segment of the row's group: first piece, how many, the row's first query in their tile
+};
+
+// LOW: at most 8 query heads; rows 8..15 of the MMA tile are then empty and their accumulators two registers that stay zero.
+template <bool LOW>
+__device__ __forceinline__ void mma_rows(float* c, float (&zero)[2], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (LOW) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(zero[0]), "+f"(zero[1])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+// Byte offset of 16-byte chunk ``chunk`` of key ``key`` in a K or V tile: 64 columns side by side, rows of 128 bytes, 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_offset(int key, int chunk) {
+  return (uint32_t)((chunk >> 3) * (TILE * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+}
+__device__ __forceinline__ void warps_barrier() { asm volatile("bar.sync 1, %0;\n" ::"n"(WARPS * 32) : "memory"); }
+
+template <int HD, bool LOW>
+__global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_kv,
+                                                                                  const __grid_constant__ CUtensorMap map_run,
+                                                                                  const DkSharedPrefixParams p) {
+  using R = Ring<HD, LOW>;
+  constexpr int NR = LOW ? 1 : 2;             // rows of the tile a thread keeps (g, and g + 8)
+  constexpr int KB = HD / 16;                 // k-blocks of Q K^T
+  constexpr int NT = HD / WARPS / 8;          // n-tiles of P V of a warp
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) unsigned long long bars[2 * R::STAGES];   // full, then empty
+  __shared__ __align__(16) RowPiece list[CAP];
+  __shared__ __align__(16) unsigned char s_p[ROWS * TILE * 2];      // weights [row][key], 16-byte chunks exchanged by the row
+  __shared__ float s_max[WARPS][ROWS], s_sum[WARPS][ROWS];
+  __shared__ int s_last;
+  __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
+  const int ps = p.ps, G = p.H / p.KV, rpt = QR / G;
+  const uint32_t full = s2u(&bars[0]), empty = full + 8 * R::STAGES, ring = s2u(smem);
+  if (tid == 0) {
+    for (int s = 0; s < R::STAGES; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, WARPS);
+    }
+    failed = stuck = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  const float sl2 = p.scale * 1.4426950408889634f;
+  int n_tile = 0;                 // tiles this block has had in the ranges before
+  bool waited = false, more = true;
+  for (int range = blockIdx.x; more; range += gridDim.x) {
+    int n_pieces;
+    {
+      auto sync = [] { __syncthreads(); };
+      const Tables t(reinterpret_cast<int*>(smem), p.rows, p.groups);
+      load_tables<true, THREADS>(p, t, tid, sync);
+      int QA = 1;
+      if (p.groups > 0)
+        QA = walk_line<THREADS>(
+                 p.groups, p.grid, -1, t.line, tid, sync, [&](int e) { return group_entry<2 * TILE>(p, t, e, rpt); },
+                 [&](int e, const Entry&, int tile, int seg) {
+                   t.tile[e] = tile;
+                   t.seg[e] = seg;
+                 },
+                 [](int, const Entry&, int, int, int, int, int, int, int) {}).Q;
+      const Line l = walk_line<THREADS>(
+          p.rows, p.rows_grid, range, t.line, tid, sync,
+          [&](int row) {
+            return Entry{p.KV, max(1, cdiv(row_keys(p, t, row, p.kv_len[row], true) - row_prefix(p, t, row), TILE))};      // (a row without a key of its own has an empty tile)
+          },
+          [&](int, const Entry&, int, int) {},
+          [&](int row, const Entry& x, int kvh, int seg, int tile, int j0, int j1, int place, int Q) {
+            const int own = row_prefix(p, t, row), first = tile / Q;
+            RowPiece d;
+            d.row = row;
+            d.kvh = kvh;
+            d.key0 = own + j0 * TILE;
+            d.limit = min(row_keys(p, t, row, p.kv_len[row], false), own + j1 * TILE);
+            d.id = seg + range;
+            d.index = range - first;
+            d.pieces = (tile + x.tiles - 1) / Q - first + 1;
+            d.group_id = d.group_n = d.r0 = 0;
+            if (own > 0) {
+              const int m = t.member[row], gr = group_of(p, t, m), i = m - t.start[gr], pt = cdiv(own, 2 * TILE), s = i / rpt * p.KV + kvh;
+              const int a = t.tile[gr] + s * pt, f = a / QA;
+              d.group_id = t.seg[gr] + s + f;
+              d.group_n = (a + pt - 1) / QA - f + 1;
+              d.r0 = i % rpt * G;
+            }
+            list[place] = d;
+          });
+      n_pieces = l.pieces;
+      more = l.more;
+      fence_async_smem();       // the ring is TMA's from here on
+      __syncthreads();
+    }
+    if (warp == WARPS) {
+      // ---------------------------------------------------------------- producer
+      const int rows_of_box = min(ps, TILE), ppt = TILE / rows_of_box;      // a tile's pages, at most 8
+      int n = n_tile;
+      for (int i = 0; i < n_pieces && !failed; ++i) {
+        const RowPiece& w = list[i];
+        const int* table = p.block_table + (size_t)w.row * p.max_pages;
+        const int kvh = w.kvh, limit = w.limit;
+        int kb = w.key0;
+        do {
+          const int held_pages = min(ppt, cdiv(limit - kb, rows_of_box)), lp = kb / ps + lane;
+          int page = -1;
+          if (lane < held_pages) {
+            page = table[lp];            // below max_pages: limits are checked when the list is made
+            if (page < 0 || page >= p.num_pages) {
+              dk_report(p.err, DK_DEV_BAD_PAGE, w.row, lp, page);
+              page = -1;
+            }
+          }
+          const int first = __shfl_sync(0xffffffffu, page, 0);
+          const bool run = ppt > 1 && __all_sync(0xffffffffu, lane >= ppt || (page >= 0 && page == first + lane));
+          const int held = __popc(__ballot_sync(0xffffffffu, page >= 0));
+          const int s = ring_slot(n, R::STAGES);
+          bool ok = true;
+          if (n >= R::STAGES) ok = mbar_wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
+          if (!__all_sync(0xffffffffu, ok && !stuck)) { failed = 1; break; }
+          const uint32_t k_dst = ring + s * R::STAGE, v_dst = k_dst + R::KV_BYTES, bar = full + 8 * s;
+          const bool with_q = kb == w.key0 && limit > w.key0;
+          if (lane == 0) {
+            mbar_expect_tx(bar, (uint32_t)(held * rows_of_box * 128 * R::HALVES * 2 + (with_q ? G * HD * 2 : 0)));
+            if (with_q)
+              bulk_load(v_dst + R::KV_BYTES, reinterpret_cast<const __nv_bfloat16*>(p.q) + w.row * p.q_stride + kvh * G * HD, (uint32_t)(G * HD * 2), bar);
+          }
+          __syncwarp();
+          if (run) {
+            if (lane == 0)
+              for (int half = 0; half < R::HALVES; ++half) {
+                tma_load_4d(k_dst + half * (TILE * 128), &map_run, half * 64, 0, kvh, first, bar);
+                tma_load_4d(v_dst + half * (TILE * 128), &map_run, half * 64, 0, p.KV + kvh, first, bar);
+              }
+          } else if (page >= 0) {
+            const int grow = (page * 2 * p.KV + kvh) * ps + kb % ps;      // row of the cache seen as [pages * 2 * KV * ps, hd]
+            for (int half = 0; half < R::HALVES; ++half) {
+              tma_load_2d(k_dst + half * (TILE * 128) + lane * rows_of_box * 128, &map_kv, half * 64, grow, bar);
+              tma_load_2d(v_dst + half * (TILE * 128) + lane * rows_of_box * 128, &map_kv, half * 64, grow + p.KV * ps, bar);
+            }
+          }
+          ++n;
+          kb += TILE;
+        } while (kb < limit);
+      }
+      if (lane == 0) ring_drain(n, R::STAGES, [&](int slot, uint32_t parity) { return mbar_wait(full + 8 * slot, parity); });   // its copies have arrived
+      __syncwarp();
+      n_tile = n;
+    } else {
+      // ---------------------------------------------------------------- the four warps
+      int n = n_tile;
+      bool bad = false;
+      for (int i = 0; i < n_pieces && !bad; ++i) {
+        const RowPiece w = list[i];
+        uint32_t qa[KB][4];
+        float o[NT][2 * NR], zero[2] = {0.f, 0.f}, m_run[NR], l_run[NR];
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int c = 0; c < 2 * NR; ++c) o[k][c] = 0.f;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          m_run[r] = -INFINITY;
+          l_run[r] = 0.f;
+        }
+        int kb = w.key0;
+        do {
+          const int s = ring_slot(n, R::STAGES);
+          const bool ok = mbar_wait(full + 8 * s, ring_parity(n, R::STAGES));
+          if (!ok) stuck = 1;
+          const uint32_t k_tile = ring + s * R::STAGE, v_tile = k_tile + R::KV_BYTES;
+          const int keys = min(TILE, w.limit - kb);
+          if (kb == w.key0 && keys > 0) {
+            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(smem + s * R::STAGE + 2 * R::KV_BYTES);
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+              const int c = k * 16 + 2 * tq;
+              qa[k][0] = g < G ? *reinterpret_cast<const uint32_t*>(q + g * HD + c) : 0u;
+              qa[k][1] = (!LOW && g + 8 < G) ? *reinterpret_cast<const uint32_t*>(q + (g + 8) * HD + c) : 0u;
+              qa[k][2] = g < G ? *reinterpret_cast<const uint32_t*>(q + g * HD + c + 8) : 0u;
+              qa[k][3] = (!LOW && g + 8 < G) ? *reinterpret_cast<const uint32_t*>(q + (g + 8) * HD + c + 8) : 0u;
+            }
+          }
+          float sc[2][2 * NR], mx[NR];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) sc[j][c] = 0.f;
+            const int key = warp * 16 + j * 8 + (lane & 7);
+#pragma unroll
+            for (int k = 0; k < KB; k += 2) {
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4(b0, b1, b2, b3, k_tile + tile_offset(key, 2 * k + (lane >> 3)));
+              mma_rows<LOW>(sc[j], zero, qa[k], b0, b1);
+              mma_rows<LOW>(sc[j], zero, qa[k + 1], b2, b3);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            mx[r] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float& v = sc[j][2 * r + c];
+                v = warp * 16 + j * 8 + 2 * tq + c < keys ? v * sl2 : -INFINITY;
+                mx[r] = fmaxf(mx[r], v);
+              }
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            if (tq == 0) s_max[warp][g + 8 * r] = mx[r];
+          }
+          warps_barrier();
+          // written by these warps only, before this barrier or behind the next one: the same for all four
+          bad = stuck != 0;
+          if (bad) break;
+          float keep[NR];
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            const int row = g + 8 * r;
+            const float m_new = fmaxf(fmaxf(m_run[r], fmaxf(s_max[0][row], s_max[1][row])), fmaxf(s_max[2][row], s_max[3][row]));
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            keep[r] = exp2f(m_run[r] - m_use);       // 0 before the first key
+            m_run[r] = m_new;
+            l_run[r] *= keep[r];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float p0 = exp2f(sc[j][2 * r] - m_use), p1 = exp2f(sc[j][2 * r + 1] - m_use);
+              l_run[r] += p0 + p1;        // the sum in 32 bits; the weights are rounded to bfloat16 for the product
+              const int key = warp * 16 + j * 8 + 2 * tq;
+              *reinterpret_cast<uint32_t*>(s_p + row * (TILE * 2) + (((key >> 3) ^ (row & 7)) << 4) + (key & 7) * 2) = pack_bf16(p0, p1);
+            }
+          }
+          warps_barrier();
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) o[k][c] *= keep[c >> 1];
+#pragma unroll
+          for (int kk = 0; kk < TILE / 16; ++kk) {
+            if (kk * 16 >= keys) break;
+            uint32_t a[4];
+            const int arow = (lane & 7) + ((lane >> 3) & 1) * 8;      // rows 0-7, 8-15 of keys 0-7, then of keys 8-15
+            ldmatrix_x4(a[0], a[1], a[2], a[3], s2u(s_p) + arow * (TILE * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4));
+            if (LOW) a[1] = a[3] = 0u;
+            // what lies behind the last key may be anything, and 0 times infinity is no zero
+            const int k0 = kk * 16 + 2 * tq;
+            const uint32_t low = (k0 < keys ? 0xffffu : 0u) | (k0 + 1 < keys ? 0xffff0000u : 0u);
+            const uint32_t high = (k0 + 8 < keys ? 0xffffu : 0u) | (k0 + 9 < keys ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int k = 0; k < NT; k += 2) {
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4_trans(b0, b1, b2, b3, v_tile + tile_offset(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, warp * NT + k + (lane >> 4)));
+              mma_rows<LOW>(o[k], zero, a, b0 & low, b1 & high);
+              mma_rows<LOW>(o[k + 1], zero, a, b2 & low, b3 & high);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * s);
+          ++n;
+          kb += TILE;
+        } while (kb < w.limit);
+        if (bad) break;
+        // ---- the segment's end: sums over the warps, then the merge
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+          l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+          if (tq == 0) s_sum[warp][g + 8 * r] = l_run[r];
+        }
+        warps_barrier();
+#pragma unroll
+        for (int r = 0; r < NR; ++r) l_run[r] = (s_sum[0][g + 8 * r] + s_sum[1][g + 8 * r]) + (s_sum[2][g + 8 * r] + s_sum[3][g + 8 * r]);
+        if (!waited) {          // the pieces of the groups and the counters
+          asm volatile("griddepcontrol.wait;\n" ::: "memory");
+          waited = true;
+        }
+        bool finish = true;
+        const int first_id = w.id - w.index;
+        if (w.pieces > 1) {
+          float* part = row_piece(p, QR, w.id);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+            if (g + 8 * r < G) {
+#pragma unroll
+              for (int k = 0; k < NT; ++k)
+                *reinterpret_cast<float2*>(part + (size_t)(g + 8 * r) * HD + (warp * NT + k) * 8 + 2 * tq) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
+              if (warp == 0 && tq == 0) *reinterpret_cast<float2*>(part + (size_t)G * HD + 2 * (g + 8 * r)) = make_float2(m_run[r], l_run[r]);
+            }
+          __threadfence();
+          warps_barrier();
+          if (tid == 0) s_last = atomicAdd(&counters(p)[w.row * p.KV + w.kvh], 1) == w.pieces - 1;
+          warps_barrier();
+          finish = s_last != 0;
+          if (finish) __threadfence();
+        }
+        if (finish) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            const int qh = g + 8 * r;
+            if (qh >= G) continue;
+            float M = -INFINITY, L = 0.f, acc[2 * NT];
+#pragma unroll
+            for (int k = 0; k < 2 * NT; ++k) acc[k] = 0.f;
+            auto add = [&](float m, float l, const float (&v)[2 * NT]) {
+              const float m_new = fmaxf(M, m), m_use = m_new == -INFINITY ? 0.f : m_new;
+              const float have = exp2f(M - m_use), f = exp2f(m - m_use);
+              M = m_new;
+              L = L * have + l * f;
+#pragma unroll
+              for (int k = 0; k < 2 * NT; ++k) acc[k] = acc[k] * have + v[k] * f;
+            };
+            // four pieces asked for at once, added in order
+            constexpr int AT_ONCE = 4;
+            const long long gs = group_piece_floats(QR, HD), rs = row_piece_floats(G, HD);
+            const float* gp = group_piece(p, QR, w.group_id);
+            for (int x = 0; x < w.group_n; x += AT_ONCE) {
+              float2 ml[AT_ONCE];
+              float v[AT_ONCE][2 * NT];
+#pragma unroll
+              for (int y = 0; y < AT_ONCE; ++y)
+                if (x + y < w.group_n) {
+                  const float* part = gp + (x + y) * gs;
+                  ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)QR * HD + 2 * (w.r0 + qh)));
+#pragma unroll
+                  for (int k = 0; k < NT; ++k) {
+                    const float2 f = __ldcg(reinterpret_cast<const float2*>(part + ((size_t)((warp * NT + k) * 2 + tq / 2) * QR + w.r0 + qh) * 4 + (tq & 1) * 2));
+                    v[y][2 * k] = f.x;
+                    v[y][2 * k + 1] = f.y;
+                  }
+                }
+#pragma unroll
+              for (int y = 0; y < AT_ONCE; ++y)
+                if (x + y < w.group_n) add(ml[y].x, ml[y].y, v[y]);
+            }
+            if (w.pieces == 1) {
+              float v[2 * NT];
+#pragma unroll
+              for (int k = 0; k < NT; ++k) {
+                v[2 * k] = o[k][2 * r];
+                v[2 * k + 1] = o[k][2 * r + 1];
+              }
+              add(m_run[r], l_run[r], v);
+            } else {
+              const float* rp = row_piece(p, QR, first_id);
+              for (int x = 0; x < w.pieces; x += AT_ONCE) {
+                float2 ml[AT_ONCE];
+                float v[AT_ONCE][2 * NT];
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y)
+                  if (x + y < w.pieces) {
+                    const float* part = rp + (x + y) * rs;
+                    ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)G * HD + 2 * qh));
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                      const float2 f = __ldcg(reinterpret_cast<const float2*>(part + (size_t)qh * HD + (warp * NT + k) * 8 + 2 * tq));
+                      v[y][2 * k] = f.x;
+                      v[y][2 * k + 1] = f.y;
+                    }
+                  }
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y)
+                  if (x + y < w.pieces) add(ml[y].x, ml[y].y, v[y]);
+              }
+            }
+            const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + qh) * HD;
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+              *reinterpret_cast<__nv_bfloat162*>(out + (warp * NT + k) * 8 + 2 * tq) = __floats2bfloat162_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+          }
+        }
+      }
+      n_tile = n;
+    }
+    __syncthreads();
+    if (failed || stuck) {
+      if (tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_pieces);
+      break;
+    }
+  }
+}
+
+template <int HD, bool LOW>
+int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
+  using R = Ring<HD, LOW>;
+  CUtensorMap map_kv, map_run;
+  const int rows = p.ps < TILE ? p.ps : TILE;
+  DK_REQUIRE(make_tensor_map_bf16(&map_kv, p.kv, (long long)p.num_pages * 2 * p.KV * p.ps, HD, HD, rows), "attention_shared_prefix: cannot encode the tensor map of the cache");
+  // the cache as [page][K|V, head][offset][hd]: a run of pages of one head in one box
+  const unsigned long long dims[4] = {(unsigned long long)HD, (unsigned long long)p.ps, (unsigned long long)(2 * p.KV), (unsigned long long)p.num_pages};
+  const unsigned long long strides[3] = {(unsigned long long)HD * 2, (unsigned long long)p.ps * HD * 2, (unsigned long long)2 * p.KV * p.ps * HD * 2};
+  DK_REQUIRE(make_tensor_map_bf16_4d(&map_run, p.kv, dims, strides, rows, TILE / rows), "attention_shared_prefix: cannot encode the tensor map of runs of pages");
+  static bool configured_on[DK_MAX_DEVICES] = {false};
+  bool& configured = configured_on[dk_current_device()];
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(attention_shared_prefix_rows_kernel<HD, LOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::TOTAL);
+    if (e != cudaSuccess) {
+      dk_set_error("attention_shared_prefix: cannot get %d bytes of shared memory: %s", R::TOTAL, cudaGetErrorString(e));
+      return DK_ERR_LAUNCH;
+    }
+    configured = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.rows_grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = R::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // it may start while the kernel of the groups runs
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_shared_prefix_rows_kernel<HD, LOW>, map_kv, map_run, p);
+  if (e != cudaSuccess) {
+    dk_set_error("attention_shared_prefix: launch of the rows' kernel failed: %s", cudaGetErrorString(e));
+    return DK_ERR_LAUNCH;
+  }
+  return dk_check_launch("attention_shared_prefix_rows");
+}
+}  // namespace
+
+int dk_shared_prefix_rows_tile() { return TILE; }
+int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p) { return (p.hd == 128 && p.H / p.KV > 8 ? 1 : 2) * dk_sm_count(); }
+int dk_shared_prefix_rows_launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
+  const bool low = p.H / p.KV <= 8;
+  if (p.hd == 64) return low ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
+  return low ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
+}

@@ -1,16 +1,16 @@
-// Attention over shared prefixes on the tcgen05 tensor cores: bfloat16, heads of 64 or 128 (the mathematics and the merge of
-// the pieces are in attention_shared_prefix.cu, how the work is cut in shared_prefix.cuh).
+// Attention over shared prefixes on the tcgen05 tensor cores, bfloat16, heads of 64 or 128: the keys that the rows of a group share.  (The
+// mathematics is in attention_shared_prefix.cu, how the work is cut in shared_prefix.cuh, the rows' own keys and the merge in
+// attention_shared_prefix_rows.cu.)
 //
-// A block walks its pieces one after the other: up to 128 queries (a group's rows with their G heads of one key-value head;
-// of a row's own keys G queries) over tiles of 128 keys.  Both products are tcgen05.mma with accumulators in tensor memory:
+// A block walks its pieces one after the other: up to 128 queries (rows of a group with their G heads of one key-value head)
+// over tiles of 128 keys.  Both products are tcgen05.mma with accumulators in tensor memory:
 //
 //   S = Q K^T   A = Q [128 x hd], B = K [128 keys x hd] from shared memory, K-major; S[128 x 128] float
 //   O += P V    A = P [128 x 128 keys] bfloat16 from shared memory, B = V as it lies in the cache ("MN-major"); O[128 x hd] float
 //
 // Tiles alternate between two halves of the block that do not wait for each other (half w: softmax warps 4w..4w+3, scores S_w,
 // accumulator O_w, weights P_w; tiles w, w + 2, ...), merged at the end of a piece: while one half exponentiates, the tensor
-// cores work for the other.  The same product with M = 128 also serves pieces of G queries: the empty rows cost the
-// tensor cores less time than the tile's 64 KB take to arrive from memory, and warps without a query exponentiate nothing.
+// cores work for the other.  Warps without a query exponentiate nothing.
 //
 //   warps 0-7   softmax: thread r of a half owns query r.  They also fetch the queries, whose rows lie anywhere: the next
 //               piece's are asked for before the merge of this one and stored when its last scores are made.
@@ -50,7 +50,7 @@ struct Layout {
   static constexpr int OFF_P = OFF_V + 2 * TILE_BYTES;    // P of each half: two boxes [128 x 64 keys]
   static constexpr int P_BYTES = 2 * BOX_BYTES;
   static constexpr int TOTAL = OFF_P + 2 * P_BYTES + 1024;   // 1024 to start on a swizzle boundary
-  static_assert(4 * scratch_ints(MAX_ROWS, MAX_GROUPS) <= 4 * TILE_BYTES, "the list is made in the buffers of K and V");
+  static_assert(4 * Tables::ints(0, MAX_GROUPS) <= 4 * TILE_BYTES, "the list is made in the buffers of K and V");
 };
 
 // 2^x by the special-function unit (two units in the last place; results below 2^-126 become 0)
@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
   auto row_stat = [&](int w) { return reinterpret_cast<float2*>(smem + L::OFF_P + w * L::P_BYTES); };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room
+  for (int i = blockIdx.x * THREADS + tid; i < p.rows * p.KV; i += gridDim.x * THREADS) counters(p)[i] = 0;
   const int ps = p.ps, G = p.H / p.KV, rpt = QT / G;
   const uint32_t bar0 = s2u(&bars[0]);
   const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = k_full + 16, s_full = v_full + 16, p_full = s_full + 16, o_done = p_full + 16,
@@ -122,15 +124,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     const uint32_t full = kind ? v_full : k_full, done = kind ? o_done : s_full, sm_dst = kind ? sm_v : sm_k;
     for (int range = blockIdx.x;; range += gridDim.x) {
       {
-        bool left = false;
-        const int n = build<KT, 128>(p, rpt, range, list, reinterpret_cast<int*>(smem + L::OFF_K), tid - PRODUCER_WARP0 * 32,
-                                     [] { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }, range == 0, left);
-        if (warp == PRODUCER_WARP0 && lane == 0) {
-          n_listed = n;
-          ranges_left = left;
+        const int t4 = tid - PRODUCER_WARP0 * 32;
+        auto sync = [] { asm volatile("bar.sync 1, 128;\n" ::: "memory"); };
+        const Tables t(reinterpret_cast<int*>(smem + L::OFF_K), 0, p.groups);
+        load_tables<false, 128>(p, t, t4, sync);
+        const Line l = walk_line<128>(
+            p.groups, p.grid, range, t.line, t4, sync, [&](int e) { return group_entry<KT>(p, t, e, rpt); }, [](int, const Entry&, int, int) {},
+            [&](int e, const Entry&, int i, int seg, int, int j0, int j1, int place, int) { list[place] = piece_of_group<KT>(p, t, e, rpt, i, seg + range, j0, j1); });
+        if (t4 == 0) {
+          n_listed = l.pieces;
+          ranges_left = l.more;
         }
         fence_async_smem();       // the buffers are TMA's from here on
-        asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
       }
       block_barrier();
       const int n_pieces = n_listed;
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         for (int i = 0; i < n_pieces && !failed; ++i) {
           const Piece w(list[i]);
           const int n_tiles = cdiv(w.limit - w.key0, KT);
-          int row = w.of_group ? p.members[w.first] : w.first;
+          int row = p.members[w.first];
           if (row < 0 || row >= p.rows) row = 0;        // recorded when the list was made
           const int* table = p.block_table + (size_t)row * p.max_pages;
           for (int j = 0; j < n_tiles; ++j) {
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     const int qi = r / G, qh = r - qi * G;
     auto ask_q = [&](const Piece& pc, uint4 (&v)[QC]) {
       int row = -1;
-      if (qi < pc.n_rows) row = pc.of_group ? p.members[pc.first + qi] : pc.first;
+      if (qi < pc.n_rows) row = p.members[pc.first + qi];
       const bool held = row >= 0 && row < p.rows;
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (held ? row : 0) * p.q_stride + (pc.kvh * G + qh) * HD + w * (HD / 2));
 #pragma unroll
@@ -424,8 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         const float l_all = l_sum * f_mine + other.y * f_other;
         const float f0 = w == 0 ? f_mine : f_other, f1 = w == 0 ? f_other : f_mine;
         const bool two = n_tiles > 1;                     // O_1 holds nothing when there was one tile
-        const int n = pc.of_group ? QT : G;
-        float* part = pc.of_group ? group_piece(p, QT, pc.id) : row_piece(p, QT, pc.id);
+        float* part = group_piece(p, QT, pc.id);
         if (!busy) {
           tc_fence_before();
           mbar_arrive(piece_done);
@@ -448,10 +452,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
               for (int k = 0; k < 32; ++k) o0[k] = two ? o0[k] * f0 + o1[k] * f1 : o0[k] * f0;
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                *reinterpret_cast<float4*>(part + ((size_t)(col / 4 + k) * n + r) * 4) = make_float4(o0[4 * k], o0[4 * k + 1], o0[4 * k + 2], o0[4 * k + 3]);
+                *reinterpret_cast<float4*>(part + ((size_t)(col / 4 + k) * QT + r) * 4) = make_float4(o0[4 * k], o0[4 * k + 1], o0[4 * k + 2], o0[4 * k + 3]);
             }
           }
-          if (r < queries && w == 0) *reinterpret_cast<float2*>(part + (size_t)n * HD + 2 * r) = make_float2(m_all, l_all);
+          if (r < queries && w == 0) *reinterpret_cast<float2*>(part + (size_t)QT * HD + 2 * r) = make_float2(m_all, l_all);
         }
         ++n_done;
       }
@@ -492,7 +496,7 @@ int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
 }  // namespace
 
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p) {
-  return p.dtype == DK_BF16 && (p.hd == 64 || p.hd == 128) && (p.ps == 8 || p.ps == 16 || p.ps == 32 || p.ps == 64 || p.ps == 128) &&
+  return p.dtype == DK_BF16 && p.H / p.KV <= 16 && (p.hd == 64 || p.hd == 128) && (p.ps == 8 || p.ps == 16 || p.ps == 32 || p.ps == 64 || p.ps == 128) &&
          (long long)p.num_pages * 2 * p.KV * p.ps < (1ll << 31);
 }
 

@@ -1,13 +1,15 @@
-// How the attention over shared prefixes cuts its work: the arguments, the list of pieces that a block takes, and
-// where the partial results lie.  Used by the kernel on the FMA units, the one on the tensor cores and the merge.
+// How the attention over shared prefixes cuts its work: the arguments, the lists of pieces that blocks take, and where the
+// partial results lie.
 //
 // Work comes in segments.  A segment of a group is a tile of its queries (``rpt`` rows with their G query heads of
 // one key-value head) over the group's shared keys; a segment of a row is its G query heads over the keys it holds
-// alone.  A segment is walked in tiles of KT keys.  All tiles of all segments, groups first, stand in one line, which
-// is cut into ranges of Q tiles (as many ranges as blocks run at once): so every block has the same number of tiles
-// whatever the prefixes, the rows and their lengths are, and at most one segment is cut at each border.  A piece is
-// what a range holds of a segment.  Pieces are numbered segment + range: every step from one piece to the next
-// moves to the next segment or to the next range, so no two pieces have one number.
+// alone.  A segment is walked in tiles of KT keys.  The tiles of all segments stand in one line, which is cut into ranges
+// of Q tiles (as many ranges as blocks run at once): so every block has the same number of tiles whatever the prefixes, the
+// rows and their lengths are, and at most one segment is cut at each border.  A piece is what a range holds of a segment.
+// Pieces are numbered segment + range: every step from one piece to the next moves to the next segment or to the next
+// range, so no two pieces have one number.
+//
+// The kernel on the FMA units has groups and rows in one line; on the tensor cores each has a line and a kernel of its own.
 #pragma once
 #include "common.cuh"
 
@@ -22,12 +24,14 @@ struct DkSharedPrefixParams {
   const int* members;        // [n_members] rows, group by group
   const int* group_start;    // [groups + 1] first member of each group
   const int* group_prefix;   // [groups] shared keys (rounded down to whole pages)
-  float* work;               // row records, then the pieces' partial results
+  float* work;               // row records and counters, then the pieces' partial results
   int* err;                  // device error record, 4 ints; or null
   long long q_stride, out_stride;   // elements
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
   float scale;
-  int grid, prefix_pieces;   // set by the launcher: blocks of the first kernel, pieces of groups that the work buffer holds
+  // set by the launcher: blocks over the line of groups (or the only line) and over the line of rows, pieces of groups that the
+  // work buffer holds, and the keys that a group must save for its prefix to be read apart
+  int grid, rows_grid, group_pieces, min_saved;
 };
 
 namespace shared_prefix {
@@ -35,127 +39,136 @@ constexpr int MAX_ROWS = 1024, MAX_GROUPS = 1024, MAX_G = 32;
 constexpr int CAP = 96;            // tiles of a range, so also the most pieces of one
 constexpr int ROW_INTS = 8;        // a row's record for the merge
 
-// ints of shared memory that build() works in
-__host__ __device__ constexpr int scratch_ints(int rows, int groups) { return rows + 4 * groups + 1 + 2 * 32 + 8; }
 __host__ __device__ constexpr int cdiv(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ constexpr int round4(int a) { return (a + 3) / 4 * 4; }
 
-struct Piece {
-  int first;      // of a group: its first member's place in ``members``; of a row: the row
-  int kvh, n_rows, id, key0, limit;
-  bool of_group;
-  __device__ __forceinline__ Piece(const int4& d)
-      : first(d.x & 0x7fffffff), kvh(d.y & 255), n_rows((d.y >> 8) & 255), id((unsigned)d.y >> 16), key0(d.z), limit(d.w), of_group(d.x < 0) {}
-};
-
-// Floats of one piece: outputs as [hd / 4][rows][4] (neighbouring rows lie side by side), then {maximum, sum} per row.
+// Floats of one piece: of a group as [hd / 4][rows][4] (neighbouring rows lie side by side), then {maximum, sum} per row.
 __host__ __device__ __forceinline__ long long group_piece_floats(int qr, int hd) { return (long long)qr * (hd + 2); }
 __host__ __device__ __forceinline__ long long row_piece_floats(int G, int hd) { return ((long long)G * (hd + 2) + 3) / 4 * 4; }
+// ints at the front of the work buffer: a record per row, a counter per row and key-value head
+__host__ __device__ __forceinline__ int front_ints(int rows, int KV) { return round4(rows * ROW_INTS) + round4(rows * KV); }
 
+// The most pieces there can be with these sizes, whatever the device's tables say.
 struct Bounds {
-  long long tiles_of_groups, tiles, group_pieces, row_pieces, floats;
+  long long tiles, group_pieces, row_pieces, floats;
 };
-// The most there can be with these sizes, whatever the device's tables say.
-static inline Bounds bounds(const DkSharedPrefixParams& p, int qr, int kt, int grid) {
+static inline Bounds bounds(const DkSharedPrefixParams& p, int qr, int kt, int grid, int rows_kt, int rows_grid) {
   Bounds b;
   const int G = p.H / p.KV, rpt = qr / G;
-  const long long keys = (long long)p.max_pages * p.ps, tiles = (keys + kt - 1) / kt;
-  const long long segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
-  b.tiles_of_groups = segments * tiles;
-  b.tiles = b.tiles_of_groups + (long long)p.rows * p.KV * tiles;
-  auto ranges = [&](long long n) { return (n + CAP - 1) / CAP > grid ? (n + CAP - 1) / CAP : (long long)grid; };
-  b.group_pieces = segments > 0 ? segments + ranges(b.tiles_of_groups) : 0;
-  b.row_pieces = (long long)p.rows * p.KV + ranges(b.tiles);
-  b.floats = ((long long)p.rows * ROW_INTS + 3) / 4 * 4 + b.group_pieces * group_piece_floats(qr, p.hd) + b.row_pieces * row_piece_floats(G, p.hd);
+  const long long keys = (long long)p.max_pages * p.ps, segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
+  const long long of_groups = segments * ((keys + kt - 1) / kt), of_rows = (long long)p.rows * p.KV * ((keys + rows_kt - 1) / rows_kt);
+  auto ranges = [&](long long n, int blocks) { return (n + CAP - 1) / CAP > blocks ? (n + CAP - 1) / CAP : (long long)blocks; };
+  b.tiles = of_groups + of_rows;
+  b.group_pieces = segments > 0 ? segments + ranges(of_groups, grid) : 0;
+  b.row_pieces = (long long)p.rows * p.KV + ranges(b.tiles, rows_grid);
+  b.floats = front_ints(p.rows, p.KV) + b.group_pieces * group_piece_floats(qr, p.hd) + b.row_pieces * row_piece_floats(G, p.hd);
   return b;
 }
+__device__ __forceinline__ int* row_record(const DkSharedPrefixParams& p, int row) { return reinterpret_cast<int*>(p.work) + row * ROW_INTS; }
+__device__ __forceinline__ int* counters(const DkSharedPrefixParams& p) { return reinterpret_cast<int*>(p.work) + round4(p.rows * ROW_INTS); }
 __device__ __forceinline__ float* group_piece(const DkSharedPrefixParams& p, int qr, int id) {
-  return p.work + (p.rows * ROW_INTS + 3) / 4 * 4 + id * group_piece_floats(qr, p.hd);
+  return p.work + front_ints(p.rows, p.KV) + id * group_piece_floats(qr, p.hd);
 }
 __device__ __forceinline__ float* row_piece(const DkSharedPrefixParams& p, int qr, int id) {
-  return group_piece(p, qr, p.prefix_pieces) + id * row_piece_floats(p.H / p.KV, p.hd);
+  return group_piece(p, qr, p.group_pieces) + id * row_piece_floats(p.H / p.KV, p.hd);
 }
 
-// Fills ``list`` with the pieces of range number ``range`` and returns how many there are; ``ranges_left`` tells whether a range
-// ``range + grid`` exists.  Called by NT threads that can be synchronised with ``sync``; ``s`` holds scratch_ints ints.  With
-// ``write_rows`` the rows' records for the merge are written too.
-template <int KT, int NT, typename Sync>
-__device__ int build(const DkSharedPrefixParams& p, int rpt, int range, int4* list, int* s, int tid, Sync sync, bool write_rows, bool& ranges_left) {
-  int* s_member = s;                       // [rows] the row's place in members, -1: of no group
-  int* s_start = s_member + p.rows;        // [groups + 1]
-  int* s_prefix = s_start + p.groups + 1;  // [groups] shared keys
-  int* s_tile = s_prefix + p.groups;       // [groups] first tile
-  int* s_seg = s_tile + p.groups;          // [groups] first segment
-  int* s_warp = s_seg + p.groups;          // [2][32]
-  int* s_out = s_warp + 64;                // first segment of the range, last one, segments of groups
-  const int lane = tid & 31, warp = tid >> 5;
+// The tables of a call in shared memory.
+struct Tables {
+  int *member, *start, *prefix, *tile, *seg, *line;
+  // [rows] the row's place in members, -1: of no group; [groups + 1]; [groups] keys that are read apart; [groups] first tile and segment in the
+  // line of groups; what walk_line works in
+  static __host__ __device__ constexpr int ints(int rows, int groups) { return rows + 4 * groups + 1 + 64 + 4; }
+  __device__ __forceinline__ Tables(int* s, int rows, int groups)
+      : member(s), start(s + rows), prefix(start + groups + 1), tile(prefix + groups), seg(tile + groups), line(seg + groups) {}
+};
+
+// The last group that starts at member m or before it.
+__device__ __forceinline__ int group_of(const DkSharedPrefixParams& p, const Tables& t, int m) {
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.start[mid] <= m) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Starts and prefixes of the groups, checked.  ROWS: also each row's place among the members.  Ends with a sync.
+template <bool ROWS, int NT, typename Sync>
+__device__ void load_tables(const DkSharedPrefixParams& p, const Tables& t, int tid, Sync sync) {
   const int max_keys = p.max_pages * p.ps;
-  for (int r = tid; r < p.rows; r += NT) s_member[r] = -1;
+  // what the steps below read is asked for at once
+  const int m_first = ROWS && tid < p.n_members ? p.members[tid] : -1;
   for (int g = tid; g <= p.groups; g += NT) {
-    int a = p.groups > 0 ? p.group_start[g] : 0;
-    if (a < 0 || a > p.n_members) {
-      dk_report(p.err, DK_DEV_BAD_GROUP, g, a, p.n_members);
-      a = 0;
-    }
-    s_start[g] = a;
+    int a = 0, b = 0, k = 0;
+    if (p.groups > 0) a = p.group_start[g];
     if (g < p.groups) {
-      int k = p.group_prefix[g];
-      if (k < 0 || k > max_keys) {
-        dk_report(p.err, DK_DEV_BAD_GROUP, g, k, max_keys);
-        k = 0;
-      }
-      s_prefix[g] = k / p.ps * p.ps;
+      b = p.group_start[g + 1];
+      k = p.group_prefix[g];
+    }
+    if (a < 0 || a > p.n_members || (g < p.groups && (b < a || k < 0 || k > max_keys))) {
+      dk_report(p.err, DK_DEV_BAD_GROUP, g, a < 0 || a > p.n_members ? a : (b < a ? b : k), b < a ? p.n_members : max_keys);
+      a = min(max(a, 0), p.n_members);
+      k = 0;
+    }
+    t.start[g] = a;
+    // one row shares nothing, and what saves few keys is read by each row itself
+    if (g < p.groups) t.prefix[g] = (long long)(min(b, p.n_members) - a - 1) * k >= max(p.min_saved, 1) ? k / p.ps * p.ps : 0;
+  }
+  if (ROWS)
+    for (int r = tid; r < p.rows; r += NT) t.member[r] = -1;
+  sync();
+  if (ROWS && p.groups > 0) {
+    const int end = min(t.start[p.groups], p.n_members);
+    for (int m = tid; m < end; m += NT) {
+      if (m < t.start[0]) continue;
+      const int row = m == tid ? m_first : p.members[m];
+      if (row < 0 || row >= p.rows || atomicCAS(&t.member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, group_of(p, t, m), row, p.rows);
     }
   }
-  if (tid == 0) s_out[0] = s_out[1] = -1;
-  sync();
-  auto group_of = [&](int m) {             // the last group that starts at m or before it
-    int lo = 0, hi = p.groups;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_start[mid] <= m) lo = mid;
-      else hi = mid;
-    }
-    return lo;
-  };
-  for (int g = tid; g < p.groups; g += NT)
-    if (s_start[g + 1] < s_start[g]) dk_report(p.err, DK_DEV_BAD_GROUP, g, s_start[g + 1], s_start[g]);
-  if (p.groups > 0)
-    for (int m = s_start[0] + tid; m < s_start[p.groups]; m += NT) {
-      const int row = p.members[m];
-      if (row < 0 || row >= p.rows || atomicCAS(&s_member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, group_of(m), row, p.rows);
-    }
-  sync();
-  // An entry is a group or a row.  Neighbouring threads take neighbouring runs of entries.
-  struct Entry {
-    int segments, tiles, prefix, len;
-  };
-  auto entry = [&](int e, bool report) {
-    Entry x = {0, 0, 0, 0};
-    if (e < p.groups) {
-      const int n = s_start[e + 1] - s_start[e];
-      x.prefix = s_prefix[e];
-      if (n > 0 && x.prefix > 0) {
-        x.tiles = cdiv(x.prefix, KT);
-        x.segments = cdiv(n, rpt) * p.KV;
-      }
-    } else {
-      const int row = e - p.groups, m = s_member[row];
-      x.prefix = m >= 0 ? s_prefix[group_of(m)] : 0;
-      x.len = p.kv_len[row];
-      if (x.len < x.prefix || x.len > max_keys) {
-        if (report) dk_report(p.err, DK_DEV_BAD_GROUP, row, x.len, x.len < x.prefix ? x.prefix : max_keys);
-        x.len = x.prefix;
-      }
-      x.tiles = cdiv(x.len - x.prefix, KT);
-      x.segments = x.tiles > 0 ? p.KV : 0;
-    }
-    return x;
-  };
-  const int entries = p.groups + p.rows, per = cdiv(entries, NT);
-  const int e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
+  if (ROWS) sync();
+}
+
+// An entry of a line: a group or a row, with its segments and the tiles of each.
+struct Entry {
+  int segments, tiles;
+};
+template <int KT>
+__device__ __forceinline__ Entry group_entry(const DkSharedPrefixParams& p, const Tables& t, int g, int rpt) {
+  const int n = t.start[g + 1] - t.start[g], k = t.prefix[g];
+  return n > 0 && k > 0 ? Entry{cdiv(n, rpt) * p.KV, cdiv(k, KT)} : Entry{0, 0};
+}
+// Keys that are read with the row's group, and all of its keys (checked).
+__device__ __forceinline__ int row_prefix(const DkSharedPrefixParams& p, const Tables& t, int row) {
+  const int m = t.member[row];
+  if (m < 0) return 0;
+  const int g = group_of(p, t, m);
+  return m - t.start[g] < t.start[g + 1] - t.start[g] ? t.prefix[g] : 0;
+}
+__device__ __forceinline__ int row_keys(const DkSharedPrefixParams& p, const Tables& t, int row, int n, bool report) {
+  const int m = t.member[row], max_keys = p.max_pages * p.ps;
+  const int shared = m >= 0 ? min(max(p.group_prefix[group_of(p, t, m)], 0), max_keys) / p.ps * p.ps : 0;
+  if (n < shared || n > max_keys) {
+    if (report) dk_report(p.err, DK_DEV_BAD_GROUP, row, n, n < shared ? shared : max_keys);
+    n = row_prefix(p, t, row);
+  }
+  return n;
+}
+
+struct Line {
+  int pieces, total, Q;     // pieces of the range, tiles of the line, tiles of a range
+  bool more;                // whether range + grid exists
+};
+// Walks a line of entries: ``at(e, x, tile, segment)`` for every entry by the thread that owns it, then, behind a sync, ``emit(e, x, i, segment,
+// tile, j0, j1, place, Q)`` for segment i of entry e that the range holds from its tile j0 to j1, at ``place`` of the range's list.  Ends with a sync.
+template <int NT, typename Sync, typename Of, typename At, typename Emit>
+__device__ Line walk_line(int entries, int grid, int range, int* s, int tid, Sync sync, Of of, At at, Emit emit) {
+  const int lane = tid & 31, warp = tid >> 5;
+  const int per = cdiv(entries, NT), e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
   int tiles = 0, segs = 0;
   for (int e = e0; e < e1; ++e) {
-    const Entry x = entry(e, write_rows);
+    const Entry x = of(e);
     tiles += x.segments * x.tiles;
     segs += x.segments;
   }
@@ -169,83 +182,67 @@ __device__ int build(const DkSharedPrefixParams& p, int rpt, int range, int4* li
     }
   }
   if (lane == 31) {
-    s_warp[warp] = tiles_to;
-    s_warp[32 + warp] = segs_to;
+    s[warp] = tiles_to;
+    s[32 + warp] = segs_to;
   }
+  if (tid == 0) s[64] = s[65] = -1;
   sync();
-  int total = 0;
+  Line l;
+  l.total = 0;
   for (int w = 0; w < NT / 32; ++w) {
     if (w < warp) {
-      tiles_to += s_warp[w];
-      segs_to += s_warp[32 + w];
+      tiles_to += s[w];
+      segs_to += s[32 + w];
     }
-    total += s_warp[w];
+    l.total += s[w];
   }
-  const int Q = max(1, min(cdiv(total, p.grid), CAP));
-  const int lo = range * Q, hi = min(total, lo + Q);
-  ranges_left = (range + p.grid) * Q < total;
-  int at = tiles_to - tiles, seg = segs_to - segs;
+  l.Q = max(1, min(cdiv(l.total, grid), CAP));
+  const int lo = range * l.Q, hi = min(l.total, lo + l.Q);
+  l.more = (range + grid) * l.Q < l.total;
+  const int first_tile = tiles_to - tiles, first_seg = segs_to - segs;
+  int a = first_tile, seg = first_seg;
   for (int e = e0; e < e1; ++e) {
-    const Entry x = entry(e, false);
-    const int end = at + x.segments * x.tiles;
-    if (e < p.groups) {
-      s_tile[e] = at;
-      s_seg[e] = seg;
-    }
-    if (at <= lo && lo < end) s_out[0] = seg + (lo - at) / x.tiles;
-    if (at < hi && hi <= end) s_out[1] = seg + (hi - 1 - at) / x.tiles;
-    if (e == p.groups - 1) s_out[2] = seg + x.segments;      // segments of groups
-    at = end;
+    const Entry x = of(e);
+    const int end = a + x.segments * x.tiles;
+    if (a <= lo && lo < end) s[64] = seg + (lo - a) / x.tiles;
+    if (a < hi && hi <= end) s[65] = seg + (hi - 1 - a) / x.tiles;
+    at(e, x, a, seg);
+    a = end;
     seg += x.segments;
   }
-  if (p.groups == 0 && tid == 0) s_out[2] = 0;
   sync();
-  const int first_seg = s_out[0], group_segs = s_out[2];
-  at = tiles_to - tiles;
-  seg = segs_to - segs;
+  const int seg0 = s[64];
+  l.pieces = lo < hi ? s[65] - seg0 + 1 : 0;
+  a = first_tile;
+  seg = first_seg;
   for (int e = e0; e < e1; ++e) {
-    const Entry x = entry(e, false);
-    const int end = at + x.segments * x.tiles;
-    const bool of_group = e < p.groups;
-    if (lo < hi && x.segments > 0 && at < hi && end > lo) {
-      const int i0 = max(0, (lo - at) / x.tiles), i1 = min(x.segments - 1, (hi - 1 - at) / x.tiles);
+    const Entry x = of(e);
+    const int end = a + x.segments * x.tiles;
+    if (lo < hi && x.segments > 0 && a < hi && end > lo) {
+      const int i0 = max(0, (lo - a) / x.tiles), i1 = min(x.segments - 1, (hi - 1 - a) / x.tiles);
       for (int i = i0; i <= i1; ++i) {
-        const int a = at + i * x.tiles, j0 = max(0, lo - a), j1 = min(x.tiles, hi - a);
-        int4 d;
-        if (of_group) {
-          const int m0 = s_start[e] + (i / p.KV) * rpt, n = min(rpt, s_start[e + 1] - m0);
-          d.x = (int)(0x80000000u | (unsigned)m0);
-          d.y = (i % p.KV) | (n << 8) | ((seg + i + range) << 16);
-          d.z = j0 * KT;
-          d.w = min(x.prefix, j1 * KT);
-        } else {
-          d.x = e - p.groups;
-          d.y = i | (1 << 8) | ((seg + i - group_segs + range) << 16);
-          d.z = x.prefix + j0 * KT;
-          d.w = min(x.len, x.prefix + j1 * KT);
-        }
-        list[seg + i - first_seg] = d;
+        const int b = a + i * x.tiles;
+        emit(e, x, i, seg + i, b, max(0, lo - b), min(x.tiles, hi - b), seg + i - seg0, l.Q);
       }
     }
-    if (write_rows && !of_group) {
-      const int row = e - p.groups, m = s_member[row];
-      int* rec = reinterpret_cast<int*>(p.work) + row * ROW_INTS;
-      int r[ROW_INTS] = {0, 0, 0, 0, seg - group_segs, at, x.tiles, Q};
-      const int g = m >= 0 ? group_of(m) : 0, i = m - s_start[g];
-      if (x.prefix > 0 && i < s_start[g + 1] - s_start[g]) {      // (a start below the one before it was recorded)
-        const int pt = cdiv(x.prefix, KT), qt = i / rpt;
-        r[0] = s_seg[g] + qt * p.KV;
-        r[1] = s_tile[g] + qt * p.KV * pt;
-        r[2] = pt;
-        r[3] = i % rpt * (p.H / p.KV);
-      }
-      for (int i = 0; i < ROW_INTS; ++i) rec[i] = r[i];
-    }
-    at = end;
+    a = end;
     seg += x.segments;
   }
-  const int n = lo < hi ? s_out[1] - first_seg + 1 : 0;
   sync();
-  return n;
+  return l;
+}
+
+// A piece of a group, 16 bytes: x the place of its first member (bit 31 set), y key-value head, rows and number, z first key, w key behind the last.
+// A piece of a row in the line of both: x the row.
+struct Piece {
+  int first, kvh, n_rows, id, key0, limit;
+  bool of_group;
+  __device__ __forceinline__ Piece(const int4& d)
+      : first(d.x & 0x7fffffff), kvh(d.y & 255), n_rows((d.y >> 8) & 255), id((unsigned)d.y >> 16), key0(d.z), limit(d.w), of_group(d.x < 0) {}
+};
+template <int KT>
+__device__ __forceinline__ int4 piece_of_group(const DkSharedPrefixParams& p, const Tables& t, int g, int rpt, int i, int id, int j0, int j1) {
+  const int m0 = t.start[g] + i / p.KV * rpt, n = min(rpt, t.start[g + 1] - m0);
+  return make_int4((int)(0x80000000u | (unsigned)m0), (i % p.KV) | (n << 8) | (id << 16), j0 * KT, min(t.prefix[g], j1 * KT));
 }
 }  // namespace shared_prefix
