@@ -16,9 +16,11 @@
 // It is bound by the FMA units and the shared-memory reads that feed them (nine 16-byte reads for 32 FMAs).
 #include "shared_prefix.cuh"
 
+// shared_prefix_plan.cu
+int dk_shared_prefix_plan_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
 // attention_shared_prefix_tc.cu
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
-int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
+int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream);
 // attention_shared_prefix_rows.cu
 int dk_shared_prefix_rows_tile();
 int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p);
@@ -46,62 +48,6 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
-// The range's pieces; the block of range 0 also writes the rows' records.
-__device__ int make_list(const DkSharedPrefixParams& p, int rpt, int range, int4* list, int* scratch, int tid, bool& more) {
-  const Tables t(scratch, p.rows, p.groups);
-  auto sync = [] { __syncthreads(); };
-  load_tables<true, THREADS>(p, t, tid, sync);
-  // segments of groups come first, those of rows are numbered from zero again: how many there are stands in t.line[67]
-  if (tid == 0) t.line[67] = 0;
-  auto keys_of = [&](int row, bool report) { return row_keys(p, t, row, p.kv_len[row], report); };
-  const Line l = walk_line<THREADS>(
-      p.groups + p.rows, p.grid, range, t.line, tid, sync,
-      [&](int e) {
-        if (e < p.groups) return group_entry<KT>(p, t, e, rpt);
-        const int tiles = cdiv(keys_of(e - p.groups, range == 0) - row_prefix(p, t, e - p.groups), KT);
-        return Entry{tiles > 0 ? p.KV : 0, tiles};
-      },
-      [&](int e, const Entry& x, int tile, int seg) {
-        if (e < p.groups) {
-          t.tile[e] = tile;
-          t.seg[e] = seg;
-          if (e == p.groups - 1) t.line[67] = seg + x.segments;
-        }
-        if (range == 0 && e >= p.groups) {
-          int* rec = row_record(p, e - p.groups);
-          rec[4] = seg;
-          rec[5] = tile;
-          rec[6] = x.tiles;
-        }
-      },
-      [&](int e, const Entry&, int i, int seg, int, int j0, int j1, int place, int) {
-        if (e < p.groups) {
-          list[place] = piece_of_group<KT>(p, t, e, rpt, i, seg + range, j0, j1);
-        } else {
-          const int row = e - p.groups, own = row_prefix(p, t, row);
-          list[place] = make_int4(row, i | (1 << 8) | ((seg - t.line[67] + range) << 16), own + j0 * KT, min(keys_of(row, false), own + j1 * KT));
-        }
-      });
-  if (range == 0)
-    for (int row = tid; row < p.rows; row += THREADS) {
-      const int m = t.member[row], k = row_prefix(p, t, row);
-      int* rec = row_record(p, row);
-      rec[2] = 0;
-      if (k > 0) {
-        const int g = group_of(p, t, m), i = m - t.start[g], pt = cdiv(k, KT);
-        rec[0] = t.seg[g] + i / rpt * p.KV;
-        rec[1] = t.tile[g] + i / rpt * p.KV * pt;
-        rec[2] = pt;
-        rec[3] = i % rpt * (p.H / p.KV);
-      }
-      rec[4] -= t.line[67];
-      rec[7] = l.Q;
-    }
-  more = l.more;
-  __syncthreads();
-  return l.pieces;
-}
-
 // HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
 __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
@@ -112,151 +58,157 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
   float* s_k = s_q + QR * hd;          // [KT][hd + 4]
   float* s_v = s_k + KT * ks;          // [KT][hd]
   float* s_p = s_v + KT * hd;          // [QR][KT + 4]
-  __shared__ int4 list[CAP];
   __shared__ int s_page[KT];
   const int tid = threadIdx.x, r = tid / EIGHT, c = tid % EIGHT;
-  const int G = p.H / p.KV, rpt = QR / G;
+  const int G = p.H / p.KV;
   const float sl2 = p.scale * 1.4426950408889634f;
-  bool more = true;
-  for (int range = blockIdx.x; more; range += gridDim.x) {
-    const int n_pieces = make_list(p, rpt, range, list, reinterpret_cast<int*>(smem), tid, more);
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
-    for (int i = 0; i < n_pieces; ++i) {
-      const Piece w(list[i]);
-      const int rows = w.n_rows * G;
-      auto row_at = [&](int k) { return w.of_group ? p.members[w.first + k] : w.first; };
-      for (int x = tid; x < QR * c4s; x += THREADS) {
-        const int qr = x / c4s, col = x % c4s * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (qr < rows) {
-          const int row = row_at(qr / G);
-          if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
-        }
-        *reinterpret_cast<float4*>(s_q + qr * hd + col) = v;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
+  const Plan plan(p);
+  const int n_ranges = plan.head[0], row_pieces = plan.head[1];
+  // first the pieces of the block's ranges of groups, then its pieces of rows
+  int range = blockIdx.x, i = 0, row_piece = gridDim.x - 1 - blockIdx.x;
+  for (;;) {
+    const bool of_group = range < n_ranges;
+    GroupPiece w;
+    if (of_group) {
+      w = plan.group_pieces[plan.ranges[2 * range] + i];
+      if (++i == plan.ranges[2 * range + 1]) {
+        i = 0;
+        range += gridDim.x;
       }
-      const int table_row = row_at(0);
-      const int* table = p.block_table + (size_t)((table_row >= 0 && table_row < p.rows) ? table_row : 0) * p.max_pages;
-      float o[OC][4];
+    } else if (row_piece < row_pieces) {
+      const RowPiece x = plan.row_pieces[row_piece];
+      w = {x.row, 1, x.kvh, row_piece, x.key0, x.limit, x.row, 0};
+      row_piece += gridDim.x;
+    } else {
+      break;
+    }
+    const int rows = w.rows * G;
+    auto row_at = [&](int k) { return of_group ? p.members[w.first + k] : w.first; };
+    for (int x = tid; x < QR * c4s; x += THREADS) {
+      const int qr = x / c4s, col = x % c4s * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (qr < rows) {
+        const int row = row_at(qr / G);
+        if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
+      }
+      *reinterpret_cast<float4*>(s_q + qr * hd + col) = v;
+    }
+    const int* table = p.block_table + (size_t)w.table_row * p.max_pages;
+    float o[OC][4];
+#pragma unroll
+    for (int k = 0; k < OC; ++k)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[k][d] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    for (int kb = w.key0; kb < w.limit; kb += KT) {
+      const int n = min(KT, w.limit - kb);
+      __syncthreads();        // the tile before is no longer read
+      if (tid < KT) {
+        int page = -1;
+        if (tid < n) {
+          const int lp = (kb + tid) / p.ps;        // below max_pages: the plan's limits are checked
+          page = table[lp];
+          if (page < 0 || page >= p.num_pages) {
+            dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
+            page = -1;
+          }
+        }
+        s_page[tid] = page;
+      }
+      __syncthreads();
+      for (int x = tid; x < KT * c4s; x += THREADS) {
+        const int key = x / c4s, col = x % c4s * 4, page = s_page[key];
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+        if (page >= 0) {
+          const T* src = reinterpret_cast<const T*>(p.kv) + (((size_t)page * 2 * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd + col;
+          k = load4(src);
+          v = load4(src + (size_t)p.KV * p.ps * hd);
+        }
+        *reinterpret_cast<float4*>(s_k + key * ks + col) = k;
+        *reinterpret_cast<float4*>(s_v + key * hd + col) = v;
+      }
+      __syncthreads();
+      float s[KT / EIGHT];
+#pragma unroll
+      for (int j = 0; j < KT / EIGHT; ++j) s[j] = 0.f;
+#pragma unroll 2
+      for (int d = 0; d < hd; d += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(s_q + r * hd + d);
+#pragma unroll
+        for (int j = 0; j < KT / EIGHT; ++j) {
+          const float4 b = *reinterpret_cast<const float4*>(s_k + (j * EIGHT + c) * ks + d);
+          s[j] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[j]))));
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < KT / EIGHT; ++j) {
+        s[j] = j * EIGHT + c < n ? s[j] * sl2 : -INFINITY;
+        mx = fmaxf(mx, s[j]);
+      }
+#pragma unroll
+      for (int x = 1; x < EIGHT; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float m_new = fmaxf(m_run, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float keep = exp2f(m_run - m_use);       // 0 before the first key
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < KT / EIGHT; ++j) {
+        const float e = exp2f(s[j] - m_use);
+        sum += e;
+        s_p[r * p_stride() + j * EIGHT + c] = e;
+      }
+      l_run = l_run * keep + sum;
+      m_run = m_new;
 #pragma unroll
       for (int k = 0; k < OC; ++k)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) o[k][d] = 0.f;
-      float m_run = -INFINITY, l_run = 0.f;
-      for (int kb = w.key0; kb < w.limit; kb += KT) {
-        const int n = min(KT, w.limit - kb);
-        __syncthreads();        // the tile before (and what the list was built in) is no longer read
-        if (tid < KT) {
-          int page = -1;
-          if (tid < n) {
-            const int lp = (kb + tid) / p.ps;        // below max_pages: limits are checked when the list is built
-            page = table[lp];
-            if (page < 0 || page >= p.num_pages) {
-              dk_report(p.err, DK_DEV_BAD_PAGE, table_row, lp, page);
-              page = -1;
-            }
-          }
-          s_page[tid] = page;
-        }
-        __syncthreads();
-        for (int x = tid; x < KT * c4s; x += THREADS) {
-          const int key = x / c4s, col = x % c4s * 4, page = s_page[key];
-          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-          if (page >= 0) {
-            const T* src = reinterpret_cast<const T*>(p.kv) + (((size_t)page * 2 * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd + col;
-            k = load4(src);
-            v = load4(src + (size_t)p.KV * p.ps * hd);
-          }
-          *reinterpret_cast<float4*>(s_k + key * ks + col) = k;
-          *reinterpret_cast<float4*>(s_v + key * hd + col) = v;
-        }
-        __syncthreads();
-        float s[KT / EIGHT];
+        for (int d = 0; d < 4; ++d) o[k][d] *= keep;
+      __syncwarp();           // a query's eight threads are of one warp
+      for (int key = 0; key < n; ++key) {
+        const float e = s_p[r * p_stride() + key];
 #pragma unroll
-        for (int j = 0; j < KT / EIGHT; ++j) s[j] = 0.f;
-#pragma unroll 2
-        for (int d = 0; d < hd; d += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(s_q + r * hd + d);
-#pragma unroll
-          for (int j = 0; j < KT / EIGHT; ++j) {
-            const float4 b = *reinterpret_cast<const float4*>(s_k + (j * EIGHT + c) * ks + d);
-            s[j] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[j]))));
-          }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < KT / EIGHT; ++j) {
-          s[j] = j * EIGHT + c < n ? s[j] * sl2 : -INFINITY;
-          mx = fmaxf(mx, s[j]);
-        }
-#pragma unroll
-        for (int x = 1; x < EIGHT; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        const float m_new = fmaxf(m_run, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float keep = exp2f(m_run - m_use);       // 0 before the first key
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < KT / EIGHT; ++j) {
-          const float e = exp2f(s[j] - m_use);
-          sum += e;
-          s_p[r * p_stride() + j * EIGHT + c] = e;
-        }
-        l_run = l_run * keep + sum;
-        m_run = m_new;
-#pragma unroll
-        for (int k = 0; k < OC; ++k)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) o[k][d] *= keep;
-        __syncwarp();           // a query's eight threads are of one warp
-        for (int key = 0; key < n; ++key) {
-          const float e = s_p[r * p_stride() + key];
-#pragma unroll
-          for (int k = 0; k < OC; ++k) {
-            const int col = k * 32 + c * 4;
-            if (col < hd) {
-              const float4 v = *reinterpret_cast<const float4*>(s_v + key * hd + col);
-              o[k][0] = fmaf(e, v.x, o[k][0]);
-              o[k][1] = fmaf(e, v.y, o[k][1]);
-              o[k][2] = fmaf(e, v.z, o[k][2]);
-              o[k][3] = fmaf(e, v.w, o[k][3]);
-            }
+        for (int k = 0; k < OC; ++k) {
+          const int col = k * 32 + c * 4;
+          if (col < hd) {
+            const float4 v = *reinterpret_cast<const float4*>(s_v + key * hd + col);
+            o[k][0] = fmaf(e, v.x, o[k][0]);
+            o[k][1] = fmaf(e, v.y, o[k][1]);
+            o[k][2] = fmaf(e, v.z, o[k][2]);
+            o[k][3] = fmaf(e, v.w, o[k][3]);
           }
         }
       }
-#pragma unroll
-      for (int x = 1; x < EIGHT; x <<= 1) l_run += __shfl_xor_sync(0xffffffffu, l_run, x);
-      if (r < rows) {
-        const int n = w.of_group ? QR : G;
-        float* part = w.of_group ? group_piece(p, QR, w.id) : row_piece(p, QR, w.id);
-#pragma unroll
-        for (int k = 0; k < OC; ++k)
-          if (k * 32 + c * 4 < hd)
-            *reinterpret_cast<float4*>(part + ((size_t)(k * 8 + c) * n + r) * 4) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
-        if (c == 0) *reinterpret_cast<float2*>(part + (size_t)n * hd + 2 * r) = make_float2(m_run, l_run);
-      }
-      __syncthreads();          // the queries may be overwritten
     }
+#pragma unroll
+    for (int x = 1; x < EIGHT; x <<= 1) l_run += __shfl_xor_sync(0xffffffffu, l_run, x);
+    if (r < rows) {
+      float* part = of_group ? group_results(p, w.id) : row_results(p, w.id);
+#pragma unroll
+      for (int k = 0; k < OC; ++k)
+        if (k * 32 + c * 4 < hd)
+          *reinterpret_cast<float4*>(part + (of_group ? ((size_t)(k * 8 + c) * QR + r) * 4 : (size_t)r * hd + k * 32 + c * 4)) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
+      if (c == 0) *reinterpret_cast<float2*>(part + (size_t)(of_group ? QR : G) * hd + 2 * r) = make_float2(m_run, l_run);
+    }
+    __syncthreads();          // the queries may be overwritten
   }
 }
 
-// One block per (key-value head, row): thread (column group, head), heads fastest, as the pieces lie.
+// One block per (key-value head, row): thread (column group, head), heads fastest.
 template <typename T>
-__global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p, const int qr) {
+__global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p) {
   const int kvh = blockIdx.x, row = blockIdx.y, G = p.H / p.KV;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int4 a = *reinterpret_cast<const int4*>(p.work + row * ROW_INTS), b = *reinterpret_cast<const int4*>(p.work + row * ROW_INTS + 4);
-  const int Q = b.w;
-  // pieces of the shared keys: segment a.x + kvh, tiles [a.y + kvh a.z, + a.z); of the row's own: b.x + kvh, [b.y + kvh b.z, + b.z)
-  const int pf = a.z > 0 ? (a.y + kvh * a.z) / Q : 0, pn = a.z > 0 ? (a.y + kvh * a.z + a.z - 1) / Q - pf + 1 : 0;
-  const int sf = b.z > 0 ? (b.y + kvh * b.z) / Q : 0, sn = b.z > 0 ? (b.y + kvh * b.z + b.z - 1) / Q - sf + 1 : 0;
-  const long long gs = group_piece_floats(qr, p.hd), rs = row_piece_floats(G, p.hd);
-  const float* gp = group_piece(p, qr, a.x + kvh + pf);
-  const float* rp = row_piece(p, qr, b.x + kvh + sf);
+  const Plan plan(p);
+  const RowPiece w = plan.row_pieces[plan.rows[2 * row] + kvh * plan.rows[2 * row + 1]];
+  const long long gs = group_piece_floats(QR, p.hd), rs = row_piece_floats(G, p.hd);
+  const float* gp = group_results(p, w.group_id);
+  const float* rp = row_results(p, w.first_id);
   for (int x = threadIdx.x; x < G * (p.hd / 4); x += blockDim.x) {
     const int g = x % G, c4 = x / G;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float* part, int n, int r) {
-      const float2 ml = *reinterpret_cast<const float2*>(part + (size_t)n * p.hd + 2 * r);
-      const float4 o = *reinterpret_cast<const float4*>(part + ((size_t)c4 * n + r) * 4);
+    auto add = [&](const float2 ml, const float4 o) {
       const float m_new = fmaxf(M, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
       const float keep = exp2f(M - m_use), f = exp2f(ml.x - m_use);
       M = m_new;
@@ -266,8 +218,25 @@ __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams 
       acc.z = acc.z * keep + o.z * f;
       acc.w = acc.w * keep + o.w * f;
     };
-    for (int i = 0; i < pn; ++i) add(gp + i * gs, qr, a.w + g);
-    for (int i = 0; i < sn; ++i) add(rp + i * rs, G, g);
+    constexpr int AT_ONCE = 8;        // pieces asked for together, added in order
+    for (int i = 0; i < w.group_n + w.pieces; i += AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float4 o[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int n = i + j;
+        if (n < w.group_n) {
+          ml[j] = *reinterpret_cast<const float2*>(gp + n * gs + (size_t)QR * p.hd + 2 * (w.r0 + g));
+          o[j] = *reinterpret_cast<const float4*>(gp + n * gs + ((size_t)c4 * QR + w.r0 + g) * 4);
+        } else if (n < w.group_n + w.pieces) {
+          ml[j] = *reinterpret_cast<const float2*>(rp + (n - w.group_n) * rs + (size_t)G * p.hd + 2 * g);
+          o[j] = *reinterpret_cast<const float4*>(rp + (n - w.group_n) * rs + (size_t)g * p.hd + c4 * 4);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (i + j < w.group_n + w.pieces) add(ml[j], o[j]);
+    }
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
     T* out = reinterpret_cast<T*>(p.out) + row * p.out_stride + (kvh * G + g) * p.hd + c4 * 4;
     if constexpr (sizeof(T) == 4) {
@@ -281,8 +250,7 @@ __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams 
 
 template <typename T, int HDM>
 int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
-  const size_t need = smem_floats(p.hd), scratch = Tables::ints(p.rows, p.groups);
-  const size_t smem = 4 * (need > scratch ? need : scratch);
+  const size_t smem = 4 * smem_floats(p.hd);
   static size_t granted_on[DK_MAX_DEVICES] = {0};
   size_t& granted = granted_on[dk_current_device()];
   if (smem > granted) {
@@ -307,7 +275,7 @@ int launch_sized(const DkSharedPrefixParams& p, cudaStream_t stream) {
 
 int fma_grid() { return 2 * dk_sm_count(); }
 
-int merge(const DkSharedPrefixParams& p, int qr, cudaStream_t stream) {
+int merge(const DkSharedPrefixParams& p, cudaStream_t stream) {
   const int work = p.H / p.KV * (p.hd / 4);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.KV, p.rows);
@@ -318,8 +286,8 @@ int merge(const DkSharedPrefixParams& p, int qr, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = p.dtype == DK_F32 ? cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<float>, p, qr)
-                                    : cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<__nv_bfloat16>, p, qr);
+  cudaError_t e = p.dtype == DK_F32 ? cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<float>, p)
+                                    : cudaLaunchKernelEx(&cfg, attention_shared_prefix_merge_kernel<__nv_bfloat16>, p);
   if (e != cudaSuccess) {
     dk_set_error("attention_shared_prefix: launch of the merge failed: %s", cudaGetErrorString(e));
     return DK_ERR_LAUNCH;
@@ -342,59 +310,70 @@ int check_sizes(const DkSharedPrefixParams& p) {
   return 0;
 }
 
-// Whether the tensor cores take these sizes, and how the work is cut then: queries and keys of a tile, blocks; the same for rows.
-struct Cut {
-  bool tc;
-  int qr, kt, grid, rows_kt, rows_grid;
-  Bounds of(const DkSharedPrefixParams& p) const { return bounds(p, qr, kt, grid, rows_kt, rows_grid); }
-};
-Cut cut_for(const DkSharedPrefixParams& p) {
-  if (dk_shared_prefix_tc_takes(p)) return {true, 128, 128, dk_sm_count(), dk_shared_prefix_rows_tile(), dk_shared_prefix_rows_grid(p)};
-  return {false, QR, KT, fma_grid(), KT, fma_grid()};
+// How the work is cut: by the tensor cores' kernels where they take the sizes, else for the FMA units.  Returns which.
+bool cut(DkSharedPrefixParams& p) {
+  const bool tc = dk_shared_prefix_tc_takes(p);
+  p.qr = tc ? 128 : QR;
+  p.kt = tc ? 128 : KT;
+  p.grid = tc ? dk_sm_count() : fma_grid();
+  p.rows_kt = tc ? dk_shared_prefix_rows_tile() : KT;
+  p.rows_grid = tc ? dk_shared_prefix_rows_grid(p) : fma_grid();
+  p.min_saved = 1;
+  return tc;
 }
 
-int floats_needed(const DkSharedPrefixParams& p, long long* floats) {
-  const Bounds b = cut_for(p).of(p);
-  DK_REQUIRE(b.tiles < (1ll << 30) && b.group_pieces < 65536 && b.row_pieces < 65536,
-             "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call", p.rows, p.KV, p.max_pages);
-  *floats = b.floats;
+int sizes(DkSharedPrefixParams& p, bool* tc, Bounds* b) {
+  if (int rc = check_sizes(p)) return rc;
+  *tc = cut(p);
+  *b = bounds(p);
+  DK_REQUIRE(b->tiles < (1ll << 30) && b->plan_ints < (1ll << 30), "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call",
+             p.rows, p.KV, p.max_pages);
   return 0;
 }
 }  // namespace
 
-// Floats of working memory that a call with these sizes needs.
-extern "C" int dk_attention_shared_prefix_floats(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, int dtype, long long* floats) {
+// Ints that the plan and floats that the working memory of a call with these sizes need: need[0] and need[1].
+extern "C" int dk_attention_shared_prefix_sizes(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, int dtype, long long* need) {
   DkSharedPrefixParams p = {};
   p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = num_pages; p.dtype = dtype;
-  if (int rc = check_sizes(p)) return rc;
-  return floats_needed(p, floats);
+  bool tc;
+  Bounds b;
+  if (int rc = sizes(p, &tc, &b)) return rc;
+  need[0] = b.plan_ints;
+  need[1] = b.work_floats;
+  return 0;
 }
 
+// make_plan: the plan is worked out first, else it holds what an earlier call with the same tables and sizes left.  q null: nothing else is done.
 extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, void* out, long long out_stride, const void* kv, const int* block_table, const int* kv_len,
-                                          const int* members, const int* group_start, const int* group_prefix, void* work, long long work_floats, int rows, int groups,
-                                          int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale, int dtype, int* err, cudaStream_t stream) {
-  DkSharedPrefixParams p = {q, out, kv, block_table, kv_len, members, group_start, group_prefix, (float*)work, err, q_stride, out_stride,
-                            rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype, scale, 0, 0, 0, 0};
-  int rc = check_sizes(p);
-  if (rc != 0) return rc;
+                                          const int* members, const int* group_start, const int* group_prefix, int* plan, long long plan_ints, int make_plan, void* work,
+                                          long long work_floats, int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale,
+                                          int dtype, int* err, cudaStream_t stream) {
+  DkSharedPrefixParams p = {};
+  p.q = q; p.out = out; p.kv = kv; p.block_table = block_table; p.kv_len = kv_len; p.members = members; p.group_start = group_start; p.group_prefix = group_prefix;
+  p.plan = plan; p.work = (float*)work; p.err = err; p.q_stride = q_stride; p.out_stride = out_stride;
+  p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = num_pages; p.dtype = dtype;
+  p.scale = scale;
+  bool tc;
+  Bounds b;
+  if (int rc = sizes(p, &tc, &b)) return rc;
   if (rows == 0) return 0;
-  long long need = 0;
-  if ((rc = floats_needed(p, &need)) != 0) return rc;
-  DK_REQUIRE(q && out && kv && block_table && kv_len && work && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
-  DK_REQUIRE(work_floats >= need, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, need);
-  DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
-  DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
-             "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
-  const Cut c = cut_for(p);
-  DK_REQUIRE(!c.tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
-  p.grid = c.tc && p.groups == 0 ? 1 : c.grid;
-  p.rows_grid = c.rows_grid;
-  p.group_pieces = (int)c.of(p).group_pieces;
-  p.min_saved = 1;
-  if (c.tc) {
-    rc = dk_shared_prefix_tc_launch(p, stream);
+  DK_REQUIRE(kv_len && plan && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a table is missing");
+  DK_REQUIRE(plan_ints >= b.plan_ints && ((uintptr_t)plan % 16) == 0, "attention_shared_prefix: a plan of %lld ints is given, %lld on a 16-byte boundary are needed", plan_ints, b.plan_ints);
+  if (q != nullptr) {
+    DK_REQUIRE(out && kv && block_table && work, "attention_shared_prefix: a tensor is missing");
+    DK_REQUIRE(work_floats >= b.work_floats, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, b.work_floats);
+    DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
+    DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
+               "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
+    DK_REQUIRE(!tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
+  }
+  int rc = make_plan ? dk_shared_prefix_plan_launch(p, stream) : 0;
+  if (rc != 0 || q == nullptr) return rc;
+  if (tc) {
+    rc = dk_shared_prefix_tc_launch(p, make_plan != 0, stream);
     return rc != 0 ? rc : dk_shared_prefix_rows_launch(p, stream);
   }
   rc = dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);
-  return rc != 0 ? rc : merge(p, c.qr, stream);
+  return rc != 0 ? rc : merge(p, stream);
 }

@@ -2,8 +2,8 @@
 // kernel of the groups (attention_shared_prefix_tc.cu) leaves.
 //
 // A row's G <= 16 query heads of one key-value head are the rows of a warp-level MMA tile; the kernel is bound by the bytes of
-// K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM, each over a range of tiles of 64 keys that may
-// begin and end inside a row's segment.  Tiles flow through a ring without a stop between rows:
+// K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM and take pieces in turn; their tiles of 64 keys flow
+// through a ring without a stop between pieces:
 //
 //   warp 4     fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
 //              box per page; pages behind the last key are left out), and with a segment's first tile its queries
@@ -12,7 +12,7 @@
 //              between them at a segment's end.
 //
 // Behind a segment's last tile its row is finished: the pieces of its group's shared keys are added in their order, then the row's own, and
-// the result is rounded once.  Where a segment is cut between blocks, each leaves its piece in the work buffer and counts itself; the one that comes
+// the result is rounded once.  Where a segment is cut, each block leaves its piece's results in the work buffer and counts itself; the one that comes
 // last adds them all, in their order, so the result does not depend on who that is.  The counters are cleared by the kernel of the groups.
 // This kernel starts while that one runs and waits for its end before it touches what it wrote.
 #include "shared_prefix.cuh"
@@ -23,7 +23,7 @@
 namespace {
 using namespace shared_prefix;
 constexpr int TILE = 64;           // keys of a tile
-constexpr int QR = 128;            // queries of a group's piece
+constexpr int LISTED = 32;         // pieces whose records lie in shared memory at once
 constexpr int ROWS = 16;           // rows of the MMA tile
 constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
 
@@ -37,14 +37,6 @@ struct Ring {
   static constexpr int STAGES = HD == 128 && LOW ? 3 : 5;
   static constexpr int BLOCKS = HD == 128 && !LOW ? 1 : 2;            // on an SM
   static constexpr int TOTAL = STAGES * STAGE + 1024;                // 1024 to start on a swizzle boundary
-  static_assert(4 * Tables::ints(MAX_ROWS, MAX_GROUPS) <= STAGES * STAGE, "the list is made in the ring");
-};
-
-// What a range holds of a row's segment.
-struct RowPiece {
-  int row, kvh, key0, limit;
-  int id, index, pieces;           // number of this piece, its place among its segment's, how many those are
-  int group_id, group_n, r0;       // the segment of the row's group: first piece, how many, the row's first query in their tile
 };
 
 // LOW: at most 8 query heads; rows 8..15 of the MMA tile are then empty and their accumulators two registers that stay zero.
@@ -77,13 +69,13 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) unsigned long long bars[2 * R::STAGES];   // full, then empty
-  __shared__ __align__(16) RowPiece list[CAP];
+  __shared__ RowPiece list[LISTED];
   __shared__ __align__(16) unsigned char s_p[ROWS * TILE * 2];      // weights [row][key], 16-byte chunks exchanged by the row
   __shared__ float s_max[WARPS][ROWS], s_sum[WARPS][ROWS];
   __shared__ int s_last;
   __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
-  const int ps = p.ps, G = p.H / p.KV, rpt = QR / G;
+  const int ps = p.ps, G = p.H / p.KV;
   const uint32_t full = s2u(&bars[0]), empty = full + 8 * R::STAGES, ring = s2u(smem);
   if (tid == 0) {
     for (int s = 0; s < R::STAGES; ++s) {
@@ -94,54 +86,16 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   const float sl2 = p.scale * 1.4426950408889634f;
-  int n_tile = 0;                 // tiles this block has had in the ranges before
-  bool waited = false, more = true;
-  for (int range = blockIdx.x; more; range += gridDim.x) {
-    int n_pieces;
-    {
-      auto sync = [] { __syncthreads(); };
-      const Tables t(reinterpret_cast<int*>(smem), p.rows, p.groups);
-      load_tables<true, THREADS>(p, t, tid, sync);
-      int QA = 1;
-      if (p.groups > 0)
-        QA = walk_line<THREADS>(
-                 p.groups, p.grid, -1, t.line, tid, sync, [&](int e) { return group_entry<2 * TILE>(p, t, e, rpt); },
-                 [&](int e, const Entry&, int tile, int seg) {
-                   t.tile[e] = tile;
-                   t.seg[e] = seg;
-                 },
-                 [](int, const Entry&, int, int, int, int, int, int, int) {}).Q;
-      const Line l = walk_line<THREADS>(
-          p.rows, p.rows_grid, range, t.line, tid, sync,
-          [&](int row) {
-            return Entry{p.KV, max(1, cdiv(row_keys(p, t, row, p.kv_len[row], true) - row_prefix(p, t, row), TILE))};      // (a row without a key of its own has an empty tile)
-          },
-          [&](int, const Entry&, int, int) {},
-          [&](int row, const Entry& x, int kvh, int seg, int tile, int j0, int j1, int place, int Q) {
-            const int own = row_prefix(p, t, row), first = tile / Q;
-            RowPiece d;
-            d.row = row;
-            d.kvh = kvh;
-            d.key0 = own + j0 * TILE;
-            d.limit = min(row_keys(p, t, row, p.kv_len[row], false), own + j1 * TILE);
-            d.id = seg + range;
-            d.index = range - first;
-            d.pieces = (tile + x.tiles - 1) / Q - first + 1;
-            d.group_id = d.group_n = d.r0 = 0;
-            if (own > 0) {
-              const int m = t.member[row], gr = group_of(p, t, m), i = m - t.start[gr], pt = cdiv(own, 2 * TILE), s = i / rpt * p.KV + kvh;
-              const int a = t.tile[gr] + s * pt, f = a / QA;
-              d.group_id = t.seg[gr] + s + f;
-              d.group_n = (a + pt - 1) / QA - f + 1;
-              d.r0 = i % rpt * G;
-            }
-            list[place] = d;
-          });
-      n_pieces = l.pieces;
-      more = l.more;
-      fence_async_smem();       // the ring is TMA's from here on
-      __syncthreads();
-    }
+  int n_tile = 0;                 // tiles this block has had
+  bool waited = false;
+  const Plan plan(p);
+  // (the plan is complete: the kernel of the groups waited for it before it let this one start)
+  const int all_pieces = __ldcg(plan.head + 1);
+  for (int first = blockIdx.x; first < all_pieces; first += gridDim.x * LISTED) {
+    const int n_pieces = min(LISTED, cdiv(all_pieces - first, (int)gridDim.x));
+    for (int x = tid; x < n_pieces * (ROW_INTS / 4); x += THREADS)
+      reinterpret_cast<int4*>(list)[x] = __ldcg(reinterpret_cast<const int4*>(plan.row_pieces + first + x / (ROW_INTS / 4) * (int)gridDim.x) + x % (ROW_INTS / 4));
+    __syncthreads();
     if (warp == WARPS) {
       // ---------------------------------------------------------------- producer
       const int rows_of_box = min(ps, TILE), ppt = TILE / rows_of_box;      // a tile's pages, at most 8
@@ -155,7 +109,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           const int held_pages = min(ppt, cdiv(limit - kb, rows_of_box)), lp = kb / ps + lane;
           int page = -1;
           if (lane < held_pages) {
-            page = table[lp];            // below max_pages: limits are checked when the list is made
+            page = table[lp];            // below max_pages: the plan's limits are checked
             if (page < 0 || page >= p.num_pages) {
               dk_report(p.err, DK_DEV_BAD_PAGE, w.row, lp, page);
               page = -1;
@@ -326,9 +280,8 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           waited = true;
         }
         bool finish = true;
-        const int first_id = w.id - w.index;
         if (w.pieces > 1) {
-          float* part = row_piece(p, QR, w.id);
+          float* part = row_results(p, w.first_id + w.index);
 #pragma unroll
           for (int r = 0; r < NR; ++r)
             if (g + 8 * r < G) {
@@ -362,8 +315,8 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             };
             // four pieces asked for at once, added in order
             constexpr int AT_ONCE = 4;
-            const long long gs = group_piece_floats(QR, HD), rs = row_piece_floats(G, HD);
-            const float* gp = group_piece(p, QR, w.group_id);
+            const long long gs = group_piece_floats(p.qr, HD), rs = row_piece_floats(G, HD);
+            const float* gp = group_results(p, w.group_id);
             for (int x = 0; x < w.group_n; x += AT_ONCE) {
               float2 ml[AT_ONCE];
               float v[AT_ONCE][2 * NT];
@@ -371,10 +324,10 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
               for (int y = 0; y < AT_ONCE; ++y)
                 if (x + y < w.group_n) {
                   const float* part = gp + (x + y) * gs;
-                  ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)QR * HD + 2 * (w.r0 + qh)));
+                  ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)p.qr * HD + 2 * (w.r0 + qh)));
 #pragma unroll
                   for (int k = 0; k < NT; ++k) {
-                    const float2 f = __ldcg(reinterpret_cast<const float2*>(part + ((size_t)((warp * NT + k) * 2 + tq / 2) * QR + w.r0 + qh) * 4 + (tq & 1) * 2));
+                    const float2 f = __ldcg(reinterpret_cast<const float2*>(part + ((size_t)((warp * NT + k) * 2 + tq / 2) * p.qr + w.r0 + qh) * 4 + (tq & 1) * 2));
                     v[y][2 * k] = f.x;
                     v[y][2 * k + 1] = f.y;
                   }
@@ -392,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
               }
               add(m_run[r], l_run[r], v);
             } else {
-              const float* rp = row_piece(p, QR, first_id);
+              const float* rp = row_results(p, w.first_id);
               for (int x = 0; x < w.pieces; x += AT_ONCE) {
                 float2 ml[AT_ONCE];
                 float v[AT_ONCE][2 * NT];

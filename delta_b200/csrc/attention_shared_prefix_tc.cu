@@ -19,7 +19,7 @@
 //   warp 10     issues the score products
 //   warp 11     issues P V over the 16-key blocks that hold keys, and clears what the last of them holds behind the last key
 //               (a page's rest may hold anything, and 0 times infinity is no zero)
-//   warps 8-11  together make the list of pieces
+//   warps 8-11  fetch the list of the range's pieces
 //
 // Every wait is bounded; when one gives up the block records it, waits (bounded again) for the copies and products it has under
 // way, frees its tensor memory and returns.
@@ -45,12 +45,11 @@ struct Layout {
   static constexpr int Q_BYTES = HALVES * BOX_BYTES;
   static constexpr int TILE_BYTES = HALVES * BOX_BYTES;   // one K or V tile
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + Q_BYTES;           // two of each; the list is made here, before they are filled
+  static constexpr int OFF_K = OFF_Q + Q_BYTES;           // two of each
   static constexpr int OFF_V = OFF_K + 2 * TILE_BYTES;
   static constexpr int OFF_P = OFF_V + 2 * TILE_BYTES;    // P of each half: two boxes [128 x 64 keys]
   static constexpr int P_BYTES = 2 * BOX_BYTES;
   static constexpr int TOTAL = OFF_P + 2 * P_BYTES + 1024;   // 1024 to start on a swizzle boundary
-  static_assert(4 * Tables::ints(0, MAX_GROUPS) <= 4 * TILE_BYTES, "the list is made in the buffers of K and V");
 };
 
 // 2^x by the special-function unit (two units in the last place; results below 2^-126 become 0)
@@ -78,17 +77,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
   // barriers: q_full, k_full[2], v_full[2], s_full[2], p_full[2], o_done[2], s_free[2], merge, piece_done.  Those in pairs belong to the
   // tiles of one parity of their pieces; what a wait needs is how many of them the block has had.
   __shared__ __align__(8) unsigned long long bars[15];
-  __shared__ __align__(16) int4 list[CAP];
+  __shared__ GroupPiece list[CAP];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
-  __shared__ int n_listed, ranges_left;
+  __shared__ int n_listed;
   // row_stat(w)[query]: maximum and sum of half w's tiles, over the half's P, which is not read any more by then
   auto row_stat = [&](int w) { return reinterpret_cast<float2*>(smem + L::OFF_P + w * L::P_BYTES); };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room
-  for (int i = blockIdx.x * THREADS + tid; i < p.rows * p.KV; i += gridDim.x * THREADS) counters(p)[i] = 0;
-  const int ps = p.ps, G = p.H / p.KV, rpt = QT / G;
+  const int ps = p.ps, G = p.H / p.KV;
   const uint32_t bar0 = s2u(&bars[0]);
   const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = k_full + 16, s_full = v_full + 16, p_full = s_full + 16, o_done = p_full + 16,
                  s_free = o_done + 16, merge_bar = s_free + 16, piece_done = merge_bar + 8;
@@ -108,6 +105,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == MMA_WARP) tmem_alloc(s2u(&tmem_slot), TMEM_COLS);
+  if (warp == PRODUCER_WARP0 && lane < 2)
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(lane ? &map_run : &map_kv)) : "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");                   // the plan
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room
+  for (int i = blockIdx.x * THREADS + tid; i < p.rows * p.KV; i += gridDim.x * THREADS) counters(p)[i] = 0;
+  const Plan plan(p);
+  const int n_ranges = __ldcg(plan.head);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -122,41 +126,31 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     int asked0 = 0, asked1 = 0;   // producers: tiles of each parity asked for so far
     const int kind = warp - PRODUCER_WARP0;     // 0: K, 1: V
     const uint32_t full = kind ? v_full : k_full, done = kind ? o_done : s_full, sm_dst = kind ? sm_v : sm_k;
-    for (int range = blockIdx.x;; range += gridDim.x) {
+    for (int range = blockIdx.x; range < n_ranges; range += gridDim.x) {
       {
+        const int2 held = __ldcg(reinterpret_cast<const int2*>(plan.ranges) + range);
         const int t4 = tid - PRODUCER_WARP0 * 32;
-        auto sync = [] { asm volatile("bar.sync 1, 128;\n" ::: "memory"); };
-        const Tables t(reinterpret_cast<int*>(smem + L::OFF_K), 0, p.groups);
-        load_tables<false, 128>(p, t, t4, sync);
-        const Line l = walk_line<128>(
-            p.groups, p.grid, range, t.line, t4, sync, [&](int e) { return group_entry<KT>(p, t, e, rpt); }, [](int, const Entry&, int, int) {},
-            [&](int e, const Entry&, int i, int seg, int, int j0, int j1, int place, int) { list[place] = piece_of_group<KT>(p, t, e, rpt, i, seg + range, j0, j1); });
-        if (t4 == 0) {
-          n_listed = l.pieces;
-          ranges_left = l.more;
-        }
-        fence_async_smem();       // the buffers are TMA's from here on
+        for (int x = t4; x < min(held.y, CAP) * (GROUP_INTS / 4); x += 128)
+          reinterpret_cast<int4*>(list)[x] = __ldcg(reinterpret_cast<const int4*>(plan.group_pieces + held.x) + x);
+        if (t4 == 0) n_listed = min(held.y, CAP);
       }
       block_barrier();
-      const int n_pieces = n_listed;
-      const bool more = ranges_left != 0;       // (read before the second barrier: behind it the next list is made)
+      const int n_pieces = n_listed;       // (read before the second barrier: behind it the next list is made)
       if (warp < MMA_WARP) {
         // ----------------------------------------------------------- producers
         const int ppt = KT / ps;      // pages per tile, at most 16
         for (int i = 0; i < n_pieces && !failed; ++i) {
-          const Piece w(list[i]);
+          const GroupPiece w = list[i];
           const int n_tiles = cdiv(w.limit - w.key0, KT);
-          int row = p.members[w.first];
-          if (row < 0 || row >= p.rows) row = 0;        // recorded when the list was made
-          const int* table = p.block_table + (size_t)row * p.max_pages;
+          const int* table = p.block_table + (size_t)w.table_row * p.max_pages;
           for (int j = 0; j < n_tiles; ++j) {
             const int c = j & 1, ord = (c ? had1 : had0) + j / 2;     // the ord-th tile of its parity in this block
             const int kb = w.key0 + j * KT, pages = min(ppt, cdiv(w.limit - kb, ps)), lp = kb / ps + lane;
             int page = -1;
             if (lane < pages) {
-              page = table[lp];          // below max_pages: limits are checked when the list is made
+              page = table[lp];          // below max_pages: the plan's limits are checked
               if (page < 0 || page >= p.num_pages) {
-                dk_report(p.err, DK_DEV_BAD_PAGE, row, lp, page);
+                dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
                 page = -1;
               }
             }
@@ -192,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         const uint64_t da0 = smem_desc_k_major(sm_q);
         bool ok = true;
         for (int i = 0; ok && i < n_pieces; ++i) {
-          const Piece w(list[i]);
+          const GroupPiece w = list[i];
           const int n_tiles = cdiv(w.limit - w.key0, KT);
           ok = wait_all(q_full, n_done & 1);
           int j = 0;
@@ -224,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
         bool ok = true;
         for (int i = 0; ok && i < n_pieces; ++i) {
-          const Piece w(list[i]);
+          const GroupPiece w = list[i];
           const int n_tiles = cdiv(w.limit - w.key0, KT);
           int j = 0;
           for (; ok && j < n_tiles; ++j) {
@@ -258,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         if (!ok) failed = 1;
       }
       block_barrier();
-      if (failed || !more) break;
+      if (failed) break;
     }
     if (lane == 0) {      // what this warp has under way ends before the block leaves
       const uint32_t bar = warp < MMA_WARP ? full : (warp == MMA_WARP ? s_full : o_done);
@@ -277,9 +271,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     const float sl2 = p.scale * 1.4426950408889634f;
     constexpr int QC = HD / 16;                         // 16-byte chunks of a query that this half fetches
     const int qi = r / G, qh = r - qi * G;
-    auto ask_q = [&](const Piece& pc, uint4 (&v)[QC]) {
+    auto ask_q = [&](const GroupPiece& pc, uint4 (&v)[QC]) {
       int row = -1;
-      if (qi < pc.n_rows) row = p.members[pc.first + qi];
+      if (qi < pc.rows) row = p.members[pc.first + qi];
       const bool held = row >= 0 && row < p.rows;
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (held ? row : 0) * p.q_stride + (pc.kvh * G + qh) * HD + w * (HD / 2));
 #pragma unroll
@@ -296,19 +290,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     };
     bool good = true;
     int had_w = 0, had_other = 0;       // tiles of this half and of the other one so far
-    for (;;) {
+    for (int range = blockIdx.x; range < n_ranges; range += gridDim.x) {
       block_barrier();
-      const int n_pieces = n_listed;
-      const bool more = ranges_left != 0;       // (read before the second barrier: behind it the next list is made)
+      const int n_pieces = n_listed;       // (read before the second barrier: behind it the next list is made)
       if (n_pieces > 0) {
         uint4 v[QC];
-        ask_q(Piece(list[0]), v);
+        ask_q(list[0], v);
         store_q(v);
       }
 #pragma unroll 1
       for (int i = 0; good && i < n_pieces; ++i) {
-        const Piece pc(list[i]);
-        const int n_tiles = cdiv(pc.limit - pc.key0, KT), queries = pc.n_rows * G;
+        const GroupPiece pc = list[i];
+        const int n_tiles = cdiv(pc.limit - pc.key0, KT), queries = pc.rows * G;
         const bool busy = (warp & 3) * 32 < queries;      // some thread of this warp has a query
         float m_used = -INFINITY, l_sum = 0.f;
         int mine = 0;
@@ -405,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
           bool ok = true;
           if (i + 1 < n_pieces) {
             uint4 v[QC];
-            ask_q(Piece(list[i + 1]), v);
+            ask_q(list[i + 1], v);
             if (had_other > 0) ok = mbar_wait(s_full + 8 * (w ^ 1), (had_other - 1) & 1);
             store_q(v);
           }
@@ -429,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         const float l_all = l_sum * f_mine + other.y * f_other;
         const float f0 = w == 0 ? f_mine : f_other, f1 = w == 0 ? f_other : f_mine;
         const bool two = n_tiles > 1;                     // O_1 holds nothing when there was one tile
-        float* part = group_piece(p, QT, pc.id);
+        float* part = group_results(p, pc.id);
         if (!busy) {
           tc_fence_before();
           mbar_arrive(piece_done);
@@ -460,17 +453,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         ++n_done;
       }
       block_barrier();
-      if (failed || !more) break;
+      if (failed) break;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (failed && tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_listed);
+  if (failed && tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_ranges);
   if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 template <int HD>
-int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
+int launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream) {
   using L = Layout<HD>;
   CUtensorMap map_kv, map_run;
   const long long kv_rows = (long long)p.num_pages * 2 * p.KV * p.ps;
@@ -490,7 +483,21 @@ int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
     }
     configured = true;
   }
-  attention_shared_prefix_tc_kernel<HD><<<p.grid, THREADS, L::TOTAL, stream>>>(map_kv, map_run, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.groups > 0 ? p.grid : 1);      // (one block clears the counters)
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // it may start while the plan is made
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind_plan ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_shared_prefix_tc_kernel<HD>, map_kv, map_run, p);
+  if (e != cudaSuccess) {
+    dk_set_error("attention_shared_prefix: launch of the groups' kernel failed: %s", cudaGetErrorString(e));
+    return DK_ERR_LAUNCH;
+  }
   return dk_check_launch("attention_shared_prefix_tc");
 }
 }  // namespace
@@ -500,4 +507,7 @@ bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p) {
          (long long)p.num_pages * 2 * p.KV * p.ps < (1ll << 31);
 }
 
-int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream) { return p.hd == 64 ? launch<64>(p, stream) : launch<128>(p, stream); }
+// behind_plan: the kernel before it in the stream makes the plan
+int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream) {
+  return p.hd == 64 ? launch<64>(p, behind_plan, stream) : launch<128>(p, behind_plan, stream);
+}
