@@ -16,11 +16,9 @@
 // It is bound by the FMA units and the shared-memory reads that feed them (nine 16-byte reads for 32 FMAs).
 #include "shared_prefix.cuh"
 
-// shared_prefix_plan.cu
-int dk_shared_prefix_plan_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
 // attention_shared_prefix_tc.cu
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
-int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream);
+int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
 // attention_shared_prefix_rows.cu
 int dk_shared_prefix_rows_tile();
 int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p);
@@ -48,6 +46,9 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
+// Behind the pieces' results: the record of the first piece of every row and key-value head.
+__device__ __forceinline__ RowPiece* row_records(const DkSharedPrefixParams& p) { return reinterpret_cast<RowPiece*>(row_results(p, p.row_pieces)); }
+
 // HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
 __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
@@ -58,31 +59,50 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
   float* s_k = s_q + QR * hd;          // [KT][hd + 4]
   float* s_v = s_k + KT * ks;          // [KT][hd]
   float* s_p = s_v + KT * hd;          // [QR][KT + 4]
+  __shared__ GroupPiece list[CAP];
   __shared__ int s_page[KT];
   const int tid = threadIdx.x, r = tid / EIGHT, c = tid % EIGHT;
   const int G = p.H / p.KV;
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
-  const Plan plan(p);
-  const int n_ranges = plan.head[0], row_pieces = plan.head[1];
-  // first the pieces of the block's ranges of groups, then its pieces of rows
-  int range = blockIdx.x, i = 0, row_piece = gridDim.x - 1 - blockIdx.x;
-  for (;;) {
-    const bool of_group = range < n_ranges;
-    GroupPiece w;
-    if (of_group) {
-      w = plan.group_pieces[plan.ranges[2 * range] + i];
-      if (++i == plan.ranges[2 * range + 1]) {
-        i = 0;
-        range += gridDim.x;
-      }
-    } else if (row_piece < row_pieces) {
-      const RowPiece x = plan.row_pieces[row_piece];
-      w = {x.row, 1, x.kvh, row_piece, x.key0, x.limit, x.row, 0};
-      row_piece += gridDim.x;
-    } else {
-      break;
+  Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
+  auto tables = [&] { make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
+  tables();
+  // every row's first piece for the merge
+  if (blockIdx.x == 0)
+    for (int i = tid; i < p.rows * p.KV; i += THREADS) {
+      const int row = i / p.KV, n = ((row + 1 < p.rows ? cut.piece[row + 1] : cut.pieces) - cut.piece[row]) / p.KV;
+      row_records(p)[i] = row_piece(p, cut, cut.piece[row] + i % p.KV * n);
     }
+  const int n_ranges = cut.ranges, row_pieces = cut.pieces;
+  // first the pieces of the block's ranges of groups, then its pieces of rows
+  int range = blockIdx.x, next_row = gridDim.x - 1 - blockIdx.x, listed = 0, at = 0;
+  bool of_group = range < n_ranges, list_made = false;
+  for (;;) {
+    if (at == listed) {
+      // a list of pieces at a time; the tables are laid out where the tiles lie
+      if (list_made) tables();
+      list_made = true;
+      at = listed = 0;
+      of_group = range < n_ranges;
+      if (of_group) {
+        int first_seg;
+        listed = min(range_pieces(p, cut, range, first_seg), CAP);
+        if (tid < listed) list[tid] = group_piece(p, cut, range, first_seg + tid);
+        range += gridDim.x;
+      } else if (next_row < row_pieces) {
+        listed = min(CAP, cdiv(row_pieces - next_row, (int)gridDim.x));
+        if (tid < listed) {
+          const int id = next_row + tid * (int)gridDim.x;
+          const RowPiece x = row_piece(p, cut, id);
+          list[tid] = {x.row, 1, x.kvh, id, x.key0, x.limit, x.row, 0};
+        }
+        next_row += listed * gridDim.x;
+      }
+      __syncthreads();
+      if (listed == 0) break;
+    }
+    const GroupPiece w = list[at++];
     const int rows = w.rows * G;
     auto row_at = [&](int k) { return of_group ? p.members[w.first + k] : w.first; };
     for (int x = tid; x < QR * c4s; x += THREADS) {
@@ -107,7 +127,7 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
       if (tid < KT) {
         int page = -1;
         if (tid < n) {
-          const int lp = (kb + tid) / p.ps;        // below max_pages: the plan's limits are checked
+          const int lp = (kb + tid) / p.ps;        // below max_pages: limits were checked
           page = table[lp];
           if (page < 0 || page >= p.num_pages) {
             dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
@@ -188,7 +208,7 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
       for (int k = 0; k < OC; ++k)
         if (k * 32 + c * 4 < hd)
           *reinterpret_cast<float4*>(part + (of_group ? ((size_t)(k * 8 + c) * QR + r) * 4 : (size_t)r * hd + k * 32 + c * 4)) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
-      if (c == 0) *reinterpret_cast<float2*>(part + (size_t)(of_group ? QR : G) * hd + 2 * r) = make_float2(m_run, l_run);
+      if (c == 0) *reinterpret_cast<float2*>(part + (of_group ? (size_t)QR * hd + 4 * r : (size_t)G * hd + 2 * r)) = make_float2(m_run, l_run);
     }
     __syncthreads();          // the queries may be overwritten
   }
@@ -199,8 +219,7 @@ template <typename T>
 __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p) {
   const int kvh = blockIdx.x, row = blockIdx.y, G = p.H / p.KV;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const Plan plan(p);
-  const RowPiece w = plan.row_pieces[plan.rows[2 * row] + kvh * plan.rows[2 * row + 1]];
+  const RowPiece w = row_records(p)[row * p.KV + kvh];
   const long long gs = group_piece_floats(QR, p.hd), rs = row_piece_floats(G, p.hd);
   const float* gp = group_results(p, w.group_id);
   const float* rp = row_results(p, w.first_id);
@@ -226,7 +245,7 @@ __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams 
       for (int j = 0; j < AT_ONCE; ++j) {
         const int n = i + j;
         if (n < w.group_n) {
-          ml[j] = *reinterpret_cast<const float2*>(gp + n * gs + (size_t)QR * p.hd + 2 * (w.r0 + g));
+          ml[j] = *reinterpret_cast<const float2*>(gp + n * gs + (size_t)QR * p.hd + 4 * (w.r0 + g));
           o[j] = *reinterpret_cast<const float4*>(gp + n * gs + ((size_t)c4 * QR + w.r0 + g) * 4);
         } else if (n < w.group_n + w.pieces) {
           ml[j] = *reinterpret_cast<const float2*>(rp + (n - w.group_n) * rs + (size_t)G * p.hd + 2 * g);
@@ -250,7 +269,8 @@ __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams 
 
 template <typename T, int HDM>
 int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
-  const size_t smem = 4 * smem_floats(p.hd);
+  const size_t need = smem_floats(p.hd), tables = Cut::ints(p.rows, p.groups);
+  const size_t smem = 4 * (need > tables ? need : tables);
   static size_t granted_on[DK_MAX_DEVICES] = {0};
   size_t& granted = granted_on[dk_current_device()];
   if (smem > granted) {
@@ -311,7 +331,7 @@ int check_sizes(const DkSharedPrefixParams& p) {
 }
 
 // How the work is cut: by the tensor cores' kernels where they take the sizes, else for the FMA units.  Returns which.
-bool cut(DkSharedPrefixParams& p) {
+bool cut_for(DkSharedPrefixParams& p) {
   const bool tc = dk_shared_prefix_tc_takes(p);
   p.qr = tc ? 128 : QR;
   p.kt = tc ? 128 : KT;
@@ -322,56 +342,45 @@ bool cut(DkSharedPrefixParams& p) {
   return tc;
 }
 
-int sizes(DkSharedPrefixParams& p, bool* tc, Bounds* b) {
+int sizes(DkSharedPrefixParams& p, bool* tc, long long* floats) {
   if (int rc = check_sizes(p)) return rc;
-  *tc = cut(p);
-  *b = bounds(p);
-  DK_REQUIRE(b->tiles < (1ll << 30) && b->plan_ints < (1ll << 30), "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call",
+  *tc = cut_for(p);
+  const Bounds b = bounds(p);
+  DK_REQUIRE(b.tiles < (1ll << 30) && b.pieces < (1ll << 24), "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call",
              p.rows, p.KV, p.max_pages);
+  *floats = b.work_floats + (*tc ? 0 : (long long)p.rows * p.KV * sizeof(RowPiece) / 4);
   return 0;
 }
 }  // namespace
 
-// Ints that the plan and floats that the working memory of a call with these sizes need: need[0] and need[1].
-extern "C" int dk_attention_shared_prefix_sizes(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, int dtype, long long* need) {
+// Floats of working memory that a call with these sizes needs.
+extern "C" int dk_attention_shared_prefix_floats(int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, int dtype, long long* floats) {
   DkSharedPrefixParams p = {};
   p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = num_pages; p.dtype = dtype;
   bool tc;
-  Bounds b;
-  if (int rc = sizes(p, &tc, &b)) return rc;
-  need[0] = b.plan_ints;
-  need[1] = b.work_floats;
-  return 0;
+  return sizes(p, &tc, floats);
 }
 
-// make_plan: the plan is worked out first, else it holds what an earlier call with the same tables and sizes left.  q null: nothing else is done.
 extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, void* out, long long out_stride, const void* kv, const int* block_table, const int* kv_len,
-                                          const int* members, const int* group_start, const int* group_prefix, int* plan, long long plan_ints, int make_plan, void* work,
-                                          long long work_floats, int rows, int groups, int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale,
-                                          int dtype, int* err, cudaStream_t stream) {
+                                          const int* members, const int* group_start, const int* group_prefix, void* work, long long work_floats, int rows, int groups,
+                                          int n_members, int H, int KV, int hd, int ps, int max_pages, int num_pages, float scale, int dtype, int* err, cudaStream_t stream) {
   DkSharedPrefixParams p = {};
   p.q = q; p.out = out; p.kv = kv; p.block_table = block_table; p.kv_len = kv_len; p.members = members; p.group_start = group_start; p.group_prefix = group_prefix;
-  p.plan = plan; p.work = (float*)work; p.err = err; p.q_stride = q_stride; p.out_stride = out_stride;
+  p.work = (float*)work; p.err = err; p.q_stride = q_stride; p.out_stride = out_stride;
   p.rows = rows; p.groups = groups; p.n_members = n_members; p.H = H; p.KV = KV; p.hd = hd; p.ps = ps; p.max_pages = max_pages; p.num_pages = num_pages; p.dtype = dtype;
   p.scale = scale;
   bool tc;
-  Bounds b;
-  if (int rc = sizes(p, &tc, &b)) return rc;
-  if (rows == 0) return 0;
-  DK_REQUIRE(kv_len && plan && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a table is missing");
-  DK_REQUIRE(plan_ints >= b.plan_ints && ((uintptr_t)plan % 16) == 0, "attention_shared_prefix: a plan of %lld ints is given, %lld on a 16-byte boundary are needed", plan_ints, b.plan_ints);
-  if (q != nullptr) {
-    DK_REQUIRE(out && kv && block_table && work, "attention_shared_prefix: a tensor is missing");
-    DK_REQUIRE(work_floats >= b.work_floats, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, b.work_floats);
-    DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
-    DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
-               "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
-    DK_REQUIRE(!tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
-  }
-  int rc = make_plan ? dk_shared_prefix_plan_launch(p, stream) : 0;
-  if (rc != 0 || q == nullptr) return rc;
+  long long need;
+  int rc = sizes(p, &tc, &need);
+  if (rc != 0 || rows == 0) return rc;
+  DK_REQUIRE(q && out && kv && block_table && kv_len && work && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
+  DK_REQUIRE(work_floats >= need, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, need);
+  DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
+  DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,
+             "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
+  DK_REQUIRE(!tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
   if (tc) {
-    rc = dk_shared_prefix_tc_launch(p, make_plan != 0, stream);
+    rc = dk_shared_prefix_tc_launch(p, stream);
     return rc != 0 ? rc : dk_shared_prefix_rows_launch(p, stream);
   }
   rc = dtype == DK_F32 ? launch_sized<float>(p, stream) : launch_sized<__nv_bfloat16>(p, stream);

@@ -11,10 +11,11 @@
 //              memory, O += P V for a quarter of the columns each.  So all warps share one maximum, and nothing has to be merged
 //              between them at a segment's end.
 //
-// Behind a segment's last tile its row is finished: the pieces of its group's shared keys are added in their order, then the row's own, and
-// the result is rounded once.  Where a segment is cut, each block leaves its piece's results in the work buffer and counts itself; the one that comes
-// last adds them all, in their order, so the result does not depend on who that is.  The counters are cleared by the kernel of the groups.
-// This kernel starts while that one runs and waits for its end before it touches what it wrote.
+// Behind a piece's last tile the pieces of its row's group are added to it, in the order of their keys: they come through the ring as well, up to eight
+// a stage, one box each.  (Of a segment that is cut, only the first piece adds them.)  The result is rounded once.  Where a segment is cut, each block
+// leaves its piece's results in the work buffer and counts itself; the one that comes last adds them all, in their order, so the result does not depend on
+// who that is.  The counters are cleared by the kernel of the groups.  This kernel starts while that one runs and waits for its end before it touches
+// what it wrote.
 #include "shared_prefix.cuh"
 #include "tcgen05_helpers.cuh"
 #include "mma_helpers.cuh"
@@ -23,7 +24,9 @@
 namespace {
 using namespace shared_prefix;
 constexpr int TILE = 64;           // keys of a tile
+constexpr int QR = 128;            // queries of a group's piece
 constexpr int LISTED = 32;         // pieces whose records lie in shared memory at once
+constexpr int MERGED = 8;          // pieces of a group in a stage, at most
 constexpr int ROWS = 16;           // rows of the MMA tile
 constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
 
@@ -37,6 +40,7 @@ struct Ring {
   static constexpr int STAGES = HD == 128 && LOW ? 3 : 5;
   static constexpr int BLOCKS = HD == 128 && !LOW ? 1 : 2;            // on an SM
   static constexpr int TOTAL = STAGES * STAGE + 1024;                // 1024 to start on a swizzle boundary
+  static_assert(4 * Cut::ints(MAX_ROWS, MAX_GROUPS) <= STAGES * STAGE, "the tables are laid out in the ring");
 };
 
 // LOW: at most 8 query heads; rows 8..15 of the MMA tile are then empty and their accumulators two registers that stay zero.
@@ -56,11 +60,16 @@ __device__ __forceinline__ void mma_rows(float* c, float (&zero)[2], const uint3
 __device__ __forceinline__ uint32_t tile_offset(int key, int chunk) {
   return (uint32_t)((chunk >> 3) * (TILE * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
 __device__ __forceinline__ void warps_barrier() { asm volatile("bar.sync 1, %0;\n" ::"n"(WARPS * 32) : "memory"); }
 
 template <int HD, bool LOW>
 __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_kv,
                                                                                   const __grid_constant__ CUtensorMap map_run,
+                                                                                  const __grid_constant__ CUtensorMap map_merge,
                                                                                   const DkSharedPrefixParams p) {
   using R = Ring<HD, LOW>;
   constexpr int NR = LOW ? 1 : 2;             // rows of the tile a thread keeps (g, and g + 8)
@@ -88,13 +97,16 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   const float sl2 = p.scale * 1.4426950408889634f;
   int n_tile = 0;                 // tiles this block has had
   bool waited = false;
-  const Plan plan(p);
-  // (the plan is complete: the kernel of the groups waited for it before it let this one start)
-  const int all_pieces = __ldcg(plan.head + 1);
+  Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
+  make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); });
+  const int all_pieces = cut.pieces;
+  // the pieces of a group in a stage: G queries each in a slot of its own
+  const int slot_bytes = (G * 16 * (HD / 4 + 1) + 127) / 128 * 128, per_stage = min(MERGED, R::STAGE / slot_bytes);
   for (int first = blockIdx.x; first < all_pieces; first += gridDim.x * LISTED) {
     const int n_pieces = min(LISTED, cdiv(all_pieces - first, (int)gridDim.x));
-    for (int x = tid; x < n_pieces * (ROW_INTS / 4); x += THREADS)
-      reinterpret_cast<int4*>(list)[x] = __ldcg(reinterpret_cast<const int4*>(plan.row_pieces + first + x / (ROW_INTS / 4) * (int)gridDim.x) + x % (ROW_INTS / 4));
+    if (first != (int)blockIdx.x) make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); });      // (the ring was used meanwhile)
+    if (tid < n_pieces) list[tid] = row_piece(p, cut, first + tid * (int)gridDim.x);
+    fence_async_smem();         // the ring is TMA's from here on
     __syncthreads();
     if (warp == WARPS) {
       // ---------------------------------------------------------------- producer
@@ -109,7 +121,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           const int held_pages = min(ppt, cdiv(limit - kb, rows_of_box)), lp = kb / ps + lane;
           int page = -1;
           if (lane < held_pages) {
-            page = table[lp];            // below max_pages: the plan's limits are checked
+            page = table[lp];            // below max_pages: limits were checked
             if (page < 0 || page >= p.num_pages) {
               dk_report(p.err, DK_DEV_BAD_PAGE, w.row, lp, page);
               page = -1;
@@ -146,6 +158,21 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           ++n;
           kb += TILE;
         } while (kb < limit);
+        if (failed || w.index != 0 || w.group_n == 0) continue;
+        if (!waited) {          // the pieces of the groups
+          asm volatile("griddepcontrol.wait;\n" ::: "memory");
+          asm volatile("fence.proxy.async;\n" ::: "memory");       // written with ordinary stores, read by TMA
+          waited = true;
+        }
+        for (int x = 0; x < w.group_n; x += per_stage, ++n) {
+          const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
+          bool ok = true;
+          if (n >= R::STAGES) ok = mbar_wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
+          if (!__all_sync(0xffffffffu, ok && !stuck)) { failed = 1; break; }
+          if (lane == 0) mbar_expect_tx(full + 8 * s, (uint32_t)(m * G * 16 * (HD / 4 + 1)));
+          __syncwarp();
+          if (lane < m) tma_load_3d(ring + s * R::STAGE + lane * slot_bytes, &map_merge, w.r0 * 4, 0, w.group_id + x + lane, full + 8 * s);
+        }
       }
       if (lane == 0) ring_drain(n, R::STAGES, [&](int slot, uint32_t parity) { return mbar_wait(full + 8 * slot, parity); });   // its copies have arrived
       __syncwarp();
@@ -275,12 +302,44 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         warps_barrier();
 #pragma unroll
         for (int r = 0; r < NR; ++r) l_run[r] = (s_sum[0][g + 8 * r] + s_sum[1][g + 8 * r]) + (s_sum[2][g + 8 * r] + s_sum[3][g + 8 * r]);
-        if (!waited) {          // the pieces of the groups and the counters
-          asm volatile("griddepcontrol.wait;\n" ::: "memory");
-          waited = true;
-        }
+        // {maximum, sum, outputs} of a piece added to this thread's queries
+        auto add = [&](int r, float m, float l, const float (&v)[2 * NT]) {
+          const float m_new = fmaxf(m_run[r], m), m_use = m_new == -INFINITY ? 0.f : m_new;
+          const float have = exp2f(m_run[r] - m_use), f = exp2f(m - m_use);
+          m_run[r] = m_new;
+          l_run[r] = l_run[r] * have + l * f;
+#pragma unroll
+          for (int k = 0; k < 2 * NT; ++k) o[k / 2][2 * r + k % 2] = o[k / 2][2 * r + k % 2] * have + v[k] * f;
+        };
+        if (w.index == 0)
+          for (int x = 0; x < w.group_n; x += per_stage, ++n) {
+            const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
+            if (!mbar_wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
+            for (int y = 0; y < m; ++y) {
+              const unsigned char* part = smem + s * R::STAGE + y * slot_bytes;
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+                if (g + 8 * r < G) {
+                  const float2 ml = *reinterpret_cast<const float2*>(part + (HD / 4 * G + g + 8 * r) * 16);
+                  float v[2 * NT];
+#pragma unroll
+                  for (int k = 0; k < NT; ++k) {
+                    const float2 f = *reinterpret_cast<const float2*>(part + (((warp * NT + k) * 2 + tq / 2) * G + g + 8 * r) * 16 + (tq & 1) * 8);
+                    v[2 * k] = f.x;
+                    v[2 * k + 1] = f.y;
+                  }
+                  add(r, ml.x, ml.y, v);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * s);
+          }
         bool finish = true;
         if (w.pieces > 1) {
+          if (!waited) {          // the counters were cleared by the kernel of the groups
+            asm volatile("griddepcontrol.wait;\n" ::: "memory");
+            waited = true;
+          }
           float* part = row_results(p, w.first_id + w.index);
 #pragma unroll
           for (int r = 0; r < NR; ++r)
@@ -295,83 +354,50 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           if (tid == 0) s_last = atomicAdd(&counters(p)[w.row * p.KV + w.kvh], 1) == w.pieces - 1;
           warps_barrier();
           finish = s_last != 0;
-          if (finish) __threadfence();
-        }
-        if (finish) {
+          if (finish) {
+            __threadfence();
+            constexpr int AT_ONCE = 4;        // pieces asked for together, added in order
+            const long long rs = row_piece_floats(G, HD);
+            const float* rp = row_results(p, w.first_id);
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const int qh = g + 8 * r;
-            if (qh >= G) continue;
-            float M = -INFINITY, L = 0.f, acc[2 * NT];
+            for (int r = 0; r < NR; ++r) {
+              m_run[r] = -INFINITY;
+              l_run[r] = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2 * NT; ++k) acc[k] = 0.f;
-            auto add = [&](float m, float l, const float (&v)[2 * NT]) {
-              const float m_new = fmaxf(M, m), m_use = m_new == -INFINITY ? 0.f : m_new;
-              const float have = exp2f(M - m_use), f = exp2f(m - m_use);
-              M = m_new;
-              L = L * have + l * f;
-#pragma unroll
-              for (int k = 0; k < 2 * NT; ++k) acc[k] = acc[k] * have + v[k] * f;
-            };
-            // four pieces asked for at once, added in order
-            constexpr int AT_ONCE = 4;
-            const long long gs = group_piece_floats(p.qr, HD), rs = row_piece_floats(G, HD);
-            const float* gp = group_results(p, w.group_id);
-            for (int x = 0; x < w.group_n; x += AT_ONCE) {
-              float2 ml[AT_ONCE];
-              float v[AT_ONCE][2 * NT];
-#pragma unroll
-              for (int y = 0; y < AT_ONCE; ++y)
-                if (x + y < w.group_n) {
-                  const float* part = gp + (x + y) * gs;
-                  ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)p.qr * HD + 2 * (w.r0 + qh)));
-#pragma unroll
-                  for (int k = 0; k < NT; ++k) {
-                    const float2 f = __ldcg(reinterpret_cast<const float2*>(part + ((size_t)((warp * NT + k) * 2 + tq / 2) * p.qr + w.r0 + qh) * 4 + (tq & 1) * 2));
-                    v[y][2 * k] = f.x;
-                    v[y][2 * k + 1] = f.y;
-                  }
-                }
-#pragma unroll
-              for (int y = 0; y < AT_ONCE; ++y)
-                if (x + y < w.group_n) add(ml[y].x, ml[y].y, v[y]);
-            }
-            if (w.pieces == 1) {
-              float v[2 * NT];
-#pragma unroll
-              for (int k = 0; k < NT; ++k) {
-                v[2 * k] = o[k][2 * r];
-                v[2 * k + 1] = o[k][2 * r + 1];
-              }
-              add(m_run[r], l_run[r], v);
-            } else {
-              const float* rp = row_results(p, w.first_id);
+              for (int k = 0; k < NT; ++k) o[k][2 * r] = o[k][2 * r + 1] = 0.f;
+              if (g + 8 * r >= G) continue;
               for (int x = 0; x < w.pieces; x += AT_ONCE) {
                 float2 ml[AT_ONCE];
                 float v[AT_ONCE][2 * NT];
 #pragma unroll
                 for (int y = 0; y < AT_ONCE; ++y)
                   if (x + y < w.pieces) {
-                    const float* part = rp + (x + y) * rs;
-                    ml[y] = __ldcg(reinterpret_cast<const float2*>(part + (size_t)G * HD + 2 * qh));
+                    const float* from = rp + (x + y) * rs;
+                    ml[y] = __ldcg(reinterpret_cast<const float2*>(from + (size_t)G * HD + 2 * (g + 8 * r)));
 #pragma unroll
                     for (int k = 0; k < NT; ++k) {
-                      const float2 f = __ldcg(reinterpret_cast<const float2*>(part + (size_t)qh * HD + (warp * NT + k) * 8 + 2 * tq));
+                      const float2 f = __ldcg(reinterpret_cast<const float2*>(from + (size_t)(g + 8 * r) * HD + (warp * NT + k) * 8 + 2 * tq));
                       v[y][2 * k] = f.x;
                       v[y][2 * k + 1] = f.y;
                     }
                   }
 #pragma unroll
                 for (int y = 0; y < AT_ONCE; ++y)
-                  if (x + y < w.pieces) add(ml[y].x, ml[y].y, v[y]);
+                  if (x + y < w.pieces) add(r, ml[y].x, ml[y].y, v[y]);
               }
             }
-            const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + qh) * HD;
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-              *reinterpret_cast<__nv_bfloat162*>(out + (warp * NT + k) * 8 + 2 * tq) = __floats2bfloat162_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
           }
+        }
+        if (finish) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+            if (g + 8 * r < G) {
+              const float inv = l_run[r] > 0.f ? 1.f / l_run[r] : (l_run[r] == 0.f ? 0.f : l_run[r]);      // no key: zeros; a NaN stays one
+              __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + g + 8 * r) * HD;
+#pragma unroll
+              for (int k = 0; k < NT; ++k)
+                *reinterpret_cast<__nv_bfloat162*>(out + (warp * NT + k) * 8 + 2 * tq) = __floats2bfloat162_rn(o[k][2 * r] * inv, o[k][2 * r + 1] * inv);
+            }
         }
       }
       n_tile = n;
@@ -384,16 +410,28 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   }
 }
 
+bool make_map_of_pieces(CUtensorMap* m, const float* base, int pieces, int G, int hd) {
+  TensorMapEncodeFn fn = tensor_map_encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {4 * QR, (cuuint64_t)(hd / 4 + 1), (cuuint64_t)pieces};
+  const cuuint64_t strides[2] = {16 * QR, (cuuint64_t)(4 * group_piece_floats(QR, hd))};
+  const cuuint32_t box[3] = {(cuuint32_t)(4 * G), (cuuint32_t)(hd / 4 + 1), 1}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD, bool LOW>
 int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
   using R = Ring<HD, LOW>;
-  CUtensorMap map_kv, map_run;
+  CUtensorMap map_kv, map_run, map_merge;
   const int rows = p.ps < TILE ? p.ps : TILE;
   DK_REQUIRE(make_tensor_map_bf16(&map_kv, p.kv, (long long)p.num_pages * 2 * p.KV * p.ps, HD, HD, rows), "attention_shared_prefix: cannot encode the tensor map of the cache");
   // the cache as [page][K|V, head][offset][hd]: a run of pages of one head in one box
   const unsigned long long dims[4] = {(unsigned long long)HD, (unsigned long long)p.ps, (unsigned long long)(2 * p.KV), (unsigned long long)p.num_pages};
   const unsigned long long strides[3] = {(unsigned long long)HD * 2, (unsigned long long)p.ps * HD * 2, (unsigned long long)2 * p.KV * p.ps * HD * 2};
   DK_REQUIRE(make_tensor_map_bf16_4d(&map_run, p.kv, dims, strides, rows, TILE / rows), "attention_shared_prefix: cannot encode the tensor map of runs of pages");
+  // the results of groups' pieces as [piece][hd / 4 + 1][queries x 4]: G queries of a piece in one box
+  DK_REQUIRE(make_map_of_pieces(&map_merge, group_results(p, 0), p.group_pieces > 0 ? p.group_pieces : 1, p.H / p.KV, HD), "attention_shared_prefix: cannot encode the tensor map of the pieces");
   static bool configured_on[DK_MAX_DEVICES] = {false};
   bool& configured = configured_on[dk_current_device()];
   if (!configured) {
@@ -414,7 +452,7 @@ int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_shared_prefix_rows_kernel<HD, LOW>, map_kv, map_run, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_shared_prefix_rows_kernel<HD, LOW>, map_kv, map_run, map_merge, p);
   if (e != cudaSuccess) {
     dk_set_error("attention_shared_prefix: launch of the rows' kernel failed: %s", cudaGetErrorString(e));
     return DK_ERR_LAUNCH;

@@ -19,7 +19,7 @@
 //   warp 10     issues the score products
 //   warp 11     issues P V over the 16-key blocks that hold keys, and clears what the last of them holds behind the last key
 //               (a page's rest may hold anything, and 0 times infinity is no zero)
-//   warps 8-11  fetch the list of the range's pieces
+//   warps 8-11  together make the list of the range's pieces
 //
 // Every wait is bounded; when one gives up the block records it, waits (bounded again) for the copies and products it has under
 // way, frees its tensor memory and returns.
@@ -45,11 +45,12 @@ struct Layout {
   static constexpr int Q_BYTES = HALVES * BOX_BYTES;
   static constexpr int TILE_BYTES = HALVES * BOX_BYTES;   // one K or V tile
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + Q_BYTES;           // two of each
+  static constexpr int OFF_K = OFF_Q + Q_BYTES;           // two of each; the list is made here, before they are filled
   static constexpr int OFF_V = OFF_K + 2 * TILE_BYTES;
   static constexpr int OFF_P = OFF_V + 2 * TILE_BYTES;    // P of each half: two boxes [128 x 64 keys]
   static constexpr int P_BYTES = 2 * BOX_BYTES;
   static constexpr int TOTAL = OFF_P + 2 * P_BYTES + 1024;   // 1024 to start on a swizzle boundary
+  static_assert(4 * Cut::ints(0, MAX_GROUPS) <= 4 * TILE_BYTES, "the list is made in the buffers of K and V");
 };
 
 // 2^x by the special-function unit (two units in the last place; results below 2^-126 become 0)
@@ -80,11 +81,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
   __shared__ GroupPiece list[CAP];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
-  __shared__ int n_listed;
+  __shared__ int n_listed, ranges_left;
   // row_stat(w)[query]: maximum and sum of half w's tiles, over the half's P, which is not read any more by then
   auto row_stat = [&](int w) { return reinterpret_cast<float2*>(smem + L::OFF_P + w * L::P_BYTES); };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room
+  for (int i = blockIdx.x * THREADS + tid; i < p.rows * p.KV; i += gridDim.x * THREADS) counters(p)[i] = 0;
   const int ps = p.ps, G = p.H / p.KV;
   const uint32_t bar0 = s2u(&bars[0]);
   const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = k_full + 16, s_full = v_full + 16, p_full = s_full + 16, o_done = p_full + 16,
@@ -107,11 +110,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
   if (warp == MMA_WARP) tmem_alloc(s2u(&tmem_slot), TMEM_COLS);
   if (warp == PRODUCER_WARP0 && lane < 2)
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(lane ? &map_run : &map_kv)) : "memory");
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");                   // the plan
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room
-  for (int i = blockIdx.x * THREADS + tid; i < p.rows * p.KV; i += gridDim.x * THREADS) counters(p)[i] = 0;
-  const Plan plan(p);
-  const int n_ranges = __ldcg(plan.head);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -126,16 +124,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     int asked0 = 0, asked1 = 0;   // producers: tiles of each parity asked for so far
     const int kind = warp - PRODUCER_WARP0;     // 0: K, 1: V
     const uint32_t full = kind ? v_full : k_full, done = kind ? o_done : s_full, sm_dst = kind ? sm_v : sm_k;
-    for (int range = blockIdx.x; range < n_ranges; range += gridDim.x) {
+    for (int range = blockIdx.x;; range += gridDim.x) {
       {
-        const int2 held = __ldcg(reinterpret_cast<const int2*>(plan.ranges) + range);
         const int t4 = tid - PRODUCER_WARP0 * 32;
-        for (int x = t4; x < min(held.y, CAP) * (GROUP_INTS / 4); x += 128)
-          reinterpret_cast<int4*>(list)[x] = __ldcg(reinterpret_cast<const int4*>(plan.group_pieces + held.x) + x);
-        if (t4 == 0) n_listed = min(held.y, CAP);
+        auto sync = [] { asm volatile("bar.sync 1, 128;\n" ::: "memory"); };
+        Cut cut(reinterpret_cast<int*>(smem + L::OFF_K), 0, p.groups);
+        make_cut<false, 128>(p, cut, t4, sync);
+        int n = 0, first_seg = 0;
+        if (range < cut.ranges) n = min(range_pieces(p, cut, range, first_seg), CAP);
+        if (t4 < n) list[t4] = group_piece(p, cut, range, first_seg + t4);
+        if (t4 == 0) {
+          n_listed = n;
+          ranges_left = range + (int)gridDim.x < cut.ranges;
+        }
+        fence_async_smem();       // the buffers are TMA's from here on
       }
       block_barrier();
       const int n_pieces = n_listed;       // (read before the second barrier: behind it the next list is made)
+      const bool more = ranges_left != 0;
       if (warp < MMA_WARP) {
         // ----------------------------------------------------------- producers
         const int ppt = KT / ps;      // pages per tile, at most 16
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
             const int kb = w.key0 + j * KT, pages = min(ppt, cdiv(w.limit - kb, ps)), lp = kb / ps + lane;
             int page = -1;
             if (lane < pages) {
-              page = table[lp];          // below max_pages: the plan's limits are checked
+              page = table[lp];          // below max_pages: limits were checked
               if (page < 0 || page >= p.num_pages) {
                 dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
                 page = -1;
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
         if (!ok) failed = 1;
       }
       block_barrier();
-      if (failed) break;
+      if (failed || !more) break;
     }
     if (lane == 0) {      // what this warp has under way ends before the block leaves
       const uint32_t bar = warp < MMA_WARP ? full : (warp == MMA_WARP ? s_full : o_done);
@@ -290,9 +296,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
     };
     bool good = true;
     int had_w = 0, had_other = 0;       // tiles of this half and of the other one so far
-    for (int range = blockIdx.x; range < n_ranges; range += gridDim.x) {
+    for (;;) {
       block_barrier();
       const int n_pieces = n_listed;       // (read before the second barrier: behind it the next list is made)
+      const bool more = ranges_left != 0;
       if (n_pieces > 0) {
         uint4 v[QC];
         ask_q(list[0], v);
@@ -448,22 +455,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
                 *reinterpret_cast<float4*>(part + ((size_t)(col / 4 + k) * QT + r) * 4) = make_float4(o0[4 * k], o0[4 * k + 1], o0[4 * k + 2], o0[4 * k + 3]);
             }
           }
-          if (r < queries && w == 0) *reinterpret_cast<float2*>(part + (size_t)QT * HD + 2 * r) = make_float2(m_all, l_all);
+          if (r < queries && w == 0) *reinterpret_cast<float4*>(part + (size_t)QT * HD + 4 * r) = make_float4(m_all, l_all, 0.f, 0.f);
         }
         ++n_done;
       }
       block_barrier();
-      if (failed) break;
+      if (failed || !more) break;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (failed && tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_ranges);
+  if (failed && tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_listed);
   if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 template <int HD>
-int launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream) {
+int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
   using L = Layout<HD>;
   CUtensorMap map_kv, map_run;
   const long long kv_rows = (long long)p.num_pages * 2 * p.KV * p.ps;
@@ -483,21 +490,7 @@ int launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream)
     }
     configured = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.groups > 0 ? p.grid : 1);      // (one block clears the counters)
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = L::TOTAL;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // it may start while the plan is made
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = behind_plan ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_shared_prefix_tc_kernel<HD>, map_kv, map_run, p);
-  if (e != cudaSuccess) {
-    dk_set_error("attention_shared_prefix: launch of the groups' kernel failed: %s", cudaGetErrorString(e));
-    return DK_ERR_LAUNCH;
-  }
+  attention_shared_prefix_tc_kernel<HD><<<p.groups > 0 ? p.grid : 1, THREADS, L::TOTAL, stream>>>(map_kv, map_run, p);      // (one block clears the counters)
   return dk_check_launch("attention_shared_prefix_tc");
 }
 }  // namespace
@@ -507,7 +500,4 @@ bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p) {
          (long long)p.num_pages * 2 * p.KV * p.ps < (1ll << 31);
 }
 
-// behind_plan: the kernel before it in the stream makes the plan
-int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, bool behind_plan, cudaStream_t stream) {
-  return p.hd == 64 ? launch<64>(p, behind_plan, stream) : launch<128>(p, behind_plan, stream);
-}
+int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream) { return p.hd == 64 ? launch<64>(p, stream) : launch<128>(p, stream); }

@@ -1,4 +1,4 @@
-// How the attention over shared prefixes cuts its work: the arguments, the plan and where the partial results lie.
+// How the attention over shared prefixes cuts its work: the arguments, the pieces and where the partial results lie.
 //
 // Work comes in segments.  A segment of a group is a tile of its queries (``rpt`` rows with their G query heads of one
 // key-value head) over the group's shared keys; a segment of a row is its G query heads over the keys it holds alone.  A segment
@@ -7,12 +7,13 @@
 //   groups  the tiles of all segments stand in one line, which is cut into ranges of Q tiles, as many as blocks run at once: every block
 //           has the same number of tiles whatever the groups are, and at most one segment is cut at each border.  A piece is what a
 //           range holds of a segment, and its number is segment + range: every step from one piece to the next moves to the next
-//           segment or the next range, so no two pieces have one number and those of a range follow one another.
+//           segment or the next range, so no two pieces have one number and those of a segment follow one another.
 //   rows    every segment is cut into equal pieces of at most C tiles, numbered through, and a block takes every ``grid``-th.  C is what
-//           levels the blocks, but eight tiles at least: a cut costs a row about as much as three tiles, since its pieces go through memory.
+//           levels the blocks, but MIN_ROW_TILES at least: the pieces of a cut segment go through memory, which takes as long as several tiles.
 //
-// One small kernel works the plan out from the tables on the device, so that a captured call follows them, and the kernels that
-// compute read it.  A plan holds for every layer that has the same tables.
+// Every block works this out for itself from the tables on the device (a captured call follows them): a kernel of its own for it was
+// measured to cost 3 us more before the first tile.  Whatever comes from the tables is checked here, so the kernels stay inside their
+// tensors (page ids they check themselves).
 #pragma once
 #include "common.cuh"
 
@@ -27,21 +28,20 @@ struct DkSharedPrefixParams {
   const int* members;        // [n_members] rows, group by group
   const int* group_start;    // [groups + 1] first member of each group
   const int* group_prefix;   // [groups] shared keys (rounded down to whole pages)
-  int* plan;
   float* work;               // counters, then the pieces' partial results
   int* err;                  // device error record, 4 ints; or null
   long long q_stride, out_stride;   // elements
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
   float scale;
-  // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), the blocks that compute, the most pieces and
-  // ranges there can be, and the keys that a group must save for its prefix to be read apart
-  int qr, kt, rows_kt, grid, rows_grid, group_ranges, group_pieces, row_pieces, min_saved;
+  // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), the blocks that compute, the most pieces
+  // there can be, and the keys that a group must save for its prefix to be read apart
+  int qr, kt, rows_kt, grid, rows_grid, group_pieces, row_pieces, min_saved;
 };
 
 namespace shared_prefix {
 constexpr int MAX_ROWS = 1024, MAX_GROUPS = 1023, MAX_G = 32;
 constexpr int CAP = 48;            // tiles of a range, so also the most pieces of one
-constexpr int MIN_ROW_TILES = 8;
+constexpr int MIN_ROW_TILES = 16;
 
 __host__ __device__ constexpr int cdiv(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ constexpr int round4(int a) { return (a + 3) / 4 * 4; }
@@ -56,47 +56,239 @@ struct __align__(16) GroupPiece {
 struct __align__(16) RowPiece {
   int row, kvh, key0, limit, index, pieces, first_id, group_id, group_n, r0, unused[2];
 };
-// The plan in ints: {ranges of groups, pieces of rows, 0, 0}, per range {first piece, pieces}, per row {first piece, pieces of a segment}, the pieces.
-constexpr int HEAD = 4, GROUP_INTS = sizeof(GroupPiece) / 4, ROW_INTS = sizeof(RowPiece) / 4;
-struct Plan {
-  int *head, *ranges, *rows;
-  GroupPiece* group_pieces;
-  RowPiece* row_pieces;
-  __host__ __device__ __forceinline__ Plan(const DkSharedPrefixParams& p)
-      : head(p.plan), ranges(head + HEAD), rows(ranges + round4(2 * p.group_ranges)), group_pieces(reinterpret_cast<GroupPiece*>(rows + round4(2 * p.rows))),
-        row_pieces(reinterpret_cast<RowPiece*>(group_pieces + p.group_pieces)) {}
-};
-
-// Floats of one piece's results: of a group as [hd / 4][queries][4] (neighbouring rows lie side by side), then {maximum, sum} per query; of a row as
-// [query][hd], then the same.
-__host__ __device__ __forceinline__ long long group_piece_floats(int qr, int hd) { return (long long)qr * (hd + 2); }
+// Floats of one piece's results: of a group as [hd / 4 + 1][queries][4] (neighbouring queries lie side by side; the last row of four holds maximum and
+// sum, then nothing); of a row as [query][hd], then {maximum, sum} per query.
+__host__ __device__ __forceinline__ long long group_piece_floats(int qr, int hd) { return (long long)qr * (hd + 4); }
 __host__ __device__ __forceinline__ long long row_piece_floats(int G, int hd) { return ((long long)G * (hd + 2) + 3) / 4 * 4; }
 
-// Fills in the most ranges and pieces that there can be with these sizes, whatever the device's tables say, and tells what they need.
+// Fills in the most pieces that there can be with these sizes, whatever the device's tables say, and tells what they need.
 struct Bounds {
-  long long tiles, group_ranges, group_pieces, row_pieces, plan_ints, work_floats;
+  long long tiles, pieces, work_floats;
 };
 static inline Bounds bounds(DkSharedPrefixParams& p) {
   Bounds b;
   const int G = p.H / p.KV, rpt = p.qr / G;
   const long long keys = (long long)p.max_pages * p.ps, segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
-  const long long of_groups = segments * ((keys + p.kt - 1) / p.kt);
+  const long long of_groups = segments * ((keys + p.kt - 1) / p.kt), capped = (of_groups + CAP - 1) / CAP;
+  const long long group_pieces = segments > 0 ? segments + (capped > p.grid ? capped : (long long)p.grid) : 0;
+  const long long row_pieces = (long long)p.rows * p.KV + p.rows_grid;      // a segment's last piece, and tiles / C of full ones, which are no more than blocks
   b.tiles = of_groups + (long long)p.rows * p.KV * ((keys + p.rows_kt - 1) / p.rows_kt);
-  b.group_ranges = segments > 0 ? ((of_groups + CAP - 1) / CAP > p.grid ? (of_groups + CAP - 1) / CAP : (long long)p.grid) : 0;
-  b.group_pieces = segments > 0 ? segments + b.group_ranges : 0;
-  b.row_pieces = (long long)p.rows * p.KV + p.rows_grid;      // a segment's last piece, and tiles / C of full ones, which are no more than blocks
-  b.plan_ints = HEAD + 2 * b.group_ranges + 4 + 2ll * p.rows + 4 + b.group_pieces * GROUP_INTS + b.row_pieces * ROW_INTS;
-  b.work_floats = round4(p.rows * p.KV) + b.group_pieces * group_piece_floats(p.qr, p.hd) + b.row_pieces * row_piece_floats(G, p.hd);
-  p.group_ranges = (int)b.group_ranges;
-  p.group_pieces = (int)b.group_pieces;
-  p.row_pieces = (int)b.row_pieces;
+  b.pieces = group_pieces + row_pieces;
+  b.work_floats = round4(p.rows * p.KV) + group_pieces * group_piece_floats(p.qr, p.hd) + row_pieces * row_piece_floats(G, p.hd);
+  p.group_pieces = (int)group_pieces;
+  p.row_pieces = (int)row_pieces;
   return b;
 }
+// The work buffer: a counter per row and key-value head, the results of groups' pieces, of rows' pieces. 
 __device__ __forceinline__ int* counters(const DkSharedPrefixParams& p) { return reinterpret_cast<int*>(p.work); }
-__device__ __forceinline__ float* group_results(const DkSharedPrefixParams& p, int id) {
+__host__ __device__ __forceinline__ float* group_results(const DkSharedPrefixParams& p, int id) {
   return p.work + round4(p.rows * p.KV) + id * group_piece_floats(p.qr, p.hd);
 }
 __device__ __forceinline__ float* row_results(const DkSharedPrefixParams& p, int id) {
   return group_results(p, p.group_pieces) + id * row_piece_floats(p.H / p.KV, p.hd);
+}
+
+// The last place whose value is not above v; a[0] <= v.
+__device__ __forceinline__ int last_not_above(const int* a, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The tables of a call in shared memory, checked, and how they are cut.
+struct Cut {
+  int *start, *prefix, *declared, *tile, *seg;      // groups: first member [groups + 1], keys read apart, keys said to be shared, first tile and segment in their line
+  int *member, *len, *own, *piece;                  // rows: place in members (-1: of no group), keys, keys read with the group, first piece
+  int* sums;
+  int Q, tiles, ranges, C, pieces;                  // tiles of a range, tiles of the line, ranges; tiles of a row's piece, rows' pieces
+  static __host__ __device__ constexpr int ints(int rows, int groups) { return 5 * groups + 1 + 4 * rows + 3 * 32; }
+  __device__ __forceinline__ Cut(int* s, int rows, int groups)
+      : start(s), prefix(start + groups + 1), declared(prefix + groups), tile(declared + groups), seg(tile + groups), member(seg + groups), len(member + rows),
+        own(len + rows), piece(own + rows), sums(piece + rows) {}
+};
+
+// Sums of N values over the threads before this one, and over all; one sync.
+template <int N, int NT, typename Sync>
+__device__ __forceinline__ void scan(const int (&v)[N], int (&before)[N], int (&total)[N], int* s, int tid, Sync sync) {
+  const int lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+  for (int i = 0; i < N; ++i) before[i] = v[i];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int a = __shfl_up_sync(0xffffffffu, before[i], o);
+      if (lane >= o) before[i] += a;
+    }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (lane == 31) s[i * 32 + warp] = before[i];
+    total[i] = 0;
+    before[i] -= v[i];
+  }
+  sync();
+  for (int w = 0; w < NT / 32; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = s[i * 32 + w];
+      total[i] += x;
+      if (w < warp) before[i] += x;
+    }
+}
+
+// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well.  Ends with a sync.
+template <bool ROWS, int NT, typename Sync>
+__device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid, Sync sync) {
+  const int rpt = p.qr / (p.H / p.KV), max_keys = p.max_pages * p.ps;
+  // what the steps below read is asked for at once
+  const int m_first = ROWS && tid < p.n_members && p.groups > 0 ? p.members[tid] : -1;
+  if (ROWS)
+    for (int r = tid; r < p.rows; r += NT) {
+      c.len[r] = p.kv_len[r];
+      c.member[r] = -1;
+    }
+  for (int g = tid; g <= p.groups; g += NT) {
+    int a = 0, b = 0, k = 0;
+    if (p.groups > 0) a = p.group_start[g];
+    if (g < p.groups) {
+      b = p.group_start[g + 1];
+      k = p.group_prefix[g];
+    }
+    if (a < 0 || a > p.n_members || (g < p.groups && (b < a || b > p.n_members || k < 0 || k > max_keys))) {
+      const bool at_start = a < 0 || a > p.n_members, at_end = b < a || b > p.n_members;
+      dk_report(p.err, DK_DEV_BAD_GROUP, g, at_start ? a : at_end ? b : k, at_start || at_end ? p.n_members : max_keys);
+      a = min(max(a, 0), p.n_members);
+      b = a;
+      k = 0;
+    }
+    c.start[g] = a;
+    if (g < p.groups) {
+      k = k / p.ps * p.ps;
+      c.declared[g] = k;
+      c.prefix[g] = (long long)(b - a - 1) * k >= p.min_saved ? k : 0;      // one row shares nothing, and what saves few keys is read by each row itself
+    }
+  }
+  sync();
+  if (ROWS) {
+    if (p.groups > 0) {
+      const int end = c.start[p.groups];
+      for (int m = tid; m < end; m += NT) {
+        if (m < c.start[0]) continue;
+        const int row = m == tid ? m_first : p.members[m];
+        if (row < 0 || row >= p.rows || atomicCAS(&c.member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, last_not_above(c.start, p.groups, m), row, p.rows);
+      }
+    }
+    sync();
+  }
+  // neighbouring threads take neighbouring groups and rows
+  const int g_per = cdiv(p.groups, NT), g0 = min(p.groups, tid * g_per), g1 = min(p.groups, g0 + g_per);
+  const int r_per = cdiv(p.rows, NT), r0 = ROWS ? min(p.rows, tid * r_per) : 0, r1 = ROWS ? min(p.rows, r0 + r_per) : 0;
+  auto segments = [&](int g) {
+    const int n = c.start[g + 1] - c.start[g];
+    return n > 0 && c.prefix[g] > 0 ? cdiv(n, rpt) * p.KV : 0;
+  };
+  int v[3] = {0, 0, 0}, before[3], total[3];
+  for (int g = g0; g < g1; ++g) {
+    const int x = segments(g);
+    v[0] += x * cdiv(c.prefix[g], p.kt);
+    v[1] += x;
+  }
+  for (int r = r0; r < r1; ++r) {
+    const int m = c.member[r];
+    int len = c.len[r], own = 0, said = 0;
+    if (m >= 0) {
+      const int g = last_not_above(c.start, p.groups, m);
+      if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
+        own = c.prefix[g];
+        said = c.declared[g];
+      }
+    }
+    if (len < said || len > max_keys) {
+      dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
+      c.len[r] = len = own;
+    }
+    c.own[r] = own;
+    const int tiles = max(1, cdiv(len - own, p.rows_kt));       // a row without a key of its own has an empty piece
+    c.piece[r] = tiles;
+    v[2] += tiles;
+  }
+  scan<3, NT>(v, before, total, c.sums, tid, sync);
+  c.tiles = total[0];
+  c.Q = max(1, min(cdiv(total[0], p.grid), CAP));
+  c.ranges = cdiv(total[0], c.Q);
+  c.C = max(MIN_ROW_TILES, cdiv(total[2] * p.KV, p.rows_grid));
+  for (int g = g0; g < g1; ++g) {
+    c.tile[g] = before[0];
+    c.seg[g] = before[1];
+    const int x = segments(g);
+    before[0] += x * cdiv(c.prefix[g], p.kt);
+    before[1] += x;
+  }
+  sync();
+  if (ROWS) {
+    int w[1] = {0}, w_before[1], w_total[1];
+    for (int r = r0; r < r1; ++r) w[0] += cdiv(c.piece[r], c.C) * p.KV;
+    scan<1, NT>(w, w_before, w_total, c.sums, tid, sync);
+    c.pieces = w_total[0];
+    for (int r = r0; r < r1; ++r) {
+      const int n = cdiv(c.piece[r], c.C) * p.KV;
+      c.piece[r] = w_before[0];
+      w_before[0] += n;
+    }
+    sync();
+  }
+}
+
+// Segment that holds tile ``x`` of the groups' line.
+__device__ __forceinline__ int segment_at(const DkSharedPrefixParams& p, const Cut& c, int x) {
+  const int g = last_not_above(c.tile, p.groups, x);       // the last one: groups without tiles before it start at the same place
+  return c.seg[g] + (x - c.tile[g]) / cdiv(c.prefix[g], p.kt);
+}
+__device__ __forceinline__ int range_pieces(const DkSharedPrefixParams& p, const Cut& c, int range, int& first_seg) {
+  const int lo = range * c.Q, hi = min(c.tiles, lo + c.Q);
+  first_seg = segment_at(p, c, lo);
+  return segment_at(p, c, hi - 1) - first_seg + 1;
+}
+// What range ``range`` holds of segment ``seg``.
+__device__ __forceinline__ GroupPiece group_piece(const DkSharedPrefixParams& p, const Cut& c, int range, int seg) {
+  const int lo = range * c.Q, hi = min(c.tiles, lo + c.Q), g = last_not_above(c.seg, p.groups, seg), rpt = p.qr / (p.H / p.KV);
+  const int tiles = cdiv(c.prefix[g], p.kt), i = seg - c.seg[g], a = c.tile[g] + i * tiles, m0 = c.start[g] + i / p.KV * rpt;
+  const int row = p.members[m0];
+  GroupPiece x;
+  x.first = m0;
+  x.rows = min(rpt, c.start[g + 1] - m0);
+  x.kvh = i % p.KV;
+  x.id = seg + range;
+  x.key0 = max(0, lo - a) * p.kt;
+  x.limit = min(c.prefix[g], min(tiles, hi - a) * p.kt);
+  x.table_row = row >= 0 && row < p.rows ? row : 0;        // (a row out of range was recorded)
+  x.unused = 0;
+  return x;
+}
+// Piece number ``id`` of the rows.
+__device__ __forceinline__ RowPiece row_piece(const DkSharedPrefixParams& p, const Cut& c, int id) {
+  const int row = last_not_above(c.piece, p.rows, id), shared = c.own[row], keys = c.len[row];
+  const int tiles = max(1, cdiv(keys - shared, p.rows_kt)), pieces = cdiv(tiles, c.C), per = cdiv(tiles, pieces), at = id - c.piece[row];
+  RowPiece x;
+  x.row = row;
+  x.kvh = at / pieces;
+  x.index = at - x.kvh * pieces;
+  x.key0 = min(keys, shared + x.index * per * p.rows_kt);
+  x.limit = min(keys, shared + (x.index + 1) * per * p.rows_kt);
+  x.pieces = pieces;
+  x.first_id = id - x.index;
+  x.group_id = x.group_n = x.r0 = x.unused[0] = x.unused[1] = 0;
+  if (shared > 0) {
+    const int G = p.H / p.KV, rpt = p.qr / G, m = c.member[row], g = last_not_above(c.start, p.groups, m), i = m - c.start[g];
+    const int t = cdiv(shared, p.kt), seg = i / rpt * p.KV + x.kvh, a = c.tile[g] + seg * t, f = a / c.Q;
+    x.group_id = c.seg[g] + seg + f;
+    x.group_n = (a + t - 1) / c.Q - f + 1;
+    x.r0 = i % rpt * G;
+  }
+  return x;
 }
 }  // namespace shared_prefix

@@ -164,8 +164,8 @@ _SIGNATURES = {
     "dk_experts_gemm": [P, P, P, P, P, I, I, I, I, I, F, F, F, P, I, P],
     "dk_experts_combine": [P, P, I, P, P, I, P, I, I, P, P, I, I, I, P],
     "dk_experts_tile_rows": [],
-    "dk_attention_shared_prefix_sizes": [I, I, I, I, I, I, I, I, I, I, C.POINTER(L)],
-    "dk_attention_shared_prefix": [P, L, P, L, P, P, P, P, P, P, P, L, I, P, L, I, I, I, I, I, I, I, I, I, F, I, P, P],
+    "dk_attention_shared_prefix_floats": [I, I, I, I, I, I, I, I, I, I, C.POINTER(L)],
+    "dk_attention_shared_prefix": [P, L, P, L, P, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, P, P],
     "dk_sizeof_copy_tensor": [],
     "dk_copy_items_inline": [],
     "dk_copy_items_order": [P, I, P, P, P, I, L, P, P],

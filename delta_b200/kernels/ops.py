@@ -1435,42 +1435,24 @@ def _head_rows(t: torch.Tensor, name: str, rows: int, H: int, hd: int, dtype):
     return t.data_ptr(), t.stride(0) if rows > 1 else H * hd
 
 
-_shared_prefix_sizes = {}
+_shared_prefix_floats = {}
 
 
-def attention_shared_prefix_sizes(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype):
-    """(int32 of a plan, float32 of working memory) that ``attention_shared_prefix`` needs for these sizes on the current device."""
+def attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype) -> int:
+    """Float32 of working memory that ``attention_shared_prefix`` needs for these sizes on the current device."""
     key = (rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype, _device_index())
-    n = _shared_prefix_sizes.get(key)
+    n = _shared_prefix_floats.get(key)
     if n is None:
-        need = (C.c_longlong * 2)()
-        _l.check(_l.load().dk_attention_shared_prefix_sizes(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype_code(dtype), need),
+        out = C.c_longlong()
+        _l.check(_l.load().dk_attention_shared_prefix_floats(rows, groups, members, H, KV, hd, ps, max_pages, num_pages, dtype_code(dtype), C.byref(out)),
                  "attention_shared_prefix", 0)
-        if len(_shared_prefix_sizes) >= 4096:
-            _shared_prefix_sizes.clear()
-        n = _shared_prefix_sizes[key] = (-(-need[0] // 4) * 4, need[1])
+        if len(_shared_prefix_floats) >= 4096:
+            _shared_prefix_floats.clear()
+        n = _shared_prefix_floats[key] = out.value
     return n
 
 
-def shared_prefix_plan(kv_len, members, group_start, group_prefix, *, H, KV, hd, ps, max_pages, num_pages, dtype, err=None, plan=None):
-    """How ``attention_shared_prefix`` cuts its work for these tables, as an int32 tensor on the device (``plan``, where one that is large enough is
-    given): for calls with the same tables and sizes, the layers of a step for instance, which then need not work it out each.  One launch."""
-    i32 = torch.int32
-    rows, groups, n = kv_len.numel(), group_prefix.numel(), members.numel()
-    if group_start.numel() != groups + 1:
-        raise KernelError(f"shared_prefix_plan: {groups} prefixes and {group_start.numel()} starts of groups")
-    _on_this_device("shared_prefix_plan", kv_len, members, group_start, group_prefix, err, plan)
-    need, _ = attention_shared_prefix_sizes(rows, groups, n, H, KV, hd, ps, max_pages, num_pages, dtype)
-    if plan is None:
-        plan = torch.empty(need, dtype=i32, device=kv_len.device)
-    _l.check(_l.load().dk_attention_shared_prefix(
-        None, 0, None, 0, None, None, _ptr(kv_len, "kv_len", i32), _ptr(members, "members", i32), _ptr(group_start, "group_start", i32),
-        _ptr(group_prefix, "group_prefix", i32), _ptr(plan, "plan", i32), plan.numel(), 1, None, 0, rows, groups, n, H, KV, hd, ps, max_pages, num_pages,
-        1.0, dtype_code(dtype), _ptr(err, "err", i32), _stream()), "shared_prefix_plan", 1 if rows else 0)
-    return plan
-
-
-def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_start, group_prefix, *, scale, err=None, plan=None, work=None):
+def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_start, group_prefix, *, scale, err=None, work=None):
     """Attention of single tokens, with the keys that rows share read once: row r of ``q`` [rows, H, hd] attends to the first ``kv_len[r]``
     keys of row r of ``block_table`` [rows, max_pages] in the pages ``kv`` [pages, 2, KV, ps, hd] (its own key among them, appended before).
 
@@ -1480,10 +1462,7 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
     row for each.  All tables are int32 on the device, so a captured call reads them anew at every replay; what does not fit
     (a row named twice or out of range, a row shorter than its group's prefix, a bad page) is recorded in ``err`` and skipped.
     Rows of ``q`` and ``out`` may lie apart.  Two products with float sums, the softmax in 32 bits; bfloat16 rounds the weights of the values once
-    and the result once.
-
-    ``plan``: what ``shared_prefix_plan`` made of the same tables and sizes (worked out here when None).  ``work``: float32 of
-    ``attention_shared_prefix_sizes`` that no other call uses meanwhile (allocated here when None).
+    and the result once.  ``work``: at least ``attention_shared_prefix_floats`` float32 that no other call uses meanwhile (allocated here when None).
     """
     i32 = torch.int32
     if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or block_table.dim() != 2:
@@ -1493,27 +1472,17 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
     if kv.shape[4] != hd or kv.dtype != q.dtype or block_table.shape[0] != rows or kv_len.numel() != rows or group_start.numel() != groups + 1:
         raise KernelError(f"attention_shared_prefix: {rows} rows of heads of {hd} ({q.dtype}) do not fit pages {tuple(kv.shape)} of {kv.dtype}, a table of "
                           f"{block_table.shape[0]} rows, {kv_len.numel()} lengths, {groups} prefixes and {group_start.numel()} starts of groups")
-    _on_this_device("attention_shared_prefix", q, out, kv, block_table, kv_len, members, group_start, group_prefix, err, plan, work)
+    _on_this_device("attention_shared_prefix", q, out, kv, block_table, kv_len, members, group_start, group_prefix, err, work)
     qp, qs = _head_rows(q, "q", rows, H, hd, q.dtype)
     op, os_ = _head_rows(out, "out", rows, H, hd, q.dtype)
-    plan_ints, work_floats = attention_shared_prefix_sizes(rows, groups, n, H, KV, hd, ps, block_table.shape[1], kv.shape[0], q.dtype)
-    make_plan = plan is None
+    need = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, block_table.shape[1], kv.shape[0], q.dtype)
     if work is None:
-        held = torch.empty(work_floats + (plan_ints if make_plan else 0), dtype=torch.float32, device=q.device)
-        wp, wn = held.data_ptr(), work_floats
-        if make_plan:       # the plan lies in front
-            pp, pn, wp = wp, plan_ints, wp + 4 * plan_ints
-    else:
-        wp, wn = _ptr(work, "work", torch.float32), work.numel()
-        if make_plan:
-            plan = torch.empty(plan_ints, dtype=i32, device=q.device)
-    if plan is not None:
-        pp, pn = _ptr(plan, "plan", i32), plan.numel()
+        work = torch.empty(need, dtype=torch.float32, device=q.device)
     _l.check(_l.load().dk_attention_shared_prefix(
         qp, qs, op, os_, _ptr(kv, "kv"), _ptr(block_table, "block_table", i32), _ptr(kv_len, "kv_len", i32), _ptr(members, "members", i32),
-        _ptr(group_start, "group_start", i32), _ptr(group_prefix, "group_prefix", i32), pp, pn, int(make_plan), wp, wn, rows, groups, n,
+        _ptr(group_start, "group_start", i32), _ptr(group_prefix, "group_prefix", i32), _ptr(work, "work", torch.float32), work.numel(), rows, groups, n,
         H, KV, hd, ps, block_table.shape[1], kv.shape[0], float(scale), dtype_code(q.dtype), _ptr(err, "err", i32), _stream()),
-        "attention_shared_prefix", (2 + make_plan) if rows else 0)
+        "attention_shared_prefix", 2 if rows else 0)
     return out
 
 

@@ -221,20 +221,6 @@ def test_wrong_tables_are_recorded(dtype):
     check(dtype, make(dtype, 32, 4, 128, 16, [(4, 320), (2, 64)], 1, [5, 6, 7, 8, 9, 150, 11], seed=11))
 
 
-@pytest.mark.parametrize("dtype", list(DT))
-def test_a_plan_serves_several_layers(dtype):
-    from delta_b200.kernels import ops
-    c = make(dtype, 32, 4, 128, 16, [(5, 700), (3, 64)], 2, [1, 40, 128, 129, 300, 5, 6, 7, 90, 91], seed=13)
-    tables = {k: c[k] for k in ("kv_len", "members", "group_start", "group_prefix")}
-    want = call(c)
-    plan = ops.shared_prefix_plan(**tables, H=32, KV=4, hd=128, ps=16, max_pages=c["block_table"].shape[1], num_pages=c["kv"].shape[0], dtype=DT[dtype])
-    work = torch.full((ops.attention_shared_prefix_sizes(10, 2, 8, 32, 4, 128, 16, c["block_table"].shape[1], c["kv"].shape[0], DT[dtype])[1],), float("nan"), device="cuda")
-    for layer in range(3):
-        assert torch.equal(call(c, plan=plan, work=work), want)
-        other = {**c, "q": c["q"] * 0.5, "kv": c["kv"].flip(4).contiguous()}
-        assert (call(other, plan=plan, work=work).double().cpu() - reference(other)).abs().amax() <= tolerance(dtype, 1000)
-
-
 def test_refusals():
     from delta_b200.kernels import ops
     from delta_b200.kernels.lib import KernelError
@@ -253,7 +239,6 @@ def test_refusals():
     refused("is on 'cpu'", members=c["members"].cpu())
     refused("must be positive", scale=-1.0)
     refused("floats of working memory", work=torch.empty(8, device="cuda"))
-    refused("a plan of 8 ints", plan=torch.empty(8, dtype=torch.int32, device="cuda"))
     refused("16-byte", kv=torch.empty(c["kv"].numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view_as(c["kv"]))
     many = 1025
     refused("at most", out=torch.empty(many, 8, 64, dtype=torch.bfloat16, device="cuda"), q=torch.empty(many, 8, 64, dtype=torch.bfloat16, device="cuda"),
