@@ -66,13 +66,13 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
   Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
-  auto tables = [&] { make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
+  auto tables = [&] { make_cut<true, KT, KT, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
   tables();
   // every row's first piece for the merge
   if (blockIdx.x == 0)
     for (int i = tid; i < p.rows * p.KV; i += THREADS) {
       const int row = i / p.KV, n = ((row + 1 < p.rows ? cut.piece[row + 1] : cut.pieces) - cut.piece[row]) / p.KV;
-      row_records(p)[i] = row_piece(p, cut, cut.piece[row] + i % p.KV * n);
+      row_records(p)[i] = row_piece<KT, KT>(p, cut, cut.piece[row] + i % p.KV * n);
     }
   const int n_ranges = cut.ranges, row_pieces = cut.pieces;
   // first the pieces of the block's ranges of groups, then its pieces of rows
@@ -87,14 +87,14 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
       of_group = range < n_ranges;
       if (of_group) {
         int first_seg;
-        listed = min(range_pieces(p, cut, range, first_seg), CAP);
-        if (tid < listed) list[tid] = group_piece(p, cut, range, first_seg + tid);
+        listed = min(range_pieces<KT>(p, cut, range, first_seg), CAP);
+        if (tid < listed) list[tid] = group_piece<KT>(p, cut, range, first_seg + tid);
         range += gridDim.x;
       } else if (next_row < row_pieces) {
         listed = min(CAP, cdiv(row_pieces - next_row, (int)gridDim.x));
         if (tid < listed) {
           const int id = next_row + tid * (int)gridDim.x;
-          const RowPiece x = row_piece(p, cut, id);
+          const RowPiece x = row_piece<KT, KT>(p, cut, id);
           list[tid] = {x.row, 1, x.kvh, id, x.key0, x.limit, x.row, 0};
         }
         next_row += listed * gridDim.x;

@@ -5,7 +5,8 @@
 // K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM and take pieces in turn; their tiles of 64 keys flow
 // through a ring without a stop between pieces:
 //
-//   warp 4     fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
+//   warps 4, 5 work out which pieces the block has; warp 4 then
+//              fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
 //              box per page; pages behind the last key are left out), and with a segment's first tile its queries
 //   warps 0-3  S = Q K^T for 16 keys each, the maximum over the tile through shared memory, P in bfloat16 through shared
 //              memory, O += P V for a quarter of the columns each.  So all warps share one maximum, and nothing has to be merged
@@ -28,7 +29,7 @@ constexpr int QR = 128;            // queries of a group's piece
 constexpr int LISTED = 32;         // pieces whose records lie in shared memory at once
 constexpr int MERGED = 8;          // pieces of a group in a stage, at most
 constexpr int ROWS = 16;           // rows of the MMA tile
-constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
+constexpr int WARPS = 4, CONTROL = 64, THREADS = WARPS * 32 + CONTROL;
 
 // One block of five stages an SM where two of three do not fit (heads of 128 with more than 8 to a key-value head).
 template <int HD, bool LOW>
@@ -47,11 +48,11 @@ struct Ring {
 template <bool LOW>
 __device__ __forceinline__ void mma_rows(float* c, float (&zero)[2], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (LOW) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(zero[0]), "+f"(zero[1])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
@@ -81,10 +82,10 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   __shared__ RowPiece list[LISTED];
   __shared__ __align__(16) unsigned char s_p[ROWS * TILE * 2];      // weights [row][key], 16-byte chunks exchanged by the row
   __shared__ float s_max[WARPS][ROWS], s_sum[WARPS][ROWS];
-  __shared__ int s_last;
+  __shared__ int s_last, s_pieces;
   __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
-  const int ps = p.ps, G = p.H / p.KV;
+  const int ps = p.ps, G = p.G;
   const uint32_t full = s2u(&bars[0]), empty = full + 8 * R::STAGES, ring = s2u(smem);
   if (tid == 0) {
     for (int s = 0; s < R::STAGES; ++s) {
@@ -94,21 +95,30 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
     failed = stuck = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
+  __syncthreads();
   const float sl2 = p.scale * 1.4426950408889634f;
   int n_tile = 0;                 // tiles this block has had
-  bool waited = false;
-  Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
-  make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); });
-  const int all_pieces = cut.pieces;
+  bool waited = false, dry = true;
   // the pieces of a group in a stage: G queries each in a slot of its own
   const int slot_bytes = (G * 16 * (HD / 4 + 1) + 127) / 128 * 128, per_stage = min(MERGED, R::STAGE / slot_bytes);
-  for (int first = blockIdx.x; first < all_pieces; first += gridDim.x * LISTED) {
-    const int n_pieces = min(LISTED, cdiv(all_pieces - first, (int)gridDim.x));
-    if (first != (int)blockIdx.x) make_cut<true, THREADS>(p, cut, tid, [] { __syncthreads(); });      // (the ring was used meanwhile)
-    if (tid < n_pieces) list[tid] = row_piece(p, cut, first + tid * (int)gridDim.x);
-    fence_async_smem();         // the ring is TMA's from here on
-    __syncthreads();
-    if (warp == WARPS) {
+  for (int first = blockIdx.x;; first += gridDim.x * LISTED) {
+    if (tid >= WARPS * 32) {
+      const int t = tid - WARPS * 32;
+      Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
+      make_cut<true, 2 * TILE, TILE, CONTROL>(p, cut, t, [] { asm volatile("bar.sync 2, %0;\n" ::"n"(CONTROL) : "memory"); });
+      if (t == 0) s_pieces = cut.pieces;
+      if (t < LISTED && first + t * (int)gridDim.x < cut.pieces) list[t] = row_piece<2 * TILE, TILE>(p, cut, first + t * (int)gridDim.x);
+      fence_async_smem();         // the ring is TMA's from here on
+    }
+    int n_pieces = 1, all_pieces = 0;
+    auto listed = [&] {
+      __syncthreads();
+      all_pieces = s_pieces;
+      n_pieces = first < all_pieces ? min(LISTED, cdiv(all_pieces - first, (int)gridDim.x)) : 0;
+    };
+    if (warp >= WARPS || !dry) listed();
+    if (warp > WARPS) {
+    } else if (warp == WARPS) {
       // ---------------------------------------------------------------- producer
       const int rows_of_box = min(ps, TILE), ppt = TILE / rows_of_box;      // a tile's pages, at most 8
       int n = n_tile;
@@ -179,10 +189,13 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
       n_tile = n;
     } else {
       // ---------------------------------------------------------------- the four warps
+    pieces:
       int n = n_tile;
       bool bad = false;
       for (int i = 0; i < n_pieces && !bad; ++i) {
-        const RowPiece w = list[i];
+        RowPiece w;
+        if (dry) w = {0, 0, 0, 0, 0, 1, 0, 0, 0, 0, {0, 0}};      // no key: nothing comes of it
+        else w = list[i];
         uint32_t qa[KB][4];
         float o[NT][2 * NR], zero[2] = {0.f, 0.f}, m_run[NR], l_run[NR];
 #pragma unroll
@@ -197,8 +210,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         int kb = w.key0;
         do {
           const int s = ring_slot(n, R::STAGES);
-          const bool ok = mbar_wait(full + 8 * s, ring_parity(n, R::STAGES));
-          if (!ok) stuck = 1;
+          if (!dry && !mbar_wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
           const uint32_t k_tile = ring + s * R::STAGE, v_tile = k_tile + R::KV_BYTES;
           const int keys = min(TILE, w.limit - kb);
           if (kb == w.key0 && keys > 0) {
@@ -212,20 +224,37 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
               qa[k][3] = (!LOW && g + 8 < G) ? *reinterpret_cast<const uint32_t*>(q + (g + 8) * HD + c + 8) : 0u;
             }
           }
-          float sc[2][2 * NR], mx[NR];
+          // fragments first, then four chains of products: even and odd k-blocks of two groups of eight keys
+          float sc[2][2 * NR], odd[2][2 * NR], mx[NR];
+          uint32_t kf[2][KB / 2][4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int k = 0; k < KB / 2; ++k)
 #pragma unroll
-            for (int c = 0; c < 2 * NR; ++c) sc[j][c] = 0.f;
-            const int key = warp * 16 + j * 8 + (lane & 7);
+            for (int j = 0; j < 2; ++j)
+              ldmatrix_x4(kf[j][k][0], kf[j][k][1], kf[j][k][2], kf[j][k][3], k_tile + tile_offset(warp * 16 + j * 8 + (lane & 7), 4 * k + (lane >> 3)));
 #pragma unroll
-            for (int k = 0; k < KB; k += 2) {
-              uint32_t b0, b1, b2, b3;
-              ldmatrix_x4(b0, b1, b2, b3, k_tile + tile_offset(key, 2 * k + (lane >> 3)));
-              mma_rows<LOW>(sc[j], zero, qa[k], b0, b1);
-              mma_rows<LOW>(sc[j], zero, qa[k + 1], b2, b3);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) sc[j][c] = odd[j][c] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KB / 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mma_rows<LOW>(sc[j], zero, qa[2 * k], kf[j][k][0], kf[j][k][1]);
+              mma_rows<LOW>(odd[j], zero, qa[2 * k + 1], kf[j][k][2], kf[j][k][3]);
             }
-          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) sc[j][c] += odd[j][c];
+          // V's fragments are asked for before the softmax
+          uint32_t vf[TILE / 16][NT / 2][4];
+#pragma unroll
+          for (int kk = 0; kk < TILE / 16; ++kk)
+#pragma unroll
+            for (int k = 0; k < NT / 2; ++k)
+              ldmatrix_x4_trans(vf[kk][k][0], vf[kk][k][1], vf[kk][k][2], vf[kk][k][3],
+                                v_tile + tile_offset(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, warp * NT + 2 * k + (lane >> 4)));
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             mx[r] = -INFINITY;
@@ -267,25 +296,37 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           for (int k = 0; k < NT; ++k)
 #pragma unroll
             for (int c = 0; c < 2 * NR; ++c) o[k][c] *= keep[c >> 1];
+          uint32_t a[TILE / 16][4];
 #pragma unroll
           for (int kk = 0; kk < TILE / 16; ++kk) {
-            if (kk * 16 >= keys) break;
-            uint32_t a[4];
             const int arow = (lane & 7) + ((lane >> 3) & 1) * 8;      // rows 0-7, 8-15 of keys 0-7, then of keys 8-15
-            ldmatrix_x4(a[0], a[1], a[2], a[3], s2u(s_p) + arow * (TILE * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4));
-            if (LOW) a[1] = a[3] = 0u;
+            ldmatrix_x4(a[kk][0], a[kk][1], a[kk][2], a[kk][3], s2u(s_p) + arow * (TILE * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4));
+            if (LOW) a[kk][1] = a[kk][3] = 0u;
+          }
+          if (keys < TILE) {
             // what lies behind the last key may be anything, and 0 times infinity is no zero
-            const int k0 = kk * 16 + 2 * tq;
-            const uint32_t low = (k0 < keys ? 0xffffu : 0u) | (k0 + 1 < keys ? 0xffff0000u : 0u);
-            const uint32_t high = (k0 + 8 < keys ? 0xffffu : 0u) | (k0 + 9 < keys ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int k = 0; k < NT; k += 2) {
-              uint32_t b0, b1, b2, b3;
-              ldmatrix_x4_trans(b0, b1, b2, b3, v_tile + tile_offset(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, warp * NT + k + (lane >> 4)));
-              mma_rows<LOW>(o[k], zero, a, b0 & low, b1 & high);
-              mma_rows<LOW>(o[k + 1], zero, a, b2 & low, b3 & high);
+            for (int kk = 0; kk < TILE / 16; ++kk) {
+              const int k0 = kk * 16 + 2 * tq;
+              const uint32_t low = (k0 < keys ? 0xffffu : 0u) | (k0 + 1 < keys ? 0xffff0000u : 0u);
+              const uint32_t high = (k0 + 8 < keys ? 0xffffu : 0u) | (k0 + 9 < keys ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int k = 0; k < NT / 2; ++k) {
+                vf[kk][k][0] &= low;
+                vf[kk][k][1] &= high;
+                vf[kk][k][2] &= low;
+                vf[kk][k][3] &= high;
+              }
             }
           }
+#pragma unroll
+          for (int kk = 0; kk < TILE / 16; ++kk)
+#pragma unroll
+            for (int k = 0; k < NT / 2; ++k) {
+              mma_rows<LOW>(o[2 * k], zero, a[kk], vf[kk][k][0], vf[kk][k][1]);
+              mma_rows<LOW>(o[2 * k + 1], zero, a[kk], vf[kk][k][2], vf[kk][k][3]);
+            }
+          if (dry) break;
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * s);
           ++n;
@@ -388,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             }
           }
         }
-        if (finish) {
+        if (finish && !dry) {
 #pragma unroll
           for (int r = 0; r < NR; ++r)
             if (g + 8 * r < G) {
@@ -401,12 +442,18 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         }
       }
       n_tile = n;
+      if (dry) {
+        dry = false;
+        listed();
+        goto pieces;
+      }
     }
     __syncthreads();
     if (failed || stuck) {
       if (tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_pieces);
       break;
     }
+    if (first + (long long)gridDim.x * LISTED >= all_pieces) break;
   }
 }
 

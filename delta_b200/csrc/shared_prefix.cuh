@@ -33,9 +33,9 @@ struct DkSharedPrefixParams {
   long long q_stride, out_stride;   // elements
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
   float scale;
-  // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), the blocks that compute, the most pieces
-  // there can be, and the keys that a group must save for its prefix to be read apart
-  int qr, kt, rows_kt, grid, rows_grid, group_pieces, row_pieces, min_saved;
+  // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), query heads of a key-value head, rows of a
+  // group's tile, the blocks that compute, the most pieces there can be, and the keys that a group must save for its prefix to be read apart
+  int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved;
 };
 
 namespace shared_prefix {
@@ -44,6 +44,8 @@ constexpr int CAP = 48;            // tiles of a range, so also the most pieces 
 constexpr int MIN_ROW_TILES = 16;
 
 __host__ __device__ constexpr int cdiv(int a, int b) { return (a + b - 1) / b; }
+// the same for a that seldom passes b (a division by a number the compiler does not know takes some hundred cycles)
+__device__ __forceinline__ int few(int a, int b) { return a <= 0 ? 0 : a <= b ? 1 : cdiv(a, b); }
 __host__ __device__ constexpr int round4(int a) { return (a + 3) / 4 * 4; }
 
 // A piece of a group: the first member's place in ``members``, how many rows, the key-value head, its number, the first key, the key behind the last,
@@ -67,7 +69,7 @@ struct Bounds {
 };
 static inline Bounds bounds(DkSharedPrefixParams& p) {
   Bounds b;
-  const int G = p.H / p.KV, rpt = p.qr / G;
+  const int G = p.G = p.H / p.KV, rpt = p.rpt = p.qr / G;
   const long long keys = (long long)p.max_pages * p.ps, segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
   const long long of_groups = segments * ((keys + p.kt - 1) / p.kt), capped = (of_groups + CAP - 1) / CAP;
   const long long group_pieces = segments > 0 ? segments + (capped > p.grid ? capped : (long long)p.grid) : 0;
@@ -105,7 +107,7 @@ struct Cut {
   int *member, *len, *own, *piece;                  // rows: place in members (-1: of no group), keys, keys read with the group, first piece
   int* sums;
   int Q, tiles, ranges, C, pieces;                  // tiles of a range, tiles of the line, ranges; tiles of a row's piece, rows' pieces
-  static __host__ __device__ constexpr int ints(int rows, int groups) { return 5 * groups + 1 + 4 * rows + 3 * 32; }
+  static __host__ __device__ constexpr int ints(int rows, int groups) { return 5 * groups + 1 + 4 * rows + 4 * 32; }
   __device__ __forceinline__ Cut(int* s, int rows, int groups)
       : start(s), prefix(start + groups + 1), declared(prefix + groups), tile(declared + groups), seg(tile + groups), member(seg + groups), len(member + rows),
         own(len + rows), piece(own + rows), sums(piece + rows) {}
@@ -113,7 +115,7 @@ struct Cut {
 
 // Sums of N values over the threads before this one, and over all; one sync.
 template <int N, int NT, typename Sync>
-__device__ __forceinline__ void scan(const int (&v)[N], int (&before)[N], int (&total)[N], int* s, int tid, Sync sync) {
+__device__ __forceinline__ void scan(const int* v, int* before, int* total, int* s, int tid, Sync sync) {
   const int lane = tid & 31, warp = tid >> 5;
 #pragma unroll
   for (int i = 0; i < N; ++i) before[i] = v[i];
@@ -140,10 +142,10 @@ __device__ __forceinline__ void scan(const int (&v)[N], int (&before)[N], int (&
     }
 }
 
-// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well.  Ends with a sync.
-template <bool ROWS, int NT, typename Sync>
+// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well; KT, ROWS_KT: p.kt, p.rows_kt.  Ends with a sync.
+template <bool ROWS, int KT, int ROWS_KT, int NT, typename Sync>
 __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid, Sync sync) {
-  const int rpt = p.qr / (p.H / p.KV), max_keys = p.max_pages * p.ps;
+  const int max_keys = p.max_pages * p.ps;
   // what the steps below read is asked for at once
   const int m_first = ROWS && tid < p.n_members && p.groups > 0 ? p.members[tid] : -1;
   if (ROWS)
@@ -189,12 +191,12 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
   const int r_per = cdiv(p.rows, NT), r0 = ROWS ? min(p.rows, tid * r_per) : 0, r1 = ROWS ? min(p.rows, r0 + r_per) : 0;
   auto segments = [&](int g) {
     const int n = c.start[g + 1] - c.start[g];
-    return n > 0 && c.prefix[g] > 0 ? cdiv(n, rpt) * p.KV : 0;
+    return c.prefix[g] > 0 ? few(n, p.rpt) * p.KV : 0;
   };
-  int v[3] = {0, 0, 0}, before[3], total[3];
+  int v[4] = {0, 0, 0, 0}, before[4], total[4];
   for (int g = g0; g < g1; ++g) {
     const int x = segments(g);
-    v[0] += x * cdiv(c.prefix[g], p.kt);
+    v[0] += x * cdiv(c.prefix[g], KT);
     v[1] += x;
   }
   for (int r = r0; r < r1; ++r) {
@@ -212,82 +214,89 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
       c.len[r] = len = own;
     }
     c.own[r] = own;
-    const int tiles = max(1, cdiv(len - own, p.rows_kt));       // a row without a key of its own has an empty piece
+    const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece
     c.piece[r] = tiles;
     v[2] += tiles;
+    v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
   }
-  scan<3, NT>(v, before, total, c.sums, tid, sync);
+  scan<ROWS ? 4 : 2, NT>(v, before, total, c.sums, tid, sync);
   c.tiles = total[0];
-  c.Q = max(1, min(cdiv(total[0], p.grid), CAP));
-  c.ranges = cdiv(total[0], c.Q);
-  c.C = max(MIN_ROW_TILES, cdiv(total[2] * p.KV, p.rows_grid));
+  c.Q = max(1, min(few(total[0], p.grid), CAP));
+  c.ranges = c.Q == 1 ? total[0] : cdiv(total[0], c.Q);
+  if (ROWS) c.C = total[2] * p.KV <= MIN_ROW_TILES * p.rows_grid ? MIN_ROW_TILES : cdiv(total[2] * p.KV, p.rows_grid);
   for (int g = g0; g < g1; ++g) {
     c.tile[g] = before[0];
     c.seg[g] = before[1];
     const int x = segments(g);
-    before[0] += x * cdiv(c.prefix[g], p.kt);
+    before[0] += x * cdiv(c.prefix[g], KT);
     before[1] += x;
   }
-  sync();
   if (ROWS) {
-    int w[1] = {0}, w_before[1], w_total[1];
-    for (int r = r0; r < r1; ++r) w[0] += cdiv(c.piece[r], c.C) * p.KV;
-    scan<1, NT>(w, w_before, w_total, c.sums, tid, sync);
-    c.pieces = w_total[0];
+    if (c.C != MIN_ROW_TILES) {
+      sync();                     // (the sums were read)
+      v[0] = 0;
+      for (int r = r0; r < r1; ++r) v[0] += cdiv(c.piece[r], c.C) * p.KV;
+      scan<1, NT>(v, before + 3, total + 3, c.sums, tid, sync);
+    }
+    c.pieces = total[3];
     for (int r = r0; r < r1; ++r) {
       const int n = cdiv(c.piece[r], c.C) * p.KV;
-      c.piece[r] = w_before[0];
-      w_before[0] += n;
+      c.piece[r] = before[3];
+      before[3] += n;
     }
-    sync();
   }
+  sync();
 }
 
 // Segment that holds tile ``x`` of the groups' line.
+template <int KT>
 __device__ __forceinline__ int segment_at(const DkSharedPrefixParams& p, const Cut& c, int x) {
   const int g = last_not_above(c.tile, p.groups, x);       // the last one: groups without tiles before it start at the same place
-  return c.seg[g] + (x - c.tile[g]) / cdiv(c.prefix[g], p.kt);
+  return c.seg[g] + (x - c.tile[g]) / cdiv(c.prefix[g], KT);
 }
+template <int KT>
 __device__ __forceinline__ int range_pieces(const DkSharedPrefixParams& p, const Cut& c, int range, int& first_seg) {
   const int lo = range * c.Q, hi = min(c.tiles, lo + c.Q);
-  first_seg = segment_at(p, c, lo);
-  return segment_at(p, c, hi - 1) - first_seg + 1;
+  first_seg = segment_at<KT>(p, c, lo);
+  return segment_at<KT>(p, c, hi - 1) - first_seg + 1;
 }
 // What range ``range`` holds of segment ``seg``.
+template <int KT>
 __device__ __forceinline__ GroupPiece group_piece(const DkSharedPrefixParams& p, const Cut& c, int range, int seg) {
-  const int lo = range * c.Q, hi = min(c.tiles, lo + c.Q), g = last_not_above(c.seg, p.groups, seg), rpt = p.qr / (p.H / p.KV);
-  const int tiles = cdiv(c.prefix[g], p.kt), i = seg - c.seg[g], a = c.tile[g] + i * tiles, m0 = c.start[g] + i / p.KV * rpt;
+  const int lo = range * c.Q, hi = min(c.tiles, lo + c.Q), g = last_not_above(c.seg, p.groups, seg);
+  const int tiles = cdiv(c.prefix[g], KT), i = seg - c.seg[g], a = c.tile[g] + i * tiles, qt = i < p.KV ? 0 : i / p.KV, m0 = c.start[g] + qt * p.rpt;
   const int row = p.members[m0];
   GroupPiece x;
   x.first = m0;
-  x.rows = min(rpt, c.start[g + 1] - m0);
-  x.kvh = i % p.KV;
+  x.rows = min(p.rpt, c.start[g + 1] - m0);
+  x.kvh = i - qt * p.KV;
   x.id = seg + range;
-  x.key0 = max(0, lo - a) * p.kt;
-  x.limit = min(c.prefix[g], min(tiles, hi - a) * p.kt);
+  x.key0 = max(0, lo - a) * KT;
+  x.limit = min(c.prefix[g], min(tiles, hi - a) * KT);
   x.table_row = row >= 0 && row < p.rows ? row : 0;        // (a row out of range was recorded)
   x.unused = 0;
   return x;
 }
 // Piece number ``id`` of the rows.
+template <int KT, int ROWS_KT>
 __device__ __forceinline__ RowPiece row_piece(const DkSharedPrefixParams& p, const Cut& c, int id) {
   const int row = last_not_above(c.piece, p.rows, id), shared = c.own[row], keys = c.len[row];
-  const int tiles = max(1, cdiv(keys - shared, p.rows_kt)), pieces = cdiv(tiles, c.C), per = cdiv(tiles, pieces), at = id - c.piece[row];
+  const int tiles = max(1, cdiv(keys - shared, ROWS_KT)), pieces = few(tiles, c.C), per = pieces == 1 ? tiles : cdiv(tiles, pieces), at = id - c.piece[row];
   RowPiece x;
   x.row = row;
-  x.kvh = at / pieces;
+  x.kvh = pieces == 1 ? at : at / pieces;
   x.index = at - x.kvh * pieces;
-  x.key0 = min(keys, shared + x.index * per * p.rows_kt);
-  x.limit = min(keys, shared + (x.index + 1) * per * p.rows_kt);
+  x.key0 = min(keys, shared + x.index * per * ROWS_KT);
+  x.limit = min(keys, shared + (x.index + 1) * per * ROWS_KT);
   x.pieces = pieces;
   x.first_id = id - x.index;
   x.group_id = x.group_n = x.r0 = x.unused[0] = x.unused[1] = 0;
   if (shared > 0) {
-    const int G = p.H / p.KV, rpt = p.qr / G, m = c.member[row], g = last_not_above(c.start, p.groups, m), i = m - c.start[g];
-    const int t = cdiv(shared, p.kt), seg = i / rpt * p.KV + x.kvh, a = c.tile[g] + seg * t, f = a / c.Q;
+    const int m = c.member[row], g = last_not_above(c.start, p.groups, m), i = m - c.start[g], qt = i < p.rpt ? 0 : i / p.rpt;
+    const int t = cdiv(shared, KT), seg = qt * p.KV + x.kvh, a = c.tile[g] + seg * t, f = c.Q == 1 ? a : a / c.Q, l = c.Q == 1 ? a + t - 1 : (a + t - 1) / c.Q;
     x.group_id = c.seg[g] + seg + f;
-    x.group_n = (a + t - 1) / c.Q - f + 1;
-    x.r0 = i % rpt * G;
+    x.group_n = l - f + 1;
+    x.r0 = (i - qt * p.rpt) * p.G;
   }
   return x;
 }
