@@ -46,9 +46,6 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
-// Behind the pieces' results: the record of the first piece of every row and key-value head.
-__device__ __forceinline__ RowPiece* row_records(const DkSharedPrefixParams& p) { return reinterpret_cast<RowPiece*>(row_results(p, p.row_pieces)); }
-
 // HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
 __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
@@ -72,9 +69,9 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
   if (blockIdx.x == 0)
     for (int i = tid; i < p.rows * p.KV; i += THREADS) {
       const int row = i / p.KV, n = ((row + 1 < p.rows ? cut.piece[row + 1] : cut.pieces) - cut.piece[row]) / p.KV;
-      row_records(p)[i] = row_piece<KT, KT>(p, cut, cut.piece[row] + i % p.KV * n);
+      row_pieces(p)[i] = row_piece<KT, KT>(p, cut, cut.piece[row] + i % p.KV * n);
     }
-  const int n_ranges = cut.ranges, row_pieces = cut.pieces;
+  const int n_ranges = cut.ranges, n_row_pieces = cut.pieces;
   // first the pieces of the block's ranges of groups, then its pieces of rows
   int range = blockIdx.x, next_row = gridDim.x - 1 - blockIdx.x, listed = 0, at = 0;
   bool of_group = range < n_ranges, list_made = false;
@@ -90,8 +87,8 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
         listed = min(range_pieces<KT>(p, cut, range, first_seg), CAP);
         if (tid < listed) list[tid] = group_piece<KT>(p, cut, range, first_seg + tid);
         range += gridDim.x;
-      } else if (next_row < row_pieces) {
-        listed = min(CAP, cdiv(row_pieces - next_row, (int)gridDim.x));
+      } else if (next_row < n_row_pieces) {
+        listed = min(CAP, cdiv(n_row_pieces - next_row, (int)gridDim.x));
         if (tid < listed) {
           const int id = next_row + tid * (int)gridDim.x;
           const RowPiece x = row_piece<KT, KT>(p, cut, id);
@@ -219,7 +216,7 @@ template <typename T>
 __global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p) {
   const int kvh = blockIdx.x, row = blockIdx.y, G = p.H / p.KV;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const RowPiece w = row_records(p)[row * p.KV + kvh];
+  const RowPiece w = row_pieces(p)[row * p.KV + kvh];
   const long long gs = group_piece_floats(QR, p.hd), rs = row_piece_floats(G, p.hd);
   const float* gp = group_results(p, w.group_id);
   const float* rp = row_results(p, w.first_id);
@@ -335,7 +332,7 @@ bool cut_for(DkSharedPrefixParams& p) {
   const bool tc = dk_shared_prefix_tc_takes(p);
   p.qr = tc ? 128 : QR;
   p.kt = tc ? 128 : KT;
-  p.grid = tc ? dk_sm_count() : fma_grid();
+  p.grid = tc ? dk_sm_count() - 1 : fma_grid();      // (one block of the tensor cores' first kernel prepares the second)
   p.rows_kt = tc ? dk_shared_prefix_rows_tile() : KT;
   p.rows_grid = tc ? dk_shared_prefix_rows_grid(p) : fma_grid();
   p.min_saved = 1;
@@ -348,7 +345,7 @@ int sizes(DkSharedPrefixParams& p, bool* tc, long long* floats) {
   const Bounds b = bounds(p);
   DK_REQUIRE(b.tiles < (1ll << 30) && b.pieces < (1ll << 24), "attention_shared_prefix: %d rows of %d key-value heads over tables of %d pages are too much for one call",
              p.rows, p.KV, p.max_pages);
-  *floats = b.work_floats + (*tc ? 0 : (long long)p.rows * p.KV * sizeof(RowPiece) / 4);
+  *floats = b.work_floats;
   return 0;
 }
 }  // namespace

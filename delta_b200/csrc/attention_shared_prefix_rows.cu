@@ -5,8 +5,7 @@
 // K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM and take pieces in turn; their tiles of 64 keys flow
 // through a ring without a stop between pieces:
 //
-//   warps 4, 5 work out which pieces the block has; warp 4 then
-//              fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
+//   warp 4     fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
 //              box per page; pages behind the last key are left out), and with a segment's first tile its queries
 //   warps 0-3  S = Q K^T for 16 keys each, the maximum over the tile through shared memory, P in bfloat16 through shared
 //              memory, O += P V for a quarter of the columns each.  So all warps share one maximum, and nothing has to be merged
@@ -15,8 +14,8 @@
 // Behind a piece's last tile the pieces of its row's group are added to it, in the order of their keys: they come through the ring as well, up to eight
 // a stage, one box each.  (Of a segment that is cut, only the first piece adds them.)  The result is rounded once.  Where a segment is cut, each block
 // leaves its piece's results in the work buffer and counts itself; the one that comes last adds them all, in their order, so the result does not depend on
-// who that is.  The counters are cleared by the kernel of the groups.  This kernel starts while that one runs and waits for its end before it touches
-// what it wrote.
+// who that is.  This kernel starts while that one runs and waits for its end before it touches what it wrote; the list of pieces and the cleared counters
+// alone are there before: the block that writes them lets this kernel start when they are.
 #include "shared_prefix.cuh"
 #include "tcgen05_helpers.cuh"
 #include "mma_helpers.cuh"
@@ -29,7 +28,7 @@ constexpr int QR = 128;            // queries of a group's piece
 constexpr int LISTED = 32;         // pieces whose records lie in shared memory at once
 constexpr int MERGED = 8;          // pieces of a group in a stage, at most
 constexpr int ROWS = 16;           // rows of the MMA tile
-constexpr int WARPS = 4, CONTROL = 64, THREADS = WARPS * 32 + CONTROL;
+constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
 
 // One block of five stages an SM where two of three do not fit (heads of 128 with more than 8 to a key-value head).
 template <int HD, bool LOW>
@@ -41,7 +40,6 @@ struct Ring {
   static constexpr int STAGES = HD == 128 && LOW ? 3 : 5;
   static constexpr int BLOCKS = HD == 128 && !LOW ? 1 : 2;            // on an SM
   static constexpr int TOTAL = STAGES * STAGE + 1024;                // 1024 to start on a swizzle boundary
-  static_assert(4 * Cut::ints(MAX_ROWS, MAX_GROUPS) <= STAGES * STAGE, "the tables are laid out in the ring");
 };
 
 // LOW: at most 8 query heads; rows 8..15 of the MMA tile are then empty and their accumulators two registers that stay zero.
@@ -65,6 +63,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
+__device__ __noinline__ bool long_wait(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity); }
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || long_wait(bar, parity); }
+// 2^x by the special-function unit (two units in the last place; results below 2^-126 become 0)
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void warps_barrier() { asm volatile("bar.sync 1, %0;\n" ::"n"(WARPS * 32) : "memory"); }
 
 template <int HD, bool LOW>
@@ -82,7 +88,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   __shared__ RowPiece list[LISTED];
   __shared__ __align__(16) unsigned char s_p[ROWS * TILE * 2];      // weights [row][key], 16-byte chunks exchanged by the row
   __shared__ float s_max[WARPS][ROWS], s_sum[WARPS][ROWS];
-  __shared__ int s_last, s_pieces;
+  __shared__ int s_last;
   __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
   const int ps = p.ps, G = p.G;
@@ -98,27 +104,20 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   __syncthreads();
   const float sl2 = p.scale * 1.4426950408889634f;
   int n_tile = 0;                 // tiles this block has had
-  bool waited = false, dry = true;
+  bool waited = false;
   // the pieces of a group in a stage: G queries each in a slot of its own
   const int slot_bytes = (G * 16 * (HD / 4 + 1) + 127) / 128 * 128, per_stage = min(MERGED, R::STAGE / slot_bytes);
-  for (int first = blockIdx.x;; first += gridDim.x * LISTED) {
-    if (tid >= WARPS * 32) {
-      const int t = tid - WARPS * 32;
-      Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
-      make_cut<true, 2 * TILE, TILE, CONTROL>(p, cut, t, [] { asm volatile("bar.sync 2, %0;\n" ::"n"(CONTROL) : "memory"); });
-      if (t == 0) s_pieces = cut.pieces;
-      if (t < LISTED && first + t * (int)gridDim.x < cut.pieces) list[t] = row_piece<2 * TILE, TILE>(p, cut, first + t * (int)gridDim.x);
-      fence_async_smem();         // the ring is TMA's from here on
+  const int all_pieces = __ldcg(reinterpret_cast<const int*>(p.work));
+  for (int first = blockIdx.x; first < p.row_pieces; first += gridDim.x * LISTED) {
+    // (records behind the last piece are read with the others, so that nothing waits for the count, and not used)
+    for (int x = tid; x < LISTED * (ROW_INTS / 4); x += THREADS) {
+      const int id = first + x / (ROW_INTS / 4) * (int)gridDim.x;
+      if (id < p.row_pieces) reinterpret_cast<int4*>(list)[x] = __ldcg(reinterpret_cast<const int4*>(row_pieces(p) + id) + x % (ROW_INTS / 4));
     }
-    int n_pieces = 1, all_pieces = 0;
-    auto listed = [&] {
-      __syncthreads();
-      all_pieces = s_pieces;
-      n_pieces = first < all_pieces ? min(LISTED, cdiv(all_pieces - first, (int)gridDim.x)) : 0;
-    };
-    if (warp >= WARPS || !dry) listed();
-    if (warp > WARPS) {
-    } else if (warp == WARPS) {
+    const int n_pieces = first < all_pieces ? min(LISTED, cdiv(all_pieces - first, (int)gridDim.x)) : 0;
+    if (n_pieces == 0) break;
+    __syncthreads();
+    if (warp == WARPS) {
       // ---------------------------------------------------------------- producer
       const int rows_of_box = min(ps, TILE), ppt = TILE / rows_of_box;      // a tile's pages, at most 8
       int n = n_tile;
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           const int held = __popc(__ballot_sync(0xffffffffu, page >= 0));
           const int s = ring_slot(n, R::STAGES);
           bool ok = true;
-          if (n >= R::STAGES) ok = mbar_wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
+          if (n >= R::STAGES) ok = wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
           if (!__all_sync(0xffffffffu, ok && !stuck)) { failed = 1; break; }
           const uint32_t k_dst = ring + s * R::STAGE, v_dst = k_dst + R::KV_BYTES, bar = full + 8 * s;
           const bool with_q = kb == w.key0 && limit > w.key0;
@@ -177,25 +176,22 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         for (int x = 0; x < w.group_n; x += per_stage, ++n) {
           const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
           bool ok = true;
-          if (n >= R::STAGES) ok = mbar_wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
+          if (n >= R::STAGES) ok = wait(empty + 8 * s, ring_parity(n - R::STAGES, R::STAGES));
           if (!__all_sync(0xffffffffu, ok && !stuck)) { failed = 1; break; }
           if (lane == 0) mbar_expect_tx(full + 8 * s, (uint32_t)(m * G * 16 * (HD / 4 + 1)));
           __syncwarp();
           if (lane < m) tma_load_3d(ring + s * R::STAGE + lane * slot_bytes, &map_merge, w.r0 * 4, 0, w.group_id + x + lane, full + 8 * s);
         }
       }
-      if (lane == 0) ring_drain(n, R::STAGES, [&](int slot, uint32_t parity) { return mbar_wait(full + 8 * slot, parity); });   // its copies have arrived
+      if (lane == 0) ring_drain(n, R::STAGES, [&](int slot, uint32_t parity) { return long_wait(full + 8 * slot, parity); });   // its copies have arrived
       __syncwarp();
       n_tile = n;
     } else {
       // ---------------------------------------------------------------- the four warps
-    pieces:
       int n = n_tile;
       bool bad = false;
       for (int i = 0; i < n_pieces && !bad; ++i) {
-        RowPiece w;
-        if (dry) w = {0, 0, 0, 0, 0, 1, 0, 0, 0, 0, {0, 0}};      // no key: nothing comes of it
-        else w = list[i];
+        const RowPiece w = list[i];
         uint32_t qa[KB][4];
         float o[NT][2 * NR], zero[2] = {0.f, 0.f}, m_run[NR], l_run[NR];
 #pragma unroll
@@ -210,18 +206,22 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         int kb = w.key0;
         do {
           const int s = ring_slot(n, R::STAGES);
-          if (!dry && !mbar_wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
+          if (!wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
           const uint32_t k_tile = ring + s * R::STAGE, v_tile = k_tile + R::KV_BYTES;
           const int keys = min(TILE, w.limit - kb);
           if (kb == w.key0 && keys > 0) {
-            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(smem + s * R::STAGE + 2 * R::KV_BYTES);
+            // (rows from G on hold whatever lay there: a row of the products depends on its own queries alone)
+            const uint32_t q = v_tile + R::KV_BYTES;
+            if (LOW) {
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-              const int c = k * 16 + 2 * tq;
-              qa[k][0] = g < G ? *reinterpret_cast<const uint32_t*>(q + g * HD + c) : 0u;
-              qa[k][1] = (!LOW && g + 8 < G) ? *reinterpret_cast<const uint32_t*>(q + (g + 8) * HD + c) : 0u;
-              qa[k][2] = g < G ? *reinterpret_cast<const uint32_t*>(q + g * HD + c + 8) : 0u;
-              qa[k][3] = (!LOW && g + 8 < G) ? *reinterpret_cast<const uint32_t*>(q + (g + 8) * HD + c + 8) : 0u;
+              for (int k = 0; k < KB; k += 2) {
+                ldmatrix_x4(qa[k][0], qa[k][2], qa[k + 1][0], qa[k + 1][2], q + (lane & 7) * (HD * 2) + (2 * k + (lane >> 3)) * 16);
+                qa[k][1] = qa[k][3] = qa[k + 1][1] = qa[k + 1][3] = 0u;
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < KB; ++k)
+                ldmatrix_x4(qa[k][0], qa[k][1], qa[k][2], qa[k][3], q + ((lane & 7) + ((lane >> 3) & 1) * 8) * (HD * 2) + (2 * k + (lane >> 4)) * 16);
             }
           }
           // fragments first, then four chains of products: even and odd k-blocks of two groups of eight keys
@@ -280,12 +280,12 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             const int row = g + 8 * r;
             const float m_new = fmaxf(fmaxf(m_run[r], fmaxf(s_max[0][row], s_max[1][row])), fmaxf(s_max[2][row], s_max[3][row]));
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            keep[r] = exp2f(m_run[r] - m_use);       // 0 before the first key
+            keep[r] = fast_exp2(m_run[r] - m_use);       // 0 before the first key
             m_run[r] = m_new;
             l_run[r] *= keep[r];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float p0 = exp2f(sc[j][2 * r] - m_use), p1 = exp2f(sc[j][2 * r + 1] - m_use);
+              const float p0 = fast_exp2(sc[j][2 * r] - m_use), p1 = fast_exp2(sc[j][2 * r + 1] - m_use);
               l_run[r] += p0 + p1;        // the sum in 32 bits; the weights are rounded to bfloat16 for the product
               const int key = warp * 16 + j * 8 + 2 * tq;
               *reinterpret_cast<uint32_t*>(s_p + row * (TILE * 2) + (((key >> 3) ^ (row & 7)) << 4) + (key & 7) * 2) = pack_bf16(p0, p1);
@@ -326,7 +326,6 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
               mma_rows<LOW>(o[2 * k], zero, a[kk], vf[kk][k][0], vf[kk][k][1]);
               mma_rows<LOW>(o[2 * k + 1], zero, a[kk], vf[kk][k][2], vf[kk][k][3]);
             }
-          if (dry) break;
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * s);
           ++n;
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         // {maximum, sum, outputs} of a piece added to this thread's queries
         auto add = [&](int r, float m, float l, const float (&v)[2 * NT]) {
           const float m_new = fmaxf(m_run[r], m), m_use = m_new == -INFINITY ? 0.f : m_new;
-          const float have = exp2f(m_run[r] - m_use), f = exp2f(m - m_use);
+          const float have = fast_exp2(m_run[r] - m_use), f = fast_exp2(m - m_use);
           m_run[r] = m_new;
           l_run[r] = l_run[r] * have + l * f;
 #pragma unroll
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         if (w.index == 0)
           for (int x = 0; x < w.group_n; x += per_stage, ++n) {
             const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
-            if (!mbar_wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
+            if (!wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
             for (int y = 0; y < m; ++y) {
               const unsigned char* part = smem + s * R::STAGE + y * slot_bytes;
 #pragma unroll
@@ -429,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             }
           }
         }
-        if (finish && !dry) {
+        if (finish) {
 #pragma unroll
           for (int r = 0; r < NR; ++r)
             if (g + 8 * r < G) {
@@ -442,18 +441,12 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
         }
       }
       n_tile = n;
-      if (dry) {
-        dry = false;
-        listed();
-        goto pieces;
-      }
     }
     __syncthreads();
     if (failed || stuck) {
       if (tid == 0) dk_report(p.err, DK_DEV_TIMEOUT, (int)blockIdx.x, (int)gridDim.x, n_pieces);
       break;
     }
-    if (first + (long long)gridDim.x * LISTED >= all_pieces) break;
   }
 }
 

@@ -11,9 +11,8 @@
 //   rows    every segment is cut into equal pieces of at most C tiles, numbered through, and a block takes every ``grid``-th.  C is what
 //           levels the blocks, but MIN_ROW_TILES at least: the pieces of a cut segment go through memory, which takes as long as several tiles.
 //
-// Every block works this out for itself from the tables on the device (a captured call follows them): a kernel of its own for it was
-// measured to cost 3 us more before the first tile.  Whatever comes from the tables is checked here, so the kernels stay inside their
-// tensors (page ids they check themselves).
+// All this is worked out on the device from the tables, so that a captured call follows them.  Whatever comes from the tables is checked here, so
+// the kernels stay inside their tensors (page ids they check themselves).
 #pragma once
 #include "common.cuh"
 
@@ -28,7 +27,7 @@ struct DkSharedPrefixParams {
   const int* members;        // [n_members] rows, group by group
   const int* group_start;    // [groups + 1] first member of each group
   const int* group_prefix;   // [groups] shared keys (rounded down to whole pages)
-  float* work;               // counters, then the pieces' partial results
+  float* work;               // the rows' pieces, counters, the pieces' results
   int* err;                  // device error record, 4 ints; or null
   long long q_stride, out_stride;   // elements
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
@@ -58,11 +57,15 @@ struct __align__(16) GroupPiece {
 struct __align__(16) RowPiece {
   int row, kvh, key0, limit, index, pieces, first_id, group_id, group_n, r0, unused[2];
 };
+constexpr int ROW_INTS = sizeof(RowPiece) / 4;
+
 // Floats of one piece's results: of a group as [hd / 4 + 1][queries][4] (neighbouring queries lie side by side; the last row of four holds maximum and
 // sum, then nothing); of a row as [query][hd], then {maximum, sum} per query.
 __host__ __device__ __forceinline__ long long group_piece_floats(int qr, int hd) { return (long long)qr * (hd + 4); }
 __host__ __device__ __forceinline__ long long row_piece_floats(int G, int hd) { return ((long long)G * (hd + 2) + 3) / 4 * 4; }
 
+// The work buffer: how many pieces the rows have and their records, a counter per row and key-value head, the results of groups' pieces, of rows' pieces.
+__host__ __device__ __forceinline__ long long front_ints(const DkSharedPrefixParams& p) { return 4 + (long long)p.row_pieces * ROW_INTS; }
 // Fills in the most pieces that there can be with these sizes, whatever the device's tables say, and tells what they need.
 struct Bounds {
   long long tiles, pieces, work_floats;
@@ -76,15 +79,15 @@ static inline Bounds bounds(DkSharedPrefixParams& p) {
   const long long row_pieces = (long long)p.rows * p.KV + p.rows_grid;      // a segment's last piece, and tiles / C of full ones, which are no more than blocks
   b.tiles = of_groups + (long long)p.rows * p.KV * ((keys + p.rows_kt - 1) / p.rows_kt);
   b.pieces = group_pieces + row_pieces;
-  b.work_floats = round4(p.rows * p.KV) + group_pieces * group_piece_floats(p.qr, p.hd) + row_pieces * row_piece_floats(G, p.hd);
   p.group_pieces = (int)group_pieces;
   p.row_pieces = (int)row_pieces;
+  b.work_floats = front_ints(p) + round4(p.rows * p.KV) + group_pieces * group_piece_floats(p.qr, p.hd) + row_pieces * row_piece_floats(G, p.hd);
   return b;
 }
-// The work buffer: a counter per row and key-value head, the results of groups' pieces, of rows' pieces. 
-__device__ __forceinline__ int* counters(const DkSharedPrefixParams& p) { return reinterpret_cast<int*>(p.work); }
+__device__ __forceinline__ RowPiece* row_pieces(const DkSharedPrefixParams& p) { return reinterpret_cast<RowPiece*>(p.work + 4); }
+__device__ __forceinline__ int* counters(const DkSharedPrefixParams& p) { return reinterpret_cast<int*>(p.work + front_ints(p)); }
 __host__ __device__ __forceinline__ float* group_results(const DkSharedPrefixParams& p, int id) {
-  return p.work + round4(p.rows * p.KV) + id * group_piece_floats(p.qr, p.hd);
+  return p.work + front_ints(p) + round4(p.rows * p.KV) + id * group_piece_floats(p.qr, p.hd);
 }
 __device__ __forceinline__ float* row_results(const DkSharedPrefixParams& p, int id) {
   return group_results(p, p.group_pieces) + id * row_piece_floats(p.H / p.KV, p.hd);
