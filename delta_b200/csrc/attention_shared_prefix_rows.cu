@@ -355,20 +355,35 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           for (int x = 0; x < w.group_n; x += per_stage, ++n) {
             const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
             if (!wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
-            for (int y = 0; y < m; ++y) {
-              const unsigned char* part = smem + s * R::STAGE + y * slot_bytes;
+            // the stage's pieces at once: their common maximum first, so that nothing but the sums is done one after the other
+            const unsigned char* part = smem + s * R::STAGE;
 #pragma unroll
-              for (int r = 0; r < NR; ++r)
-                if (g + 8 * r < G) {
-                  const float2 ml = *reinterpret_cast<const float2*>(part + (HD / 4 * G + g + 8 * r) * 16);
-                  float v[2 * NT];
+            for (int r = 0; r < NR; ++r) {
+              const int qh = g + 8 * r;
+              if (qh >= G) continue;
+              float f[MERGED], m_new = m_run[r];
+#pragma unroll
+              for (int y = 0; y < MERGED; ++y) {
+                f[y] = y < m ? *reinterpret_cast<const float*>(part + y * slot_bytes + (HD / 4 * G + qh) * 16) : -INFINITY;
+                m_new = fmaxf(m_new, f[y]);
+              }
+              const float m_use = m_new == -INFINITY ? 0.f : m_new, have = fast_exp2(m_run[r] - m_use);
+              m_run[r] = m_new;
+              l_run[r] *= have;
+#pragma unroll
+              for (int k = 0; k < 2 * NT; ++k) o[k / 2][2 * r + k % 2] *= have;
+#pragma unroll
+              for (int y = 0; y < MERGED; ++y)
+                if (y < m) {
+                  const unsigned char* from = part + y * slot_bytes;
+                  const float w_y = fast_exp2(f[y] - m_use);
+                  l_run[r] += w_y * *reinterpret_cast<const float*>(from + (HD / 4 * G + qh) * 16 + 4);
 #pragma unroll
                   for (int k = 0; k < NT; ++k) {
-                    const float2 f = *reinterpret_cast<const float2*>(part + (((warp * NT + k) * 2 + tq / 2) * G + g + 8 * r) * 16 + (tq & 1) * 8);
-                    v[2 * k] = f.x;
-                    v[2 * k + 1] = f.y;
+                    const float2 v = *reinterpret_cast<const float2*>(from + (((warp * NT + k) * 2 + tq / 2) * G + qh) * 16 + (tq & 1) * 8);
+                    o[k][2 * r] = fmaf(w_y, v.x, o[k][2 * r]);
+                    o[k][2 * r + 1] = fmaf(w_y, v.y, o[k][2 * r + 1]);
                   }
-                  add(r, ml.x, ml.y, v);
                 }
             }
             __syncwarp();

@@ -125,8 +125,8 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
       seg_base += seg_end;
     }
     if (pass == 0) {
-      Q = max(1, min(few(tile_base, p.grid), CAP));
-      ranges = Q == 1 ? tile_base : cdiv(tile_base, Q);
+      Q = range_tiles(p, tile_base, seg_base);
+      ranges = cdiv(tile_base, Q);
       lo = range * Q;
       hi = min(tile_base, lo + Q);
       if (lo >= hi) return 0;
@@ -211,21 +211,25 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
       const uint32_t t_s = tmem + lane_base + COL_S + w * KT;
       const uint32_t t_o = tmem + lane_base + COL_O + w * HD;
       const float sl2 = p.scale * 1.4426950408889634f;
-      constexpr int QC = HD / 16;                         // 16-byte chunks of a query that this half fetches
+      // This half's columns of the queries: LANES neighbouring lanes fetch a row's 16-byte chunks, so a warp's request covers whole lines.
+      constexpr int LANES = HD / 16, AT_ONCE = 32 / LANES;       // lanes to a row, rows to a request
       const int qi = r / G, qh = r - qi * G;
-      uint4 qv[QC];
-      auto ask_q = [&](const GroupPiece& pc) {
+      uint4 qv[LANES];
+      auto ask_q = [&](const GroupPiece& pc) {      // (a row of the tile without a query gets some other: nothing comes of it)
         const int row = qi < pc.rows ? p.members[pc.first + qi] : -1;
-        const bool held = row >= 0 && row < p.rows;
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (held ? row : 0) * p.q_stride + (pc.kvh * G + qh) * HD + w * (HD / 2));
+        const long long mine = row >= 0 && row < p.rows ? row * p.q_stride + (pc.kvh * G + qh) * HD : -1;
 #pragma unroll
-        for (int c = 0; c < QC; ++c) qv[c] = held ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        for (int x = 0; x < LANES; ++x) {
+          const long long at = __shfl_sync(0xffffffffu, mine, x * AT_ONCE + lane / LANES);
+          qv[x] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (at < 0 ? 0 : at) + w * (HD / 2) + lane % LANES * 8);
+        }
       };
       auto store_q = [&] {
+        const int col = w * LANES + lane % LANES;       // 16-byte chunk of a query's row
 #pragma unroll
-        for (int c = 0; c < QC; ++c) {
-          const int col = w * QC + c;       // 16-byte chunk of the query's row
-          *reinterpret_cast<uint4*>(smem + L::OFF_Q + (col / 8) * BOX_BYTES + r * 128 + (((col % 8) ^ (r & 7)) << 4)) = qv[c];
+        for (int x = 0; x < LANES; ++x) {
+          const int to = (warp & 3) * 32 + x * AT_ONCE + lane / LANES;
+          *reinterpret_cast<uint4*>(smem + L::OFF_Q + (col / 8) * BOX_BYTES + to * 128 + (((col % 8) ^ (to & 7)) << 4)) = qv[x];
         }
         fence_async_smem();
         mbar_arrive(q_full);
