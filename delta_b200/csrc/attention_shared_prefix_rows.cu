@@ -1,15 +1,15 @@
 // Attention over shared prefixes, bfloat16: the keys that each row holds alone, and the merge with the pieces that the
 // kernel of the groups (attention_shared_prefix_tc.cu) leaves.
 //
-// A row's G <= 16 query heads of one key-value head are the rows of a warp-level MMA tile; the kernel is bound by the bytes of
+// A row's G <= 16 query heads of one key-value head are the columns of warp-level MMA tiles; the kernel is bound by the bytes of
 // K and V, which nobody shares, so the legacy MMA is enough.  Two blocks run on an SM and take pieces in turn; their tiles of 64 keys flow
 // through a ring without a stop between pieces:
 //
 //   warp 4     fetches by TMA: a tile's K and V (one box per 64 columns where its pages follow one another in the pool, else a
 //              box per page; pages behind the last key are left out), and with a segment's first tile its queries
-//   warps 0-3  S = Q K^T for 16 keys each, the maximum over the tile through shared memory, P in bfloat16 through shared
-//              memory, O += P V for a quarter of the columns each.  So all warps share one maximum, and nothing has to be merged
-//              between them at a segment's end.
+//   warps 0-3  16 keys of a tile each, as S^T = K Q^T and O^T += V^T P^T: the queries are the eight columns of an MMA, so that none of it is
+//              spent on empty rows (an MMA takes a warp some 35 cycles here, which was most of the time with queries as its 16 rows).  Each
+//              warp has a maximum of its own; they are merged at a piece's end.
 //
 // Behind a piece's last tile the pieces of its row's group are added to it, in the order of their keys: they come through the ring as well, up to eight
 // a stage, one box each.  (Of a segment that is cut, only the first piece adds them.)  The result is rounded once.  Where a segment is cut, each block
@@ -27,7 +27,7 @@ constexpr int TILE = 64;           // keys of a tile
 constexpr int QR = 128;            // queries of a group's piece
 constexpr int LISTED = 32;         // pieces whose records lie in shared memory at once
 constexpr int MERGED = 8;          // pieces of a group in a stage, at most
-constexpr int ROWS = 16;           // rows of the MMA tile
+constexpr int ROWS = 16;           // queries of a piece, at most
 constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
 
 // One block of five stages an SM where two of three do not fit (heads of 128 with more than 8 to a key-value head).
@@ -42,18 +42,11 @@ struct Ring {
   static constexpr int TOTAL = STAGES * STAGE + 1024;                // 1024 to start on a swizzle boundary
 };
 
-// LOW: at most 8 query heads; rows 8..15 of the MMA tile are then empty and their accumulators two registers that stay zero.
-template <bool LOW>
-__device__ __forceinline__ void mma_rows(float* c, float (&zero)[2], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (LOW) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(zero[0]), "+f"(zero[1])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
+// The 8 x 8 matrix of 16-bit entries that lies over the warp as a fragment, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  return d;
 }
 // Byte offset of 16-byte chunk ``chunk`` of key ``key`` in a K or V tile: 64 columns side by side, rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_offset(int key, int chunk) {
@@ -79,15 +72,14 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
                                                                                   const __grid_constant__ CUtensorMap map_merge,
                                                                                   const DkSharedPrefixParams p) {
   using R = Ring<HD, LOW>;
-  constexpr int NR = LOW ? 1 : 2;             // rows of the tile a thread keeps (g, and g + 8)
-  constexpr int KB = HD / 16;                 // k-blocks of Q K^T
-  constexpr int NT = HD / WARPS / 8;          // n-tiles of P V of a warp
+  constexpr int NQ = LOW ? 1 : 2, ROWS_USED = 8 * NQ;      // tiles of eight queries
+  constexpr int KB = HD / 16, MT = HD / 16;   // blocks of 16 columns: the depth of K Q^T, the rows of V^T P^T
+  constexpr int LANES = HD / 4, PASSES = ROWS_USED * LANES / (WARPS * 32);      // threads to a query at the end, queries of each
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) unsigned long long bars[2 * R::STAGES];   // full, then empty
   __shared__ RowPiece list[LISTED];
-  __shared__ __align__(16) unsigned char s_p[ROWS * TILE * 2];      // weights [row][key], 16-byte chunks exchanged by the row
-  __shared__ float s_max[WARPS][ROWS], s_sum[WARPS][ROWS];
+  __shared__ float s_max[2][WARPS][ROWS], s_sum[2][WARPS][ROWS];      // in turns for the pieces
   __shared__ int s_last;
   __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
@@ -189,221 +181,219 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
     } else {
       // ---------------------------------------------------------------- the four warps
       int n = n_tile;
-      bool bad = false;
+      bool bad = false, dead = false;         // bad: some warp of these gave up a wait; dead: this one did
       for (int i = 0; i < n_pieces && !bad; ++i) {
         const RowPiece w = list[i];
-        uint32_t qa[KB][4];
-        float o[NT][2 * NR], zero[2] = {0.f, 0.f}, m_run[NR], l_run[NR];
+        // S^T = K Q^T and O^T += V^T P^T: the queries are the eight columns of an MMA, a warp's 16 keys its rows and then its depth.  A thread has
+        // queries 2 tq and 2 tq + 1 (and 8 more behind them).
+        uint32_t qb[KB][NQ][2];
+        float o[MT][NQ][4], m_run[NQ][2], l_run[NQ][2];
 #pragma unroll
-        for (int k = 0; k < NT; ++k)
+        for (int x = 0; x < NQ; ++x) {
 #pragma unroll
-          for (int c = 0; c < 2 * NR; ++c) o[k][c] = 0.f;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          m_run[r] = -INFINITY;
-          l_run[r] = 0.f;
+          for (int k = 0; k < MT; ++k) o[k][x][0] = o[k][x][1] = o[k][x][2] = o[k][x][3] = 0.f;
+          m_run[x][0] = m_run[x][1] = -INFINITY;
+          l_run[x][0] = l_run[x][1] = 0.f;
         }
-        int kb = w.key0;
-        do {
-          const int s = ring_slot(n, R::STAGES);
-          if (!wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
-          const uint32_t k_tile = ring + s * R::STAGE, v_tile = k_tile + R::KV_BYTES;
-          const int keys = min(TILE, w.limit - kb);
-          if (kb == w.key0 && keys > 0) {
-            // (rows from G on hold whatever lay there: a row of the products depends on its own queries alone)
-            const uint32_t q = v_tile + R::KV_BYTES;
-            if (LOW) {
-#pragma unroll
-              for (int k = 0; k < KB; k += 2) {
-                ldmatrix_x4(qa[k][0], qa[k][2], qa[k + 1][0], qa[k + 1][2], q + (lane & 7) * (HD * 2) + (2 * k + (lane >> 3)) * 16);
-                qa[k][1] = qa[k][3] = qa[k + 1][1] = qa[k + 1][3] = 0u;
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < KB; ++k)
-                ldmatrix_x4(qa[k][0], qa[k][1], qa[k][2], qa[k][3], q + ((lane & 7) + ((lane >> 3) & 1) * 8) * (HD * 2) + (2 * k + (lane >> 4)) * 16);
-            }
+        int kb = w.key0, s;
+        for (;;) {
+          s = ring_slot(n, R::STAGES);
+          if (!dead && !wait(full + 8 * s, ring_parity(n, R::STAGES))) {
+            dead = true;
+            stuck = 1;
           }
-          // fragments first, then four chains of products: even and odd k-blocks of two groups of eight keys
-          float sc[2][2 * NR], odd[2][2 * NR], mx[NR];
-          uint32_t kf[2][KB / 2][4];
+          const uint32_t k_tile = ring + s * R::STAGE, v_tile = k_tile + R::KV_BYTES;
+          const int keys = min(16, w.limit - kb - warp * 16);      // of this warp
+          if (kb == w.key0) {
+            // (rows from G on hold whatever lay there: a query's scores depend on nobody else's)
+            const uint32_t q = v_tile + R::KV_BYTES;
 #pragma unroll
-          for (int k = 0; k < KB / 2; ++k)
+            for (int k = 0; k < KB; k += 2)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              ldmatrix_x4(kf[j][k][0], kf[j][k][1], kf[j][k][2], kf[j][k][3], k_tile + tile_offset(warp * 16 + j * 8 + (lane & 7), 4 * k + (lane >> 3)));
+              for (int x = 0; x < NQ; ++x)
+                ldmatrix_x4(qb[k][x][0], qb[k][x][1], qb[k + 1][x][0], qb[k + 1][x][1], q + (x * 8 + (lane & 7)) * (HD * 2) + (2 * k + (lane >> 3)) * 16);
+          }
+          if (keys > 0) {
+            uint32_t a[KB][4];
+            const int row = warp * 16 + (lane & 7);
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+            for (int k = 0; k < KB; ++k) ldmatrix_x4(a[k][0], a[k][1], a[k][2], a[k][3], k_tile + tile_offset(row + ((lane >> 3) & 1) * 8, 2 * k + (lane >> 4)));
+            float sc[NQ][4], odd[NQ][4];      // two chains of products: even and odd k-blocks
 #pragma unroll
-            for (int c = 0; c < 2 * NR; ++c) sc[j][c] = odd[j][c] = 0.f;
+            for (int x = 0; x < NQ; ++x)
 #pragma unroll
-          for (int k = 0; k < KB / 2; ++k)
+              for (int c = 0; c < 4; ++c) sc[x][c] = odd[x][c] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              mma_rows<LOW>(sc[j], zero, qa[2 * k], kf[j][k][0], kf[j][k][1]);
-              mma_rows<LOW>(odd[j], zero, qa[2 * k + 1], kf[j][k][2], kf[j][k][3]);
+            for (int k = 0; k < KB; k += 2)
+#pragma unroll
+              for (int x = 0; x < NQ; ++x) {
+                mma_bf16(sc[x], a[k], qb[k][x][0], qb[k][x][1]);
+                mma_bf16(odd[x], a[k + 1], qb[k + 1][x][0], qb[k + 1][x][1]);
+              }
+            // V's fragments are asked for before the softmax, into the registers of K's: keys are the depth now
+            uint32_t v[MT][4];
+#pragma unroll
+            for (int k = 0; k < MT; ++k)
+              ldmatrix_x4_trans(v[k][0], v[k][1], v[k][2], v[k][3], v_tile + tile_offset(row + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)));
+            if (keys < 16) {
+              // what lies behind the last key may be anything, and 0 times infinity is no zero
+              const uint32_t low = (2 * tq < keys ? 0xffffu : 0u) | (2 * tq + 1 < keys ? 0xffff0000u : 0u);
+              const uint32_t high = (2 * tq + 8 < keys ? 0xffffu : 0u) | (2 * tq + 9 < keys ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int k = 0; k < MT; ++k) {
+                v[k][0] &= low;
+                v[k][1] &= low;
+                v[k][2] &= high;
+                v[k][3] &= high;
+              }
             }
+            uint32_t pb[NQ][2];
+            bool moved = false;
+            float keep[NQ][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+            for (int x = 0; x < NQ; ++x) {
 #pragma unroll
-            for (int c = 0; c < 2 * NR; ++c) sc[j][c] += odd[j][c];
-          // V's fragments are asked for before the softmax
-          uint32_t vf[TILE / 16][NT / 2][4];
-#pragma unroll
-          for (int kk = 0; kk < TILE / 16; ++kk)
-#pragma unroll
-            for (int k = 0; k < NT / 2; ++k)
-              ldmatrix_x4_trans(vf[kk][k][0], vf[kk][k][1], vf[kk][k][2], vf[kk][k][3],
-                                v_tile + tile_offset(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, warp * NT + 2 * k + (lane >> 4)));
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            mx[r] = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
+              for (int c = 0; c < 4; ++c) sc[x][c] = g + (c >> 1) * 8 < keys ? (sc[x][c] + odd[x][c]) * sl2 : -INFINITY;
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float& v = sc[j][2 * r + c];
-                v = warp * 16 + j * 8 + 2 * tq + c < keys ? v * sl2 : -INFINITY;
-                mx[r] = fmaxf(mx[r], v);
+                float mx = fmaxf(sc[x][c], sc[x][c + 2]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                const float m_new = fmaxf(m_run[x][c], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+                keep[x][c] = fast_exp2(m_run[x][c] - m_use);       // 0 before the first key
+                moved |= m_new != m_run[x][c];
+                m_run[x][c] = m_new;
+                sc[x][c] = fast_exp2(sc[x][c] - m_use);
+                sc[x][c + 2] = fast_exp2(sc[x][c + 2] - m_use);
+                l_run[x][c] = l_run[x][c] * keep[x][c] + (sc[x][c] + sc[x][c + 2]);        // the sum in 32 bits; the weights are rounded to bfloat16 for the product
               }
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            if (tq == 0) s_max[warp][g + 8 * r] = mx[r];
-          }
-          warps_barrier();
-          // written by these warps only, before this barrier or behind the next one: the same for all four
-          bad = stuck != 0;
-          if (bad) break;
-          float keep[NR];
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const int row = g + 8 * r;
-            const float m_new = fmaxf(fmaxf(m_run[r], fmaxf(s_max[0][row], s_max[1][row])), fmaxf(s_max[2][row], s_max[3][row]));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            keep[r] = fast_exp2(m_run[r] - m_use);       // 0 before the first key
-            m_run[r] = m_new;
-            l_run[r] *= keep[r];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float p0 = fast_exp2(sc[j][2 * r] - m_use), p1 = fast_exp2(sc[j][2 * r + 1] - m_use);
-              l_run[r] += p0 + p1;        // the sum in 32 bits; the weights are rounded to bfloat16 for the product
-              const int key = warp * 16 + j * 8 + 2 * tq;
-              *reinterpret_cast<uint32_t*>(s_p + row * (TILE * 2) + (((key >> 3) ^ (row & 7)) << 4) + (key & 7) * 2) = pack_bf16(p0, p1);
+              pb[x][0] = transposed(pack_bf16(sc[x][0], sc[x][1]));
+              pb[x][1] = transposed(pack_bf16(sc[x][2], sc[x][3]));
             }
-          }
-          warps_barrier();
+            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-          for (int k = 0; k < NT; ++k)
+              for (int k = 0; k < MT; ++k)
 #pragma unroll
-            for (int c = 0; c < 2 * NR; ++c) o[k][c] *= keep[c >> 1];
-          uint32_t a[TILE / 16][4];
+                for (int x = 0; x < NQ; ++x)
 #pragma unroll
-          for (int kk = 0; kk < TILE / 16; ++kk) {
-            const int arow = (lane & 7) + ((lane >> 3) & 1) * 8;      // rows 0-7, 8-15 of keys 0-7, then of keys 8-15
-            ldmatrix_x4(a[kk][0], a[kk][1], a[kk][2], a[kk][3], s2u(s_p) + arow * (TILE * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4));
-            if (LOW) a[kk][1] = a[kk][3] = 0u;
-          }
-          if (keys < TILE) {
-            // what lies behind the last key may be anything, and 0 times infinity is no zero
-#pragma unroll
-            for (int kk = 0; kk < TILE / 16; ++kk) {
-              const int k0 = kk * 16 + 2 * tq;
-              const uint32_t low = (k0 < keys ? 0xffffu : 0u) | (k0 + 1 < keys ? 0xffff0000u : 0u);
-              const uint32_t high = (k0 + 8 < keys ? 0xffffu : 0u) | (k0 + 9 < keys ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int k = 0; k < NT / 2; ++k) {
-                vf[kk][k][0] &= low;
-                vf[kk][k][1] &= high;
-                vf[kk][k][2] &= low;
-                vf[kk][k][3] &= high;
-              }
+                  for (int c = 0; c < 4; ++c) o[k][x][c] *= keep[x][c & 1];
             }
+#pragma unroll
+            for (int k = 0; k < MT; ++k)
+#pragma unroll
+              for (int x = 0; x < NQ; ++x) mma_bf16(o[k][x], v[k], pb[x][0], pb[x][1]);
           }
-#pragma unroll
-          for (int kk = 0; kk < TILE / 16; ++kk)
-#pragma unroll
-            for (int k = 0; k < NT / 2; ++k) {
-              mma_rows<LOW>(o[2 * k], zero, a[kk], vf[kk][k][0], vf[kk][k][1]);
-              mma_rows<LOW>(o[2 * k + 1], zero, a[kk], vf[kk][k][2], vf[kk][k][3]);
-            }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(empty + 8 * s);
           ++n;
           kb += TILE;
-        } while (kb < w.limit);
-        if (bad) break;
-        // ---- the segment's end: sums over the warps, then the merge
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-          l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-          if (tq == 0) s_sum[warp][g + 8 * r] = l_run[r];
+          if (kb >= w.limit) break;       // (the last tile's stage is kept for what follows)
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * s);
         }
+        // ---- the segment's end: the four warps' results added in the last tile's stage, under their common maximum
+        float(*maxima)[ROWS] = s_max[i & 1], (*sums)[ROWS] = s_sum[i & 1];
+#pragma unroll
+        for (int x = 0; x < NQ; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l_run[x][c] += __shfl_xor_sync(0xffffffffu, l_run[x][c], d);
+            if (g == 0) {
+              maxima[warp][x * 8 + 2 * tq + c] = m_run[x][c];
+              sums[warp][x * 8 + 2 * tq + c] = l_run[x][c];
+            }
+          }
         warps_barrier();
+        bad = stuck != 0;       // set before this barrier or behind the next one: the same for all four warps
+        if (bad) break;
+        float* scratch = reinterpret_cast<float*>(smem + s * R::STAGE);       // [warp][query][HD + 4]
 #pragma unroll
-        for (int r = 0; r < NR; ++r) l_run[r] = (s_sum[0][g + 8 * r] + s_sum[1][g + 8 * r]) + (s_sum[2][g + 8 * r] + s_sum[3][g + 8 * r]);
-        // {maximum, sum, outputs} of a piece added to this thread's queries
-        auto add = [&](int r, float m, float l, const float (&v)[2 * NT]) {
-          const float m_new = fmaxf(m_run[r], m), m_use = m_new == -INFINITY ? 0.f : m_new;
-          const float have = fast_exp2(m_run[r] - m_use), f = fast_exp2(m - m_use);
-          m_run[r] = m_new;
-          l_run[r] = l_run[r] * have + l * f;
+        for (int x = 0; x < NQ; ++x)
 #pragma unroll
-          for (int k = 0; k < 2 * NT; ++k) o[k / 2][2 * r + k % 2] = o[k / 2][2 * r + k % 2] * have + v[k] * f;
+          for (int c = 0; c < 2; ++c) {
+            const int q = x * 8 + 2 * tq + c;
+            const float M = fmaxf(fmaxf(maxima[0][q], maxima[1][q]), fmaxf(maxima[2][q], maxima[3][q]));
+            const float f = M == -INFINITY ? 0.f : fast_exp2(m_run[x][c] - M);
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+              scratch[(warp * ROWS_USED + q) * (HD + 4) + k * 16 + g] = o[k][x][c] * f;
+              scratch[(warp * ROWS_USED + q) * (HD + 4) + k * 16 + g + 8] = o[k][x][c + 2] * f;
+            }
+          }
+        warps_barrier();
+        // from here on a thread has four columns of PASSES queries
+        const int col = tid % LANES * 4, q0 = tid / LANES;
+        float M[PASSES], L[PASSES];
+        float4 acc[PASSES];
+#pragma unroll
+        for (int j = 0; j < PASSES; ++j) {
+          const int q = q0 + j * (WARPS * 32 / LANES);
+          M[j] = fmaxf(fmaxf(maxima[0][q], maxima[1][q]), fmaxf(maxima[2][q], maxima[3][q]));
+          L[j] = 0.f;
+          acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int y = 0; y < WARPS; ++y) {
+            const float4 v = *reinterpret_cast<const float4*>(scratch + (y * ROWS_USED + q) * (HD + 4) + col);
+            acc[j] = make_float4(acc[j].x + v.x, acc[j].y + v.y, acc[j].z + v.z, acc[j].w + v.w);
+            L[j] += M[j] == -INFINITY ? 0.f : sums[y][q] * fast_exp2(maxima[y][q] - M[j]);
+          }
+        }
+        fence_async_smem();       // the stage is TMA's again
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * s);
+        // ``count`` pieces added to a query's state, under their common maximum: piece y has {maximum, sum} at ml(y) and this thread's columns at at(y)
+        auto add = [&](int j, int count, auto ml, auto at) {
+          float m[MERGED], m_new = M[j];
+#pragma unroll
+          for (int y = 0; y < MERGED; ++y) {
+            m[y] = y < count ? ml(y).x : -INFINITY;
+            m_new = fmaxf(m_new, m[y]);
+          }
+          const float m_use = m_new == -INFINITY ? 0.f : m_new, have = fast_exp2(M[j] - m_use);
+          M[j] = m_new;
+          L[j] *= have;
+          acc[j] = make_float4(acc[j].x * have, acc[j].y * have, acc[j].z * have, acc[j].w * have);
+#pragma unroll
+          for (int y = 0; y < MERGED; ++y)
+            if (y < count) {
+              const float f = fast_exp2(m[y] - m_use);
+              const float4 v = at(y);
+              L[j] = fmaf(f, ml(y).y, L[j]);
+              acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z), fmaf(f, v.w, acc[j].w));
+            }
         };
         if (w.index == 0)
           for (int x = 0; x < w.group_n; x += per_stage, ++n) {
-            const int s = ring_slot(n, R::STAGES), m = min(per_stage, w.group_n - x);
-            if (!wait(full + 8 * s, ring_parity(n, R::STAGES))) stuck = 1;
-            // the stage's pieces at once: their common maximum first, so that nothing but the sums is done one after the other
+            s = ring_slot(n, R::STAGES);
+            if (!dead && !wait(full + 8 * s, ring_parity(n, R::STAGES))) {
+              dead = true;
+              stuck = 1;
+            }
             const unsigned char* part = smem + s * R::STAGE;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              const int qh = g + 8 * r;
-              if (qh >= G) continue;
-              float f[MERGED], m_new = m_run[r];
-#pragma unroll
-              for (int y = 0; y < MERGED; ++y) {
-                f[y] = y < m ? *reinterpret_cast<const float*>(part + y * slot_bytes + (HD / 4 * G + qh) * 16) : -INFINITY;
-                m_new = fmaxf(m_new, f[y]);
-              }
-              const float m_use = m_new == -INFINITY ? 0.f : m_new, have = fast_exp2(m_run[r] - m_use);
-              m_run[r] = m_new;
-              l_run[r] *= have;
-#pragma unroll
-              for (int k = 0; k < 2 * NT; ++k) o[k / 2][2 * r + k % 2] *= have;
-#pragma unroll
-              for (int y = 0; y < MERGED; ++y)
-                if (y < m) {
-                  const unsigned char* from = part + y * slot_bytes;
-                  const float w_y = fast_exp2(f[y] - m_use);
-                  l_run[r] += w_y * *reinterpret_cast<const float*>(from + (HD / 4 * G + qh) * 16 + 4);
-#pragma unroll
-                  for (int k = 0; k < NT; ++k) {
-                    const float2 v = *reinterpret_cast<const float2*>(from + (((warp * NT + k) * 2 + tq / 2) * G + qh) * 16 + (tq & 1) * 8);
-                    o[k][2 * r] = fmaf(w_y, v.x, o[k][2 * r]);
-                    o[k][2 * r + 1] = fmaf(w_y, v.y, o[k][2 * r + 1]);
-                  }
-                }
+            for (int j = 0; j < PASSES; ++j) {
+              const int q = q0 + j * (WARPS * 32 / LANES);
+              if (q < G)
+                add(j, min(per_stage, w.group_n - x), [&](int y) { return *reinterpret_cast<const float2*>(part + y * slot_bytes + (HD / 4 * G + q) * 16); },
+                    [&](int y) { return *reinterpret_cast<const float4*>(part + y * slot_bytes + (col / 4 * G + q) * 16); });
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + 8 * s);
           }
         bool finish = true;
         if (w.pieces > 1) {
-          if (!waited) {          // the counters were cleared by the kernel of the groups
+          if (!waited) {          // the last call's pieces are nobody's any more
             asm volatile("griddepcontrol.wait;\n" ::: "memory");
             waited = true;
           }
           float* part = row_results(p, w.first_id + w.index);
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (g + 8 * r < G) {
-#pragma unroll
-              for (int k = 0; k < NT; ++k)
-                *reinterpret_cast<float2*>(part + (size_t)(g + 8 * r) * HD + (warp * NT + k) * 8 + 2 * tq) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
-              if (warp == 0 && tq == 0) *reinterpret_cast<float2*>(part + (size_t)G * HD + 2 * (g + 8 * r)) = make_float2(m_run[r], l_run[r]);
+          for (int j = 0; j < PASSES; ++j) {
+            const int q = q0 + j * (WARPS * 32 / LANES);
+            if (q < G) {
+              *reinterpret_cast<float4*>(part + (size_t)q * HD + col) = acc[j];
+              if (col == 0) *reinterpret_cast<float2*>(part + (size_t)G * HD + 2 * q) = make_float2(M[j], L[j]);
             }
+          }
           __threadfence();
           warps_barrier();
           if (tid == 0) s_last = atomicAdd(&counters(p)[w.row * p.KV + w.kvh], 1) == w.pieces - 1;
@@ -411,48 +401,31 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
           finish = s_last != 0;
           if (finish) {
             __threadfence();
-            constexpr int AT_ONCE = 4;        // pieces asked for together, added in order
             const long long rs = row_piece_floats(G, HD);
-            const float* rp = row_results(p, w.first_id);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              m_run[r] = -INFINITY;
-              l_run[r] = 0.f;
-#pragma unroll
-              for (int k = 0; k < NT; ++k) o[k][2 * r] = o[k][2 * r + 1] = 0.f;
-              if (g + 8 * r >= G) continue;
-              for (int x = 0; x < w.pieces; x += AT_ONCE) {
-                float2 ml[AT_ONCE];
-                float v[AT_ONCE][2 * NT];
-#pragma unroll
-                for (int y = 0; y < AT_ONCE; ++y)
-                  if (x + y < w.pieces) {
-                    const float* from = rp + (x + y) * rs;
-                    ml[y] = __ldcg(reinterpret_cast<const float2*>(from + (size_t)G * HD + 2 * (g + 8 * r)));
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) {
-                      const float2 f = __ldcg(reinterpret_cast<const float2*>(from + (size_t)(g + 8 * r) * HD + (warp * NT + k) * 8 + 2 * tq));
-                      v[y][2 * k] = f.x;
-                      v[y][2 * k + 1] = f.y;
-                    }
-                  }
-#pragma unroll
-                for (int y = 0; y < AT_ONCE; ++y)
-                  if (x + y < w.pieces) add(r, ml[y].x, ml[y].y, v[y]);
-              }
+            for (int j = 0; j < PASSES; ++j) {
+              const int q = q0 + j * (WARPS * 32 / LANES);
+              M[j] = -INFINITY;
+              L[j] = 0.f;
+              acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (q < G)
+                for (int x = 0; x < w.pieces; x += MERGED) {
+                  const float* from = row_results(p, w.first_id + x);
+                  add(j, min(MERGED, w.pieces - x), [&](int y) { return __ldcg(reinterpret_cast<const float2*>(from + y * rs + (size_t)G * HD + 2 * q)); },
+                      [&](int y) { return __ldcg(reinterpret_cast<const float4*>(from + y * rs + (size_t)q * HD + col)); });
+                }
             }
           }
         }
         if (finish) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (g + 8 * r < G) {
-              const float inv = l_run[r] > 0.f ? 1.f / l_run[r] : (l_run[r] == 0.f ? 0.f : l_run[r]);      // no key: zeros; a NaN stays one
-              __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + g + 8 * r) * HD;
-#pragma unroll
-              for (int k = 0; k < NT; ++k)
-                *reinterpret_cast<__nv_bfloat162*>(out + (warp * NT + k) * 8 + 2 * tq) = __floats2bfloat162_rn(o[k][2 * r] * inv, o[k][2 * r + 1] * inv);
-            }
+          for (int j = 0; j < PASSES; ++j) {
+            const int q = q0 + j * (WARPS * 32 / LANES);
+            const float inv = L[j] > 0.f ? 1.f / L[j] : (L[j] == 0.f ? 0.f : L[j]);      // no key: zeros; a NaN stays one
+            if (q < G)
+              *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + q) * HD + col) =
+                  make_uint2(pack_bf16(acc[j].x * inv, acc[j].y * inv), pack_bf16(acc[j].z * inv, acc[j].w * inv));
+          }
         }
       }
       n_tile = n;
