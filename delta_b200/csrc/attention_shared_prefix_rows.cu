@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   using R = Ring<HD, LOW>;
   constexpr int NQ = LOW ? 1 : 2, ROWS_USED = 8 * NQ;      // tiles of eight queries
   constexpr int KB = HD / 16, MT = HD / 16;   // blocks of 16 columns: the depth of K Q^T, the rows of V^T P^T
-  constexpr int LANES = HD / 4, PASSES = ROWS_USED * LANES / (WARPS * 32);      // threads to a query at the end, queries of each
+  constexpr int STEP = WARPS * 32 / ROWS_USED, PASSES = HD / 4 / STEP;      // at a piece's end: threads to a query, groups of four columns of each
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) unsigned long long bars[2 * R::STAGES];   // full, then empty
@@ -320,45 +320,49 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             }
           }
         warps_barrier();
-        // from here on a thread has four columns of PASSES queries
-        const int col = tid % LANES * 4, q0 = tid / LANES;
-        float M[PASSES], L[PASSES];
+        // from here on a thread has one query and PASSES times four columns (neighbouring threads have neighbouring queries, as the pieces lie)
+        const int q = tid % ROWS_USED, c4 = tid / ROWS_USED;
+        float M = fmaxf(fmaxf(maxima[0][q], maxima[1][q]), fmaxf(maxima[2][q], maxima[3][q])), L = 0.f;
         float4 acc[PASSES];
 #pragma unroll
-        for (int j = 0; j < PASSES; ++j) {
-          const int q = q0 + j * (WARPS * 32 / LANES);
-          M[j] = fmaxf(fmaxf(maxima[0][q], maxima[1][q]), fmaxf(maxima[2][q], maxima[3][q]));
-          L[j] = 0.f;
-          acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < PASSES; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int y = 0; y < WARPS; ++y) {
-            const float4 v = *reinterpret_cast<const float4*>(scratch + (y * ROWS_USED + q) * (HD + 4) + col);
+        for (int y = 0; y < WARPS; ++y) {
+          L += M == -INFINITY ? 0.f : sums[y][q] * fast_exp2(maxima[y][q] - M);
+#pragma unroll
+          for (int j = 0; j < PASSES; ++j) {
+            const float4 v = *reinterpret_cast<const float4*>(scratch + (y * ROWS_USED + q) * (HD + 4) + (c4 + j * STEP) * 4);
             acc[j] = make_float4(acc[j].x + v.x, acc[j].y + v.y, acc[j].z + v.z, acc[j].w + v.w);
-            L[j] += M[j] == -INFINITY ? 0.f : sums[y][q] * fast_exp2(maxima[y][q] - M[j]);
           }
         }
         fence_async_smem();       // the stage is TMA's again
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + 8 * s);
-        // ``count`` pieces added to a query's state, under their common maximum: piece y has {maximum, sum} at ml(y) and this thread's columns at at(y)
-        auto add = [&](int j, int count, auto ml, auto at) {
-          float m[MERGED], m_new = M[j];
+        // ``count`` pieces added, under their common maximum: piece y has {maximum, sum} at ml(y) and four columns at at(y, c)
+        auto add = [&](int count, auto ml, auto at) {
+          float2 m[MERGED];
+          float m_new = M;
 #pragma unroll
           for (int y = 0; y < MERGED; ++y) {
-            m[y] = y < count ? ml(y).x : -INFINITY;
-            m_new = fmaxf(m_new, m[y]);
+            m[y] = make_float2(-INFINITY, 0.f);
+            if (y < count) m[y] = ml(y);
+            m_new = fmaxf(m_new, m[y].x);
           }
-          const float m_use = m_new == -INFINITY ? 0.f : m_new, have = fast_exp2(M[j] - m_use);
-          M[j] = m_new;
-          L[j] *= have;
-          acc[j] = make_float4(acc[j].x * have, acc[j].y * have, acc[j].z * have, acc[j].w * have);
+          const float m_use = m_new == -INFINITY ? 0.f : m_new, have = fast_exp2(M - m_use);
+          M = m_new;
+          L *= have;
+#pragma unroll
+          for (int j = 0; j < PASSES; ++j) acc[j] = make_float4(acc[j].x * have, acc[j].y * have, acc[j].z * have, acc[j].w * have);
 #pragma unroll
           for (int y = 0; y < MERGED; ++y)
             if (y < count) {
-              const float f = fast_exp2(m[y] - m_use);
-              const float4 v = at(y);
-              L[j] = fmaf(f, ml(y).y, L[j]);
-              acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z), fmaf(f, v.w, acc[j].w));
+              const float f = fast_exp2(m[y].x - m_use);
+              L = fmaf(f, m[y].y, L);
+#pragma unroll
+              for (int j = 0; j < PASSES; ++j) {
+                const float4 v = at(y, c4 + j * STEP);
+                acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z), fmaf(f, v.w, acc[j].w));
+              }
             }
         };
         if (w.index == 0)
@@ -368,14 +372,10 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
               dead = true;
               stuck = 1;
             }
-            const unsigned char* part = smem + s * R::STAGE;
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) {
-              const int q = q0 + j * (WARPS * 32 / LANES);
-              if (q < G)
-                add(j, min(per_stage, w.group_n - x), [&](int y) { return *reinterpret_cast<const float2*>(part + y * slot_bytes + (HD / 4 * G + q) * 16); },
-                    [&](int y) { return *reinterpret_cast<const float4*>(part + y * slot_bytes + (col / 4 * G + q) * 16); });
-            }
+            const unsigned char* part = smem + s * R::STAGE + q * 16;
+            if (q < G)
+              add(min(per_stage, w.group_n - x), [&](int y) { return *reinterpret_cast<const float2*>(part + y * slot_bytes + HD / 4 * G * 16); },
+                  [&](int y, int c) { return *reinterpret_cast<const float4*>(part + y * slot_bytes + c * G * 16); });
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + 8 * s);
           }
@@ -385,47 +385,35 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
             asm volatile("griddepcontrol.wait;\n" ::: "memory");
             waited = true;
           }
-          float* part = row_results(p, w.first_id + w.index);
+          if (q < G) {
+            float* part = row_results(p, w.first_id + w.index);
 #pragma unroll
-          for (int j = 0; j < PASSES; ++j) {
-            const int q = q0 + j * (WARPS * 32 / LANES);
-            if (q < G) {
-              *reinterpret_cast<float4*>(part + (size_t)q * HD + col) = acc[j];
-              if (col == 0) *reinterpret_cast<float2*>(part + (size_t)G * HD + 2 * q) = make_float2(M[j], L[j]);
-            }
+            for (int j = 0; j < PASSES; ++j) *reinterpret_cast<float4*>(part + (size_t)q * HD + (c4 + j * STEP) * 4) = acc[j];
+            if (c4 == 0) *reinterpret_cast<float2*>(part + (size_t)G * HD + 2 * q) = make_float2(M, L);
           }
           __threadfence();
           warps_barrier();
           if (tid == 0) s_last = atomicAdd(&counters(p)[w.row * p.KV + w.kvh], 1) == w.pieces - 1;
           warps_barrier();
           finish = s_last != 0;
-          if (finish) {
+          if (finish && q < G) {
             __threadfence();
             const long long rs = row_piece_floats(G, HD);
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) {
-              const int q = q0 + j * (WARPS * 32 / LANES);
-              M[j] = -INFINITY;
-              L[j] = 0.f;
-              acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (q < G)
-                for (int x = 0; x < w.pieces; x += MERGED) {
-                  const float* from = row_results(p, w.first_id + x);
-                  add(j, min(MERGED, w.pieces - x), [&](int y) { return __ldcg(reinterpret_cast<const float2*>(from + y * rs + (size_t)G * HD + 2 * q)); },
-                      [&](int y) { return __ldcg(reinterpret_cast<const float4*>(from + y * rs + (size_t)q * HD + col)); });
-                }
+            M = -INFINITY;
+            L = 0.f;
+            for (int x = 0; x < w.pieces; x += MERGED) {
+              const float* from = row_results(p, w.first_id + x);
+              add(min(MERGED, w.pieces - x), [&](int y) { return __ldcg(reinterpret_cast<const float2*>(from + y * rs + (size_t)G * HD + 2 * q)); },
+                  [&](int y, int c) { return __ldcg(reinterpret_cast<const float4*>(from + y * rs + (size_t)q * HD + c * 4)); });
             }
           }
         }
-        if (finish) {
+        if (finish && q < G) {
+          const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
+          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + q) * HD;
 #pragma unroll
-          for (int j = 0; j < PASSES; ++j) {
-            const int q = q0 + j * (WARPS * 32 / LANES);
-            const float inv = L[j] > 0.f ? 1.f / L[j] : (L[j] == 0.f ? 0.f : L[j]);      // no key: zeros; a NaN stays one
-            if (q < G)
-              *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + w.row * p.out_stride + (w.kvh * G + q) * HD + col) =
-                  make_uint2(pack_bf16(acc[j].x * inv, acc[j].y * inv), pack_bf16(acc[j].z * inv, acc[j].w * inv));
-          }
+          for (int j = 0; j < PASSES; ++j)
+            *reinterpret_cast<uint2*>(out + (c4 + j * STEP) * 4) = make_uint2(pack_bf16(acc[j].x * inv, acc[j].y * inv), pack_bf16(acc[j].z * inv, acc[j].w * inv));
         }
       }
       n_tile = n;
