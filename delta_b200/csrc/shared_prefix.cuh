@@ -75,7 +75,8 @@ static inline Bounds bounds(DkSharedPrefixParams& p) {
   const int G = p.G = p.H / p.KV, rpt = p.rpt = p.qr / G;
   const long long keys = (long long)p.max_pages * p.ps, segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
   const long long of_groups = segments * ((keys + p.kt - 1) / p.kt), capped = (of_groups + CAP - 1) / CAP;
-  const long long group_pieces = segments > 0 ? segments + (capped > p.grid ? capped : (long long)p.grid) : 0;
+  const long long ranges = capped > p.grid ? capped : (of_groups < p.grid ? of_groups : (long long)p.grid);      // (no range is empty)
+  const long long group_pieces = segments > 0 ? segments + ranges : 0;
   const long long row_pieces = (long long)p.rows * p.KV + p.rows_grid;      // a segment's last piece, and tiles / C of full ones, which are no more than blocks
   b.tiles = of_groups + (long long)p.rows * p.KV * ((keys + p.rows_kt - 1) / p.rows_kt);
   b.pieces = group_pieces + row_pieces;

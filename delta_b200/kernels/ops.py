@@ -8,9 +8,9 @@ the CPU and no library model code is called.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from typing import Optional
 
-import numpy as np
 import torch
 
 from . import lib as _l
@@ -1424,13 +1424,26 @@ def _on_this_device(what: str, *tensors) -> None:
             raise KernelError(f"{what}: a tensor is on '{t.device}' and the current device is cuda:{_device_index()}")
 
 
-def _head_rows(t: torch.Tensor, name: str, rows: int, H: int, hd: int, dtype):
+def _table(what: str, t: torch.Tensor, name: str, dtype, device: int) -> int:
+    """The address of a dense tensor of this type on the current device (one test where nothing is wrong)."""
+    if not (t.is_cuda and t.dtype is dtype and t.is_contiguous() and t.get_device() == device):
+        _ptr(t, name, dtype)
+        _on_this_device(what, t)
+    return t.data_ptr()
+
+
+def _head_rows(what: str, t: torch.Tensor, name: str, shape, dtype, device: int):
     """Address and row stride of [rows, H, hd] whose rows may lie apart."""
-    if not t.is_cuda:
-        raise KernelError(f"{name} is on '{t.device}': the kernels run on CUDA tensors only and there is no CPU path")
-    if tuple(t.shape) != (rows, H, hd) or t.dtype != dtype:
+    rows, H, hd = shape
+    if not (t.is_cuda and t.get_device() == device):
+        if not t.is_cuda:
+            raise KernelError(f"{name} is on '{t.device}': the kernels run on CUDA tensors only and there is no CPU path")
+        _on_this_device(what, t)
+    if t.shape != shape or t.dtype is not dtype:
         raise KernelError(f"{name} has shape {tuple(t.shape)} / {t.dtype}, expected [{rows}, {H}, {hd}] of {dtype}")
-    if rows and (t.stride(2) != 1 or (H > 1 and t.stride(1) != hd) or (rows > 1 and t.stride(0) < H * hd)):
+    if t.is_contiguous():
+        return t.data_ptr(), H * hd
+    if t.stride(2) != 1 or (H > 1 and t.stride(1) != hd) or (rows > 1 and t.stride(0) < H * hd):
         raise KernelError(f"{name}: a row's heads must lie one behind the other, the strides are {t.stride()}")
     return t.data_ptr(), t.stride(0) if rows > 1 else H * hd
 
@@ -1464,61 +1477,77 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
     Rows of ``q`` and ``out`` may lie apart.  Two products with float sums, the softmax in 32 bits; bfloat16 rounds the weights of the values once
     and the result once.  ``work``: at least ``attention_shared_prefix_floats`` float32 that no other call uses meanwhile (allocated here when None).
     """
-    i32 = torch.int32
-    if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or block_table.dim() != 2:
-        raise KernelError(f"attention_shared_prefix: q, pages and table have shapes {tuple(q.shape)}, {tuple(kv.shape)}, {tuple(block_table.shape)}")
-    (rows, H, hd), KV, ps = q.shape, kv.shape[2], kv.shape[3]
+    what, i32, shape, pages, table, dtype = "attention_shared_prefix", torch.int32, q.shape, kv.shape, block_table.shape, q.dtype
+    if len(pages) != 5 or pages[1] != 2 or len(shape) != 3 or len(table) != 2:
+        raise KernelError(f"attention_shared_prefix: q, pages and table have shapes {tuple(shape)}, {tuple(pages)}, {tuple(table)}")
+    (rows, H, hd), (num_pages, _, KV, ps, width), (table_rows, max_pages) = shape, pages, table
     groups, n = group_prefix.numel(), members.numel()
-    if kv.shape[4] != hd or kv.dtype != q.dtype or block_table.shape[0] != rows or kv_len.numel() != rows or group_start.numel() != groups + 1:
-        raise KernelError(f"attention_shared_prefix: {rows} rows of heads of {hd} ({q.dtype}) do not fit pages {tuple(kv.shape)} of {kv.dtype}, a table of "
-                          f"{block_table.shape[0]} rows, {kv_len.numel()} lengths, {groups} prefixes and {group_start.numel()} starts of groups")
-    _on_this_device("attention_shared_prefix", q, out, kv, block_table, kv_len, members, group_start, group_prefix, err, work)
-    qp, qs = _head_rows(q, "q", rows, H, hd, q.dtype)
-    op, os_ = _head_rows(out, "out", rows, H, hd, q.dtype)
-    need = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, block_table.shape[1], kv.shape[0], q.dtype)
+    if width != hd or kv.dtype is not dtype or table_rows != rows or kv_len.numel() != rows or group_start.numel() != groups + 1:
+        raise KernelError(f"attention_shared_prefix: {rows} rows of heads of {hd} ({dtype}) do not fit pages {tuple(pages)} of {kv.dtype}, a table of "
+                          f"{table_rows} rows, {kv_len.numel()} lengths, {groups} prefixes and {group_start.numel()} starts of groups")
+    device = _device_index() if q.is_cuda else -1
+    qp, q_stride = _head_rows(what, q, "q", shape, dtype, device)
+    op, out_stride = _head_rows(what, out, "out", shape, dtype, device)
+    kvp = _table(what, kv, "kv", dtype, device)
+    bp = _table(what, block_table, "block_table", i32, device)
+    lp = _table(what, kv_len, "kv_len", i32, device)
+    mp = _table(what, members, "members", i32, device)
+    sp = _table(what, group_start, "group_start", i32, device)
+    pp = _table(what, group_prefix, "group_prefix", i32, device)
+    ep = _table(what, err, "err", i32, device) if err is not None else None
     if work is None:
-        work = torch.empty(need, dtype=torch.float32, device=q.device)
-    _l.check(_l.load().dk_attention_shared_prefix(
-        qp, qs, op, os_, _ptr(kv, "kv"), _ptr(block_table, "block_table", i32), _ptr(kv_len, "kv_len", i32), _ptr(members, "members", i32),
-        _ptr(group_start, "group_start", i32), _ptr(group_prefix, "group_prefix", i32), _ptr(work, "work", torch.float32), work.numel(), rows, groups, n,
-        H, KV, hd, ps, block_table.shape[1], kv.shape[0], float(scale), dtype_code(q.dtype), _ptr(err, "err", i32), _stream()),
-        "attention_shared_prefix", 2 if rows else 0)
+        floats = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, max_pages, num_pages, dtype)
+        work = torch.empty(floats, dtype=torch.float32, device=q.device)
+    else:
+        floats = work.numel()
+    wp = _table(what, work, "work", torch.float32, device)
+    _l.check(_l.load().dk_attention_shared_prefix(qp, q_stride, op, out_stride, kvp, bp, lp, mp, sp, pp, wp, floats, rows, groups, n, H, KV, hd, ps,
+                                                  max_pages, num_pages, scale, dtype_code(dtype), ep, _stream()), what, 2 if rows else 0)
     return out
 
 
-def _host_ints(v, name: str) -> np.ndarray:
+def _host_ints(v, name: str) -> array:
     if isinstance(v, torch.Tensor):
         if v.is_cuda:
             raise KernelError(f"{name} is on '{v.device}': which items are copied is said on the host")
-        v = v.numpy()
-    a = np.asarray(v)
-    if a.size and (a.dtype.kind not in "iu" or a.ndim != 1 or a.min() < -(1 << 31) or a.max() >= 1 << 31):
-        raise KernelError(f"{name} must be a list of whole numbers, not {a.dtype} of shape {a.shape}")
-    return np.ascontiguousarray(a, dtype=np.int32)
+        v = v.tolist()
+    try:
+        return array("i", v)
+    except (TypeError, OverflowError) as e:
+        raise KernelError(f"{name} must be a list of whole numbers of 32 bits: {e}") from None
 
 
-def _copy_items(what: str, records, device, src, dst, tokens, n_items: int) -> None:
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _copy_items(what: str, records, n_tensors: int, device, src, dst, tokens, n_items: int) -> None:
+    """records: five 64-bit numbers for each tensor, as ``DkCopyTensor`` in csrc/copy_items.cu has them."""
     lib = _l.load()
     src, dst = _host_ints(src, "src"), _host_ints(dst, "dst")
-    tokens = _host_ints(tokens, "tokens") if tokens is not None else None
-    n = src.size
-    if dst.size != n or (tokens is not None and tokens.size != n):
-        raise KernelError(f"{what}: {n} sources, {dst.size} targets" + (f", {tokens.size} counts of tokens" if tokens is not None else ""))
+    n, counts = len(src), None
+    if tokens is not None:
+        tokens = _host_ints(tokens, "tokens")
+        counts = _address(tokens)
+    if len(dst) != n or (tokens is not None and len(tokens) != n):
+        raise KernelError(f"{what}: {n} sources, {len(dst)} targets" + (f", {len(tokens)} counts of tokens" if tokens is not None else ""))
     if n == 0:
         return
-    table = np.array(records, dtype=np.int64)
-    addresses = (src.ctypes.data, dst.ctypes.data, tokens.ctypes.data if tokens is not None else None)
-    if n <= lib.dk_copy_items_inline():
-        _l.check(lib.dk_copy_items(table.ctypes.data, len(records), *addresses, n, n_items, None, None, 0, _stream()), what)
+    table = array("q", records)
+    if n <= _COPIES_INLINE:
+        _l.check(lib.dk_copy_items(_address(table), n_tensors, _address(src), _address(dst), counts, n, n_items, None, None, 0, _stream()), what)
         return
     if torch.cuda.is_current_stream_capturing():
-        raise KernelError(f"{what}: {n} copies go through a list that is made on the host; a captured call takes at most {lib.dk_copy_items_inline()}")
-    order = np.empty(5 * n + 2, dtype=np.int32)
-    lanes = lib.dk_copy_items_order(table.ctypes.data, len(records), *addresses, n, n_items, order.ctypes.data, order.ctypes.data + 16 * n)
+        raise KernelError(f"{what}: {n} copies go through a list that is made on the host; a captured call takes at most {_COPIES_INLINE}")
+    order = torch.empty(5 * n + 2, dtype=torch.int32)
+    lanes = lib.dk_copy_items_order(_address(table), n_tensors, _address(src), _address(dst), counts, n, n_items, order.data_ptr(), order.data_ptr() + 16 * n)
     _l.check(min(lanes, 0), what, 0)
     if lanes > 0:
-        held = torch.from_numpy(order).to(device)
-        _l.check(lib.dk_copy_items(table.ctypes.data, len(records), None, None, None, n, n_items, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what)
+        held = order.to(device)
+        _l.check(lib.dk_copy_items(_address(table), n_tensors, None, None, None, n, n_items, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what)
+
+
+_COPIES_INLINE = 96      # copies that travel in a launch's arguments (csrc/copy_items.cu)
 
 
 def _two_ints(lo: int, hi: int) -> int:
@@ -1530,42 +1559,39 @@ def copy_pages(pages, src, dst, *, tokens=None, token_axis=None):
     may be read by several copies and may be the source of one and the target of another, so a cache can be permuted in place.  No page is the
     target of two.  ``tokens[i]``: only the first so many tokens of the page are copied and the others of the target stay; ``token_axis`` says
     which axis of the layout counts a page's tokens.  Sources, targets and counts are host lists.  One launch."""
-    if pages.dim() < 3:
-        raise KernelError(f"copy_pages: pages have shape {tuple(pages.shape)}, expected [layers, pages, *layout]")
-    _ptr(pages, "pages")
-    _on_this_device("copy_pages", pages)
-    layers, n, layout, size = pages.shape[0], pages.shape[1], pages.shape[2:], pages.element_size()
-    if pages.numel() == 0:
-        raise KernelError(f"copy_pages: there is nothing to copy in pages of shape {tuple(pages.shape)}")
-    item = pages[0, 0].numel() * size
+    shape, size = pages.shape, pages.element_size()
+    if len(shape) < 3:
+        raise KernelError(f"copy_pages: pages have shape {tuple(shape)}, expected [layers, pages, *layout]")
+    at = _table("copy_pages", pages, "pages", pages.dtype, _device_index() if pages.is_cuda else -1)
+    layers, n, total = shape[0], shape[1], pages.numel()
+    if total == 0:
+        raise KernelError(f"copy_pages: there is nothing to copy in pages of shape {tuple(shape)}")
+    item = total // (layers * n) * size
     if item >= 1 << 31:
         raise KernelError(f"copy_pages: a page of {item} bytes is too large")
     token_bytes = per_page = 0
     if tokens is not None:
-        if token_axis is None or not 0 <= token_axis < len(layout):
-            raise KernelError(f"copy_pages: counts of tokens need the token axis of the layout {tuple(layout)}, got {token_axis}")
-        per_page = layout[token_axis]
-        token_bytes = size
-        for d in layout[token_axis + 1:]:
-            token_bytes *= d
-    _copy_items("copy_pages", [[pages.data_ptr(), item, item * n, _two_ints(layers, item), _two_ints(token_bytes, per_page)]], pages.device, src, dst, tokens, n)
+        if token_axis is None or not 0 <= token_axis < len(shape) - 2:
+            raise KernelError(f"copy_pages: counts of tokens need the token axis of the layout {tuple(shape[2:])}, got {token_axis}")
+        per_page, token_bytes = shape[2 + token_axis], pages.stride(2 + token_axis) * size
+    _copy_items("copy_pages", (at, item, item * n, _two_ints(layers, item), _two_ints(token_bytes, per_page)), 1, pages.device, src, dst, tokens, n)
 
 
 def copy_slots(states, src, dst):
     """Copies slot ``src[i]`` to slot ``dst[i]`` of every tensor [slots, ...] in ``states``, as if all were read before any is written.  Slots are
     host lists; no slot is the target of two.  One launch for up to 32 tensors."""
     states = list(states.values()) if isinstance(states, dict) else list(states)
-    records, slots = [], None
+    records, slots, device = [], states[0].shape[0] if states and states[0].dim() else 0, _device_index() if states and states[0].is_cuda else -1
     for s in states:
-        _ptr(s, "a state")
-        _on_this_device("copy_slots", s)
-        if s.dim() < 1 or (slots is not None and s.shape[0] != slots):
+        at = _table("copy_slots", s, "a state", s.dtype, device)
+        if s.dim() < 1 or s.shape[0] != slots:
             raise KernelError(f"copy_slots: states have shapes {[tuple(x.shape) for x in states]}; all need the same number of slots")
-        slots = s.shape[0]
-        item = s.numel() // max(1, slots) * s.element_size()
-        if item >= 1 << 31:
-            raise KernelError(f"copy_slots: a slot of {item} bytes is too large")
-        if item:
-            records.append([s.data_ptr(), item, 0, _two_ints(1, item), 0])
-    for i in range(0, len(records), 32):
-        _copy_items("copy_slots", records[i:i + 32], states[0].device, src, dst, None, slots)
+        total = s.numel()
+        if total:
+            item = total // slots * s.element_size()
+            if item >= 1 << 31:
+                raise KernelError(f"copy_slots: a slot of {item} bytes is too large")
+            records += (at, item, 0, 1 | item << 32, 0)
+    for i in range(0, len(records), 160):      # 32 tensors a launch
+        part = records[i:i + 160]
+        _copy_items("copy_slots", part, len(part) // 5, states[0].device, src, dst, None, slots)

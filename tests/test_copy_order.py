@@ -63,6 +63,11 @@ def test_refused():
         order([0], [1], 4, tokens=[17], whole=16)
 
 
+def test_a_launch_takes_as_many_copies_as_its_caller_says():
+    assert lib.load().dk_copy_items_inline() == ops._COPIES_INLINE
+    assert lib.load().dk_sizeof_copy_tensor() == 5 * 8
+
+
 def test_no_cpu_path():
     with pytest.raises(KernelError, match="no CPU path"):
         ops.copy_pages(torch.zeros(1, 4, 8), [0], [1])
