@@ -32,7 +32,7 @@ constexpr int SAVE = 1, TAKE = 2;          // keep the target's old unit; write 
 struct Tensor {
   char* base;
   long long item_stride, layer_stride;
-  int layers, units, unit, first_block;
+  int layers, units, unit, first_block, layer_blocks;
   int units_per_token, tokens;             // 0: whole items
 };
 struct Args {
@@ -46,15 +46,14 @@ struct Args {
 
 template <typename U>
 __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int begin, int end) {
-  const long long at = ((long long)blockIdx.x - t.first_block) * THREADS + threadIdx.x;
-  if (at >= (long long)t.layers * t.units) return;
-  const int layer = (int)(at / t.units), unit = (int)(at - (long long)layer * t.units);
+  const int block = (int)blockIdx.x - t.first_block, layer = block / t.layer_blocks, unit = (block - layer * t.layer_blocks) * (int)blockDim.x + (int)threadIdx.x;
+  if (unit >= t.units) return;
   char* place = t.base + layer * t.layer_stride + (long long)unit * sizeof(U);
   const int token = t.units_per_token > 0 ? unit / t.units_per_token % t.tokens : 0;
   U kept = U();
   for (int i = begin; i < end; i += AHEAD) {
     U v[AHEAD];
-    int to[AHEAD];
+    int to[AHEAD], from = -1;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       to[j] = -1;
@@ -63,8 +62,13 @@ __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int beg
         if (c.w & SAVE) kept = *reinterpret_cast<const U*>(place + c.y * t.item_stride);
         if (token < c.z) {
           to[j] = c.y;
+          // (a fork's copies have one source: it is read once)
           if (c.w & TAKE) v[j] = kept;
+          else if (j > 0 && c.x == from) v[j] = v[j > 0 ? j - 1 : 0];
           else v[j] = *reinterpret_cast<const U*>(place + c.x * t.item_stride);
+          from = c.w & TAKE ? -1 : c.x;
+        } else {
+          from = -1;
         }
       }
     }
@@ -161,10 +165,10 @@ int order_copies(const int* src, const int* dst, const int* tokens, int n, long 
   return left;
 }
 
-// Fills a.t; returns the blocks that one lane takes, or a negative code.
-int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a) {
+// Fills a.t; returns the blocks that one lane takes, or a negative code.  ``threads``: of a block.
+int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a, int& threads) {
   DK_REQUIRE(n_tensors >= 1 && n_tensors <= MAX_TENSORS, "copy_items: %d tensors; 1 to %d are taken in one call", n_tensors, MAX_TENSORS);
-  long long blocks = 0;
+  int most = 1;
   for (int k = 0; k < n_tensors; ++k) {
     const DkCopyTensor& x = tensors[k];
     DK_REQUIRE(x.base != nullptr && x.layers >= 0 && x.item_bytes >= 0 && x.token_bytes >= 0 && x.tokens >= 0, "copy_items: tensor %d is missing or has a negative size", k);
@@ -180,18 +184,27 @@ int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a) {
     t.units = x.item_bytes / unit;
     t.units_per_token = x.token_bytes / unit;
     t.tokens = x.tokens > 0 ? x.tokens : 1;
+    if (t.units > most) most = t.units;
+  }
+  threads = std::min(THREADS, (most + 31) / 32 * 32);
+  long long blocks = 0;
+  for (int k = 0; k < n_tensors; ++k) {
+    Tensor& t = a.t[k];
     t.first_block = (int)blocks;
-    blocks += ((long long)t.layers * t.units + THREADS - 1) / THREADS;
+    t.layer_blocks = std::max(1, (t.units + threads - 1) / threads);
+    blocks += (long long)t.layers * t.layer_blocks;
     DK_REQUIRE(blocks < (1ll << 31) - 1, "copy_items: items of too many bytes");
   }
   a.n_tensors = n_tensors;
   return (int)blocks;
 }
 
+// As many lanes as leave AHEAD copies to each, while there are fewer than LEVEL blocks for an SM: then the last round of blocks, which does not fill the
+// device, costs little (16 layers, 1,100 pages of 32 KB: 4.1 rounds of long blocks 223 us).
 int lanes_for(int blocks, int n) {
-  // four rounds of eight blocks an SM: enough to fill the device and to level the ends
-  const long long want = blocks > 0 ? (32ll * dk_sm_count() + blocks - 1) / blocks : 1;
-  return (int)std::max(1ll, std::min({want, (long long)std::max(1, n), 65535ll}));
+  constexpr int LEVEL = 128;
+  const long long want = blocks > 0 ? ((long long)LEVEL * dk_sm_count() + blocks - 1) / blocks : 1;
+  return (int)std::max(1ll, std::min({want, (long long)(n + AHEAD - 1) / AHEAD, 65535ll}));
 }
 }  // namespace
 
@@ -202,7 +215,8 @@ extern "C" int dk_copy_items_inline() { return INLINE; }
 extern "C" int dk_copy_items_order(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, int* list, int* starts) {
   try {
     Args a = {};
-    const int blocks = lay_out(tensors, n_tensors, a);
+    int threads = THREADS;
+    const int blocks = lay_out(tensors, n_tensors, a, threads);
     if (blocks < 0) return blocks;
     int lanes = 0;
     const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), reinterpret_cast<int4*>(list), starts, &lanes);
@@ -218,7 +232,8 @@ extern "C" int dk_copy_items(const DkCopyTensor* tensors, int n_tensors, const i
                              const int* list, const int* starts, int lanes, cudaStream_t stream) {
   try {
     Args a = {};
-    const int blocks = lay_out(tensors, n_tensors, a);
+    int threads = THREADS;
+    const int blocks = lay_out(tensors, n_tensors, a, threads);
     if (blocks < 0) return blocks;
     if (list == nullptr) {
       DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
@@ -232,7 +247,7 @@ extern "C" int dk_copy_items(const DkCopyTensor* tensors, int n_tensors, const i
     }
     a.lanes = lanes;
     if (blocks == 0 || lanes <= 0) return 0;
-    copy_items_kernel<<<dim3(blocks, lanes), THREADS, 0, stream>>>(a);
+    copy_items_kernel<<<dim3(blocks, lanes), threads, 0, stream>>>(a);
     return dk_check_launch("copy_items");
   } catch (const std::bad_alloc&) {
     dk_set_error("copy_items: no memory on the host to order %d copies", n);
