@@ -6,10 +6,12 @@
 //
 // A thread owns one unit (16 bytes where sizes and addresses allow it) at one place of an item and carries it through the
 // whole list: units at different places never meet, so nothing has to be synchronised however the copies depend on
-// one another.  It reads eight copies ahead before it writes, which the order allows (a reader stands before the writer or
-// beside it).  Components that do not depend on one another are dealt to lanes (blockIdx.y), as many as fill the device.
-// The kernel is bound by the bytes it moves; a short list travels in the kernel's arguments, so a fork is one launch and no
-// copy from the host.
+// one another.  Components that do not depend on one another are dealt to lanes (blockIdx.y).  The list travels in the kernel's arguments up to
+// 1,500 copies, so there is one launch and no copy from the host.
+//
+// Bound by the bytes it moves.  With the device full of blocks a thread reads one copy at a time (16 layers, 1,100 pages of 32 KB: 179 us = 6.4 TB/s;
+// two reads ahead 192, four 208, eight 235); a few long chains leave it nearly empty, and then four reads stand in front of four writes, which the
+// order allows: a reader stands before its writer or beside it.
 #include "common.cuh"
 #include <algorithm>
 #include <new>
@@ -24,9 +26,9 @@ struct DkCopyTensor {
 
 namespace {
 constexpr int THREADS = 256;
-constexpr int AHEAD = 8;
 constexpr int MAX_TENSORS = 32;
-constexpr int INLINE = 96;                 // copies that travel in the kernel's arguments
+constexpr int FEW = 96, INLINE = 1500;     // copies that travel in the arguments of the two kernels
+constexpr int FULL = 8;                    // blocks for an SM from which on threads need not read ahead
 constexpr int SAVE = 1, TAKE = 2;          // keep the target's old unit; write the kept unit
 
 struct Tensor {
@@ -35,16 +37,18 @@ struct Tensor {
   int layers, units, unit, first_block, layer_blocks;
   int units_per_token, tokens;             // 0: whole items
 };
+template <int N>
 struct Args {
   Tensor t[MAX_TENSORS];
   int n_tensors, lanes;
   const int4* list;                        // {source, target, tokens, flags}; null: in ``copies``
   const int* starts;                       // [lanes + 1]
-  int4 copies[INLINE];
-  short inline_starts[INLINE + 2];
+  int4 copies[N];
+  short inline_starts[N + 2];
 };
+static_assert(sizeof(Args<FEW>) <= 4096 && sizeof(Args<INLINE>) <= 32764, "a kernel's arguments");
 
-template <typename U>
+template <int AHEAD, typename U>
 __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int begin, int end) {
   const int block = (int)blockIdx.x - t.first_block, layer = block / t.layer_blocks, unit = (block - layer * t.layer_blocks) * (int)blockDim.x + (int)threadIdx.x;
   if (unit >= t.units) return;
@@ -53,7 +57,7 @@ __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int beg
   U kept = U();
   for (int i = begin; i < end; i += AHEAD) {
     U v[AHEAD];
-    int to[AHEAD], from = -1;
+    int to[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       to[j] = -1;
@@ -62,13 +66,8 @@ __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int beg
         if (c.w & SAVE) kept = *reinterpret_cast<const U*>(place + c.y * t.item_stride);
         if (token < c.z) {
           to[j] = c.y;
-          // (a fork's copies have one source: it is read once)
           if (c.w & TAKE) v[j] = kept;
-          else if (j > 0 && c.x == from) v[j] = v[j > 0 ? j - 1 : 0];
           else v[j] = *reinterpret_cast<const U*>(place + c.x * t.item_stride);
-          from = c.w & TAKE ? -1 : c.x;
-        } else {
-          from = -1;
         }
       }
     }
@@ -78,7 +77,8 @@ __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int beg
   }
 }
 
-__global__ void __launch_bounds__(THREADS) copy_items_kernel(const __grid_constant__ Args a) {
+template <int N, int AHEAD>
+__global__ void __launch_bounds__(THREADS) copy_items_kernel(const __grid_constant__ Args<N> a) {
   int k = 0;
   while (k + 1 < a.n_tensors && (int)blockIdx.x >= a.t[k + 1].first_block) ++k;
   const Tensor& t = a.t[k];
@@ -86,11 +86,11 @@ __global__ void __launch_bounds__(THREADS) copy_items_kernel(const __grid_consta
   const int begin = a.list ? a.starts[blockIdx.y] : a.inline_starts[blockIdx.y];
   const int end = a.list ? a.starts[blockIdx.y + 1] : a.inline_starts[blockIdx.y + 1];
   switch (t.unit) {
-    case 16: carry<uint4>(t, list, begin, end); break;
-    case 8: carry<uint2>(t, list, begin, end); break;
-    case 4: carry<uint32_t>(t, list, begin, end); break;
-    case 2: carry<unsigned short>(t, list, begin, end); break;
-    default: carry<unsigned char>(t, list, begin, end); break;
+    case 16: carry<AHEAD, uint4>(t, list, begin, end); break;
+    case 8: carry<AHEAD, uint2>(t, list, begin, end); break;
+    case 4: carry<AHEAD, uint32_t>(t, list, begin, end); break;
+    case 2: carry<AHEAD, unsigned short>(t, list, begin, end); break;
+    default: carry<AHEAD, unsigned char>(t, list, begin, end); break;
   }
 }
 
@@ -98,16 +98,28 @@ __global__ void __launch_bounds__(THREADS) copy_items_kernel(const __grid_consta
 // left (a copy of an item to itself is none), or a negative code.
 int order_copies(const int* src, const int* dst, const int* tokens, int n, long long n_items, int whole, int want_lanes, int4* list, int* starts, int* lanes) {
   DK_REQUIRE(n >= 0, "copy_items: a negative number of copies");
-  std::vector<int> by_target;
-  by_target.reserve(n);
   for (int i = 0; i < n; ++i) {
     DK_REQUIRE(src[i] >= 0 && src[i] < n_items && dst[i] >= 0 && dst[i] < n_items, "copy_items: copy %d goes from item %d to item %d of %lld", i, src[i], dst[i], n_items);
     DK_REQUIRE(tokens == nullptr || (tokens[i] >= 0 && tokens[i] <= whole), "copy_items: copy %d asks for %d tokens of an item of %d", i, tokens ? tokens[i] : 0, whole);
-    by_target.push_back(i);
   }
-  std::sort(by_target.begin(), by_target.end(), [&](int a, int b) { return dst[a] < dst[b]; });
-  for (int i = 1; i < n; ++i)
-    DK_REQUIRE(dst[by_target[i]] != dst[by_target[i - 1]], "copy_items: item %d is written twice", dst[by_target[i]]);
+  // which copy writes an item: a table of the items, or, where there are far more items than copies, the copies sorted by their targets
+  const bool direct = n_items <= 64ll * n;
+  std::vector<int> by_target(direct ? (size_t)n_items : (size_t)n, -1);
+  if (direct) {
+    for (int i = 0; i < n; ++i) {
+      DK_REQUIRE(by_target[dst[i]] < 0, "copy_items: item %d is written twice", dst[i]);
+      by_target[dst[i]] = i;
+    }
+  } else {
+    for (int i = 0; i < n; ++i) by_target[i] = i;
+    std::sort(by_target.begin(), by_target.end(), [&](int a, int b) { return dst[a] < dst[b]; });
+    for (int i = 1; i < n; ++i) DK_REQUIRE(dst[by_target[i]] != dst[by_target[i - 1]], "copy_items: item %d is written twice", dst[by_target[i]]);
+  }
+  auto writer = [&](int item) {
+    if (direct) return by_target[item];
+    const auto it = std::lower_bound(by_target.begin(), by_target.end(), item, [&](int a, int v) { return dst[a] < v; });
+    return it == by_target.end() || dst[*it] != item ? -1 : *it;
+  };
   // next[i]: the copy that writes what copy i reads
   std::vector<int> next(n, -1), readers(n, 0), root(n);
   auto find = [&](int i) {
@@ -118,11 +130,11 @@ int order_copies(const int* src, const int* dst, const int* tokens, int n, long 
   auto moot = [&](int i) { return src[i] == dst[i] || (tokens != nullptr && tokens[i] == 0); };
   for (int i = 0; i < n; ++i) {
     if (moot(i)) continue;
-    const auto it = std::lower_bound(by_target.begin(), by_target.end(), src[i], [&](int a, int v) { return dst[a] < v; });
-    if (it == by_target.end() || dst[*it] != src[i] || moot(*it)) continue;
-    next[i] = *it;
-    ++readers[*it];
-    root[find(i)] = find(*it);
+    const int j = writer(src[i]);
+    if (j < 0 || moot(j)) continue;
+    next[i] = j;
+    ++readers[j];
+    root[find(i)] = find(j);
   }
   std::vector<int> order, flags(n, 0);
   order.reserve(n);
@@ -166,7 +178,8 @@ int order_copies(const int* src, const int* dst, const int* tokens, int n, long 
 }
 
 // Fills a.t; returns the blocks that one lane takes, or a negative code.  ``threads``: of a block.
-int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a, int& threads) {
+template <int N>
+int lay_out(const DkCopyTensor* tensors, int n_tensors, Args<N>& a, int& threads) {
   DK_REQUIRE(n_tensors >= 1 && n_tensors <= MAX_TENSORS, "copy_items: %d tensors; 1 to %d are taken in one call", n_tensors, MAX_TENSORS);
   int most = 1;
   for (int k = 0; k < n_tensors; ++k) {
@@ -199,26 +212,47 @@ int lay_out(const DkCopyTensor* tensors, int n_tensors, Args& a, int& threads) {
   return (int)blocks;
 }
 
-// As many lanes as leave AHEAD copies to each, while there are fewer than LEVEL blocks for an SM: then the last round of blocks, which does not fill the
-// device, costs little (16 layers, 1,100 pages of 32 KB: 4.1 rounds of long blocks 223 us).
+// As many lanes as leave eight copies to each (a fork's one source is then read for every eighth target only: 63 targets, one and eight to a lane, 18.3 and
+// 11.2 us), while there are fewer than LEVEL blocks for an SM, which is enough to level the ends.
 int lanes_for(int blocks, int n) {
-  constexpr int LEVEL = 128;
+  constexpr int LEVEL = 64, EACH = 8;
   const long long want = blocks > 0 ? ((long long)LEVEL * dk_sm_count() + blocks - 1) / blocks : 1;
-  return (int)std::max(1ll, std::min({want, (long long)(n + AHEAD - 1) / AHEAD, 65535ll}));
+  return (int)std::max(1ll, std::min({want, (long long)(n + EACH - 1) / EACH, 65535ll}));
+}
+
+template <int N>
+int launch(const Args<N>& a, int blocks, int lanes, int threads, cudaStream_t stream) {
+  if (blocks == 0 || lanes <= 0) return 0;
+  const dim3 grid(blocks, lanes);
+  if ((long long)blocks * lanes >= (long long)FULL * dk_sm_count()) copy_items_kernel<N, 1><<<grid, threads, 0, stream>>>(a);
+  else copy_items_kernel<N, 4><<<grid, threads, 0, stream>>>(a);
+  return dk_check_launch("copy_items");
+}
+
+template <int N>
+int copy_inline(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, cudaStream_t stream) {
+  Args<N> a = {};
+  int threads = THREADS, lanes = 0;
+  const int blocks = lay_out(tensors, n_tensors, a, threads);
+  if (blocks < 0) return blocks;
+  int s[N + 2];
+  const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), a.copies, s, &lanes);
+  if (rc < 0) return rc;
+  for (int i = 0; i <= lanes; ++i) a.inline_starts[i] = (short)s[i];
+  return launch(a, blocks, lanes, threads, stream);
 }
 }  // namespace
 
 extern "C" int dk_sizeof_copy_tensor() { return (int)sizeof(DkCopyTensor); }
 extern "C" int dk_copy_items_inline() { return INLINE; }
 
-// Puts n copies in order for a list on the device: list [n][4] ints and starts [n + 1].  Returns the number of lanes (0: nothing to copy) or a negative code.
+// Puts n copies in order for a list on the device: list [n][4] ints and starts [n + 2].  Returns the number of lanes (0: nothing to copy) or a negative code.
 extern "C" int dk_copy_items_order(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, int* list, int* starts) {
   try {
-    Args a = {};
-    int threads = THREADS;
+    Args<1> a = {};
+    int threads = THREADS, lanes = 0;
     const int blocks = lay_out(tensors, n_tensors, a, threads);
     if (blocks < 0) return blocks;
-    int lanes = 0;
     const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), reinterpret_cast<int4*>(list), starts, &lanes);
     return rc < 0 ? rc : lanes;
   } catch (const std::bad_alloc&) {
@@ -231,24 +265,18 @@ extern "C" int dk_copy_items_order(const DkCopyTensor* tensors, int n_tensors, c
 extern "C" int dk_copy_items(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items,
                              const int* list, const int* starts, int lanes, cudaStream_t stream) {
   try {
-    Args a = {};
+    if (list == nullptr) {
+      DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
+      return n <= FEW ? copy_inline<FEW>(tensors, n_tensors, src, dst, tokens, n, n_items, stream)
+                      : copy_inline<INLINE>(tensors, n_tensors, src, dst, tokens, n, n_items, stream);
+    }
+    Args<1> a = {};
     int threads = THREADS;
     const int blocks = lay_out(tensors, n_tensors, a, threads);
     if (blocks < 0) return blocks;
-    if (list == nullptr) {
-      DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
-      int s[INLINE + 2];
-      const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), a.copies, s, &lanes);
-      if (rc < 0) return rc;
-      for (int i = 0; i <= lanes; ++i) a.inline_starts[i] = (short)s[i];
-    } else {
-      a.list = reinterpret_cast<const int4*>(list);
-      a.starts = starts;
-    }
-    a.lanes = lanes;
-    if (blocks == 0 || lanes <= 0) return 0;
-    copy_items_kernel<<<dim3(blocks, lanes), threads, 0, stream>>>(a);
-    return dk_check_launch("copy_items");
+    a.list = reinterpret_cast<const int4*>(list);
+    a.starts = starts;
+    return launch(a, blocks, lanes, threads, stream);
   } catch (const std::bad_alloc&) {
     dk_set_error("copy_items: no memory on the host to order %d copies", n);
     return DK_ERR_ARG;

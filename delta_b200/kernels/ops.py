@@ -1547,7 +1547,7 @@ def _copy_items(what: str, records, n_tensors: int, device, src, dst, tokens, n_
         _l.check(lib.dk_copy_items(_address(table), n_tensors, None, None, None, n, n_items, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what)
 
 
-_COPIES_INLINE = 96      # copies that travel in a launch's arguments (csrc/copy_items.cu)
+_COPIES_INLINE = 1500    # copies that travel in a launch's arguments (csrc/copy_items.cu)
 
 
 def _two_ints(lo: int, hi: int) -> int:

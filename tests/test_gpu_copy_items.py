@@ -30,7 +30,7 @@ KINDS = ["apart", "one to many", "cycle", "chain", "swaps", "nothing moves", "an
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("pages", [2, 9, 60, 400])
+@pytest.mark.parametrize("pages", [2, 9, 60, 400, 2000])
 @pytest.mark.parametrize("layout", [(2, 4, 16, 128), (16, 36), (3, 5), (1,)], ids=str)
 def test_pages(kind, pages, layout):
     from delta_b200.kernels import ops
@@ -104,10 +104,10 @@ def test_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(x, want)
-    big = torch.zeros(1, 400, 16, device="cuda")
+    big = torch.zeros(1, 4000, 16, device="cuda")
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         with pytest.raises(KernelError, match="captured"):
-            ops.copy_pages(big, list(range(200)), list(range(200, 400)))
+            ops.copy_pages(big, list(range(2000)), list(range(2000, 4000)))
         big.zero_()
 
 
