@@ -10,10 +10,10 @@
 //   m = max_i m_i,   out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i      (maxima in units of log2).
 //
 // This file holds the merge and the kernel on the FMA units: 32-bit keys and values, and every head size and page
-// size that the kernel on the tensor cores (attention_shared_prefix_tc.cu) does not take.  A block of 256 threads
-// keeps 32 queries; eight threads share a query.  K and V tiles of 64 keys lie in shared memory as floats, rows of K
-// four floats apart from a multiple of 32 so that eight threads read eight rows without bank conflicts.
-// It is bound by the FMA units and the shared-memory reads that feed them (nine 16-byte reads for 32 FMAs).
+// size that the kernels on the tensor cores (attention_shared_prefix_tc.cu, attention_shared_prefix_rows.cu) do not take.  A block of 128 threads
+// keeps 32 queries; K and then V of a tile of 64 keys lie in one buffer in shared memory as floats, so that three blocks fit on an SM and one loads
+// while others compute.  A thread has four queries and four keys of the scores (twelve 16-byte wavefronts of shared memory for 64 FMAs), then four
+// queries and eight columns of the result (five for 32).  The FMA units bound it.
 #include "shared_prefix.cuh"
 
 // attention_shared_prefix_tc.cu
@@ -28,12 +28,13 @@ namespace {
 using namespace shared_prefix;
 constexpr int QR = 32;        // queries of a tile
 constexpr int KT = 64;        // keys of a tile
-constexpr int THREADS = 256;
-constexpr int EIGHT = 8;      // threads that share a query
+constexpr int THREADS = 128, WARPS = THREADS / 32;
+constexpr int SHARE = 16;     // threads that share four queries
+constexpr int P_STRIDE = QR + 4;
 
-__host__ __device__ constexpr int k_stride(int hd) { return hd + 4; }
-__host__ __device__ constexpr int p_stride() { return KT + 4; }
-static size_t smem_floats(int hd) { return (size_t)QR * hd + (size_t)KT * k_stride(hd) + (size_t)KT * hd + (size_t)QR * p_stride(); }
+// rows four floats apart from a multiple of 32: threads that read neighbouring rows meet no bank twice
+__host__ __device__ constexpr int row_stride(int hd) { return hd + 4; }
+static size_t smem_floats(int hd) { return (size_t)QR * row_stride(hd) + (size_t)KT * row_stride(hd) + (size_t)KT * P_STRIDE; }
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -46,20 +47,19 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
-// HDM: the head size rounded up to 32, 64, 128 or 256 (sizes the registers)
+// HDM: the head size rounded up to 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
-__global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
-  constexpr int OC = HDM / 32;     // groups of four output columns of a thread
+__global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
+  constexpr int OC = HDM <= 64 ? 1 : HDM / 64;     // groups of four output columns of a thread
   extern __shared__ __align__(16) float smem[];
-  const int hd = p.hd, ks = k_stride(hd), c4s = hd / 4;
-  float* s_q = smem;                   // [QR][hd]
-  float* s_k = s_q + QR * hd;          // [KT][hd + 4]
-  float* s_v = s_k + KT * ks;          // [KT][hd]
-  float* s_p = s_v + KT * hd;          // [QR][KT + 4]
+  const int hd = p.hd, ks = row_stride(hd), c4s = hd / 4;
+  float* s_q = smem;                   // [QR][hd + 4]
+  float* s_kv = s_q + QR * ks;         // [KT][hd + 4]: keys, then values
+  float* s_p = s_kv + KT * ks;         // [KT][QR + 4]
   __shared__ GroupPiece list[CAP];
   __shared__ int s_page[KT];
-  const int tid = threadIdx.x, r = tid / EIGHT, c = tid % EIGHT;
-  const int G = p.H / p.KV;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = tid / SHARE * 4, c = tid % SHARE;
+  const int G = p.G;
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
   Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
@@ -102,22 +102,23 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
     const GroupPiece w = list[at++];
     const int rows = w.rows * G;
     auto row_at = [&](int k) { return of_group ? p.members[w.first + k] : w.first; };
-    for (int x = tid; x < QR * c4s; x += THREADS) {
-      const int qr = x / c4s, col = x % c4s * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (qr < rows) {
-        const int row = row_at(qr / G);
+    for (int qr = warp; qr < QR; qr += WARPS) {
+      const int row = qr < rows ? row_at(qr / G) : -1;
+      for (int col = lane * 4; col < hd; col += 128) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
+        *reinterpret_cast<float4*>(s_q + qr * ks + col) = v;
       }
-      *reinterpret_cast<float4*>(s_q + qr * hd + col) = v;
     }
     const int* table = p.block_table + (size_t)w.table_row * p.max_pages;
-    float o[OC][4];
+    float o[4][OC][4], m_run[4], l_run[4];
 #pragma unroll
-    for (int k = 0; k < OC; ++k)
+    for (int i = 0; i < 4; ++i) {
+      m_run[i] = -INFINITY;
+      l_run[i] = 0.f;
 #pragma unroll
-      for (int d = 0; d < 4; ++d) o[k][d] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
+      for (int k = 0; k < OC; ++k) o[i][k][0] = o[i][k][1] = o[i][k][2] = o[i][k][3] = 0.f;
+    }
     for (int kb = w.key0; kb < w.limit; kb += KT) {
       const int n = min(KT, w.limit - kb);
       __syncthreads();        // the tile before is no longer read
@@ -134,78 +135,91 @@ __global__ void __launch_bounds__(THREADS) attention_shared_prefix_kernel(const 
         s_page[tid] = page;
       }
       __syncthreads();
-      for (int x = tid; x < KT * c4s; x += THREADS) {
-        const int key = x / c4s, col = x % c4s * 4, page = s_page[key];
-        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-        if (page >= 0) {
-          const T* src = reinterpret_cast<const T*>(p.kv) + (((size_t)page * 2 * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd + col;
-          k = load4(src);
-          v = load4(src + (size_t)p.KV * p.ps * hd);
+      auto load_tile = [&](int kind) {       // 0: keys, 1: values; zeros where there is none
+#pragma unroll 8
+        for (int key = warp; key < KT; key += WARPS) {
+          const int page = s_page[key];
+          const T* src = reinterpret_cast<const T*>(p.kv) + ((((size_t)max(page, 0) * 2 + kind) * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd;
+          for (int col = lane * 4; col < hd; col += 128)
+            *reinterpret_cast<float4*>(s_kv + key * ks + col) = page >= 0 ? load4(src + col) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        *reinterpret_cast<float4*>(s_k + key * ks + col) = k;
-        *reinterpret_cast<float4*>(s_v + key * hd + col) = v;
-      }
+      };
+      load_tile(0);
       __syncthreads();
-      float s[KT / EIGHT];
+      float s[4][4];
 #pragma unroll
-      for (int j = 0; j < KT / EIGHT; ++j) s[j] = 0.f;
+      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll 2
       for (int d = 0; d < hd; d += 4) {
-        const float4 a = *reinterpret_cast<const float4*>(s_q + r * hd + d);
+        float4 a[4], b[4];
 #pragma unroll
-        for (int j = 0; j < KT / EIGHT; ++j) {
-          const float4 b = *reinterpret_cast<const float4*>(s_k + (j * EIGHT + c) * ks + d);
-          s[j] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[j]))));
+        for (int i = 0; i < 4; ++i) {
+          a[i] = *reinterpret_cast<const float4*>(s_q + (q4 + i) * ks + d);
+          b[i] = *reinterpret_cast<const float4*>(s_kv + (c + i * SHARE) * ks + d);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
       }
-      float mx = -INFINITY;
+      __syncthreads();        // the keys are no longer read
+      load_tile(1);
 #pragma unroll
-      for (int j = 0; j < KT / EIGHT; ++j) {
-        s[j] = j * EIGHT + c < n ? s[j] * sl2 : -INFINITY;
-        mx = fmaxf(mx, s[j]);
+      for (int i = 0; i < 4; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = c + j * SHARE < n ? s[i][j] * sl2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int x = 1; x < SHARE; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        const float m_new = fmaxf(m_run[i], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = exp2f(m_run[i] - m_use);       // 0 before the first key
+        m_run[i] = m_new;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = exp2f(s[i][j] - m_use);
+        l_run[i] = l_run[i] * keep + ((s[i][0] + s[i][1]) + (s[i][2] + s[i][3]));
+#pragma unroll
+        for (int k = 0; k < OC; ++k)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[i][k][d] *= keep;
       }
 #pragma unroll
-      for (int x = 1; x < EIGHT; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float m_new = fmaxf(m_run, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float keep = exp2f(m_run - m_use);       // 0 before the first key
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < KT / EIGHT; ++j) {
-        const float e = exp2f(s[j] - m_use);
-        sum += e;
-        s_p[r * p_stride() + j * EIGHT + c] = e;
-      }
-      l_run = l_run * keep + sum;
-      m_run = m_new;
-#pragma unroll
-      for (int k = 0; k < OC; ++k)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[k][d] *= keep;
-      __syncwarp();           // a query's eight threads are of one warp
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(s_p + (c + j * SHARE) * P_STRIDE + q4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+      __syncthreads();
+#pragma unroll 4
       for (int key = 0; key < n; ++key) {
-        const float e = s_p[r * p_stride() + key];
+        const float4 e = *reinterpret_cast<const float4*>(s_p + key * P_STRIDE + q4);
 #pragma unroll
-        for (int k = 0; k < OC; ++k) {
-          const int col = k * 32 + c * 4;
-          if (col < hd) {
-            const float4 v = *reinterpret_cast<const float4*>(s_v + key * hd + col);
-            o[k][0] = fmaf(e, v.x, o[k][0]);
-            o[k][1] = fmaf(e, v.y, o[k][1]);
-            o[k][2] = fmaf(e, v.z, o[k][2]);
-            o[k][3] = fmaf(e, v.w, o[k][3]);
+        for (int k = 0; k < OC; ++k)
+          if (k * 64 + c * 4 < hd) {
+            const float4 v = *reinterpret_cast<const float4*>(s_kv + key * ks + k * 64 + c * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float f = i == 0 ? e.x : i == 1 ? e.y : i == 2 ? e.z : e.w;
+              o[i][k][0] = fmaf(f, v.x, o[i][k][0]);
+              o[i][k][1] = fmaf(f, v.y, o[i][k][1]);
+              o[i][k][2] = fmaf(f, v.z, o[i][k][2]);
+              o[i][k][3] = fmaf(f, v.w, o[i][k][3]);
+            }
           }
-        }
       }
     }
+    float* part = of_group ? group_results(p, w.id) : row_results(p, w.id);
 #pragma unroll
-    for (int x = 1; x < EIGHT; x <<= 1) l_run += __shfl_xor_sync(0xffffffffu, l_run, x);
-    if (r < rows) {
-      float* part = of_group ? group_results(p, w.id) : row_results(p, w.id);
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int k = 0; k < OC; ++k)
-        if (k * 32 + c * 4 < hd)
-          *reinterpret_cast<float4*>(part + (of_group ? ((size_t)(k * 8 + c) * QR + r) * 4 : (size_t)r * hd + k * 32 + c * 4)) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
-      if (c == 0) *reinterpret_cast<float2*>(part + (of_group ? (size_t)QR * hd + 4 * r : (size_t)G * hd + 2 * r)) = make_float2(m_run, l_run);
+      for (int x = 1; x < SHARE; x <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], x);
+      const int r = q4 + i;
+      if (r < rows) {
+#pragma unroll
+        for (int k = 0; k < OC; ++k)
+          if (k * 64 + c * 4 < hd)
+            *reinterpret_cast<float4*>(part + (of_group ? ((size_t)(k * 16 + c) * QR + r) * 4 : (size_t)r * hd + k * 64 + c * 4)) =
+                make_float4(o[i][k][0], o[i][k][1], o[i][k][2], o[i][k][3]);
+        if (c == 0) *reinterpret_cast<float2*>(part + (of_group ? (size_t)QR * hd + 4 * r : (size_t)G * hd + 2 * r)) = make_float2(m_run[i], l_run[i]);
+      }
     }
     __syncthreads();          // the queries may be overwritten
   }
@@ -284,13 +298,12 @@ int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
 
 template <typename T>
 int launch_sized(const DkSharedPrefixParams& p, cudaStream_t stream) {
-  if (p.hd <= 32) return launch<T, 32>(p, stream);
   if (p.hd <= 64) return launch<T, 64>(p, stream);
   if (p.hd <= 128) return launch<T, 128>(p, stream);
   return launch<T, 256>(p, stream);
 }
 
-int fma_grid() { return 2 * dk_sm_count(); }
+int fma_grid() { return 3 * dk_sm_count(); }
 
 int merge(const DkSharedPrefixParams& p, cudaStream_t stream) {
   const int work = p.H / p.KV * (p.hd / 4);
@@ -336,6 +349,7 @@ bool cut_for(DkSharedPrefixParams& p) {
   p.rows_kt = tc ? dk_shared_prefix_rows_tile() : KT;
   p.rows_grid = tc ? dk_shared_prefix_rows_grid(p) : fma_grid();
   p.min_saved = 1;
+  p.least_tiles = tc ? 4 : 1;
   return tc;
 }
 

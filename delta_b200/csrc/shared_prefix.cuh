@@ -33,8 +33,8 @@ struct DkSharedPrefixParams {
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
   float scale;
   // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), query heads of a key-value head, rows of a
-  // group's tile, the blocks that compute, the most pieces there can be, and the keys that a group must save for its prefix to be read apart
-  int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved;
+  // group's tile, the blocks that compute, the most pieces there can be, the keys that a group must save for its prefix to be read apart, and the tiles that a range of long segments has at least
+  int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved, least_tiles;
 };
 
 namespace shared_prefix {
@@ -117,10 +117,10 @@ struct Cut {
         own(len + rows), piece(own + rows), sums(piece + rows) {}
 };
 
-// Tiles of a range, for a line of ``tiles`` in ``segments``.  Long segments are cut into ranges of up to four tiles even where that leaves blocks
-// idle: every piece is one more for the rows to read, eight at a time.  (8 rows x 4,096 keys, 1, 2 and 4 tiles a range: 21.6, 18.6 and 17.4 us.)
+// Tiles of a range, for a line of ``tiles`` in ``segments``.  Long segments are cut into ranges of up to ``least_tiles`` even where that leaves blocks
+// idle: every piece is one more for the rows to read, eight at a time.  (Tensor cores, 8 rows x 4,096 keys, 1, 2 and 4 tiles a range: 21.6, 18.6 and 17.4 us.)
 __device__ __forceinline__ int range_tiles(const DkSharedPrefixParams& p, int tiles, int segments) {
-  return min(max(few(tiles, p.grid), tiles > 24 * segments ? 4 : max(1, few(tiles, 8 * segments))), CAP);
+  return min(max(few(tiles, p.grid), min(p.least_tiles, tiles > 24 * segments ? 4 : max(1, few(tiles, 8 * segments)))), CAP);
 }
 
 // Sums of N values over the threads before this one, and over all; one sync.
