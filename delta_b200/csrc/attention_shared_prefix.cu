@@ -11,10 +11,11 @@
 //
 // This file holds the merge and the kernel on the FMA units: 32-bit keys and values, and every head size and page
 // size that the kernels on the tensor cores (attention_shared_prefix_tc.cu, attention_shared_prefix_rows.cu) do not take.  A block of 128 threads
-// keeps 32 queries; K and then V of a tile of 64 keys lie in one buffer in shared memory as floats, so that three blocks fit on an SM and one loads
-// while others compute.  A thread has four queries and four keys of the scores (twelve 16-byte wavefronts of shared memory for 64 FMAs), then four
-// queries and eight columns of the result (five for 32).  The FMA units bound it.
+// keeps 32 queries; K and V of a tile of 32 keys lie in shared memory as floats, and those of the next tile are on their way while this one is
+// computed.  A thread has four queries and two keys of the scores, then four queries and eight columns of the result (five 16-byte wavefronts of shared
+// memory for 32 FMAs).  Threads without a query only fetch.  The FMA units bound it, and in a short call the instructions' first fetch: its loops are rolled.
 #include "shared_prefix.cuh"
+#include "mma_helpers.cuh"
 
 // attention_shared_prefix_tc.cu
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
@@ -27,14 +28,14 @@ int dk_shared_prefix_rows_launch(const DkSharedPrefixParams& p, cudaStream_t str
 namespace {
 using namespace shared_prefix;
 constexpr int QR = 32;        // queries of a tile
-constexpr int KT = 64;        // keys of a tile
+constexpr int KT = 32;        // keys of a tile
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int SHARE = 16;     // threads that share four queries
 constexpr int P_STRIDE = QR + 4;
 
 // rows four floats apart from a multiple of 32: threads that read neighbouring rows meet no bank twice
 __host__ __device__ constexpr int row_stride(int hd) { return hd + 4; }
-static size_t smem_floats(int hd) { return (size_t)QR * row_stride(hd) + (size_t)KT * row_stride(hd) + (size_t)KT * P_STRIDE; }
+static size_t smem_floats(int hd) { return (size_t)(QR + 2 * KT) * row_stride(hd) + (size_t)KT * P_STRIDE; }
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -52,18 +53,19 @@ template <typename T, int HDM>
 __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
   constexpr int OC = HDM <= 64 ? 1 : HDM / 64;     // groups of four output columns of a thread
   extern __shared__ __align__(16) float smem[];
-  const int hd = p.hd, ks = row_stride(hd), c4s = hd / 4;
+  const int hd = p.hd, ks = row_stride(hd);
   float* s_q = smem;                   // [QR][hd + 4]
-  float* s_kv = s_q + QR * ks;         // [KT][hd + 4]: keys, then values
-  float* s_p = s_kv + KT * ks;         // [KT][QR + 4]
+  float* s_k = s_q + QR * ks;          // [KT][hd + 4]
+  float* s_v = s_k + KT * ks;          // [KT][hd + 4]
+  float* s_p = s_v + KT * ks;          // [KT][QR + 4]
   __shared__ GroupPiece list[CAP];
-  __shared__ int s_page[KT];
+  __shared__ long long s_row[2][KT];   // where a key's row of K begins in the cache, -1: there is none; of this tile and the next
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = tid / SHARE * 4, c = tid % SHARE;
   const int G = p.G;
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
   Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
-  auto tables = [&] { make_cut<true, KT, KT, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
+  auto tables = [&] { make_cut<true, KT, KT, 2, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
   tables();
   // every row's first piece for the merge
   if (blockIdx.x == 0)
@@ -102,8 +104,9 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
     const GroupPiece w = list[at++];
     const int rows = w.rows * G;
     auto row_at = [&](int k) { return of_group ? p.members[w.first + k] : w.first; };
-    for (int qr = warp; qr < QR; qr += WARPS) {
-      const int row = qr < rows ? row_at(qr / G) : -1;
+#pragma unroll 1
+    for (int qr = warp; qr < rows; qr += WARPS) {
+      const int row = row_at(qr / G);
       for (int col = lane * 4; col < hd; col += 128) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
@@ -119,93 +122,109 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
 #pragma unroll
       for (int k = 0; k < OC; ++k) o[i][k][0] = o[i][k][1] = o[i][k][2] = o[i][k][3] = 0.f;
     }
-    for (int kb = w.key0; kb < w.limit; kb += KT) {
-      const int n = min(KT, w.limit - kb);
-      __syncthreads();        // the tile before is no longer read
-      if (tid < KT) {
-        int page = -1;
-        if (tid < n) {
-          const int lp = (kb + tid) / p.ps;        // below max_pages: limits were checked
-          page = table[lp];
-          if (page < 0 || page >= p.num_pages) {
-            dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
-            page = -1;
-          }
-        }
-        s_page[tid] = page;
+    auto look_up = [&](int kb, int which) {       // by the first KT threads
+      if (tid >= KT) return;
+      long long row = -1;
+      if (kb + tid < w.limit) {
+        const int lp = (kb + tid) / p.ps, page = table[lp];        // below max_pages: limits were checked
+        if (page < 0 || page >= p.num_pages) dk_report(p.err, DK_DEV_BAD_PAGE, w.table_row, lp, page);
+        else row = (((long long)page * 2 * p.KV + w.kvh) * p.ps + (kb + tid - lp * p.ps)) * hd;
       }
-      __syncthreads();
-      auto load_tile = [&](int kind) {       // 0: keys, 1: values; zeros where there is none
-#pragma unroll 8
-        for (int key = warp; key < KT; key += WARPS) {
-          const int page = s_page[key];
-          const T* src = reinterpret_cast<const T*>(p.kv) + ((((size_t)max(page, 0) * 2 + kind) * p.KV + w.kvh) * p.ps + (kb + key) % p.ps) * hd;
-          for (int col = lane * 4; col < hd; col += 128)
-            *reinterpret_cast<float4*>(s_kv + key * ks + col) = page >= 0 ? load4(src + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s_row[which][tid] = row;
+    };
+    auto fetch = [&](float* to, int which, long long kind) {       // zeros where there is none
+#pragma unroll 1
+      for (int key = warp; key < KT; key += WARPS) {
+        const long long row = s_row[which][key];
+        const T* src = reinterpret_cast<const T*>(p.kv) + (row < 0 ? 0 : row + kind);
+        for (int col = lane * 4; col < hd; col += 128) {
+          if constexpr (sizeof(T) == 4) cp_async_16(smem_u32(to + key * ks + col), src + col, row >= 0);
+          else *reinterpret_cast<float4*>(to + key * ks + col) = row >= 0 ? load4(src + col) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-      };
-      load_tile(0);
-      __syncthreads();
-      float s[4][4];
+      }
+      cp_async_commit();
+    };
+    const long long values = (long long)p.KV * p.ps * hd;        // from a key's row to its value's
+    look_up(w.key0, 0);
+    __syncthreads();
+    fetch(s_k, 0, 0);
+    fetch(s_v, 0, values);
+    int which = 0;
+    const bool busy = warp * 8 < rows;        // some of the warp's eight queries is one
+#pragma unroll 1
+    for (int kb = w.key0; kb < w.limit; kb += KT, which ^= 1) {
+      look_up(kb + KT, which ^ 1);
+      cp_async_wait<1>();
+      __syncthreads();        // the keys are there
+      float s[4][2];
+      if (busy) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
 #pragma unroll 2
-      for (int d = 0; d < hd; d += 4) {
-        float4 a[4], b[4];
+        for (int d = 0; d < hd; d += 4) {
+          float4 a[4], b[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = *reinterpret_cast<const float4*>(s_q + (q4 + i) * ks + d);
-          b[i] = *reinterpret_cast<const float4*>(s_kv + (c + i * SHARE) * ks + d);
+          for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(s_q + (q4 + i) * ks + d);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const float4*>(s_k + (c + j * SHARE) * ks + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
       }
       __syncthreads();        // the keys are no longer read
-      load_tile(1);
+      fetch(s_k, which ^ 1, 0);
+      if (busy) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float mx = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j] = c + j * SHARE < n ? s[i][j] * sl2 : -INFINITY;
-          mx = fmaxf(mx, s[i][j]);
+          for (int j = 0; j < 2; ++j) {
+            s[i][j] = kb + c + j * SHARE < w.limit ? s[i][j] * sl2 : -INFINITY;
+            mx = fmaxf(mx, s[i][j]);
+          }
+#pragma unroll
+          for (int x = 1; x < SHARE; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          const float m_new = fmaxf(m_run[i], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+          const float keep = exp2f(m_run[i] - m_use);       // 0 before the first key
+          m_run[i] = m_new;
+          s[i][0] = exp2f(s[i][0] - m_use);
+          s[i][1] = exp2f(s[i][1] - m_use);
+          l_run[i] = l_run[i] * keep + (s[i][0] + s[i][1]);
+#pragma unroll
+          for (int k = 0; k < OC; ++k)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[i][k][d] *= keep;
         }
 #pragma unroll
-        for (int x = 1; x < SHARE; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        const float m_new = fmaxf(m_run[i], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float keep = exp2f(m_run[i] - m_use);       // 0 before the first key
-        m_run[i] = m_new;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = exp2f(s[i][j] - m_use);
-        l_run[i] = l_run[i] * keep + ((s[i][0] + s[i][1]) + (s[i][2] + s[i][3]));
-#pragma unroll
-        for (int k = 0; k < OC; ++k)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) o[i][k][d] *= keep;
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<float4*>(s_p + (c + j * SHARE) * P_STRIDE + q4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
       }
+      cp_async_wait<1>();
+      __syncthreads();        // the values and the weights are there
+      if (busy) {
+#pragma unroll 2
+        for (int key = 0; key < KT; ++key) {        // (behind the last key weights and values are zeros)
+          const float4 e = *reinterpret_cast<const float4*>(s_p + key * P_STRIDE + q4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(s_p + (c + j * SHARE) * P_STRIDE + q4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
-      __syncthreads();
-#pragma unroll 4
-      for (int key = 0; key < n; ++key) {
-        const float4 e = *reinterpret_cast<const float4*>(s_p + key * P_STRIDE + q4);
+          for (int k = 0; k < OC; ++k)
+            if (k * 64 + c * 4 < hd) {
+              const float4 v = *reinterpret_cast<const float4*>(s_v + key * ks + k * 64 + c * 4);
 #pragma unroll
-        for (int k = 0; k < OC; ++k)
-          if (k * 64 + c * 4 < hd) {
-            const float4 v = *reinterpret_cast<const float4*>(s_kv + key * ks + k * 64 + c * 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float f = i == 0 ? e.x : i == 1 ? e.y : i == 2 ? e.z : e.w;
-              o[i][k][0] = fmaf(f, v.x, o[i][k][0]);
-              o[i][k][1] = fmaf(f, v.y, o[i][k][1]);
-              o[i][k][2] = fmaf(f, v.z, o[i][k][2]);
-              o[i][k][3] = fmaf(f, v.w, o[i][k][3]);
+              for (int i = 0; i < 4; ++i) {
+                const float f = i == 0 ? e.x : i == 1 ? e.y : i == 2 ? e.z : e.w;
+                o[i][k][0] = fmaf(f, v.x, o[i][k][0]);
+                o[i][k][1] = fmaf(f, v.y, o[i][k][1]);
+                o[i][k][2] = fmaf(f, v.z, o[i][k][2]);
+                o[i][k][3] = fmaf(f, v.w, o[i][k][3]);
+              }
             }
-          }
+        }
       }
+      __syncthreads();        // the values are no longer read
+      fetch(s_v, which ^ 1, values);
     }
+    cp_async_wait<0>();
     float* part = of_group ? group_results(p, w.id) : row_results(p, w.id);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -35,6 +35,7 @@ using namespace shared_prefix;
 constexpr int QT = 128;            // queries of a tile (rows of both products)
 constexpr int KT = 128;            // keys of a tile
 constexpr int ROWS_KT = 64;        // keys of a tile of the rows' kernel
+constexpr int MIN_ROW_TILES = 16;  // (48 rows of 200 to 1,000 keys of their own, 8 and 16: 58.7 and 56.3 us)
 constexpr int HALF_THREADS = 128;
 constexpr int PRODUCER_WARP0 = 8, MMA_WARP = 10;
 constexpr int THREADS = (MMA_WARP + 2) * 32;
@@ -140,7 +141,7 @@ template <int HD>
 __device__ void prepare_rows(const DkSharedPrefixParams& p, int* tables, int tid) {
   for (int i = tid; i < p.rows * p.KV; i += THREADS) counters(p)[i] = 0;
   Cut cut(tables, p.rows, p.groups);
-  make_cut<true, KT, ROWS_KT, THREADS>(p, cut, tid, [] { __syncthreads(); });
+  make_cut<true, KT, ROWS_KT, MIN_ROW_TILES, THREADS>(p, cut, tid, [] { __syncthreads(); });
   for (int id = tid; id < cut.pieces; id += THREADS) row_pieces(p)[id] = row_piece<KT, ROWS_KT>(p, cut, id);
   if (tid == 0) *reinterpret_cast<int*>(p.work) = cut.pieces;
   __threadfence();

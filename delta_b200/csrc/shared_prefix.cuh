@@ -9,7 +9,7 @@
 //           range holds of a segment, and its number is segment + range: every step from one piece to the next moves to the next
 //           segment or the next range, so no two pieces have one number and those of a segment follow one another.
 //   rows    every segment is cut into equal pieces of at most C tiles, numbered through, and a block takes every ``grid``-th.  C is what
-//           levels the blocks, but MIN_ROW_TILES at least: the pieces of a cut segment go through memory, which takes as long as several tiles.
+//           levels the blocks, but a number of its own for each kernel at least: the pieces of a cut segment go through memory, which takes as long as several tiles.
 //
 // All this is worked out on the device from the tables, so that a captured call follows them.  Whatever comes from the tables is checked here, so
 // the kernels stay inside their tensors (page ids they check themselves).
@@ -40,7 +40,7 @@ struct DkSharedPrefixParams {
 namespace shared_prefix {
 constexpr int MAX_ROWS = 1024, MAX_GROUPS = 1023, MAX_G = 32;
 constexpr int CAP = 48;            // tiles of a range, so also the most pieces of one
-constexpr int MIN_ROW_TILES = 16;
+
 
 __host__ __device__ constexpr int cdiv(int a, int b) { return (a + b - 1) / b; }
 // the same for a that seldom passes b (a division by a number the compiler does not know takes some hundred cycles)
@@ -152,8 +152,8 @@ __device__ __forceinline__ void scan(const int* v, int* before, int* total, int*
     }
 }
 
-// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well; KT, ROWS_KT: p.kt, p.rows_kt.  Ends with a sync.
-template <bool ROWS, int KT, int ROWS_KT, int NT, typename Sync>
+// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well; KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
+template <bool ROWS, int KT, int ROWS_KT, int MIN_ROW_TILES, int NT, typename Sync>
 __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid, Sync sync) {
   const int max_keys = p.max_pages * p.ps;
   // what the steps below read is asked for at once
