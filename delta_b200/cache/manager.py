@@ -17,6 +17,9 @@ What differs, on purpose:
     scheduler.py:60-66).
   * Growing a request is all or nothing over the groups; ``OutOfPages`` leaves
     everything as it was, and the scheduler decides what happens then.
+  * A request can be forked: the new ones hold the same whole pages (a page counts its holders) and a copy of
+    the last one as far as it is filled, so nothing that is shared is ever written again.  The reference gives every
+    request pages of its own and computes a prompt once for every sample of it.
   * What a page holds is the mixer's business: the manager allocates
     [layers of the group][page][*layout] from the layout the mixer declares.  The
     attention part keeps [K|V][kv head][offset][head_dim], so that the keys of one
@@ -25,12 +28,13 @@ What differs, on purpose:
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
-from ..parts.base import CacheSpec, StateSpec
+from ..kernels import ops
+from ..parts.base import PAGE, CacheSpec, StateSpec
 from .page_pool import OutOfPages, PagePool
 
 
@@ -86,7 +90,9 @@ class CacheManager:
 
     def __init__(self, cache_specs: Dict[int, CacheSpec], state_specs: Dict[str, StateSpec], *, max_slots: int,
                  max_seq_len: int, page_size: int, num_pages, dtype=torch.bfloat16, device="cuda", shuffle_seed=None,
-                 page_runs: bool = True):
+                 page_runs: bool = True, states_follow_tokens: bool = True):
+        """``states_follow_tokens``: a request's states belong to the tokens it holds now, so it can be forked at its present
+        length only.  False: they are made anew in every step, and a fork at a shorter length starts with fresh ones."""
         self.max_slots, self.max_seq_len, self.page_size = int(max_slots), int(max_seq_len), int(page_size)
         self.max_pages_per_request = (self.max_seq_len + page_size - 1) // page_size
         self.device = device
@@ -110,6 +116,8 @@ class CacheManager:
         self.seq_len = np.zeros(self.max_slots, dtype=np.int64)
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
         self._live = [False] * self.max_slots
+        self.states_follow_tokens = bool(states_follow_tokens)
+        self._shared: Dict[tuple, list] = {}      # (group, slots) -> what ``shared_prefixes`` found, until a holder comes or goes
 
     # ---- slots -------------------------------------------------------------
     @property
@@ -121,6 +129,7 @@ class CacheManager:
         if not self._free_slots:
             raise RuntimeError("no free request slot")
         slot = self._free_slots.pop()
+        self._shared.clear()
         self._live[slot] = True
         self.seq_len[slot] = 0
         for g in self.groups.values():
@@ -135,6 +144,7 @@ class CacheManager:
         """Gives back every page the request holds, and the slot."""
         if not self._live[slot]:
             raise ValueError(f"slot {slot} is released twice (or was never acquired)")
+        self._shared.clear()
         for g in self.groups.values():
             g.pool.free(g.held(slot))
             g.table[slot].fill(-1)
@@ -194,24 +204,163 @@ class CacheManager:
                 g.table[slot, a:first_needed] = -1
                 g.first_page[slot] = first_needed
 
+    # ---- requests that share their beginning -----------------------------------
+    def can_fork(self, slot: int, length: int) -> bool:
+        """Whether the request still holds what a fork at its first ``length`` tokens needs."""
+        if not self._live[slot] or not 0 < length <= int(self.seq_len[slot]):
+            return False
+        if self.states and self.states_follow_tokens and length != int(self.seq_len[slot]):
+            return False
+        return all(not g.spec.reach or g.spec.first_needed(length) // g.page_size >= int(g.first_page[slot]) for g in self.groups.values())
+
+    def fork(self, slot: int, length: Optional[int] = None, count: int = 1) -> List[int]:
+        """``count`` new requests that hold the first ``length`` tokens of a live one (all of them when None), as slots: the whole pages
+        are shared, the tokens of the last page and the states are copied, one launch for each.  The copies are enqueued on the
+        current stream.  All or nothing: ``OutOfPages`` and a lack of slots leave everything as it was."""
+        length = int(self.seq_len[slot]) if length is None else int(length)
+        if not self.can_fork(slot, length):
+            raise ValueError(f"slot {slot} cannot be forked at {length} tokens: it holds {int(self.seq_len[slot]) if self._live[slot] else 0}, and what a window "
+                             "or a state has passed is gone")
+        if count > self.free_slots:
+            raise RuntimeError("no free request slot")
+        whole, rest = divmod(length, self.page_size)
+        for n, g in self.groups.items():
+            if rest and count > g.pool.free_pages:
+                raise OutOfPages(f"out of cache pages in group {n}: {count} needed for the forks' last pages, {g.pool.free_pages} free")
+        present = length == int(self.seq_len[slot])
+        new = [self.acquire_slot() for _ in range(count)]
+        for g in self.groups.values():
+            first = max(int(g.first_page[slot]), g.spec.first_needed(length) // g.page_size if g.spec.reach else 0)
+            shared = g.table[slot, first:whole].tolist() if whole > first else []
+            copies = []
+            for s in new:
+                g.table[s, first:whole] = shared
+                g.first_page[s], g.num_logical[s] = first, whole + (1 if rest else 0)
+                g.pool.share(shared)
+                if rest:
+                    page = g.pool.alloc(1, after=shared[-1] if shared else None)[0]
+                    g.table[s, whole] = page
+                    copies.append(page)
+            if copies:
+                self._copy_pages(g, [int(g.table[slot, whole])] * count, copies, [rest] * count)
+        if self.states and present:
+            self._copy_slots([slot] * count, new)
+        for s in new:
+            self.seq_len[s] = length
+        return new
+
+    def shared_prefixes(self, group: str, slots: Sequence[int]) -> List[Tuple[List[int], int]]:
+        """[(places in ``slots``, pages)]: which of these requests hold the same first pages of a group, two or more to each entry.  Where
+        some of them share more than all of them do, the way to divide them that saves the most reading is taken."""
+        key = (group, tuple(slots))
+        found = self._shared.get(key)
+        if found is None:
+            g = self.groups[group]
+            table = g.table[list(slots)]
+            n = g.num_logical[list(slots)]
+
+            def divide(rows: np.ndarray, known: int):       # rows that agree on the first ``known`` pages -> (pages saved, entries)
+                most = int(n[rows].min())
+                same = (table[rows, known:most] == table[rows[0], known:most]).all(axis=0)
+                k = known + (int(same.argmin()) if not same.all() else most - known)
+                best = ((len(rows) - 1) * k, [(rows.tolist(), k)] if k else [])
+                longer = rows[n[rows] > k]
+                parts = [divide(longer[table[longer, k] == p], k + 1) for p in np.unique(table[longer, k]) if (table[longer, k] == p).sum() > 1 and p >= 0] if len(longer) > 1 else []
+                apart = (sum(x for x, _ in parts), [e for _, es in parts for e in es])
+                return apart if apart[0] > best[0] else best
+
+            rows = np.array([i for i in range(len(slots)) if table[i, 0] >= 0 and g.pool.holders(int(table[i, 0])) > 1], dtype=np.int64)
+            found = []
+            for p in np.unique(table[rows, 0]) if len(rows) else []:
+                mine = rows[table[rows, 0] == p]
+                if len(mine) > 1:
+                    found += divide(mine, 1)[1]
+            if len(self._shared) >= 256:
+                self._shared.clear()
+            self._shared[key] = found
+        return found
+
+    def compact(self) -> Dict[str, int]:
+        """Moves pages, in place, so that a request's pages follow one another in aligned runs again (see ``PagePool``), where serving has
+        scattered them; requests that lie in runs stay where they are.  Tables, shared pages and free pages are booked anew; the copies are
+        enqueued on the current stream, one launch for each group.  Returns how many pages moved, by group."""
+        self._shared.clear()
+        return {name: self._compact_group(g) for name, g in self.groups.items()}
+
+    def _compact_group(self, g: CacheGroup) -> int:
+        R, total = g.pool.run_pages, g.pool.num_pages
+        if R == 1:
+            return 0
+        slots = [s for s in range(self.max_slots) if self._live[s]]
+        held = {s: g.held(s) for s in slots}
+
+        def broken(pages):      # steps from page to page that neither stay in a run nor begin the next one
+            return sum(1 for a, b in zip(pages, pages[1:]) if b != a + 1 and not (a % R == R - 1 and b % R == 0))
+        fixed = {p for s in slots if not broken(held[s]) for p in held[s]}
+        movable, seen = [], set(fixed)
+        for s in sorted(slots, key=lambda s: -len(held[s])):      # shared pages go with the longest request that holds them
+            mine = [p for p in held[s] if p not in seen]
+            seen.update(mine)
+            if mine:
+                movable.append(mine)
+        runs = [r for r in range(total // R) if not any(q in fixed for q in range(r * R, r * R + R))]
+        if sum(-(-len(m) // R) for m in movable) <= len(runs):
+            places, at = [], 0
+            for m in movable:
+                places += [runs[at + i // R] * R + i % R for i in range(len(m))]
+                at += -(-len(m) // R)
+        else:
+            places = [q for q in range(total) if q not in fixed]
+        moved = {p: q for p, q in zip((p for m in movable for p in m), places) if p != q}
+        if not moved:
+            return 0
+        self._copy_pages(g, list(moved), list(moved.values()), None)
+        g.pool.relocate(moved)
+        new_id = np.arange(total + 1, dtype=np.int32)
+        new_id[list(moved)] = list(moved.values())
+        for s in slots:
+            row = g.table[s]
+            row[row >= 0] = new_id[row[row >= 0]]
+        return len(moved)
+
+    def _copy_pages(self, g: CacheGroup, src, dst, tokens) -> None:
+        axis = g.spec.layout.index(PAGE)
+        if g.pages.is_cuda:
+            ops.copy_pages(g.pages, src, dst, tokens=tokens, token_axis=axis)
+        elif tokens is None:                    # the bookkeeping's tests
+            g.pages[:, dst] = g.pages[:, src]
+        else:
+            for a, b, n in zip(src, dst, tokens):
+                g.pages[:, b].narrow(axis + 1, 0, n).copy_(g.pages[:, a].narrow(axis + 1, 0, n))
+
+    def _copy_slots(self, src, dst) -> None:
+        if next(iter(self.states.values())).is_cuda:
+            ops.copy_slots(self.states, src, dst)
+        else:
+            for s in self.states.values():
+                s[dst] = s[src]
+
     # ---- views for a step ------------------------------------------------------
     def layer_pages(self, cache_id: int) -> torch.Tensor:
         g = self.group_of_cache[cache_id]
         return g.pages[g.index_of[cache_id]]
 
     def check(self) -> None:
-        """Bookkeeping invariants: every held page belongs to exactly one live request."""
+        """Bookkeeping invariants: every held page belongs to live requests, as many as it has holders."""
         for g in self.groups.values():
             g.pool.check()
-            seen = set()
+            seen: Dict[int, int] = {}
             for slot in range(self.max_slots):
                 pages = g.held(slot)
                 if pages and not self._live[slot]:
                     raise AssertionError(f"slot {slot} is free but holds pages in group {g.name}")
+                if len(set(pages)) != len(pages):
+                    raise AssertionError(f"slot {slot} holds a page of group {g.name} twice")
                 for p in pages:
-                    if p in seen:
-                        raise AssertionError(f"page {p} of group {g.name} is held twice")
-                    seen.add(p)
+                    seen[p] = seen.get(p, 0) + 1
+            for p, n in seen.items():
+                if n != g.pool.holders(p):
+                    raise AssertionError(f"page {p} of group {g.name} is held twice" if n > g.pool.holders(p) else f"page {p} of group {g.name} has lost a holder")
             if len(seen) != g.pool.held_pages:
                 raise AssertionError(f"group {g.name}: {g.pool.held_pages} pages are out, requests hold {len(seen)}")
 

@@ -16,7 +16,8 @@ pages, and a request that says which page it took last (``after``) gets
 So requests that grow by a page now and then, in turns, still hold runs, and a
 request that takes many pages at once takes them in order.  Nothing is set
 aside: a request holds the pages it asked for and no more, and every free page
-can be had by whoever asks.  With ``run_pages = 1`` this is a last-in
+can be had by whoever asks.  A page may have several holders (requests that share their beginning): it is free
+again when the last one gives it back.  With ``run_pages = 1`` this is a last-in
 first-out stack of pages.  A seeded shuffle scatters pages as the reference
 does (then ``after`` is ignored).  A double free or a foreign page is an error.
 """
@@ -39,7 +40,7 @@ class PagePool:
         self.num_pages = int(num_pages)
         self.shuffled = shuffle_seed is not None            # pages of a request lie scattered over the pool
         self.run_pages = 1 if self.shuffled else int(run_pages)
-        self._held = [False] * self.num_pages
+        self._held = [0] * self.num_pages                   # holders of each page
         self._n_free = self.num_pages
         n_runs = -(-self.num_pages // self.run_pages)
         self._free_in_run = [self._run_size(r) for r in range(n_runs)]
@@ -62,7 +63,7 @@ class PagePool:
 
     def _take(self, p: int) -> None:
         r = p // self.run_pages
-        self._held[p] = True
+        self._held[p] = 1
         self._n_free -= 1
         self._free_in_run[r] -= 1
         self._begun.pop(r, None)
@@ -93,19 +94,35 @@ class PagePool:
             last = p
         return out
 
-    def free(self, pages) -> None:
-        """Gives pages back.  Runs that become wholly free go on the stack in reverse, so that
-        runs freed together are handed out again in the order they had."""
+    def holders(self, page: int) -> int:
+        """How many hold this page (0: it is free, or none of this pool's)."""
+        return self._held[page] if 0 <= page < self.num_pages else 0
+
+    def share(self, pages) -> None:
+        """One more holder for each of these pages, which are held already."""
         pages = list(pages)
+        for p in pages:
+            if not self.holders(p):
+                raise ValueError(f"page {p} is held by nobody and cannot be shared")
+        for p in pages:
+            self._held[p] += 1
+
+    def free(self, pages) -> None:
+        """Gives pages back; one that others hold too stays theirs.  Runs that become wholly free go on the stack in reverse,
+        so that runs freed together are handed out again in the order they had."""
+        pages = list(pages)
+        gone = []
         for p in pages:
             if not (0 <= p < self.num_pages):
                 raise ValueError(f"page {p} does not belong to this pool of {self.num_pages}")
             if not self._held[p]:
                 raise ValueError(f"page {p} is freed twice (or was never handed out)")
-            self._held[p] = False
-        self._n_free += len(pages)
+            self._held[p] -= 1
+            if not self._held[p]:
+                gone.append(p)
+        self._n_free += len(gone)
         whole = []
-        for p in reversed(pages):
+        for p in reversed(gone):
             r = p // self.run_pages
             self._free_in_run[r] += 1
             self._begun.pop(r, None)
@@ -114,6 +131,27 @@ class PagePool:
             else:
                 self._begun[r] = None
         self._whole.extend(whole)
+
+    def relocate(self, moved: Dict[int, int]) -> None:
+        """Books that the held pages ``moved`` (old id -> new id) lie elsewhere now, all at once; the others stay.  What was free before
+        its new page came stays free where the page went away."""
+        held = list(self._held)
+        for p in moved:
+            if not self.holders(p):
+                raise ValueError(f"page {p} is held by nobody and cannot be moved")
+            held[p] = 0
+        for p, q in moved.items():
+            if not 0 <= q < self.num_pages or held[q]:
+                raise ValueError(f"page {p} cannot be moved to page {q}")
+            held[q] = self._held[p]
+        self._held = held
+        before = set(self._whole)
+        self._free_in_run = [sum(1 for q in range(r * self.run_pages, r * self.run_pages + self._run_size(r)) if not held[q])
+                             for r in range(len(self._free_in_run))]
+        whole = {r for r, n in enumerate(self._free_in_run) if n == self._run_size(r)}
+        # runs that stayed wholly free keep their places on the stack; new ones go below, the first on top of the last
+        self._whole = sorted(whole - before, reverse=True) + [r for r in self._whole if r in whole]
+        self._begun = {r: None for r, n in enumerate(self._free_in_run) if 0 < n < self._run_size(r)}
 
     def check(self) -> None:
         """No page lost, none both free and held, no run listed twice or in the wrong list."""
@@ -132,5 +170,5 @@ class PagePool:
                 raise AssertionError(f"run {r} with {n} free pages is {'not ' if r not in whole else ''}on the free stack")
             if (0 < n < self._run_size(r)) != (r in self._begun):
                 raise AssertionError(f"run {r} with {n} free pages is {'not ' if r not in self._begun else ''}among the begun runs")
-        if free != self._n_free or sum(self._held) + free != self.num_pages:
+        if free != self._n_free or sum(1 for h in self._held if h) + free != self.num_pages:
             raise AssertionError("pages were lost")

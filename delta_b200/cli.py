@@ -44,6 +44,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--dataset", type=str, choices=["dummy1tok", "dummy4tok", "random"], default="dummy4tok",
                    help="synthetic prompts: one or four copies of one token, or random ids of --prompt_len")
     p.add_argument("--num_samples", type=int, default=16, help="how many requests are made")
+    p.add_argument("--samples", type=int, default=1, help="requests for every prompt, which is computed once")
+    p.add_argument("--share_prefix", action="store_true", help="compute the first tokens that all prompts have in common once")
     p.add_argument("--dummy_token_id", type=int, default=None, help="the token the dummy prompts repeat (default: bos_token_id, else 1)")
     p.add_argument("--full_cache_layers", nargs="+", type=int, default=None,
                    help="indices of the layers that read every page; a full layer followed by another kind chooses the pages")
@@ -123,7 +125,7 @@ def main(argv=None) -> int:
         n = 1 if args.dataset == "dummy1tok" else 4
         prompts = [[tid] * n for _ in range(args.num_samples)]
     eng.add_requests(prompts, [args.max_len] * len(prompts), [], temperature=args.temperature, top_p=args.top_p,
-                     seed=args.seed, max_new_tokens=args.max_new_tokens)
+                     seed=args.seed, max_new_tokens=args.max_new_tokens, samples=args.samples, share_prefix=args.share_prefix)
     t0 = time.perf_counter()
     results = eng.run_scheduler_loop()
     total = time.perf_counter() - t0
@@ -131,7 +133,7 @@ def main(argv=None) -> int:
     decode = [s for s in eng.step_timings if s["tokens"] == s["active_bsz"]]
     summary = dict(total_time_s=total, requests=len(results), prompt_tokens=st["prompt_tokens"],
                    generated_tokens=st["generated_tokens"], tokens_per_second=st["generated_tokens"] / total if total else 0.0,
-                   steps=st["steps"], preemptions=st["preemptions"],
+                   steps=st["steps"], preemptions=st["preemptions"], forks=st["forks"],
                    graph_captures=eng.runner.graph_captures, graph_replays=eng.runner.graph_replays,
                    graph_fallbacks=dict(eng.runner.graph_fallbacks),
                    decode_step_ms_mean=(sum(s["model_forward_ms"] for s in decode) / len(decode)) if decode else None)

@@ -32,13 +32,16 @@ class StepContext:
     ``max_rows`` and ``max_step_tokens`` are the engine's limits on a step (rows of a
     batch, tokens of a scheduled step), for parts that size working memory once.
 
+    ``shared``: for a step of single tokens whose rows share leading pages, by cache group, the tables that
+    ``ops.attention_shared_prefix`` takes (members, group_start, group_prefix, kv_len); empty when it would not pay.
+
     ``plain_kernels``: names of kernel families ("products", "attention") for which
     the slow plain kernels are to be taken, for comparisons.
     """
 
     def __init__(self, *, device, dtype, cache: CacheManager, sections: Dict[str, torch.Tensor], block_tables,
                  host: dict, err: torch.Tensor, scratch_pool: dict, plain_kernels=frozenset(), replayable: bool = False,
-                 capture: Optional[dict] = None, max_rows: int = 0, max_step_tokens: int = 0):
+                 capture: Optional[dict] = None, max_rows: int = 0, max_step_tokens: int = 0, shared: Optional[dict] = None):
         self.device, self.dtype, self.cache = device, dtype, cache
         self.tokens = sections["tokens"]
         self.tok_row = sections["tok_row"]
@@ -51,6 +54,7 @@ class StepContext:
         self.logit_rows = sections["logit_rows"]
         self.sampling_sections = {k: v for k, v in sections.items() if k.startswith("samp_")}
         self.block_tables = block_tables
+        self.shared = shared or {}
         self.host = host
         self.num_tokens = int(self.tokens.shape[0])
         self.num_rows = int(self.row_slot.shape[0])

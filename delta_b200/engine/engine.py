@@ -116,17 +116,35 @@ class LMBackend:
 
     # ---- requests ---------------------------------------------------------------
     def add_requests(self, input_ids_list, max_lengths, eot_token_ids: Sequence[int] = (), *, temperature=0.0, top_p=1.0,
-                     seed: int = 0, max_new_tokens: Optional[int] = None):
+                     seed: int = 0, max_new_tokens: Optional[int] = None, samples: int = 1, share_prefix: bool = False):
         """One request per prompt (lists or 1-D tensors of token ids).  ``max_lengths`` is a
-        number or a list: the most tokens a request may reach, prompt included."""
-        out = []
+        number or a list: the most tokens a request may reach, prompt included.
+
+        ``samples``: so many requests for every prompt, one behind the other, each with a sampling seed of its own.  The prompt is
+        computed once: the others are forked from the first (they hold the same cache pages and a copy of the last one).
+        ``share_prefix``: the first tokens that all prompts of this call have in common are computed once likewise.  Single
+        tokens of requests that share much are decoded with the shared pages read once for all of them."""
+        out, samples = [], int(samples)
+        if samples < 1:
+            raise ValueError(f"{samples} samples of a prompt")
         for i, ids in enumerate(input_ids_list):
             ids = ids.tolist() if hasattr(ids, "tolist") else list(ids)
             ml = max_lengths[i] if isinstance(max_lengths, (list, tuple)) else max_lengths
             t = temperature[i] if isinstance(temperature, (list, tuple)) else temperature
-            sp = SamplingParams(temperature=float(t), top_p=float(top_p), seed=int(seed) + len(self.scheduler.requests))
-            out.append(self.scheduler.add_request(ids, ml, eot_token_ids, sp, max_new_tokens))
+            for _ in range(samples):
+                sp = SamplingParams(temperature=float(t), top_p=float(top_p), seed=int(seed) + len(self.scheduler.requests))
+                out.append(self.scheduler.add_request(ids, ml, eot_token_ids, sp, max_new_tokens))
+            self.scheduler.relate(out[-samples:], len(ids) - 1)
+        if share_prefix and len(out) > samples:
+            first = [r.prompt for r in out[::samples]]
+            common = next((k for k, column in enumerate(zip(*first)) if any(x != column[0] for x in column)), min(map(len, first)))
+            self.scheduler.relate(out, common)
         return out
+
+    def compact_cache(self) -> dict:
+        """Moves cache pages in place so that every request's pages follow one another again where serving has scattered them (the attention
+        kernels fetch such runs with one copy); to be called between steps.  Returns how many pages moved, by cache group."""
+        return self.runner.cache.compact()
 
     # ---- the loop -----------------------------------------------------------------
     def step(self) -> List:
@@ -244,7 +262,7 @@ class LMBackend:
         sch, runner = self.scheduler, self.runner
         if not (self.run_ahead and self.cuda_graph_decode) or self.record_timings or self.on_step_logits or sch.waiting or not plan or result is None:
             return
-        if not runner.decode_graph_ready(len(plan)):
+        if not runner.decode_graph_ready(len(plan), [RowInput(x.request.slot, [0], 0) for x in plan]):
             return
         if runner.model.has_run_state():
             # a step launched ahead may have to be dropped and run again; one that advanced a recurrent state cannot be
@@ -330,11 +348,12 @@ class LMBackend:
         return res
 
     # ---- convenience -----------------------------------------------------------------
-    def generate(self, prompts, max_new_tokens: int, *, temperature=0.0, top_p=1.0, seed=0, stop_ids=()) -> List[List[int]]:
-        """Token ids in, generated token ids out (host lists)."""
+    def generate(self, prompts, max_new_tokens: int, *, temperature=0.0, top_p=1.0, seed=0, stop_ids=(), samples: int = 1,
+                 share_prefix: bool = False) -> List[List[int]]:
+        """Token ids in, generated token ids out (host lists), ``samples`` of them for every prompt."""
         first = len(self.scheduler.requests)
         limit = self.engine_config.max_seq_len
         self.add_requests(prompts, [min(limit, len(p) + max_new_tokens) for p in prompts], stop_ids, temperature=temperature,
-                          top_p=top_p, seed=seed, max_new_tokens=max_new_tokens)
+                          top_p=top_p, seed=seed, max_new_tokens=max_new_tokens, samples=samples, share_prefix=share_prefix)
         self.run_scheduler_loop()
         return [list(r.output) for r in self.scheduler.requests[first:]]

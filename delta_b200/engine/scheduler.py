@@ -21,6 +21,9 @@ everyone's decode token, and sizes the pool so that it can never run out
     and generated tokens run as one prompt; when some part treats them otherwise (page
     selection applies to decode rows only) the prompt runs in portions and every
     generated token again as a decode row of its own, one per step, unsampled.
+  * requests that begin alike (samples of one prompt, prompts with a common first part) are a ``Family``: while one of
+    them computes what they share the others wait, and then they are forked from it (``CacheManager.fork``) instead of
+    computing it again.  When nobody holds it any more, the next one computes it.
 """
 from __future__ import annotations
 
@@ -31,6 +34,13 @@ from typing import Dict, List, Optional, Sequence
 from ..sampling.sampler import SamplingParams
 
 WAITING, RUNNING, FINISHED, FAILED = "waiting", "running", "finished", "failed"
+
+
+@dataclass(eq=False)
+class Family:
+    """Requests whose first ``shared`` tokens are the same."""
+    shared: int
+    members: List["Request"] = field(default_factory=list)
 
 
 @dataclass
@@ -50,6 +60,7 @@ class Request:
     start_time: Optional[float] = None
     end_time: Optional[float] = None
     finish_reason: str = ""
+    families: List[Family] = field(default_factory=list, repr=False, compare=False)     # the longest beginning first
 
     @property
     def tokens(self) -> List[int]:
@@ -86,7 +97,7 @@ class Scheduler:
         self._admitted = 0
         # False: no request decodes while another still has prompt tokens to run (prompts first)
         self.decode_while_prefill = True
-        self.stats = dict(prompt_tokens=0, generated_tokens=0, steps=0, prefill_steps=0, decode_steps=0, preemptions=0)
+        self.stats = dict(prompt_tokens=0, generated_tokens=0, steps=0, prefill_steps=0, decode_steps=0, preemptions=0, forks=0)
 
     # ---- intake ------------------------------------------------------------
     def add_request(self, prompt: Sequence[int], max_length: int, stop_ids: Sequence[int] = (),
@@ -105,6 +116,18 @@ class Scheduler:
         else:
             self.waiting.append(r)
         return r
+
+    def relate(self, requests: Sequence[Request], shared: int) -> None:
+        """Says that the first ``shared`` tokens of these prompts are the same.  At least one token of each is left to compute."""
+        shared = min([int(shared)] + [len(r.prompt) - 1 for r in requests])
+        if shared < 1 or len(requests) < 2:
+            return
+        if any(r.prompt[:shared] != requests[0].prompt[:shared] for r in requests):
+            raise ValueError(f"the first {shared} tokens of these prompts are not the same")
+        family = Family(shared, list(requests))
+        for r in requests:
+            r.families.append(family)
+            r.families.sort(key=lambda f: -f.shared)
 
     def _fits_alone(self, n_tokens: int) -> bool:
         for g in self.cache.groups.values():
@@ -130,6 +153,9 @@ class Scheduler:
         """Chooses what runs in the next step and books the pages for it."""
         budget = self.budget
         rows: List[PlannedRow] = []
+        # 0. waiting requests whose beginning a running one holds
+        if any(r.families for r in self.waiting):
+            self._fork_waiting()
         # 1. one token for every request that is decoding (or computing a decode position again)
         # With prompts first, decoding waits only while a prompt is really under way or about to be: a
         # waiting request that cannot be admitted (no slot, no pages) must not stop those that can end.
@@ -153,7 +179,7 @@ class Scheduler:
         for r in sorted(self.running, key=lambda q: q.admitted_order):
             if r.status != RUNNING or budget < 1 or any(x.request is r for x in rows):
                 continue
-            left = self._portion_end(r) - r.computed
+            left = self._stop_for_forks(r, self._portion_end(r)) - r.computed
             if left < 1 or r.computed == r.total_len - 1:
                 continue
             count = min(left, budget)
@@ -161,25 +187,74 @@ class Scheduler:
                 continue
             rows.append(PlannedRow(r, r.computed, count, samples=(r.computed + count == r.total_len), decode=False))
             budget -= count
-        # 3. admit waiting requests, oldest first
-        while self.waiting and budget >= 1 and len(self.running) < self.max_batch and self.cache.free_slots > 0:
-            r = self.waiting[0]
+        # 3. admit waiting requests, oldest first; those whose beginning is being computed wait for it
+        at = 0
+        while at < len(self.waiting) and budget >= 1 and len(self.running) < self.max_batch and self.cache.free_slots > 0:
+            r = self.waiting[at]
+            if self._beginning_under_way(r):
+                at += 1
+                continue
             if not self._can_admit(r):
                 break
-            self.waiting.pop(0)
+            self.waiting.pop(at)
             r.slot = self.cache.acquire_slot()
-            r.status = RUNNING
             r.computed = 0
-            r.admitted_order = self._admitted
-            self._admitted += 1
-            if r.start_time is None:
-                r.start_time = self.clock()
-            self.running.append(r)
-            count = min(self._portion_end(r), budget)
+            self._start(r)
+            count = min(self._stop_for_forks(r, self._portion_end(r)), budget)
             self.cache.grow(r.slot, count)
             rows.append(PlannedRow(r, 0, count, samples=(count == r.total_len), decode=False))
             budget -= count
         return rows
+
+    def _start(self, r: Request) -> None:
+        r.status = RUNNING
+        r.admitted_order = self._admitted
+        self._admitted += 1
+        if r.start_time is None:
+            r.start_time = self.clock()
+        self.running.append(r)
+
+    # ---- requests that begin alike -----------------------------------------------
+    def _beginning_under_way(self, r: Request) -> bool:
+        """Some running request has yet to compute what ``r`` can then share."""
+        return any(m.status == RUNNING and m.computed < f.shared for f in r.families for m in f.members if m is not r)
+
+    def _stop_for_forks(self, r: Request, end: int) -> int:
+        """Where a portion of ``r`` that may go up to ``end`` stops: at a length where waiting requests are to be forked from it, when the
+        model's states make that the only place where they can."""
+        if self.cache.states and self.cache.states_follow_tokens:
+            for f in r.families:
+                if r.computed < f.shared < end and any(m.status == WAITING for m in f.members):
+                    end = f.shared
+        return end
+
+    def _fork_waiting(self) -> None:
+        """Forks waiting requests from running ones that hold what they share, as many as have a slot and pages for their whole prompt and
+        one more token; those of one source with one launch for all of them."""
+        reserve = {n: 0 for n in self.cache.groups}
+        wanted: Dict[tuple, List[Request]] = {}
+        room = min(self.max_batch - len(self.running), self.cache.free_slots)
+        for r in self.waiting:
+            if room < 1:
+                break
+            for f in r.families:
+                source = next((m for m in f.members if m.status == RUNNING and m.computed >= f.shared and self.cache.can_fork(m.slot, f.shared)), None)
+                if source is None:
+                    continue
+                need = {n: self._pages(g, r.total_len + 1) - f.shared // g.page_size if not g.spec.reach else self._pages(g, r.total_len + 1)
+                        for n, g in self.cache.groups.items()}
+                if all(reserve[n] + need[n] <= g.pool.free_pages for n, g in self.cache.groups.items()):
+                    wanted.setdefault((source.slot, f.shared), []).append(r)
+                    room -= 1
+                    for n in need:
+                        reserve[n] += need[n]
+                break
+        for (slot, length), requests in wanted.items():
+            for r, new in zip(requests, self.cache.fork(slot, length, len(requests))):
+                self.waiting.remove(r)
+                r.slot, r.computed = new, length
+                self._start(r)
+                self.stats["forks"] += 1
 
     def _portion_end(self, r: Request) -> int:
         """Where the tokens end that may run as prompt portions."""
@@ -187,14 +262,13 @@ class Scheduler:
 
     def _can_admit(self, r: Request) -> bool:
         """Room for the whole prompt and one more token in every group."""
-        need_len = r.total_len + 1
-        for g in self.cache.groups.values():
-            pages = (need_len + g.page_size - 1) // g.page_size
-            if g.spec.reach:
-                pages = min(pages, (g.spec.reach + min(self.budget, need_len) + g.page_size - 1) // g.page_size + 1)
-            if pages > g.pool.free_pages:
-                return False
-        return True
+        return all(self._pages(g, r.total_len + 1) <= g.pool.free_pages for g in self.cache.groups.values())
+
+    def _pages(self, g, need_len: int) -> int:
+        pages = (need_len + g.page_size - 1) // g.page_size
+        if g.spec.reach:
+            pages = min(pages, (g.spec.reach + min(self.budget, need_len) + g.page_size - 1) // g.page_size + 1)
+        return pages
 
     def _grow_or_preempt(self, r: Request, new_len: int, protect: List[Request]) -> bool:
         """Books pages for ``r`` to hold ``new_len`` tokens, preempting the youngest running

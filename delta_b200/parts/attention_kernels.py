@@ -8,6 +8,9 @@ rows.  32-bit rows that bring enough tokens go to a kernel with tiles of 32 quer
 Everything else (other head sizes, 32-bit rows of few tokens) goes to the plain kernel,
 which takes every size.
 
+Rows of single tokens that share leading pages (samples of one prompt, prompts with a common first part) go to kernels that read
+those pages once for all of them, where the engine found that it pays (``ctx.shared``).
+
 In a replayable step (``ctx.replayable``) nothing is chosen from the step's host data: the
 grid is the one for the longest request the engine allows, and whether pages are looked for
 in runs follows from how the pool hands pages out, not from this step's block tables.
@@ -33,6 +36,7 @@ MAX_SPLITS = int(os.environ.get("DELTA_B200_MAX_SPLITS", "64"))
 TMA_MIN_TILES = int(os.environ.get("DELTA_B200_TMA_MIN_TILES", "16"))    # tiles a block must walk for the decode kernel's TMA variant to be taken
 TC_PREFILL_MIN_TOKENS = 32   # below this a 128-query tile of the tcgen05 kernel is mostly padding
 PARTIALS = "attention.decode_partials"
+SHARED_WORK = "attention.shared_prefix"
 
 
 def decode_splits(rows: int, kv_heads: int, max_keys: int, sm_count: int, blocks_per_sm: int) -> int:
@@ -60,6 +64,23 @@ def can_fuse_rope_append(ctx, H: int, KV: int, hd: int, ps: int, interleaved: bo
     """True when the step goes to the decode kernel, which can then rotate q and k and append the
     new token's k and v itself; the separate rotary/append kernel is left out."""
     return (ctx.decode_only and not plain(ctx) and not interleaved and ops.attention_decode_supported(ctx.dtype, H, KV, hd, ps))
+
+
+def shares_prefixes(ctx, group: str, H: int, KV: int, hd: int) -> bool:
+    """True when the step goes to the kernels that read shared leading pages once (rotary positions and the append come before them)."""
+    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and hd % 4 == 0 and hd <= 256
+
+
+def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float) -> None:
+    """Attention of a step of single tokens over pages that rows share; ``qkv`` [rows, (H + 2 KV) hd] is rotated and appended already."""
+    t = ctx.shared[cache.group]
+    rows, max_pages = ctx.num_rows, ctx.max_pages
+
+    def floats(n, pages):
+        return ops.attention_shared_prefix_floats(n, n // 2, n, H, KV, hd, cache.page_size, pages, cache.pages.shape[0], qkv.dtype)
+    work = ctx.scratch(SHARED_WORK, (floats(rows, max_pages),), torch.float32, bound=(floats(max(ctx.max_rows, rows), ctx.cache.max_pages_per_request),))
+    ops.attention_shared_prefix(qkv[:, :H * hd].unflatten(1, (H, hd)), out.view(rows, H, hd), cache.pages, cache.block_table, t["kv_len"], t["members"],
+                                t["group_start"], t["group_prefix"], scale=scale, err=ctx.err, work=work)
 
 
 def _pages_scattered(ctx, group: str) -> bool:
