@@ -15,6 +15,7 @@
 #include "common.cuh"
 #include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 struct DkCopyTensor {
@@ -177,14 +178,29 @@ int order_copies(const int* src, const int* dst, const int* tokens, int n, long 
   return left;
 }
 
-// Fills a.t; returns the blocks that one lane takes, or a negative code.  ``threads``: of a block.
+// Tensors that share memory would be copied in two places at once, each overwriting what the other reads.
+int check_apart(const DkCopyTensor* tensors, int n_tensors, long long n_items) {
+  DK_REQUIRE(n_tensors >= 1, "copy_items: there is no tensor");
+  if (n_tensors == 1) return 0;
+  std::vector<std::pair<const char*, long long>> spans;
+  spans.reserve(n_tensors);
+  for (int k = 0; k < n_tensors; ++k)
+    if (tensors[k].layers > 0 && tensors[k].item_bytes > 0)
+      spans.push_back({(const char*)tensors[k].base, (tensors[k].layers - 1) * tensors[k].layer_stride + n_items * tensors[k].item_stride});
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    DK_REQUIRE(spans[i].first >= spans[i - 1].first + spans[i - 1].second, "copy_items: two of the tensors share memory");
+  return 0;
+}
+
+// Fills a.t with up to MAX_TENSORS; returns the blocks that one lane takes, or a negative code.  ``threads``: of a block.
 template <int N>
 int lay_out(const DkCopyTensor* tensors, int n_tensors, Args<N>& a, int& threads) {
-  DK_REQUIRE(n_tensors >= 1 && n_tensors <= MAX_TENSORS, "copy_items: %d tensors; 1 to %d are taken in one call", n_tensors, MAX_TENSORS);
+  n_tensors = std::min(n_tensors, MAX_TENSORS);
   int most = 1;
   for (int k = 0; k < n_tensors; ++k) {
     const DkCopyTensor& x = tensors[k];
-    DK_REQUIRE(x.base != nullptr && x.layers >= 0 && x.item_bytes >= 0 && x.token_bytes >= 0 && x.tokens >= 0, "copy_items: tensor %d is missing or has a negative size", k);
+    DK_REQUIRE((x.base != nullptr || x.item_bytes == 0) && x.layers >= 0 && x.item_bytes >= 0 && x.token_bytes >= 0 && x.tokens >= 0, "copy_items: tensor %d is missing, or its items have no size that is taken", k);
     long long bits = (long long)(uintptr_t)x.base | x.item_stride | x.layer_stride | x.item_bytes | x.token_bytes;
     int unit = 16;
     while (unit > 1 && bits % unit != 0) unit /= 2;
@@ -229,6 +245,19 @@ int launch(const Args<N>& a, int blocks, int lanes, int threads, cudaStream_t st
   return dk_check_launch("copy_items");
 }
 
+// One launch for every MAX_TENSORS tensors.
+template <int N>
+int launch_all(const DkCopyTensor* tensors, int n_tensors, Args<N>& a, int lanes, cudaStream_t stream) {
+  for (int k = 0; k < n_tensors; k += MAX_TENSORS) {
+    int threads = THREADS;
+    const int blocks = lay_out(tensors + k, n_tensors - k, a, threads);
+    if (blocks < 0) return blocks;
+    const int rc = launch(a, blocks, lanes, threads, stream);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}
+
 template <int N>
 int copy_inline(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, cudaStream_t stream) {
   Args<N> a = {};
@@ -239,7 +268,51 @@ int copy_inline(const DkCopyTensor* tensors, int n_tensors, const int* src, cons
   const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), a.copies, s, &lanes);
   if (rc < 0) return rc;
   for (int i = 0; i <= lanes; ++i) a.inline_starts[i] = (short)s[i];
-  return launch(a, blocks, lanes, threads, stream);
+  return launch_all(tensors, n_tensors, a, lanes, stream);
+}
+
+int copy_all(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, const int* list, const int* starts,
+             int lanes, cudaStream_t stream) {
+  if (list == nullptr) {
+    DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
+    if (const int rc = check_apart(tensors, n_tensors, n_items)) return rc;
+    return n <= FEW ? copy_inline<FEW>(tensors, n_tensors, src, dst, tokens, n, n_items, stream)
+                    : copy_inline<INLINE>(tensors, n_tensors, src, dst, tokens, n, n_items, stream);
+  }
+  Args<1> a = {};
+  a.list = reinterpret_cast<const int4*>(list);
+  a.starts = starts;
+  return launch_all(tensors, n_tensors, a, lanes, stream);
+}
+
+int order_all(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, int* list, int* starts) {
+  if (const int rc = check_apart(tensors, n_tensors, n_items)) return rc;
+  Args<1> a = {};
+  int threads = THREADS, lanes = 0;
+  const int blocks = lay_out(tensors, n_tensors, a, threads);
+  if (blocks < 0) return blocks;
+  const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), reinterpret_cast<int4*>(list), starts, &lanes);
+  return rc < 0 ? rc : lanes;
+}
+
+// {address, bytes} of dense tensors [slots, ...] as tensors of items.
+std::vector<DkCopyTensor> dense(const long long* pairs, int n, long long slots) {
+  std::vector<DkCopyTensor> out(n);
+  for (int k = 0; k < n; ++k) {
+    const long long item = slots > 0 ? pairs[2 * k + 1] / slots : 0;
+    out[k] = {(void*)pairs[2 * k], item, 0, item > 0 ? 1 : 0, item < (1ll << 31) ? (int)item : -1, 0, 0};      // (-1: refused as a negative size)
+  }
+  return out;
+}
+
+template <typename F>
+int guarded(int n, F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    dk_set_error("copy_items: no memory on the host to order %d copies", n);
+    return DK_ERR_ARG;
+  }
 }
 }  // namespace
 
@@ -248,37 +321,26 @@ extern "C" int dk_copy_items_inline() { return INLINE; }
 
 // Puts n copies in order for a list on the device: list [n][4] ints and starts [n + 2].  Returns the number of lanes (0: nothing to copy) or a negative code.
 extern "C" int dk_copy_items_order(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items, int* list, int* starts) {
-  try {
-    Args<1> a = {};
-    int threads = THREADS, lanes = 0;
-    const int blocks = lay_out(tensors, n_tensors, a, threads);
-    if (blocks < 0) return blocks;
-    const int rc = order_copies(src, dst, tokens, n, n_items, tensors[0].tokens, lanes_for(blocks, n), reinterpret_cast<int4*>(list), starts, &lanes);
-    return rc < 0 ? rc : lanes;
-  } catch (const std::bad_alloc&) {
-    dk_set_error("copy_items: no memory on the host to order %d copies", n);
-    return DK_ERR_ARG;
-  }
+  return guarded(n, [&] { return order_all(tensors, n_tensors, src, dst, tokens, n, n_items, list, starts); });
 }
 
 // The copies of src and dst (host) when there are at most INLINE of them, else those of a list on the device that dk_copy_items_order made.
 extern "C" int dk_copy_items(const DkCopyTensor* tensors, int n_tensors, const int* src, const int* dst, const int* tokens, int n, long long n_items,
                              const int* list, const int* starts, int lanes, cudaStream_t stream) {
-  try {
-    if (list == nullptr) {
-      DK_REQUIRE(n <= INLINE, "copy_items: %d copies need a list on the device", n);
-      return n <= FEW ? copy_inline<FEW>(tensors, n_tensors, src, dst, tokens, n, n_items, stream)
-                      : copy_inline<INLINE>(tensors, n_tensors, src, dst, tokens, n, n_items, stream);
-    }
-    Args<1> a = {};
-    int threads = THREADS;
-    const int blocks = lay_out(tensors, n_tensors, a, threads);
-    if (blocks < 0) return blocks;
-    a.list = reinterpret_cast<const int4*>(list);
-    a.starts = starts;
-    return launch(a, blocks, lanes, threads, stream);
-  } catch (const std::bad_alloc&) {
-    dk_set_error("copy_items: no memory on the host to order %d copies", n);
-    return DK_ERR_ARG;
-  }
+  return guarded(n, [&] { return copy_all(tensors, n_tensors, src, dst, tokens, n, n_items, list, starts, lanes, stream); });
+}
+
+// The same two for dense tensors [slots, ...], each given by its address and bytes.
+extern "C" int dk_copy_slots_order(const long long* pairs, int n_tensors, const int* src, const int* dst, int n, long long slots, int* list, int* starts) {
+  return guarded(n, [&] {
+    const std::vector<DkCopyTensor> t = dense(pairs, n_tensors, slots);
+    return order_all(t.data(), n_tensors, src, dst, nullptr, n, slots, list, starts);
+  });
+}
+extern "C" int dk_copy_slots(const long long* pairs, int n_tensors, const int* src, const int* dst, int n, long long slots, const int* list, const int* starts, int lanes,
+                             cudaStream_t stream) {
+  return guarded(n, [&] {
+    const std::vector<DkCopyTensor> t = dense(pairs, n_tensors, slots);
+    return copy_all(t.data(), n_tensors, src, dst, nullptr, n, slots, list, starts, lanes, stream);
+  });
 }

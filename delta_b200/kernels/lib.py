@@ -170,6 +170,8 @@ _SIGNATURES = {
     "dk_copy_items_inline": [],
     "dk_copy_items_order": [P, I, P, P, P, I, L, P, P],
     "dk_copy_items": [P, I, P, P, P, I, L, P, P, I, P],
+    "dk_copy_slots_order": [P, I, P, P, I, L, P, P],
+    "dk_copy_slots": [P, I, P, P, I, L, P, P, I, P],
 }
 
 

@@ -1521,30 +1521,33 @@ def _address(a: array) -> int:
     return a.buffer_info()[0]
 
 
-def _copy_items(what: str, records, n_tensors: int, device, src, dst, tokens, n_items: int) -> None:
-    """records: five 64-bit numbers for each tensor, as ``DkCopyTensor`` in csrc/copy_items.cu has them."""
+def _copy_items(what: str, entry: str, table, n_tensors: int, device, src, dst, tokens, n_items: int) -> None:
+    """``table``: what the C entry (``dk_copy_items`` or ``dk_copy_slots``) takes of each tensor."""
     lib = _l.load()
     src, dst = _host_ints(src, "src"), _host_ints(dst, "dst")
-    n, counts = len(src), None
+    n, counts = len(src), ()
     if tokens is not None:
         tokens = _host_ints(tokens, "tokens")
-        counts = _address(tokens)
+        counts = (_address(tokens),)
+    elif entry == "dk_copy_items":
+        counts = (None,)
     if len(dst) != n or (tokens is not None and len(tokens) != n):
         raise KernelError(f"{what}: {n} sources, {len(dst)} targets" + (f", {len(tokens)} counts of tokens" if tokens is not None else ""))
     if n == 0:
         return
-    table = array("q", records)
+    copy, launches = getattr(lib, entry), -(-n_tensors // 32)
+    args = (_address(table), n_tensors, _address(src), _address(dst), *counts, n, n_items)
     if n <= _COPIES_INLINE:
-        _l.check(lib.dk_copy_items(_address(table), n_tensors, _address(src), _address(dst), counts, n, n_items, None, None, 0, _stream()), what)
+        _l.check(copy(*args, None, None, 0, _stream()), what, launches)
         return
     if torch.cuda.is_current_stream_capturing():
         raise KernelError(f"{what}: {n} copies go through a list that is made on the host; a captured call takes at most {_COPIES_INLINE}")
     order = torch.empty(5 * n + 2, dtype=torch.int32)
-    lanes = lib.dk_copy_items_order(_address(table), n_tensors, _address(src), _address(dst), counts, n, n_items, order.data_ptr(), order.data_ptr() + 16 * n)
+    lanes = getattr(lib, entry + "_order")(*args, order.data_ptr(), order.data_ptr() + 16 * n)
     _l.check(min(lanes, 0), what, 0)
     if lanes > 0:
         held = order.to(device)
-        _l.check(lib.dk_copy_items(_address(table), n_tensors, None, None, None, n, n_items, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what)
+        _l.check(copy(*args, held.data_ptr(), held.data_ptr() + 16 * n, lanes, _stream()), what, launches)
 
 
 _COPIES_INLINE = 1500    # copies that travel in a launch's arguments (csrc/copy_items.cu)
@@ -1574,24 +1577,24 @@ def copy_pages(pages, src, dst, *, tokens=None, token_axis=None):
         if token_axis is None or not 0 <= token_axis < len(shape) - 2:
             raise KernelError(f"copy_pages: counts of tokens need the token axis of the layout {tuple(shape[2:])}, got {token_axis}")
         per_page, token_bytes = shape[2 + token_axis], pages.stride(2 + token_axis) * size
-    _copy_items("copy_pages", (at, item, item * n, _two_ints(layers, item), _two_ints(token_bytes, per_page)), 1, pages.device, src, dst, tokens, n)
+    record = array("q", (at, item, item * n, _two_ints(layers, item), _two_ints(token_bytes, per_page)))      # DkCopyTensor of csrc/copy_items.cu
+    _copy_items("copy_pages", "dk_copy_items", record, 1, pages.device, src, dst, tokens, n)
 
 
 def copy_slots(states, src, dst):
     """Copies slot ``src[i]`` to slot ``dst[i]`` of every tensor [slots, ...] in ``states``, as if all were read before any is written.  Slots are
-    host lists; no slot is the target of two.  One launch for up to 32 tensors."""
+    host lists; no slot is the target of two, and no two tensors share memory.  One launch for every 32 tensors."""
     states = list(states.values()) if isinstance(states, dict) else list(states)
-    records, slots, device = [], states[0].shape[0] if states and states[0].dim() else 0, _device_index() if states and states[0].is_cuda else -1
+    if not states:
+        return
+    first = states[0]
+    slots, device = first.shape[0] if first.dim() else -1, _device_index() if first.is_cuda else -2      # (-1 would be the CPU's)
+    pairs = []
     for s in states:
-        at = _table("copy_slots", s, "a state", s.dtype, device)
-        if s.dim() < 1 or s.shape[0] != slots:
+        if s.get_device() != device or not s.is_contiguous():
+            _table("copy_slots", s, "a state", s.dtype, device)
+        shape = s.shape
+        if not shape or shape[0] != slots:
             raise KernelError(f"copy_slots: states have shapes {[tuple(x.shape) for x in states]}; all need the same number of slots")
-        total = s.numel()
-        if total:
-            item = total // slots * s.element_size()
-            if item >= 1 << 31:
-                raise KernelError(f"copy_slots: a slot of {item} bytes is too large")
-            records += (at, item, 0, 1 | item << 32, 0)
-    for i in range(0, len(records), 160):      # 32 tensors a launch
-        part = records[i:i + 160]
-        _copy_items("copy_slots", part, len(part) // 5, states[0].device, src, dst, None, slots)
+        pairs += (s.data_ptr(), s.nbytes)
+    _copy_items("copy_slots", "dk_copy_slots", array("q", pairs), len(states), first.device, src, dst, None, slots)

@@ -77,3 +77,24 @@ def test_no_cpu_path():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(KernelError, match="no CPU path"):
         ops.attention_shared_prefix(q, q, torch.zeros(4, 2, 2, 8, 16), torch.zeros(2, 3, dtype=torch.int32), i, i, i[:2], i[:1], scale=1.0)
+
+
+@pytest.mark.parametrize("copies", [1, 4])
+def test_tensors_that_share_memory_are_refused(copies):
+    """Each would overwrite what the other still reads.  (The addresses are never followed here.)"""
+    a = np.arange(copies, dtype=np.int32)
+    out = np.zeros(5 * copies + 2, dtype=np.int32)
+
+    def call(*pairs):
+        table = np.array(pairs, dtype=np.int64)
+        to = a + copies
+        lanes = lib.load().dk_copy_slots_order(table.ctypes.data, len(pairs), a.ctypes.data, to.ctypes.data, copies, 8, out.ctypes.data, out.ctypes.data + 16 * copies)
+        lib.check(min(lanes, 0), "copy_slots", 0)
+        return lanes
+    assert call((4096, 64), (4160, 64), (8192, 800)) >= 1
+    assert call((4096, 64), (0, 0), (0, 0)) >= 1            # empty tensors
+    for pairs in [((4096, 64), (4096, 64)), ((4096, 64), (8192, 64), (4152, 64)), ((8192, 64), (4096, 8192))]:
+        with pytest.raises(KernelError, match="share memory"):
+            call(*pairs)
+    with pytest.raises(KernelError, match="no size that is taken"):
+        call((4096, 8 << 31))

@@ -128,3 +128,28 @@ def test_refusals():
         ops.copy_slots([x, x[:1]], [0], [1])
     ops.copy_pages(x, [], [])
     ops.copy_slots([], [], [])
+
+
+def test_slots_that_share_memory_are_refused():
+    from delta_b200.kernels import ops
+    from delta_b200.kernels.lib import KernelError
+    x = torch.zeros(8, 4, device="cuda")
+    keep = x.clone()
+    for states in ([x, x], {0: x, 1: torch.zeros(8, 2, device="cuda"), 2: x.view(8, 2, 2)}, [x, x.view(-1)[4:28].view(8, 3)]):
+        with pytest.raises(KernelError, match="share memory"):
+            ops.copy_slots(states, [0], [1])
+    assert torch.equal(x, keep)
+
+
+def test_many_slots_of_many_tensors():
+    """More copies than travel in a launch's arguments, more tensors than one launch takes."""
+    from delta_b200.kernels import ops
+    rnd = random.Random(5)
+    states = [torch.randn(4000, 1 + i % 5, device="cuda") for i in range(40)]
+    want = [s.clone() for s in states]
+    dst = rnd.sample(range(4000), 2500)
+    src = [rnd.randrange(4000) for _ in dst]
+    for w, s in zip(want, states):
+        w[dst] = s[src]
+    ops.copy_slots(states, src, dst)
+    assert all(torch.equal(a, b) for a, b in zip(states, want))
