@@ -12,8 +12,13 @@
 // This file holds the merge and the kernel on the FMA units: 32-bit keys and values, and every head size and page
 // size that the kernels on the tensor cores (attention_shared_prefix_tc.cu, attention_shared_prefix_rows.cu) do not take.  A block of 128 threads
 // keeps 32 queries; K and V of a tile of 32 keys lie in shared memory as floats, and those of the next tile are on their way while this one is
-// computed.  A thread has four queries and two keys of the scores, then four queries and eight columns of the result (five 16-byte wavefronts of shared
-// memory for 32 FMAs).  Threads without a query only fetch.  The FMA units bound it, and in a short call the instructions' first fetch: its loops are rolled.
+// computed.  A thread has four queries and two keys of the scores, then four queries and eight columns of the result, two products to an instruction.
+//
+// 8 rows of 32 query heads on 4 of 128 behind 2,048 shared keys: 34.5 us.  Of these 2.7 go into the tables, 1 into the list of pieces, 5 until the first
+// keys are there, 7.5 into a tile with two or three blocks to an SM, 2 into a piece's results and 5 into the merge.  32 rows behind 4,096 keys: 132 us, a quarter of
+// the FMA units' rate: latency of shared memory between four barriers a tile, which three warps to a scheduler do not hide.  (A fourth block to an SM: 40 us for
+// the small call, since its ranges are half as long and the merge reads twice the pieces.  Weights kept twice, ready to be multiplied in pairs: 36.4.  Loops rolled
+// to two steps: 35.7 and 142.)
 #include "shared_prefix.cuh"
 #include "mma_helpers.cuh"
 
@@ -32,6 +37,7 @@ constexpr int KT = 32;        // keys of a tile
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int SHARE = 16;     // threads that share four queries
 constexpr int P_STRIDE = QR + 4;
+constexpr int BLOCKS = 3;     // of an SM
 
 // rows four floats apart from a multiple of 32: threads that read neighbouring rows meet no bank twice
 __host__ __device__ constexpr int row_stride(int hd) { return hd + 4; }
@@ -48,9 +54,32 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
   return make_float4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
 }
 
+// Two floats in one register pair: a product and a sum of both is one instruction.
+using two = unsigned long long;
+__device__ __forceinline__ two pack(float a, float b) {
+  two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ two fma2(two a, two b, two c) {
+  two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ two mul2(two a, two b) {
+  two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // HDM: the head size rounded up to 64, 128 or 256 (sizes the registers)
 template <typename T, int HDM>
-__global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
+__global__ void __launch_bounds__(THREADS, HDM <= 128 ? BLOCKS : 1) attention_shared_prefix_kernel(const DkSharedPrefixParams p) {
   constexpr int OC = HDM <= 64 ? 1 : HDM / 64;     // groups of four output columns of a thread
   extern __shared__ __align__(16) float smem[];
   const int hd = p.hd, ks = row_stride(hd);
@@ -61,7 +90,7 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
   __shared__ GroupPiece list[CAP];
   __shared__ long long s_row[2][KT];   // where a key's row of K begins in the cache, -1: there is none; of this tile and the next
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = tid / SHARE * 4, c = tid % SHARE;
-  const int G = p.G;
+  const int G = p.G, inv_g = 65535 / G + 1;        // x / G = x * inv_g >> 16 for the x below QR
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
   Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
@@ -104,23 +133,15 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
     const GroupPiece w = list[at++];
     const int rows = w.rows * G;
     auto row_at = [&](int k) { return of_group ? p.members[w.first + k] : w.first; };
-#pragma unroll 1
-    for (int qr = warp; qr < rows; qr += WARPS) {
-      const int row = row_at(qr / G);
-      for (int col = lane * 4; col < hd; col += 128) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (row >= 0 && row < p.rows) v = load4(reinterpret_cast<const T*>(p.q) + row * p.q_stride + (w.kvh * G + qr % G) * hd + col);
-        *reinterpret_cast<float4*>(s_q + qr * ks + col) = v;
-      }
-    }
     const int* table = p.block_table + (size_t)w.table_row * p.max_pages;
-    float o[4][OC][4], m_run[4], l_run[4];
+    two o[4][OC][2];
+    float m_run[4], l_run[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       m_run[i] = -INFINITY;
       l_run[i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < OC; ++k) o[i][k][0] = o[i][k][1] = o[i][k][2] = o[i][k][3] = 0.f;
+      for (int k = 0; k < OC; ++k) o[i][k][0] = o[i][k][1] = 0;
     }
     auto look_up = [&](int kb, int which) {       // by the first KT threads
       if (tid >= KT) return;
@@ -145,8 +166,24 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
       cp_async_commit();
     };
     const long long values = (long long)p.KV * p.ps * hd;        // from a key's row to its value's
+    int q_row[QR / WARPS];        // asked for with the first pages
+#pragma unroll
+    for (int i = 0; i < QR / WARPS; ++i) {
+      const int qr = warp + i * WARPS;
+      q_row[i] = qr < rows ? row_at(qr * inv_g >> 16) : -1;
+    }
     look_up(w.key0, 0);
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QR / WARPS; ++i) {        // the queries, on their way with the first keys
+      const int qr = warp + i * WARPS, row = q_row[i];
+      const bool there = row >= 0 && row < p.rows;
+      const T* src = reinterpret_cast<const T*>(p.q) + (there ? row * p.q_stride + (w.kvh * G + qr - (qr * inv_g >> 16) * G) * hd : 0);
+      for (int col = lane * 4; col < hd; col += 128) {
+        if constexpr (sizeof(T) == 4) cp_async_16(smem_u32(s_q + qr * ks + col), src + col, there);
+        else *reinterpret_cast<float4*>(s_q + qr * ks + col) = there ? load4(src + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
     fetch(s_k, 0, 0);
     fetch(s_v, 0, values);
     int which = 0;
@@ -158,20 +195,28 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
       __syncthreads();        // the keys are there
       float s[4][2];
       if (busy) {
+        two t[4][2];        // even and odd places of the head apart
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
-#pragma unroll 2
+        for (int i = 0; i < 4; ++i) t[i][0] = t[i][1] = 0;
+#pragma unroll 8
         for (int d = 0; d < hd; d += 4) {
-          float4 a[4], b[2];
+          ulonglong2 a[4], b[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(s_q + (q4 + i) * ks + d);
+          for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(s_q + (q4 + i) * ks + d);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const float4*>(s_k + (c + j * SHARE) * ks + d);
+          for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(s_k + (c + j * SHARE) * ks + d);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+            for (int j = 0; j < 2; ++j) t[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, t[i][j]));
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 v = unpack(t[i][j]);
+            s[i][j] = v.x + v.y;
+          }
       }
       __syncthreads();        // the keys are no longer read
       fetch(s_k, which ^ 1, 0);
@@ -192,31 +237,32 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
           s[i][0] = exp2f(s[i][0] - m_use);
           s[i][1] = exp2f(s[i][1] - m_use);
           l_run[i] = l_run[i] * keep + (s[i][0] + s[i][1]);
+          const two keep2 = pack(keep, keep);
 #pragma unroll
-          for (int k = 0; k < OC; ++k)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) o[i][k][d] *= keep;
+          for (int k = 0; k < OC; ++k) {
+            o[i][k][0] = mul2(o[i][k][0], keep2);
+            o[i][k][1] = mul2(o[i][k][1], keep2);
+          }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) *reinterpret_cast<float4*>(s_p + (c + j * SHARE) * P_STRIDE + q4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float4*>(s_p + (c + j * SHARE) * P_STRIDE + q4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
       }
       cp_async_wait<1>();
       __syncthreads();        // the values and the weights are there
       if (busy) {
-#pragma unroll 2
+#pragma unroll 8
         for (int key = 0; key < KT; ++key) {        // (behind the last key weights and values are zeros)
-          const float4 e = *reinterpret_cast<const float4*>(s_p + key * P_STRIDE + q4);
+          const float4 x = *reinterpret_cast<const float4*>(s_p + key * P_STRIDE + q4);
+          const two e[4] = {pack(x.x, x.x), pack(x.y, x.y), pack(x.z, x.z), pack(x.w, x.w)};
 #pragma unroll
           for (int k = 0; k < OC; ++k)
             if (k * 64 + c * 4 < hd) {
-              const float4 v = *reinterpret_cast<const float4*>(s_v + key * ks + k * 64 + c * 4);
+              const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(s_v + key * ks + k * 64 + c * 4);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float f = i == 0 ? e.x : i == 1 ? e.y : i == 2 ? e.z : e.w;
-                o[i][k][0] = fmaf(f, v.x, o[i][k][0]);
-                o[i][k][1] = fmaf(f, v.y, o[i][k][1]);
-                o[i][k][2] = fmaf(f, v.z, o[i][k][2]);
-                o[i][k][3] = fmaf(f, v.w, o[i][k][3]);
+                o[i][k][0] = fma2(e[i], v.x, o[i][k][0]);
+                o[i][k][1] = fma2(e[i], v.y, o[i][k][1]);
               }
             }
         }
@@ -225,75 +271,89 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? 3 : 1) attention_shared_
       fetch(s_v, which ^ 1, values);
     }
     cp_async_wait<0>();
+    // a query's columns and a column's queries lie one step apart
     float* part = of_group ? group_results(p, w.id) : row_results(p, w.id);
+    const int per_query = of_group ? 4 : hd, per_column = of_group ? QR : 1;
+    float* to = part + q4 * per_query + c * 4 * per_column;
+    float* ml = part + (of_group ? QR : G) * hd + (of_group ? 4 : 2) * q4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int x = 1; x < SHARE; x <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], x);
-      const int r = q4 + i;
-      if (r < rows) {
+      if (q4 + i < rows) {
 #pragma unroll
         for (int k = 0; k < OC; ++k)
-          if (k * 64 + c * 4 < hd)
-            *reinterpret_cast<float4*>(part + (of_group ? ((size_t)(k * 16 + c) * QR + r) * 4 : (size_t)r * hd + k * 64 + c * 4)) =
-                make_float4(o[i][k][0], o[i][k][1], o[i][k][2], o[i][k][3]);
-        if (c == 0) *reinterpret_cast<float2*>(part + (of_group ? (size_t)QR * hd + 4 * r : (size_t)G * hd + 2 * r)) = make_float2(m_run[i], l_run[i]);
+          if (k * 64 + c * 4 < hd) *reinterpret_cast<ulonglong2*>(to + i * per_query + k * 64 * per_column) = make_ulonglong2(o[i][k][0], o[i][k][1]);
+        if (c == 0) *reinterpret_cast<float2*>(ml + i * (of_group ? 4 : 2)) = make_float2(m_run[i], l_run[i]);
       }
     }
     __syncthreads();          // the queries may be overwritten
   }
 }
 
-// One block per (key-value head, row): thread (column group, head), heads fastest.
+// One block per (key-value head, row, eight groups of four columns): thread (head, column group, lane), heads fastest.  A lane takes every ``lanes``-th
+// piece, eight at a time; the lanes' results are joined in their order.
+constexpr int MERGE_COLS = 8, MERGE_THREADS = 256;
 template <typename T>
-__global__ void attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p) {
-  const int kvh = blockIdx.x, row = blockIdx.y, G = p.H / p.KV;
+__global__ void __launch_bounds__(MERGE_THREADS) attention_shared_prefix_merge_kernel(const DkSharedPrefixParams p) {
+  const int kvh = blockIdx.x, row = blockIdx.y, G = p.G;
+  __shared__ float4 s_o[MERGE_THREADS];
+  __shared__ float2 s_ml[MERGE_THREADS];
+  const int places = G * MERGE_COLS, lanes = MERGE_THREADS / places, place = threadIdx.x % places, lane = threadIdx.x / places, g = place % G,
+            c4 = blockIdx.z * MERGE_COLS + place / G;
+  const bool mine = c4 * 4 < p.hd && lane < lanes;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const RowPiece w = row_pieces(p)[row * p.KV + kvh];
   const long long gs = group_piece_floats(QR, p.hd), rs = row_piece_floats(G, p.hd);
   const float* gp = group_results(p, w.group_id);
   const float* rp = row_results(p, w.first_id);
-  for (int x = threadIdx.x; x < G * (p.hd / 4); x += blockDim.x) {
-    const int g = x % G, c4 = x / G;
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float2 ml, const float4 o) {
-      const float m_new = fmaxf(M, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float keep = exp2f(M - m_use), f = exp2f(ml.x - m_use);
-      M = m_new;
-      L = L * keep + ml.y * f;
-      acc.x = acc.x * keep + o.x * f;
-      acc.y = acc.y * keep + o.y * f;
-      acc.z = acc.z * keep + o.z * f;
-      acc.w = acc.w * keep + o.w * f;
-    };
-    constexpr int AT_ONCE = 8;        // pieces asked for together, added in order
-    for (int i = 0; i < w.group_n + w.pieces; i += AT_ONCE) {
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float2 ml, const float4 o) {
+    const float m_new = fmaxf(M, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float keep = exp2f(M - m_use), f = exp2f(ml.x - m_use);
+    M = m_new;
+    L = L * keep + ml.y * f;
+    acc.x = acc.x * keep + o.x * f;
+    acc.y = acc.y * keep + o.y * f;
+    acc.z = acc.z * keep + o.z * f;
+    acc.w = acc.w * keep + o.w * f;
+  };
+  if (mine) {
+    constexpr int AT_ONCE = 8;        // pieces asked for together
+    const int pieces = w.group_n + w.pieces;
+#pragma unroll 1
+    for (int i = lane; i < pieces; i += AT_ONCE * lanes) {
       float2 ml[AT_ONCE];
       float4 o[AT_ONCE];
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
-        const int n = i + j;
+        const int n = i + j * lanes;
         if (n < w.group_n) {
           ml[j] = *reinterpret_cast<const float2*>(gp + n * gs + (size_t)QR * p.hd + 4 * (w.r0 + g));
           o[j] = *reinterpret_cast<const float4*>(gp + n * gs + ((size_t)c4 * QR + w.r0 + g) * 4);
-        } else if (n < w.group_n + w.pieces) {
+        } else if (n < pieces) {
           ml[j] = *reinterpret_cast<const float2*>(rp + (n - w.group_n) * rs + (size_t)G * p.hd + 2 * g);
           o[j] = *reinterpret_cast<const float4*>(rp + (n - w.group_n) * rs + (size_t)g * p.hd + c4 * 4);
         }
       }
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j)
-        if (i + j < w.group_n + w.pieces) add(ml[j], o[j]);
+        if (i + j * lanes < pieces) add(ml[j], o[j]);
     }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
-    T* out = reinterpret_cast<T*>(p.out) + row * p.out_stride + (kvh * G + g) * p.hd + c4 * 4;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(out) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    } else {
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    }
+  }
+  s_o[threadIdx.x] = acc;
+  s_ml[threadIdx.x] = make_float2(M, L);
+  __syncthreads();
+  if (!mine || lane != 0) return;
+  for (int k = 1; k < lanes; ++k) add(s_ml[k * places + place], s_o[k * places + place]);
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);      // no key: zeros; a NaN stays one
+  T* out = reinterpret_cast<T*>(p.out) + row * p.out_stride + (kvh * G + g) * p.hd + c4 * 4;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(out) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   }
 }
 
@@ -322,13 +382,12 @@ int launch_sized(const DkSharedPrefixParams& p, cudaStream_t stream) {
   return launch<T, 256>(p, stream);
 }
 
-int fma_grid() { return 3 * dk_sm_count(); }
+int fma_grid() { return BLOCKS * dk_sm_count(); }
 
 int merge(const DkSharedPrefixParams& p, cudaStream_t stream) {
-  const int work = p.H / p.KV * (p.hd / 4);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.KV, p.rows);
-  cfg.blockDim = dim3(work < 32 ? 32 : (work > 512 ? 512 : (work + 31) / 32 * 32));
+  cfg.gridDim = dim3(p.KV, p.rows, cdiv(p.hd, 4 * MERGE_COLS));
+  cfg.blockDim = dim3(MERGE_THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // its launch overlaps the first kernel's end; it waits for its results
