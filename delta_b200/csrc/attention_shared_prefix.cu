@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(THREADS, HDM <= 128 ? BLOCKS : 1) attention_sh
   const float sl2 = p.scale * 1.4426950408889634f;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the merge may be put in place (it waits for this kernel's end)
   Cut cut(reinterpret_cast<int*>(smem), p.rows, p.groups);
-  auto tables = [&] { make_cut<true, KT, KT, 2, THREADS>(p, cut, tid, [] { __syncthreads(); }); };
+  auto tables = [&] { make_cut<KT, KT, 2, THREADS>(p, cut, tid); };
   tables();
   // every row's first piece for the merge
   if (blockIdx.x == 0)
@@ -405,7 +405,7 @@ int merge(const DkSharedPrefixParams& p, cudaStream_t stream) {
 }  // namespace
 
 namespace {
-int check_sizes(const DkSharedPrefixParams& p) {
+int check_sizes(DkSharedPrefixParams& p) {
   DK_REQUIRE(p.dtype == DK_F32 || p.dtype == DK_BF16, "attention_shared_prefix: unknown element type %d", p.dtype);
   DK_REQUIRE(p.rows >= 0 && p.rows <= MAX_ROWS && p.groups >= 0 && p.groups <= MAX_GROUPS && p.n_members >= 0 && p.n_members <= MAX_ROWS,
              "attention_shared_prefix: %d rows in %d groups with %d members; at most %d rows and %d groups are taken", p.rows, p.groups,
@@ -415,6 +415,7 @@ int check_sizes(const DkSharedPrefixParams& p) {
   DK_REQUIRE(p.hd >= 4 && p.hd <= 256 && p.hd % 4 == 0, "attention_shared_prefix: head size %d is no multiple of 4 up to 256", p.hd);
   DK_REQUIRE(p.ps >= 1 && p.max_pages >= 1 && p.num_pages >= 1 && (long long)p.max_pages * p.ps < (1ll << 30),
              "attention_shared_prefix: tables of %d pages of %d tokens", p.max_pages, p.ps);
+  if (p.n_members == 0) p.groups = 0;
   return 0;
 }
 
@@ -462,7 +463,14 @@ extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, voi
   long long need;
   int rc = sizes(p, &tc, &need);
   if (rc != 0 || rows == 0) return rc;
-  DK_REQUIRE(q && out && kv && block_table && kv_len && work && (groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
+  DK_REQUIRE(q && out && kv && block_table && kv_len && work && (p.groups == 0 || (members && group_start && group_prefix)), "attention_shared_prefix: a tensor is missing");
+  {
+    // a row's pieces are read and written in no order
+    const long long size = dtype == DK_F32 ? 4 : 2, row = (long long)H * hd, away = ((const char*)out - (const char*)q) / size;
+    const bool apart = away >= (rows - 1) * q_stride + row || -away >= (rows - 1) * out_stride + row;
+    const long long in_row = q_stride > 0 ? ((away % q_stride) + q_stride) % q_stride : 0;
+    DK_REQUIRE(apart || (q_stride == out_stride && in_row >= row && in_row + row <= q_stride), "attention_shared_prefix: the results would overwrite queries that are still read");
+  }
   DK_REQUIRE(work_floats >= need, "attention_shared_prefix: %lld floats of working memory are given, %lld are needed", work_floats, need);
   DK_REQUIRE(scale > 0.f, "attention_shared_prefix: the scale of the scores must be positive");
   DK_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)kv % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)work % 16) == 0,

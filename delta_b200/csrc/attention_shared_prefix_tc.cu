@@ -83,6 +83,7 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     int tile_base = 0, seg_base = 0;
+    bool out_of_order = false;
 #pragma unroll 1
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
@@ -92,7 +93,9 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
         b = p.group_start[g + 1];
         k = p.group_prefix[g];
       }
-      if (a < 0 || b < a || b > p.n_members || k < 0 || k > max_keys) a = b = k = 0;
+      const bool bad = a < 0 || b < a || b > p.n_members;
+      out_of_order |= __any_sync(0xffffffffu, bad);
+      if (bad || k < 0 || k > max_keys) a = b = k = 0;
       k &= -p.ps;               // whole pages (a power of two)
       const int tiles = (long long)(b - a - 1) * k >= p.min_saved ? cdiv(k, KT) : 0, segs = tiles > 0 ? few(b - a, p.rpt) * p.KV : 0;
       int at = segs * tiles, seg = segs;
@@ -126,6 +129,7 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
       seg_base += seg_end;
     }
     if (pass == 0) {
+      if (out_of_order) tile_base = seg_base = 0;      // as make_cut has it
       Q = range_tiles(p, tile_base, seg_base);
       ranges = cdiv(tile_base, Q);
       lo = range * Q;
@@ -141,7 +145,7 @@ template <int HD>
 __device__ void prepare_rows(const DkSharedPrefixParams& p, int* tables, int tid) {
   for (int i = tid; i < p.rows * p.KV; i += THREADS) counters(p)[i] = 0;
   Cut cut(tables, p.rows, p.groups);
-  make_cut<true, KT, ROWS_KT, MIN_ROW_TILES, THREADS>(p, cut, tid, [] { __syncthreads(); });
+  make_cut<KT, ROWS_KT, MIN_ROW_TILES, THREADS>(p, cut, tid);
   for (int id = tid; id < cut.pieces; id += THREADS) row_pieces(p)[id] = row_piece<KT, ROWS_KT>(p, cut, id);
   if (tid == 0) *reinterpret_cast<int*>(p.work) = cut.pieces;
   __threadfence();

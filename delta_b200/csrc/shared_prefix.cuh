@@ -152,17 +152,20 @@ __device__ __forceinline__ void scan(const int* v, int* before, int* total, int*
     }
 }
 
-// Fills in ``c`` by NT threads that ``sync`` synchronises.  ROWS: the rows as well; KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
-template <bool ROWS, int KT, int ROWS_KT, int MIN_ROW_TILES, int NT, typename Sync>
-__device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid, Sync sync) {
+// Fills in ``c`` by a block of NT threads.  KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
+// Starts of groups that are out of order or out of range could make groups overlap and pieces outnumber the work buffer: then there is no group, and every
+// row reads its keys alone.
+template <int KT, int ROWS_KT, int MIN_ROW_TILES, int NT>
+__device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid) {
+  const auto sync = [] { __syncthreads(); };
   const int max_keys = p.max_pages * p.ps;
   // what the steps below read is asked for at once
-  const int m_first = ROWS && tid < p.n_members && p.groups > 0 ? p.members[tid] : -1;
-  if (ROWS)
-    for (int r = tid; r < p.rows; r += NT) {
-      c.len[r] = p.kv_len[r];
-      c.member[r] = -1;
-    }
+  const int m_first = tid < p.n_members && p.groups > 0 ? p.members[tid] : -1;
+  for (int r = tid; r < p.rows; r += NT) {
+    c.len[r] = p.kv_len[r];
+    c.member[r] = -1;
+  }
+  bool out_of_order = false;
   for (int g = tid; g <= p.groups; g += NT) {
     int a = 0, b = 0, k = 0;
     if (p.groups > 0) a = p.group_start[g];
@@ -170,11 +173,10 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
       b = p.group_start[g + 1];
       k = p.group_prefix[g];
     }
-    if (a < 0 || a > p.n_members || (g < p.groups && (b < a || b > p.n_members || k < 0 || k > max_keys))) {
-      const bool at_start = a < 0 || a > p.n_members, at_end = b < a || b > p.n_members;
+    const bool at_start = a < 0 || a > p.n_members, at_end = g < p.groups && (b < a || b > p.n_members);
+    out_of_order |= at_start || at_end;
+    if (at_start || at_end || k < 0 || k > max_keys) {
       dk_report(p.err, DK_DEV_BAD_GROUP, g, at_start ? a : at_end ? b : k, at_start || at_end ? p.n_members : max_keys);
-      a = min(max(a, 0), p.n_members);
-      b = a;
       k = 0;
     }
     c.start[g] = a;
@@ -184,21 +186,25 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
       c.prefix[g] = (long long)(b - a - 1) * k >= p.min_saved ? k : 0;      // one row shares nothing, and what saves few keys is read by each row itself
     }
   }
-  sync();
-  if (ROWS) {
-    if (p.groups > 0) {
-      const int end = c.start[p.groups];
-      for (int m = tid; m < end; m += NT) {
-        if (m < c.start[0]) continue;
-        const int row = m == tid ? m_first : p.members[m];
-        if (row < 0 || row >= p.rows || atomicCAS(&c.member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, last_not_above(c.start, p.groups, m), row, p.rows);
-      }
+  if (__syncthreads_or(out_of_order)) {
+    for (int g = tid; g <= p.groups; g += NT) {
+      c.start[g] = 0;
+      if (g < p.groups) c.declared[g] = c.prefix[g] = 0;
     }
     sync();
   }
+  if (p.groups > 0) {
+    const int end = c.start[p.groups];
+    for (int m = tid; m < end; m += NT) {
+      if (m < c.start[0]) continue;
+      const int row = m == tid ? m_first : p.members[m];
+      if (row < 0 || row >= p.rows || atomicCAS(&c.member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, last_not_above(c.start, p.groups, m), row, p.rows);
+    }
+  }
+  sync();
   // neighbouring threads take neighbouring groups and rows
   const int g_per = cdiv(p.groups, NT), g0 = min(p.groups, tid * g_per), g1 = min(p.groups, g0 + g_per);
-  const int r_per = cdiv(p.rows, NT), r0 = ROWS ? min(p.rows, tid * r_per) : 0, r1 = ROWS ? min(p.rows, r0 + r_per) : 0;
+  const int r_per = cdiv(p.rows, NT), r0 = min(p.rows, tid * r_per), r1 = min(p.rows, r0 + r_per);
   auto segments = [&](int g) {
     const int n = c.start[g + 1] - c.start[g];
     return c.prefix[g] > 0 ? few(n, p.rpt) * p.KV : 0;
@@ -229,11 +235,11 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     v[2] += tiles;
     v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
   }
-  scan<ROWS ? 4 : 2, NT>(v, before, total, c.sums, tid, sync);
+  scan<4, NT>(v, before, total, c.sums, tid, sync);
   c.tiles = total[0];
   c.Q = range_tiles(p, total[0], total[1]);
   c.ranges = cdiv(total[0], c.Q);
-  if (ROWS) c.C = total[2] * p.KV <= MIN_ROW_TILES * p.rows_grid ? MIN_ROW_TILES : cdiv(total[2] * p.KV, p.rows_grid);
+  c.C = total[2] * p.KV <= MIN_ROW_TILES * p.rows_grid ? MIN_ROW_TILES : cdiv(total[2] * p.KV, p.rows_grid);
   for (int g = g0; g < g1; ++g) {
     c.tile[g] = before[0];
     c.seg[g] = before[1];
@@ -241,19 +247,17 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     before[0] += x * cdiv(c.prefix[g], KT);
     before[1] += x;
   }
-  if (ROWS) {
-    if (c.C != MIN_ROW_TILES) {
-      sync();                     // (the sums were read)
-      v[0] = 0;
-      for (int r = r0; r < r1; ++r) v[0] += cdiv(c.piece[r], c.C) * p.KV;
-      scan<1, NT>(v, before + 3, total + 3, c.sums, tid, sync);
-    }
-    c.pieces = total[3];
-    for (int r = r0; r < r1; ++r) {
-      const int n = cdiv(c.piece[r], c.C) * p.KV;
-      c.piece[r] = before[3];
-      before[3] += n;
-    }
+  if (c.C != MIN_ROW_TILES) {
+    sync();                     // (the sums were read)
+    v[0] = 0;
+    for (int r = r0; r < r1; ++r) v[0] += cdiv(c.piece[r], c.C) * p.KV;
+    scan<1, NT>(v, before + 3, total + 3, c.sums, tid, sync);
+  }
+  c.pieces = total[3];
+  for (int r = r0; r < r1; ++r) {
+    const int n = cdiv(c.piece[r], c.C) * p.KV;
+    c.piece[r] = before[3];
+    before[3] += n;
   }
   sync();
 }

@@ -68,7 +68,7 @@ def can_fuse_rope_append(ctx, H: int, KV: int, hd: int, ps: int, interleaved: bo
 
 def shares_prefixes(ctx, group: str, H: int, KV: int, hd: int) -> bool:
     """True when the step goes to the kernels that read shared leading pages once (rotary positions and the append come before them)."""
-    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and hd % 4 == 0 and hd <= 256
+    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and KV <= 128 and hd % 4 == 0 and hd <= 256 and ctx.num_rows <= 1024
 
 
 def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float) -> None:

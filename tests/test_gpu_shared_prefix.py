@@ -246,3 +246,62 @@ def test_refusals():
     empty = ops.attention_shared_prefix(c["q"][:0], out[:0], c["kv"], c["block_table"][:0], c["kv_len"][:0], c["members"][:0], c["group_start"][:1] * 0,
                                         c["group_prefix"][:0], scale=1.0)
     assert empty.numel() == 0
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("starts", [[0, 6, 0, 6], [6, 0, 6, 0], [2, 4, 3, 6], [0, 0, 7, 6], [0, -1, 3, 6]], ids=str)
+def test_starts_out_of_order_leave_no_group(dtype, starts):
+    """Groups that overlap would be more pieces than there is room for: none is taken, which is recorded, and every row reads its keys alone."""
+    from delta_b200.kernels import ops
+    from delta_b200.kernels.lib import KernelError
+    c = make(dtype, 32, 4, 128, 16, [(6, 320), (0, 320), (0, 320)], 1, [5, 6, 7, 8, 9, 150, 11], seed=14)
+    c["group_start"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    with pytest.raises(KernelError, match="share a prefix"):
+        call(c)
+    out = torch.full_like(c["q"], 7.0)
+    ops.attention_shared_prefix(out=out, **c)
+    off = (out.double().cpu() - reference(c)).abs().amax().item()
+    assert off <= tolerance(dtype, int(c["kv_len"].max())), off
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_groups_of_nobody(dtype):
+    c = make(dtype, 8, 2, 64, 16, [], 3, [1, 20, 150], seed=15)
+    c["group_start"], c["group_prefix"] = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (5, 4))
+    check(dtype, c)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_results_over_the_queries_are_refused(dtype):
+    from delta_b200.kernels.lib import KernelError
+    c = make(dtype, 8, 2, 64, 16, [(3, 64)], 1, [1, 20, 150, 9], seed=16)
+    n = c["q"].shape[0]
+    wide = torch.zeros(n + 1, 3 * 512, dtype=DT[dtype], device="cuda")
+    side = lambda at, first=0: wide[first:first + n, at:at + 512].unflatten(1, (8, 64))      # noqa: E731
+    side(512).copy_(c["q"])
+    c["q"] = side(512)
+    for out in (side(512), side(512, 1), side(256), side(1024 - 256), wide.view(-1)[512 + 1024:][:n * 1024].view(n, 1024)[:, :512].unflatten(1, (8, 64))):
+        with pytest.raises(KernelError, match="overwrite"):
+            call(c, out=out)
+    want = reference(c)
+    for out in (side(0), side(1024), side(1024, 1)):         # columns beside them are nobody's
+        got = call(c, out=out)
+        assert (got.double().cpu() - want).abs().amax().item() <= tolerance(dtype, int(c["kv_len"].max()))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("case", [(32, 4, 128, [(700, 4096), (300, 1504)], 24), (32, 16, 64, [(1000, 160)], 24), (8, 8, 64, [(2, 32)] * 500, 24)], ids=["ranges", "pieces", "groups"])
+def test_most_rows(dtype, case):
+    """As many rows as a call takes: blocks walk several ranges of groups and several lists of pieces."""
+    H, KV, hd, groups, loose = case
+    rnd = random.Random(17)
+    rows = sum(n for n, _ in groups) + loose
+    assert rows == 1024
+    c = make(dtype, H, KV, hd, 16, groups, loose, [rnd.choice((0, 1, 15, 16, 17, 40, 70)) for _ in range(rows)], seed=17)
+    got = call(c)
+    some = torch.tensor(rnd.sample(range(rows), 40))
+    part = dict(c, q=c["q"][some.cuda()], block_table=c["block_table"][some.cuda()], kv_len=c["kv_len"][some.cuda()])
+    off = (got[some.cuda()].double().cpu() - reference(part)).abs().amax().item()
+    assert off <= tolerance(dtype, int(c["kv_len"].max())), off
+    assert torch.isfinite(got.float()).all()
+    assert torch.equal(call(c), got)
