@@ -153,8 +153,7 @@ class ModelRunner:
             if g.spec.reach or len(layout) != 4 or layout[0] != 2 or layout[2] != PAGE:      # keys and values by head, all of them read
                 continue
             found = self.cache.shared_prefixes(name, [r.slot for r in rows])
-            saved = sum((len(members) - 1) * pages for members, pages in found) * g.pages[0, 0].numel() * g.pages.element_size()
-            if found and saved >= self.shared_prefix_min_bytes:
+            if found and sum((len(members) - 1) * pages for members, pages in found) * g.pages[0, 0].numel() * g.pages.element_size() >= self.shared_prefix_min_bytes:
                 out[name] = found
         return out
 
