@@ -18,7 +18,7 @@
 // keys are there, 7.5 into a tile with two or three blocks to an SM, 2 into a piece's results and 5 into the merge.  32 rows behind 4,096 keys: 132 us, a quarter of
 // the FMA units' rate: latency of shared memory between four barriers a tile, which three warps to a scheduler do not hide.  (A fourth block to an SM: 40 us for
 // the small call, since its ranges are half as long and the merge reads twice the pieces.  Weights kept twice, ready to be multiplied in pairs: 36.4.  Loops rolled
-// to two steps: 35.7 and 142.)
+// to two steps: 35.7 and 142.  Tiles of 64 keys with 4 x 4 scores to a thread and two blocks to an SM: 55 and 171.)
 #include "shared_prefix.cuh"
 #include "mma_helpers.cuh"
 
