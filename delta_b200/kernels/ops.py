@@ -1486,22 +1486,28 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
         raise KernelError(f"attention_shared_prefix: {rows} rows of heads of {hd} ({dtype}) do not fit pages {tuple(pages)} of {kv.dtype}, a table of "
                           f"{table_rows} rows, {kv_len.numel()} lengths, {groups} prefixes and {group_start.numel()} starts of groups")
     device = _device_index() if q.is_cuda else -1
-    qp, q_stride = _head_rows(what, q, "q", shape, dtype, device)
-    op, out_stride = _head_rows(what, out, "out", shape, dtype, device)
-    kvp = _table(what, kv, "kv", dtype, device)
-    bp = _table(what, block_table, "block_table", i32, device)
-    lp = _table(what, kv_len, "kv_len", i32, device)
-    mp = _table(what, members, "members", i32, device)
-    sp = _table(what, group_start, "group_start", i32, device)
-    pp = _table(what, group_prefix, "group_prefix", i32, device)
+    # the usual call in one test; else piece by piece, which says what is wrong
+    if (device >= 0 and q.get_device() == device and out.get_device() == device and out.dtype is dtype and out.shape == shape and q.is_contiguous()
+            and out.is_contiguous()):
+        q_stride = out_stride = H * hd
+    else:
+        q_stride, out_stride = _head_rows(what, q, "q", shape, dtype, device)[1], _head_rows(what, out, "out", shape, dtype, device)[1]
+    if not (device >= 0 and block_table.dtype is i32 and kv_len.dtype is i32 and members.dtype is i32 and group_start.dtype is i32 and group_prefix.dtype is i32
+            and kv.get_device() == device and block_table.get_device() == device and kv_len.get_device() == device and members.get_device() == device
+            and group_start.get_device() == device and group_prefix.get_device() == device and kv.is_contiguous() and block_table.is_contiguous()
+            and kv_len.is_contiguous() and members.is_contiguous() and group_start.is_contiguous() and group_prefix.is_contiguous()):
+        _table(what, kv, "kv", dtype, device)
+        for t, name in ((block_table, "block_table"), (kv_len, "kv_len"), (members, "members"), (group_start, "group_start"), (group_prefix, "group_prefix")):
+            _table(what, t, name, i32, device)
     ep = _table(what, err, "err", i32, device) if err is not None else None
     if work is None:
         floats = attention_shared_prefix_floats(rows, groups, n, H, KV, hd, ps, max_pages, num_pages, dtype)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
+        wp = work.data_ptr()
     else:
-        floats = work.numel()
-    wp = _table(what, work, "work", torch.float32, device)
-    _l.check(_l.load().dk_attention_shared_prefix(qp, q_stride, op, out_stride, kvp, bp, lp, mp, sp, pp, wp, floats, rows, groups, n, H, KV, hd, ps,
+        floats, wp = work.numel(), _table(what, work, "work", torch.float32, device)
+    _l.check(_l.load().dk_attention_shared_prefix(q.data_ptr(), q_stride, out.data_ptr(), out_stride, kv.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
+                                                  members.data_ptr(), group_start.data_ptr(), group_prefix.data_ptr(), wp, floats, rows, groups, n, H, KV, hd, ps,
                                                   max_pages, num_pages, scale, dtype_code(dtype), ep, _stream()), what, 2 if rows else 0)
     return out
 
