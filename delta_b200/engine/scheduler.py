@@ -23,7 +23,8 @@ everyone's decode token, and sizes the pool so that it can never run out
     generated token again as a decode row of its own, one per step, unsampled.
   * requests that begin alike (samples of one prompt, prompts with a common first part) are a ``Family``: while one of
     them computes what they share the others wait, and then they are forked from it (``CacheManager.fork``) instead of
-    computing it again.  When nobody holds it any more, the next one computes it.
+    computing it again.  When nobody holds it any more, the next one computes it.  Of families in one another (samples of
+    prompts with a common first part) the longest beginning that somebody has or computes counts.
 """
 from __future__ import annotations
 
@@ -233,6 +234,7 @@ class Scheduler:
         one more token; those of one source with one launch for all of them."""
         reserve = {n: 0 for n in self.cache.groups}
         wanted: Dict[tuple, List[Request]] = {}
+        begun: List[Family] = []      # whose beginning a request that is forked now will go on to compute
         room = min(self.max_batch - len(self.running), self.cache.free_slots)
         for r in self.waiting:
             if room < 1:
@@ -240,11 +242,14 @@ class Scheduler:
             for f in r.families:
                 source = next((m for m in f.members if m.status == RUNNING and m.computed >= f.shared and self.cache.can_fork(m.slot, f.shared)), None)
                 if source is None:
+                    if f in begun or any(m.status == RUNNING and m.computed < f.shared for m in f.members):
+                        break         # more than a shorter family has is being computed: it is waited for
                     continue
                 need = {n: self._pages(g, r.total_len + 1) - f.shared // g.page_size if not g.spec.reach else self._pages(g, r.total_len + 1)
                         for n, g in self.cache.groups.items()}
                 if all(reserve[n] + need[n] <= g.pool.free_pages for n, g in self.cache.groups.items()):
                     wanted.setdefault((source.slot, f.shared), []).append(r)
+                    begun += [x for x in r.families if x.shared > f.shared]
                     room -= 1
                     for n in need:
                         reserve[n] += need[n]

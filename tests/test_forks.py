@@ -292,6 +292,23 @@ def test_families_under_a_short_pool():
         assert all(g.pool.held_pages == 0 for g in c.groups.values())
 
 
+@pytest.mark.parametrize("budget", [8, 16, 64, 512])
+@pytest.mark.parametrize("states", [False, True])
+def test_samples_of_prompts_with_a_common_first_part(budget, states):
+    """Two families in one another: the common part is computed once, then every prompt's rest once, and its samples wait for it."""
+    c = manager(num_pages=300, max_slots=12, states={"s": StateSpec((2,), torch.float32, 0.0)} if states else None)
+    s = Scheduler(c, max_batch=12, max_tokens_per_step=budget)
+    rs = []
+    for i in range(3):
+        mine = requests(s, [list(range(20)) + [100 * i + 60 + j for j in range(40)]] * 4, new=3)
+        s.relate(mine, 59)
+        rs += mine
+    s.relate(rs, 20)
+    done = run(s, c)
+    assert [done[r.id] for r in rs] == [60, 1, 1, 1, 40, 1, 1, 1, 40, 1, 1, 1]
+    assert s.stats["forks"] == 11 and all(r.status == FINISHED for r in rs)
+
+
 def test_a_follower_computes_for_itself_when_nobody_holds_the_beginning():
     c = manager(num_pages=64, max_slots=1)
     s = Scheduler(c, max_batch=1, max_tokens_per_step=64)

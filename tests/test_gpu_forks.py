@@ -73,6 +73,18 @@ def test_a_common_first_part(model_folders):
     assert outs == backend(model_folders["B"], page_size=8).generate([p for p in prompts[1:] for _ in range(2)], 10, temperature=0.7, seed=9)
 
 
+@pytest.mark.parametrize("budget", [32, 512])
+def test_samples_of_prompts_with_a_common_first_part_compute_each_once(model_folders, budget):
+    vocab = helpers.tiny_config("B")["vocab_size"]
+    common = helpers.random_tokens(50, vocab, 1)
+    prompts = [common + helpers.random_tokens(n, vocab, 60 + n) for n in (20, 7)]
+    e = backend(model_folders["B"], min_bytes=0, page_size=8, max_tokens_per_step=budget)
+    outs = e.generate(prompts, 6, samples=3, share_prefix=True, temperature=0.7, seed=9)
+    assert e.scheduler.stats["forks"] == 5 and e.scheduler.stats["prompt_tokens"] == 50 + 20 + 7 + 2 * 2
+    done(e)
+    assert outs == backend(model_folders["B"], page_size=8).generate([p for p in prompts for _ in range(3)], 6, temperature=0.7, seed=9)
+
+
 @pytest.mark.parametrize("design", list(DESIGNS))
 @pytest.mark.parametrize("graph", [False, True], ids=["eager", "graphs"])
 def test_every_design_can_be_forked(design, graph, tmp_path):
