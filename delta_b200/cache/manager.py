@@ -126,6 +126,13 @@ class CacheManager:
 
     def acquire_slot(self) -> int:
         """A free request slot with empty block tables and its state reset."""
+        slot = self._take_slot()
+        for k, s in self.state_specs.items():
+            self.states[k][slot] = s.fill
+        return slot
+
+    def _take_slot(self) -> int:
+        """A free slot with empty block tables; its state is what the last request left."""
         if not self._free_slots:
             raise RuntimeError("no free request slot")
         slot = self._free_slots.pop()
@@ -136,8 +143,6 @@ class CacheManager:
             g.table[slot].fill(-1)
             g.first_page[slot] = 0
             g.num_logical[slot] = 0
-        for k, s in self.state_specs.items():
-            self.states[k][slot] = s.fill
         return slot
 
     def release_slot(self, slot: int) -> None:
@@ -215,7 +220,7 @@ class CacheManager:
 
     def fork(self, slot: int, length: Optional[int] = None, count: int = 1) -> List[int]:
         """``count`` new requests that hold the first ``length`` tokens of a live one (all of them when None), as slots: the whole pages
-        are shared, the tokens of the last page and the states are copied, one launch for each.  The copies are enqueued on the
+        are shared, the tokens of the last page and the states are copied, one launch for each (states that are made anew are filled).  The copies are enqueued on the
         current stream.  All or nothing: ``OutOfPages`` and a lack of slots leave everything as it was."""
         length = int(self.seq_len[slot]) if length is None else int(length)
         if not self.can_fork(slot, length):
@@ -228,7 +233,7 @@ class CacheManager:
             if rest and count > g.pool.free_pages:
                 raise OutOfPages(f"out of cache pages in group {n}: {count} needed for the forks' last pages, {g.pool.free_pages} free")
         present = length == int(self.seq_len[slot])
-        new = [self.acquire_slot() for _ in range(count)]
+        new = [self._take_slot() for _ in range(count)]
         for g in self.groups.values():
             first = max(int(g.first_page[slot]), g.spec.first_needed(length) // g.page_size if g.spec.reach else 0)
             shared = g.table[slot, first:whole].tolist() if whole > first else []
@@ -245,6 +250,10 @@ class CacheManager:
                 self._copy_pages(g, [int(g.table[slot, whole])] * count, copies, [rest] * count)
         if self.states and present:
             self._copy_slots([slot] * count, new)
+        elif self.states and new:
+            at = torch.tensor(new, device=self.device)
+            for k, s in self.state_specs.items():
+                self.states[k].index_fill_(0, at, s.fill)
         for s in new:
             self.seq_len[s] = length
         return new

@@ -130,6 +130,34 @@ def test_fork_behind_a_window_and_with_states():
     m.check()
 
 
+@pytest.mark.parametrize("follow", [True, False])
+def test_a_fork_writes_each_state_tensor_once(follow):
+    """However many forks: one copy of the states (or one fill, where they are made anew), not a fill for every tensor and slot."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Writes(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func._schema.is_mutable:
+                self.ops.append((str(func), args[0].untyped_storage().data_ptr()))
+            return func(*args, **(kwargs or {}))
+    m = manager(num_pages=64, max_slots=12, states={k: StateSpec((3,), torch.float32, 0.5) for k in "abcde"}, states_follow_tokens=follow)
+    a = hold(m, 8)
+    for s in m.states.values():
+        s.copy_(torch.arange(13.0)[:, None].expand(13, 3))
+    with Writes() as w:
+        new = m.fork(a, 8 if follow else 4, 9)
+    storages = {s.untyped_storage().data_ptr() for s in m.states.values()}
+    assert len([x for x in w.ops if x[1] in storages]) == 5, w.ops
+    for s in m.states.values():
+        assert (s[new] == (float(a) if follow else 0.5)).all()
+        assert all((s[x] == float(x)).all() for x in range(13) if x not in new)
+    m.check()
+
+
 def test_shared_prefixes():
     m = manager(num_pages=64, max_slots=8)
     name, g = next(iter(m.groups.items()))
