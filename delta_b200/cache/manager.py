@@ -323,8 +323,8 @@ class CacheManager:
         moved = {p: q for p, q in zip((p for m in movable for p in m), places) if p != q}
         if not moved:
             return 0
+        g.pool.relocate(moved)          # (refuses, before anything is copied, what would overwrite a page that is held but stands in no table)
         self._copy_pages(g, list(moved), list(moved.values()), None)
-        g.pool.relocate(moved)
         new_id = np.arange(total + 1, dtype=np.int32)
         new_id[list(moved)] = list(moved.values())
         for s in slots:

@@ -233,6 +233,28 @@ def test_compaction_makes_runs():
     assert sum(scattered.compact().values()) == 0
 
 
+def test_compaction_that_is_refused_moves_nothing():
+    """Pages that are held but stand in no table may be a move's target: the pool refuses before any page is copied."""
+    m = manager(num_pages=32, max_slots=4, run_tokens=16)
+    name, g = next(iter(m.groups.items()))
+    foreign = g.pool.alloc(4)
+    a, b = m.acquire_slot(), m.acquire_slot()
+    pages = g.pool.alloc(16)
+    for i, s in enumerate((a, b)):
+        g.table[s, :8] = pages[i::2]
+        g.num_logical[s] = 8
+        m.seq_len[s] = 32
+    g.pages.copy_(torch.arange(33.0)[None, :, None, None, None, None].expand_as(g.pages))
+    before, table = g.pages.clone(), g.table.copy()
+    with pytest.raises(ValueError, match="cannot be moved"):
+        m.compact()
+    assert torch.equal(g.pages, before) and (g.table == table).all()
+    g.pool.check()
+    g.pool.free(foreign)
+    assert m.compact()[name] > 0
+    m.check()
+
+
 # ---------------------------------------------------------------- the scheduler
 
 def run(s, cache, tokens=lambda r: len(r.output), watch=None, steps=500):
