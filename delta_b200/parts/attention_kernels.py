@@ -37,6 +37,7 @@ TMA_MIN_TILES = int(os.environ.get("DELTA_B200_TMA_MIN_TILES", "16"))    # tiles
 TC_PREFILL_MIN_TOKENS = 32   # below this a 128-query tile of the tcgen05 kernel is mostly padding
 PARTIALS = "attention.decode_partials"
 SHARED_WORK = "attention.shared_prefix"
+SHARED_MAX_ROWS = 1024       # rows that one call over shared prefixes takes (csrc/shared_prefix.cuh)
 
 
 def decode_splits(rows: int, kv_heads: int, max_keys: int, sm_count: int, blocks_per_sm: int) -> int:
@@ -68,7 +69,7 @@ def can_fuse_rope_append(ctx, H: int, KV: int, hd: int, ps: int, interleaved: bo
 
 def shares_prefixes(ctx, group: str, H: int, KV: int, hd: int) -> bool:
     """True when the step goes to the kernels that read shared leading pages once (rotary positions and the append come before them)."""
-    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and KV <= 128 and hd % 4 == 0 and hd <= 256 and ctx.num_rows <= 1024
+    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and KV <= 128 and hd % 4 == 0 and hd <= 256 and ctx.num_rows <= SHARED_MAX_ROWS
 
 
 def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float) -> None:
@@ -78,7 +79,7 @@ def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float) -> 
 
     def floats(n, pages):
         return ops.attention_shared_prefix_floats(n, n // 2, n, H, KV, hd, cache.page_size, pages, cache.pages.shape[0], qkv.dtype)
-    work = ctx.scratch(SHARED_WORK, (floats(rows, max_pages),), torch.float32, bound=(floats(max(ctx.max_rows, rows), ctx.cache.max_pages_per_request),))
+    work = ctx.scratch(SHARED_WORK, (floats(rows, max_pages),), torch.float32, bound=(floats(max(rows, min(ctx.max_rows, SHARED_MAX_ROWS)), ctx.cache.max_pages_per_request),))
     ops.attention_shared_prefix(qkv[:, :H * hd].unflatten(1, (H, hd)), out.view(rows, H, hd), cache.pages, cache.block_table, t["kv_len"], t["members"],
                                 t["group_start"], t["group_prefix"], scale=scale, err=ctx.err, work=work)
 

@@ -172,6 +172,19 @@ def test_shared_pages_read_once_in_bfloat16(heads):
     assert off > 0           # two ways, not one
 
 
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graphs"])
+def test_an_engine_of_more_slots_than_a_call_takes_rows(model_folders, graph):
+    vocab = helpers.tiny_config("A")["vocab_size"]
+    prompt = helpers.random_tokens(40, vocab, 3)
+    e = backend(model_folders["A"], graph=graph, min_bytes=0, max_batch_size=1100, max_seq_length=64, num_pages=2000)
+    outs = e.generate([prompt], 6, samples=5, temperature=0.9, seed=4)
+    assert e.scheduler.stats["forks"] == 4
+    done(e)
+    assert outs == backend(model_folders["A"]).generate([prompt] * 5, 6, temperature=0.9, seed=4)
+    from delta_b200.parts.attention_kernels import SHARED_WORK
+    assert SHARED_WORK in e.runner._scratch
+
+
 def test_command_line(model_folders, tmp_path):
     out = tmp_path / "r.json"
     r = subprocess.run([sys.executable, "-m", "delta_b200.cli", "--model", str(model_folders["A"]), "--B", "6", "--max_len", "128", "--dataset", "random", "--num_samples",
