@@ -40,7 +40,7 @@ struct DkSharedPrefixParams {
 namespace shared_prefix {
 constexpr int MAX_ROWS = 1024, MAX_GROUPS = 1023, MAX_G = 32;
 constexpr int CAP = 48;            // tiles of a range, so also the most pieces of one
-
+constexpr int NOBODY = 0x7fffffff;
 
 __host__ __device__ constexpr int cdiv(int a, int b) { return (a + b - 1) / b; }
 // the same for a that seldom passes b (a division by a number the compiler does not know takes some hundred cycles)
@@ -108,7 +108,7 @@ __device__ __forceinline__ int last_not_above(const int* a, int n, int v) {
 // The tables of a call in shared memory, checked, and how they are cut.
 struct Cut {
   int *start, *prefix, *declared, *tile, *seg;      // groups: first member [groups + 1], keys read apart, keys said to be shared, first tile and segment in their line
-  int *member, *len, *own, *piece;                  // rows: place in members (-1: of no group), keys, keys read with the group, first piece
+  int *member, *len, *own, *piece;                  // rows: place in members (the first of several; NOBODY: of no group), keys, keys read with the group, first piece
   int* sums;
   int Q, tiles, ranges, C, pieces;                  // tiles of a range, tiles of the line, ranges; tiles of a row's piece, rows' pieces
   static __host__ __device__ constexpr int ints(int rows, int groups) { return 5 * groups + 1 + 4 * rows + 4 * 32; }
@@ -154,7 +154,7 @@ __device__ __forceinline__ void scan(const int* v, int* before, int* total, int*
 
 // Fills in ``c`` by a block of NT threads.  KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
 // Starts of groups that are out of order or out of range could make groups overlap and pieces outnumber the work buffer: then there is no group, and every
-// row reads its keys alone.
+// row reads its keys alone.  A row that is named twice belongs to its first place: every block that works the tables out finds the same pieces.
 template <int KT, int ROWS_KT, int MIN_ROW_TILES, int NT>
 __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid) {
   const auto sync = [] { __syncthreads(); };
@@ -163,7 +163,7 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
   const int m_first = tid < p.n_members && p.groups > 0 ? p.members[tid] : -1;
   for (int r = tid; r < p.rows; r += NT) {
     c.len[r] = p.kv_len[r];
-    c.member[r] = -1;
+    c.member[r] = NOBODY;
   }
   bool out_of_order = false;
   for (int g = tid; g <= p.groups; g += NT) {
@@ -198,7 +198,8 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     for (int m = tid; m < end; m += NT) {
       if (m < c.start[0]) continue;
       const int row = m == tid ? m_first : p.members[m];
-      if (row < 0 || row >= p.rows || atomicCAS(&c.member[row], -1, m) != -1) dk_report(p.err, DK_DEV_BAD_GROUP, last_not_above(c.start, p.groups, m), row, p.rows);
+      const int other = row < 0 || row >= p.rows ? -1 : atomicMin(&c.member[row], m);
+      if (other != NOBODY) dk_report(p.err, DK_DEV_BAD_GROUP, last_not_above(c.start, p.groups, max(m, other)), row, p.rows);
     }
   }
   sync();
@@ -218,7 +219,7 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
   for (int r = r0; r < r1; ++r) {
     const int m = c.member[r];
     int len = c.len[r], own = 0, said = 0;
-    if (m >= 0) {
+    if (m != NOBODY) {
       const int g = last_not_above(c.start, p.groups, m);
       if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
         own = c.prefix[g];

@@ -221,6 +221,38 @@ def test_wrong_tables_are_recorded(dtype):
     check(dtype, make(dtype, 32, 4, 128, 16, [(4, 320), (2, 64)], 1, [5, 6, 7, 8, 9, 150, 11], seed=11))
 
 
+def right_but_for(c, wrong=()):
+    """The call records an error and every row but ``wrong`` is what its keys give; twice the same bits."""
+    from delta_b200.kernels import ops
+    from delta_b200.kernels.lib import KernelError
+    with pytest.raises(KernelError, match="share a prefix|page id out of range"):      # (which comes first: a wrong first member's table is too short as well)
+        call(c)
+    outs = []
+    for _ in range(2):
+        outs.append(ops.attention_shared_prefix(out=torch.full_like(c["q"], 7.0), **c))
+    torch.cuda.synchronize()
+    keys = c["block_table"].shape[1] * c["kv"].shape[3]
+    ok = torch.tensor([r not in wrong and 0 <= n <= keys for r, n in enumerate(c["kv_len"].tolist())])
+    want = reference(dict(c, kv_len=torch.where(ok, c["kv_len"].cpu(), 0)))
+    off = (outs[0].double().cpu() - want)[ok].abs().amax().item()
+    assert off <= tolerance(str(c["q"].dtype)[6:], int(c["kv_len"].cpu()[ok].max())), off
+    assert torch.equal(outs[0][ok.cuda()], outs[1][ok.cuda()])         # (the others may be any bits)
+    return outs[0]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16), (4, 2, 16, 16)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("again", [(0, 9), (5, 9), (8, 0), (11, 10)], ids=str)
+def test_a_row_named_twice_spoils_no_other(dtype, shape, again):
+    """Place ``again[1]`` of the members names the row of place ``again[0]`` too: another place of its group, or of a group with another prefix."""
+    c = make(dtype, *shape, [(4, 1320), (4, 640), (4, 64)], 3, [random.Random(21).choice((1, 7, 40, 200)) for _ in range(15)], seed=21)
+    c["members"] = c["members"].clone()
+    row = int(c["members"][again[0]])
+    c["members"][again[1]] = row
+    # (a group reads its pages through its first member's table)
+    right_but_for(c, c["members"][:4].tolist() if again[1] == 0 else ())
+
+
 def test_refusals():
     from delta_b200.kernels import ops
     from delta_b200.kernels.lib import KernelError
