@@ -154,7 +154,8 @@ __device__ __forceinline__ void scan(const int* v, int* before, int* total, int*
 
 // Fills in ``c`` by a block of NT threads.  KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
 // Starts of groups that are out of order or out of range could make groups overlap and pieces outnumber the work buffer: then there is no group, and every
-// row reads its keys alone.  A row that is named twice belongs to its first place: every block that works the tables out finds the same pieces.
+// row reads its keys alone.  So does a row that is shorter than its group's prefix; one whose length fits no table reads nothing.  A row that is named twice belongs
+// to its first place: every block that works the tables out finds the same pieces.
 template <int KT, int ROWS_KT, int MIN_ROW_TILES, int NT>
 __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid) {
   const auto sync = [] { __syncthreads(); };
@@ -228,7 +229,8 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     }
     if (len < said || len > max_keys) {
       dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
-      c.len[r] = len = own;
+      own = 0;
+      if (len < 0 || len > max_keys) c.len[r] = len = 0;
     }
     c.own[r] = own;
     const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece

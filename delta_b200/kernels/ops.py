@@ -1473,8 +1473,9 @@ def attention_shared_prefix(q, out, kv, block_table, kv_len, members, group_star
     group g hold the same pages for their first ``group_prefix[g]`` tokens, of which the whole pages are shared and read through the table row
     of one of them.  A row of no group reads all of its keys alone; one of ``kv_len`` 0 gets zeros.  A request that brings several tokens has a
     row for each.  All tables are int32 on the device, so a captured call reads them anew at every replay; what does not fit
-    (a row out of range, a row shorter than its group's prefix, a bad page) is recorded in ``err``; a row named twice is too, and belongs to the
-    first group that names it.  Rows of other groups are what they are.
+    is recorded in ``err`` and touches no row of another group: a row named twice belongs to the first group that names it, one shorter than its
+    group's prefix reads its keys alone, one whose length is negative or beyond its table gets zeros, a member out of range is skipped, and
+    rows that read a page which does not exist have no result.
     Rows of ``q`` and ``out`` may lie apart.  Two products with float sums, the softmax in 32 bits; bfloat16 rounds the weights of the values once
     and the result once.  ``work``: at least ``attention_shared_prefix_floats`` float32 that no other call uses meanwhile (allocated here when None).
     """

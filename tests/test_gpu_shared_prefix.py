@@ -253,6 +253,19 @@ def test_a_row_named_twice_spoils_no_other(dtype, shape, again):
     right_but_for(c, c["members"][:4].tolist() if again[1] == 0 else ())
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16), (4, 2, 16, 16)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("length", [0, 1, 100, 639, -5, 1 << 30])
+def test_a_row_that_is_shorter_than_its_prefix_reads_its_keys_alone(dtype, shape, length):
+    c = make(dtype, *shape, [(4, 1320), (4, 640)], 2, [1, 7, 40, 200, 3, 90, 1, 300, 5, 66], seed=22, scattered=True)
+    row = int(c["members"][5])
+    c["kv_len"] = c["kv_len"].clone()
+    c["kv_len"][row] = length
+    out = right_but_for(c)
+    if length <= 0 or length > 5000:
+        assert (out[row] == 0).all()
+
+
 def test_refusals():
     from delta_b200.kernels import ops
     from delta_b200.kernels.lib import KernelError
