@@ -51,10 +51,11 @@ static_assert(sizeof(Args<FEW>) <= 4096 && sizeof(Args<INLINE>) <= 32764, "a ker
 
 template <int AHEAD, typename U>
 __device__ __forceinline__ void carry(const Tensor& t, const int4* list, int begin, int end) {
-  const int block = (int)blockIdx.x - t.first_block, layer = block / t.layer_blocks, unit = (block - layer * t.layer_blocks) * (int)blockDim.x + (int)threadIdx.x;
-  if (unit >= t.units) return;
+  const int block = (int)blockIdx.x - t.first_block, layer = block / t.layer_blocks;
+  const unsigned unit = (unsigned)(block - layer * t.layer_blocks) * blockDim.x + threadIdx.x;      // (an item may have 2^31 - 1 units, and its last block ends behind them)
+  if (unit >= (unsigned)t.units) return;
   char* place = t.base + layer * t.layer_stride + (long long)unit * sizeof(U);
-  const int token = t.units_per_token > 0 ? unit / t.units_per_token % t.tokens : 0;
+  const int token = t.units_per_token > 0 ? (int)(unit / (unsigned)t.units_per_token % (unsigned)t.tokens) : 0;
   U kept = U();
   for (int i = begin; i < end; i += AHEAD) {
     U v[AHEAD];
@@ -215,12 +216,12 @@ int lay_out(const DkCopyTensor* tensors, int n_tensors, Args<N>& a, int& threads
     t.tokens = x.tokens > 0 ? x.tokens : 1;
     if (t.units > most) most = t.units;
   }
-  threads = std::min(THREADS, (most + 31) / 32 * 32);
+  threads = most >= THREADS ? THREADS : (most + 31) / 32 * 32;
   long long blocks = 0;
   for (int k = 0; k < n_tensors; ++k) {
     Tensor& t = a.t[k];
     t.first_block = (int)blocks;
-    t.layer_blocks = std::max(1, (t.units + threads - 1) / threads);
+    t.layer_blocks = (int)std::max(1ll, (t.units + threads - 1ll) / threads);
     blocks += (long long)t.layers * t.layer_blocks;
     DK_REQUIRE(blocks < (1ll << 31) - 1, "copy_items: items of too many bytes");
   }

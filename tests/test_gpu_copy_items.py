@@ -153,3 +153,15 @@ def test_many_slots_of_many_tensors():
         w[dst] = s[src]
     ops.copy_slots(states, src, dst)
     assert all(torch.equal(a, b) for a, b in zip(states, want))
+
+
+def test_the_largest_slots():
+    """2^31 - 1 bytes that only fit byte by byte: the last block's places pass 2^31."""
+    n = (1 << 31) - 1
+    a = torch.zeros((2, n), dtype=torch.uint8, device="cuda")
+    a[0, ::997] = 7
+    a[0, -300:] = torch.arange(300, device="cuda").to(torch.uint8)
+    from delta_b200.kernels import ops
+    ops.copy_slots([a], [0], [1])
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], a[1]) and int(a[1, -1]) == 299 - 256
