@@ -221,7 +221,7 @@ int lay_out(const DkCopyTensor* tensors, int n_tensors, Args<N>& a, int& threads
   for (int k = 0; k < n_tensors; ++k) {
     Tensor& t = a.t[k];
     t.first_block = (int)blocks;
-    t.layer_blocks = (int)std::max(1ll, (t.units + threads - 1ll) / threads);
+    t.layer_blocks = (int)std::max(1ll, ((long long)t.units + threads - 1) / threads);
     blocks += (long long)t.layers * t.layer_blocks;
     DK_REQUIRE(blocks < (1ll << 31) - 1, "copy_items: items of too many bytes");
   }
