@@ -26,6 +26,7 @@
 bool dk_shared_prefix_tc_takes(const DkSharedPrefixParams& p);
 int dk_shared_prefix_tc_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
 // attention_shared_prefix_rows.cu
+unsigned long long dk_shared_prefix_call_number();
 int dk_shared_prefix_rows_tile();
 int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p);
 int dk_shared_prefix_rows_launch(const DkSharedPrefixParams& p, cudaStream_t stream);
@@ -477,6 +478,7 @@ extern "C" int dk_attention_shared_prefix(const void* q, long long q_stride, voi
              "attention_shared_prefix: tensors must start on 16-byte boundaries, rows on multiples of 4 entries");
   DK_REQUIRE(!tc || q_stride % 8 == 0, "attention_shared_prefix: rows of queries must lie a multiple of 8 entries apart, not %lld", q_stride);
   if (tc) {
+    p.call = dk_shared_prefix_call_number();
     rc = dk_shared_prefix_tc_launch(p, stream);
     return rc != 0 ? rc : dk_shared_prefix_rows_launch(p, stream);
   }

@@ -14,12 +14,14 @@
 // Behind a piece's last tile the pieces of its row's group are added to it, in the order of their keys: they come through the ring as well, up to eight
 // a stage, one box each.  (Of a segment that is cut, only the first piece adds them.)  The result is rounded once.  Where a segment is cut, each block
 // leaves its piece's results in the work buffer and counts itself; the one that comes last adds them all, in their order, so the result does not depend on
-// who that is.  This kernel starts while that one runs and waits for its end before it touches what it wrote; the list of pieces and the cleared counters
-// alone are there before: the block that writes them lets this kernel start when they are.
+// who that is.  This kernel starts while that one runs and waits for its end before it touches what it wrote, but for the list of pieces: the block that
+// writes it publishes it with a release of the call's number, and a block of this kernel that acquires that number may read the list; one that does not
+// waits for the other kernel's end.  The number is nobody else's, and it is taken back before this kernel ends, so a replayed call does not find its last one.
 #include "shared_prefix.cuh"
 #include "tcgen05_helpers.cuh"
 #include "mma_helpers.cuh"
 #include "ring.cuh"
+#include <atomic>
 
 namespace {
 using namespace shared_prefix;
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   __shared__ RowPiece list[LISTED];
   __shared__ float s_max[2][WARPS][ROWS], s_sum[2][WARPS][ROWS];      // in turns for the pieces
   __shared__ int s_last;
+  __shared__ bool listed;
   __shared__ volatile int failed, stuck;      // a wait of the producer, of one of the four warps gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
   const int ps = p.ps, G = p.G;
@@ -91,6 +94,9 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
       mbar_init(empty + 8 * s, WARPS);
     }
     failed = stuck = 0;
+    unsigned long long seen;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];\n" : "=l"(seen) : "l"(list_of_call(p)) : "memory");
+    listed = seen == p.call;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncthreads();
@@ -99,6 +105,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
   bool waited = false;
   // the pieces of a group in a stage: G queries each in a slot of its own
   const int slot_bytes = (G * 16 * (HD / 4 + 1) + 127) / 128 * 128, per_stage = min(MERGED, R::STAGE / slot_bytes);
+  if (!listed) asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int all_pieces = __ldcg(reinterpret_cast<const int*>(p.work));
   for (int first = blockIdx.x; first < p.row_pieces; first += gridDim.x * LISTED) {
     // (records behind the last piece are read with the others, so that nothing waits for the count, and not used)
@@ -424,6 +431,8 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
       break;
     }
   }
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");       // what follows this kernel follows the other one too
+  if (blockIdx.x == 0 && tid == 0) *list_of_call(p) = 0;
 }
 
 bool make_map_of_pieces(CUtensorMap* m, const float* base, int pieces, int G, int hd) {
@@ -477,6 +486,10 @@ int launch(const DkSharedPrefixParams& p, cudaStream_t stream) {
 }
 }  // namespace
 
+unsigned long long dk_shared_prefix_call_number() {
+  static std::atomic<unsigned long long> calls{0};
+  return 0x9e3779b97f4a7c15ull * (calls.fetch_add(1) + 1);       // (odd, so no two are alike; and never 0)
+}
 int dk_shared_prefix_rows_tile() { return TILE; }
 int dk_shared_prefix_rows_grid(const DkSharedPrefixParams& p) { return (p.hd == 128 && p.H / p.KV > 8 ? 1 : 2) * dk_sm_count(); }
 int dk_shared_prefix_rows_launch(const DkSharedPrefixParams& p, cudaStream_t stream) {

@@ -144,7 +144,7 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
   return last_seg - first_seg + 1;
 }
 
-// What the rows' kernel needs: its pieces, and the counters cleared.
+// What the rows' kernel needs: its pieces, and the counters cleared.  The list is published for its blocks that start before this kernel's end.
 template <int HD>
 __device__ void prepare_rows(const DkSharedPrefixParams& p, int* tables, int tid) {
   for (int i = tid; i < p.rows * p.KV; i += THREADS) counters(p)[i] = 0;
@@ -152,8 +152,12 @@ __device__ void prepare_rows(const DkSharedPrefixParams& p, int* tables, int tid
   make_cut<KT, ROWS_KT, MIN_ROW_TILES, THREADS>(p, cut, tid);
   for (int id = tid; id < cut.pieces; id += THREADS) row_pieces(p)[id] = row_piece<KT, ROWS_KT>(p, cut, id);
   if (tid == 0) *reinterpret_cast<int*>(p.work) = cut.pieces;
-  __threadfence();
   __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    asm volatile("st.release.gpu.global.u64 [%0], %1;\n" ::"l"(list_of_call(p)), "l"(p.call) : "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  }
 }
 
 template <int HD>
@@ -176,7 +180,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_prefix_tc_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x + 1 == gridDim.x) {
     prepare_rows<HD>(p, reinterpret_cast<int*>(smem), tid);
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     return;
   }
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // the rows' kernel may start wherever there is room, once its pieces are there

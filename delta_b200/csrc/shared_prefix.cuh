@@ -32,6 +32,7 @@ struct DkSharedPrefixParams {
   long long q_stride, out_stride;   // elements
   int rows, groups, n_members, H, KV, hd, ps, max_pages, num_pages, dtype;
   float scale;
+  unsigned long long call;          // set by the launcher: what says that this call's list of the rows' pieces is there (attention_shared_prefix_rows.cu)
   // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), query heads of a key-value head, rows of a
   // group's tile, the blocks that compute, the most pieces there can be, the keys that a group must save for its prefix to be read apart, and the tiles that a range of long segments has at least
   int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved, least_tiles;
@@ -64,7 +65,7 @@ constexpr int ROW_INTS = sizeof(RowPiece) / 4;
 __host__ __device__ __forceinline__ long long group_piece_floats(int qr, int hd) { return (long long)qr * (hd + 4); }
 __host__ __device__ __forceinline__ long long row_piece_floats(int G, int hd) { return ((long long)G * (hd + 2) + 3) / 4 * 4; }
 
-// The work buffer: how many pieces the rows have and their records, a counter per row and key-value head, the results of groups' pieces, of rows' pieces.
+// The work buffer: how many pieces the rows have, nothing, the call whose list this is (64 bits), their records, a counter per row and key-value head, the results of groups' pieces, of rows' pieces.
 __host__ __device__ __forceinline__ long long front_ints(const DkSharedPrefixParams& p) { return 4 + (long long)p.row_pieces * ROW_INTS; }
 // Fills in the most pieces that there can be with these sizes, whatever the device's tables say, and tells what they need.
 struct Bounds {
@@ -85,6 +86,7 @@ static inline Bounds bounds(DkSharedPrefixParams& p) {
   b.work_floats = front_ints(p) + round4(p.rows * p.KV) + group_pieces * group_piece_floats(p.qr, p.hd) + row_pieces * row_piece_floats(G, p.hd);
   return b;
 }
+__device__ __forceinline__ unsigned long long* list_of_call(const DkSharedPrefixParams& p) { return reinterpret_cast<unsigned long long*>(p.work + 2); }
 __device__ __forceinline__ RowPiece* row_pieces(const DkSharedPrefixParams& p) { return reinterpret_cast<RowPiece*>(p.work + 4); }
 __device__ __forceinline__ int* counters(const DkSharedPrefixParams& p) { return reinterpret_cast<int*>(p.work + front_ints(p)); }
 __host__ __device__ __forceinline__ float* group_results(const DkSharedPrefixParams& p, int id) {

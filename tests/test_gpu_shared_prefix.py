@@ -185,6 +185,43 @@ def test_same_bits_again_and_captured(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+def test_one_work_buffer_for_many_calls(dtype):
+    """Whatever an earlier call (or nobody) left in the working memory, a call takes its own list of pieces: eager ones, two recorded ones in turn."""
+    from delta_b200.kernels import ops
+    cases = [make(dtype, 32, 4, 128, 16, [(9, 1500), (4, 2000)], 1, [31 * i % 211 + 1 for i in range(14)], seed=30),
+             make(dtype, 32, 4, 128, 16, [(2, 4000)], 12, [17 * i % 907 + 1 for i in range(14)], seed=31, scattered=True),
+             make(dtype, 32, 4, 128, 16, [], 14, [61 * i % 1501 for i in range(14)], seed=32)]
+    want = [call(c).clone() for c in cases]
+    need = max(ops.attention_shared_prefix_floats(14, c["group_prefix"].numel(), c["members"].numel(), 32, 4, 128, 16, c["block_table"].shape[1], c["kv"].shape[0], c["kv"].dtype)
+               for c in cases)
+    work = torch.empty(need, device="cuda")
+    outs, graphs = [torch.empty_like(c["q"]) for c in cases], []
+
+    def run(i):
+        ops.attention_shared_prefix(out=outs[i], work=work, **cases[i])
+    for junk in (0, -1, 0x7F800001):
+        work.view(torch.int32).fill_(junk)
+        for i in (0, 1, 2, 1, 0, 0):
+            run(i)
+            assert torch.equal(outs[i], want[i])
+    for i in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(i)
+        graphs.append(g)
+    rnd = random.Random(33)
+    for n in range(60):
+        i = rnd.randrange(3)
+        outs[i].fill_(3.0)
+        if n % 4 == 0:
+            work.view(torch.int32).random_()
+        graphs[i].replay()
+        if n % 3 == 0:
+            run((i + 1) % 3)
+        assert torch.equal(outs[i], want[i])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_two_streams_at_once(dtype):
     cases = [make(dtype, 32, 4, 128, 16, [(8, 1500)], 1, [3 * i + 1 for i in range(9)], seed=s) for s in (9, 10)]
     want = [call(c).clone() for c in cases]
