@@ -133,7 +133,7 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
       seg_base += seg_end;
     }
     if (pass == 0) {
-      if (out_of_order) tile_base = seg_base = 0;      // as make_cut has it
+      if (out_of_order || tile_base > p.max_tiles) tile_base = seg_base = 0;      // as make_cut has it
       Q = range_tiles(p, tile_base, seg_base);
       ranges = cdiv(tile_base, Q);
       lo = range * Q;

@@ -35,7 +35,8 @@ struct DkSharedPrefixParams {
   unsigned long long call;          // set by the launcher: what says that this call's list of the rows' pieces is there (attention_shared_prefix_rows.cu)
   // set by the launcher: how the work is cut (queries and keys of a group's tile, keys of a row's), query heads of a key-value head, rows of a
   // group's tile, the blocks that compute, the most pieces there can be, the keys that a group must save for its prefix to be read apart, and the tiles that a range of long segments has at least
-  int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved, least_tiles;
+  // (and the tiles that the groups may have together: where the tables ask for more, every row reads its keys alone)
+  int qr, kt, rows_kt, G, rpt, grid, rows_grid, group_pieces, row_pieces, min_saved, least_tiles, max_tiles;
 };
 
 namespace shared_prefix {
@@ -68,6 +69,10 @@ __host__ __device__ __forceinline__ long long row_piece_floats(int G, int hd) { 
 // The work buffer: how many pieces the rows have, nothing, the call whose list this is (64 bits), their records, a counter per row and key-value head, the results of groups' pieces, of rows' pieces.
 __host__ __device__ __forceinline__ long long front_ints(const DkSharedPrefixParams& p) { return 4 + (long long)p.row_pieces * ROW_INTS; }
 // Fills in the most pieces that there can be with these sizes, whatever the device's tables say, and tells what they need.
+// Groups of n_g rows and k_g keys have ceil(n_g / rpt) ceil(k_g / kt) tiles for a key-value head, at most (n_g / rpt + 1) (k_g / kt + 1).  Their pages are
+// distinct, or some are held by two groups (a part of all rows shares more than all do): sum k_g <= 2 pool.  So the sum is at most
+// (n / rpt + 2 pool / longest) longest / kt and a tile for every segment, which is what the working memory is made for.  Tables that ask for more are right all the
+// same: their rows read alone.  (64 rows with tables of 131,072 tokens, 32 heads on 8 of 128, a pool of 262,144 tokens: 89 MB; with 32 groups of full tables 412.)
 struct Bounds {
   long long tiles, pieces, work_floats;
 };
@@ -75,11 +80,14 @@ static inline Bounds bounds(DkSharedPrefixParams& p) {
   Bounds b;
   const int G = p.G = p.H / p.KV, rpt = p.rpt = p.qr / G;
   const long long keys = (long long)p.max_pages * p.ps, segments = (long long)p.KV * (p.groups > 0 ? p.n_members / rpt + p.groups : 0);
-  const long long of_groups = segments * ((keys + p.kt - 1) / p.kt), capped = (of_groups + CAP - 1) / CAP;
+  const long long pool = (long long)p.num_pages * p.ps, longest = keys < pool ? keys : pool, any = segments * ((keys + p.kt - 1) / p.kt);
+  const long long held = segments + p.KV * ((p.n_members + rpt - 1) / rpt * ((longest + p.kt - 1) / p.kt) + (2 * pool + p.kt - 1) / p.kt);
+  const long long of_groups = any < held ? any : held, capped = (of_groups + CAP - 1) / CAP;
   const long long ranges = capped > p.grid ? capped : (of_groups < p.grid ? of_groups : (long long)p.grid);      // (no range is empty)
   const long long group_pieces = segments > 0 ? segments + ranges : 0;
   const long long row_pieces = (long long)p.rows * p.KV + p.rows_grid;      // a segment's last piece, and tiles / C of full ones, which are no more than blocks
-  b.tiles = of_groups + (long long)p.rows * p.KV * ((keys + p.rows_kt - 1) / p.rows_kt);
+  p.max_tiles = (int)of_groups;
+  b.tiles = any + (long long)p.rows * p.KV * ((keys + p.rows_kt - 1) / p.rows_kt);
   b.pieces = group_pieces + row_pieces;
   p.group_pieces = (int)group_pieces;
   p.row_pieces = (int)row_pieces;
@@ -213,34 +221,42 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     const int n = c.start[g + 1] - c.start[g];
     return c.prefix[g] > 0 ? few(n, p.rpt) * p.KV : 0;
   };
-  int v[4] = {0, 0, 0, 0}, before[4], total[4];
-  for (int g = g0; g < g1; ++g) {
-    const int x = segments(g);
-    v[0] += x * cdiv(c.prefix[g], KT);
-    v[1] += x;
-  }
-  for (int r = r0; r < r1; ++r) {
-    const int m = c.member[r];
-    int len = c.len[r], own = 0, said = 0;
-    if (m != NOBODY) {
-      const int g = last_not_above(c.start, p.groups, m);
-      if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
-        own = c.prefix[g];
-        said = c.declared[g];
+  int v[4], before[4], total[4];
+#pragma unroll 1
+  for (;;) {        // (once more where the groups' tiles are too many)
+    v[0] = v[1] = v[2] = v[3] = 0;
+    for (int g = g0; g < g1; ++g) {
+      const int x = segments(g);
+      v[0] += x * cdiv(c.prefix[g], KT);
+      v[1] += x;
+    }
+    for (int r = r0; r < r1; ++r) {
+      const int m = c.member[r];
+      int len = c.len[r], own = 0, said = 0;
+      if (m != NOBODY) {
+        const int g = last_not_above(c.start, p.groups, m);
+        if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
+          own = c.prefix[g];
+          said = c.declared[g];
+        }
       }
+      if (len < said || len > max_keys) {
+        dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
+        own = 0;
+        if (len < 0 || len > max_keys) c.len[r] = len = 0;
+      }
+      c.own[r] = own;
+      const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece
+      c.piece[r] = tiles;
+      v[2] += tiles;
+      v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
     }
-    if (len < said || len > max_keys) {
-      dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
-      own = 0;
-      if (len < 0 || len > max_keys) c.len[r] = len = 0;
-    }
-    c.own[r] = own;
-    const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece
-    c.piece[r] = tiles;
-    v[2] += tiles;
-    v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
+    scan<4, NT>(v, before, total, c.sums, tid, sync);
+    if (total[0] <= p.max_tiles) break;
+    sync();                     // (the sums and prefixes were read)
+    for (int g = g0; g < g1; ++g) c.declared[g] = c.prefix[g] = 0;
+    sync();
   }
-  scan<4, NT>(v, before, total, c.sums, tid, sync);
   c.tiles = total[0];
   c.Q = range_tiles(p, total[0], total[1]);
   c.ranges = cdiv(total[0], c.Q);

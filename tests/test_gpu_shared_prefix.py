@@ -347,6 +347,18 @@ def test_starts_out_of_order_leave_no_group(dtype, starts):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads", [(32, 4, 128), (4, 2, 16)], ids=str)
+def test_groups_over_the_same_pages(dtype, heads):
+    """32 groups of the same pages are more tiles than the pool has pages for: the rows read alone, and nothing is wrong.  Two groups of them are taken."""
+    for groups in (32, 2):
+        c = make(dtype, *heads, 16, [(64, 4000)], 2, [random.Random(i).choice((1, 9, 16, 30)) for i in range(66)], seed=34)
+        per = 64 // groups
+        c["group_start"] = torch.arange(0, 65, per, dtype=torch.int32, device="cuda")
+        c["group_prefix"] = torch.full((groups,), 4000, dtype=torch.int32, device="cuda")
+        check(dtype, c)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_groups_of_nobody(dtype):
     c = make(dtype, 8, 2, 64, 16, [], 3, [1, 20, 150], seed=15)
     c["group_start"], c["group_prefix"] = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (5, 4))

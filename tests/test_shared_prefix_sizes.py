@@ -42,3 +42,25 @@ def test_an_engine_of_many_slots(monkeypatch, max_rows):
     assert bound == ops.attention_shared_prefix_floats(most, most // 2, most, 2, 2, 64, 16, 64, 1000, torch.bfloat16) >= asked
     with pytest.raises(KernelError, match="at most 1024 rows"):
         ops.attention_shared_prefix_floats(1025, 4, 8, 2, 2, 64, 16, 64, 1000, torch.bfloat16)
+
+
+def megabytes(rows, keys, pool, dtype=torch.bfloat16, KV=8, H=32):
+    return ops.attention_shared_prefix_floats(rows, rows // 2, rows, H, KV, 128, 16, keys // 16, pool // 16, dtype) * 4 / 1e6
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_working_memory_goes_with_the_cache(dtype):
+    """Groups hold no more than the pool does: long tables over a small pool ask for no more than a tenth of one layer's share of it and a piece's results
+    (128 queries of 132 floats; 32 in 32 bits) for every segment and block."""
+    item = torch.empty((), dtype=dtype).element_size()
+    queries, grid = (128, 148) if dtype == torch.bfloat16 else (32, 444)
+    for rows, keys, pool in [(64, 131072, 262144), (64, 131072, 1 << 20), (256, 65536, 262144), (1024, 131072, 262144), (8, 8192, 65536)]:
+        layer = pool * 2 * 8 * 128 * item / 1e6
+        rpt = queries // 4
+        pieces = 8 * (rows // rpt + rows // 2) + grid + rows * 8 + 2 * grid
+        behind_all = rows // rpt * 8 * keys / (rpt * 4) / 48          # one group of all rows over the longest table, 48 tiles to a piece
+        assert megabytes(rows, keys, pool, dtype) < 0.1 * layer + (pieces + behind_all) * queries * 132 * 4 * 1.1 / 1e6
+    assert megabytes(64, 131072, 262144, dtype) < 0.4 * megabytes(64, 131072, 1 << 24, dtype)
+    # more rows or longer tables never ask for less: an engine's buffer is made for its largest step
+    sizes = [megabytes(r, k, 262144, dtype) for r in range(2, 200, 7) for k in (4096, 131072)]
+    assert all(a <= b for a, b in zip(sizes[::2], sizes[2::2])) and all(a <= b for a, b in zip(sizes[1::2], sizes[3::2])) and all(a <= b for a, b in zip(sizes[::2], sizes[1::2]))
