@@ -2,6 +2,7 @@
 the per-request state."""
 from __future__ import annotations
 
+import warnings
 from typing import Dict, Optional
 
 import torch
@@ -126,3 +127,15 @@ class StepContext:
             buf = torch.empty(max(n, count(bound) if bound is not None else 0, 1), dtype=dtype, device=self.device)
             self._scratch_pool[key] = buf
         return buf[:n].view(*shape)
+
+    def scratch_if_there(self, key: str, shape, dtype, bound=None) -> Optional[torch.Tensor]:
+        """``scratch`` for a path that a step can do without: None where the device has no memory left for it (the cache may hold
+        nearly all), then and in every later step, so that recorded and eager steps go the same way."""
+        declined = self._scratch_pool.setdefault("__declined__", set())
+        if key not in declined:
+            try:
+                return self.scratch(key, shape, dtype, bound)
+            except torch.OutOfMemoryError as e:
+                declined.add(key)
+                warnings.warn(f"no memory on the device for '{key}': steps go without it ({e})", RuntimeWarning, stacklevel=2)
+        return None

@@ -106,14 +106,14 @@ class GQAAttention(Mixer):
         qkv = linear.linear(ctx, x, self.w_qkv)
         table = self.position.table(x.device) if self.position is not None else None
         interleaved = bool(getattr(self.position, "interleaved", False))
-        shared = self.role == "full" and not self.window and attention_kernels.shares_prefixes(ctx, cache.group, H, KV, hd)
-        fuse = not shared and attention_kernels.can_fuse_rope_append(ctx, H, KV, hd, cache.page_size, interleaved)
+        shared = attention_kernels.shared_work(ctx, cache, H, KV, hd) if self.role == "full" and not self.window else None
+        fuse = shared is None and attention_kernels.can_fuse_rope_append(ctx, H, KV, hd, cache.page_size, interleaved)
         if not fuse:
             ops.rope_append(qkv, ctx.tok_pos, ctx.tok_row, cache.block_table, cache.pages if cache.writes else None, table,
                             H, KV, hd, cache.page_size, interleaved, err=ctx.err)
         out = torch.empty((T, H * hd), dtype=x.dtype, device=x.device)
-        if shared:
-            attention_kernels.run_shared(ctx, qkv, out, cache, H, KV, hd, self.scale)
+        if shared is not None:
+            attention_kernels.run_shared(ctx, qkv, out, cache, H, KV, hd, self.scale, shared)
             return linear.linear(ctx, out, self.w_o)
         selective = self.role != "full" and ctx.any_row_flag(ROW_DECODE)
         dump = lse = None

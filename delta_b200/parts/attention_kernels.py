@@ -67,19 +67,22 @@ def can_fuse_rope_append(ctx, H: int, KV: int, hd: int, ps: int, interleaved: bo
     return (ctx.decode_only and not plain(ctx) and not interleaved and ops.attention_decode_supported(ctx.dtype, H, KV, hd, ps))
 
 
-def shares_prefixes(ctx, group: str, H: int, KV: int, hd: int) -> bool:
-    """True when the step goes to the kernels that read shared leading pages once (rotary positions and the append come before them)."""
-    return group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and KV <= 128 and hd % 4 == 0 and hd <= 256 and ctx.num_rows <= SHARED_MAX_ROWS
-
-
-def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float) -> None:
-    """Attention of a step of single tokens over pages that rows share; ``qkv`` [rows, (H + 2 KV) hd] is rotated and appended already."""
-    t = ctx.shared[cache.group]
-    rows, max_pages = ctx.num_rows, ctx.max_pages
+def shared_work(ctx, cache, H: int, KV: int, hd: int):
+    """Working memory of the kernels that read shared leading pages once, made for the engine's largest step, where the step goes to them (rotary
+    positions and the append come before them).  None: it does not, or the device has not so much memory left, and every row reads its pages itself."""
+    rows = ctx.num_rows
+    if not (cache.group in ctx.shared and "attention" not in ctx.plain_kernels and H // KV <= 32 and KV <= 128 and hd % 4 == 0 and hd <= 256 and rows <= SHARED_MAX_ROWS):
+        return None
 
     def floats(n, pages):
-        return ops.attention_shared_prefix_floats(n, n // 2, n, H, KV, hd, cache.page_size, pages, cache.pages.shape[0], qkv.dtype)
-    work = ctx.scratch(SHARED_WORK, (floats(rows, max_pages),), torch.float32, bound=(floats(max(rows, min(ctx.max_rows, SHARED_MAX_ROWS)), ctx.cache.max_pages_per_request),))
+        return ops.attention_shared_prefix_floats(n, n // 2, n, H, KV, hd, cache.page_size, pages, cache.pages.shape[0], ctx.dtype)
+    most = floats(max(rows, min(ctx.max_rows, SHARED_MAX_ROWS)), ctx.cache.max_pages_per_request)
+    return ctx.scratch_if_there(SHARED_WORK, (floats(rows, ctx.max_pages),), torch.float32, bound=(most,))
+
+
+def run_shared(ctx, qkv, out, cache, H: int, KV: int, hd: int, scale: float, work) -> None:
+    """Attention of a step of single tokens over pages that rows share; ``qkv`` [rows, (H + 2 KV) hd] is rotated and appended already."""
+    t, rows = ctx.shared[cache.group], ctx.num_rows
     ops.attention_shared_prefix(qkv[:, :H * hd].unflatten(1, (H, hd)), out.view(rows, H, hd), cache.pages, cache.block_table, t["kv_len"], t["members"],
                                 t["group_start"], t["group_prefix"], scale=scale, err=ctx.err, work=work)
 

@@ -185,6 +185,27 @@ def test_an_engine_of_more_slots_than_a_call_takes_rows(model_folders, graph):
     assert SHARED_WORK in e.runner._scratch
 
 
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graphs"])
+def test_an_engine_without_room_for_the_working_memory(model_folders, graph, monkeypatch):
+    """Rows that share pages read them each for itself then."""
+    from delta_b200.engine.context import StepContext
+    from delta_b200.parts.attention_kernels import SHARED_WORK
+    have = StepContext.scratch
+
+    def scratch(self, key, *a, **k):
+        if key == SHARED_WORK:
+            raise torch.OutOfMemoryError("the device is full")
+        return have(self, key, *a, **k)
+    monkeypatch.setattr(StepContext, "scratch", scratch)
+    prompt = helpers.random_tokens(40, helpers.tiny_config("A")["vocab_size"], 3)
+    e = backend(model_folders["A"], graph=graph, min_bytes=0)
+    with pytest.warns(RuntimeWarning, match="no memory on the device"):
+        outs = e.generate([prompt], 8, samples=5, temperature=0.9, seed=4)
+    assert e.scheduler.stats["forks"] == 4 and not e.runner.graph_fallbacks
+    done(e)
+    assert outs == backend(model_folders["A"]).generate([prompt] * 5, 8, temperature=0.9, seed=4)
+
+
 def test_command_line(model_folders, tmp_path):
     out = tmp_path / "r.json"
     r = subprocess.run([sys.executable, "-m", "delta_b200.cli", "--model", str(model_folders["A"]), "--B", "6", "--max_len", "128", "--dataset", "random", "--num_samples",

@@ -1,5 +1,4 @@
 """What attention over shared prefixes asks for under an engine's limits: working memory, rows (no GPU: sizes and choices only)."""
-import ctypes
 import types
 
 import pytest
@@ -15,33 +14,51 @@ def on_device_0(monkeypatch):
     monkeypatch.setattr(ops, "_device_index", lambda: 0)
 
 
-def context(rows, max_rows, max_pages=64, pages=1000, scratch=None):
-    """As much of a step as the part looks at; ``calls`` gets what would be launched."""
-    calls = []
-    tables = dict(kv_len=0, members=0, group_start=0, group_prefix=0)
-    ctx = types.SimpleNamespace(shared=dict(g=tables), plain_kernels=frozenset(), num_rows=rows, max_rows=max_rows, max_pages=max_pages, err=None,
+def context(rows, max_rows, max_pages=64, dtype=torch.bfloat16):
+    """As much of a step as the part looks at; ``asked`` gets what working memory is asked for."""
+    asked = []
+    ctx = types.SimpleNamespace(shared=dict(g=None), plain_kernels=frozenset(), num_rows=rows, max_rows=max_rows, max_pages=max_pages, dtype=dtype,
                                 cache=types.SimpleNamespace(max_pages_per_request=max_pages))
-    ctx.scratch = scratch or (lambda key, shape, dtype, bound=None: calls.append((shape[0], bound[0])))
-    return ctx, calls
+    ctx.scratch_if_there = lambda key, shape, dtype, bound=None: asked.append((shape[0], bound[0])) or torch.empty(0)
+    return ctx, asked
 
 
-def cache_view(pages=1000, KV=2, ps=16, hd=64):
-    return types.SimpleNamespace(group="g", page_size=ps, block_table=None, pages=types.SimpleNamespace(shape=(pages, 2, KV, ps, hd)))
+def cache_view(pages=1000, KV=2, ps=16, hd=64, group="g"):
+    return types.SimpleNamespace(group=group, page_size=ps, pages=types.SimpleNamespace(shape=(pages, 2, KV, ps, hd)))
 
 
 @pytest.mark.parametrize("max_rows", [8, 1024, 1025, 2000, 100000])
-def test_an_engine_of_many_slots(monkeypatch, max_rows):
+def test_an_engine_of_many_slots(max_rows):
     """A call takes 1,024 rows; the engine may have more slots, and a step of few rows still goes there."""
-    monkeypatch.setattr(ops, "attention_shared_prefix", lambda *a, **k: None)
-    qkv, out = torch.zeros(8, 6 * 64, dtype=torch.bfloat16), torch.zeros(8, 2 * 64, dtype=torch.bfloat16)
     ctx, calls = context(8, max_rows)
-    attention_kernels.run_shared(ctx, qkv, out, cache_view(), 2, 2, 64, 0.125)
+    assert attention_kernels.shared_work(ctx, cache_view(), 2, 2, 64) is not None
     (asked, bound), = calls
     assert asked == ops.attention_shared_prefix_floats(8, 4, 8, 2, 2, 64, 16, 64, 1000, torch.bfloat16)
     most = min(max_rows, 1024)
     assert bound == ops.attention_shared_prefix_floats(most, most // 2, most, 2, 2, 64, 16, 64, 1000, torch.bfloat16) >= asked
     with pytest.raises(KernelError, match="at most 1024 rows"):
         ops.attention_shared_prefix_floats(1025, 4, 8, 2, 2, 64, 16, 64, 1000, torch.bfloat16)
+    assert attention_kernels.shared_work(context(1025, 2000)[0], cache_view(), 2, 2, 64) is None
+    assert attention_kernels.shared_work(context(8, 8)[0], cache_view(group="another"), 2, 2, 64) is None
+
+
+def test_a_device_without_room(monkeypatch):
+    """The cache may hold nearly all of the device: a step goes on without the kernels whose working memory is not to be had, and so do all later ones."""
+    from delta_b200.engine.context import StepContext
+    ctx = StepContext.__new__(StepContext)
+    ctx._scratch_pool, ctx.device, tries = {}, "cpu", []
+
+    def full(*a, **k):
+        tries.append(1)
+        raise torch.OutOfMemoryError("full")
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", full)
+        with pytest.warns(RuntimeWarning, match="'shared'.*without it"):
+            assert ctx.scratch_if_there("shared", (5,), torch.float32, bound=(50,)) is None
+        with pytest.raises(torch.OutOfMemoryError):
+            ctx.scratch("other", (5,), torch.float32)
+    assert ctx.scratch_if_there("shared", (5,), torch.float32) is None and len(tries) == 2
+    assert ctx.scratch_if_there("another", (5,), torch.float32, bound=(50,)).shape == (5,)
 
 
 def megabytes(rows, keys, pool, dtype=torch.bfloat16, KV=8, H=32):
