@@ -106,6 +106,14 @@ def test_one_group(dtype, shape, scattered):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(2, 1, 132, 16), (6, 2, 200, 8), (4, 4, 256, 16), (34, 2, 256, 32), (32, 1, 128, 16), (24, 1, 64, 16), (40, 2, 4, 16), (62, 2, 128, 8),
+                                   (8, 2, 128, 10), (8, 2, 64, 1), (8, 2, 128, 48), (4, 2, 128, 256), (16, 2, 64, 100)], ids=lambda s: "x".join(map(str, s)))
+def test_wide_heads_many_heads_odd_pages(dtype, shape):
+    """Heads of 129 to 256, more than 16 query heads to a key-value head, pages whose size is no power of two or larger than a tile."""
+    check(dtype, make(dtype, *shape, [(5, 700), (9, 333)], 2, [1, 40, 128, 129, 300, 2, 3, 64, 65, 31, 32, 33, 7, 100, 17, 530], seed=35, scattered=True))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("shape", SHAPES[:5], ids=lambda s: "x".join(map(str, s)))
 def test_groups_and_loose_rows(dtype, shape):
     groups = [(3, 1000), (1, 333), (20, 129), (2, 5)]
