@@ -231,7 +231,8 @@ class Scheduler:
 
     def _fork_waiting(self) -> None:
         """Forks waiting requests from running ones that hold what they share, as many as have a slot and pages for their whole prompt and
-        one more token; those of one source with one launch for all of them."""
+        one more token; those of one source with one launch for all of them.  A fork may so pass an older request that waits for pages, but only
+        in a family that somebody computes already: families that come later wait behind that request."""
         reserve = {n: 0 for n in self.cache.groups}
         wanted: Dict[tuple, List[Request]] = {}
         begun: List[Family] = []      # whose beginning a request that is forked now will go on to compute

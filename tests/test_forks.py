@@ -359,6 +359,26 @@ def test_samples_of_prompts_with_a_common_first_part(budget, states):
     assert s.stats["forks"] == 11 and all(r.status == FINISHED for r in rs)
 
 
+def test_forks_pass_an_older_request_only_while_their_family_runs():
+    """A fork needs few pages and may start before an older request that waits for many: the families under way end, later ones wait behind it."""
+    c = manager(num_pages=20, max_slots=12)
+    s = Scheduler(c, max_batch=12, max_tokens_per_step=64)
+    first = requests(s, [list(range(21))], new=12)
+    big = s.add_request([7] * 62, 64, max_new_tokens=2)
+    first += requests(s, [list(range(21))] * 3, new=12)
+    s.relate(first, 20)
+    later = []
+
+    def watch(plan):
+        if len(later) < 40:
+            mine = requests(s, [[50 + len(later)] * 9] * 2, new=3)
+            s.relate(mine, 8)
+            later.extend(mine)
+    run(s, c, watch=watch, steps=2000)
+    assert all(r.status == FINISHED for r in s.requests)
+    assert all(r.admitted_order < big.admitted_order < x.admitted_order for r in first for x in later)
+
+
 def test_a_follower_computes_for_itself_when_nobody_holds_the_beginning():
     c = manager(num_pages=64, max_slots=1)
     s = Scheduler(c, max_batch=1, max_tokens_per_step=64)
