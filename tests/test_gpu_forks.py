@@ -100,6 +100,38 @@ def test_every_design_can_be_forked(design, graph, tmp_path):
     assert outs == backend(folder, max_tokens_per_step=64).generate([prompt] * 4, 8, temperature=0.6, seed=2)
 
 
+@pytest.mark.parametrize("design", list(DESIGNS))
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graphs"])
+def test_every_design_reads_shared_pages_once(design, dtype, graph, tmp_path):
+    """Whatever else a design has in its layers, those that read every page take the shared ones once; in bfloat16 every sample runs to its end."""
+    from roletar_helpers import write_folder
+    h = DESIGNS[design]
+    cfg, weights = h.build("mix", 3)[:2] if hasattr(h, "build") else (h.config("mix"), h.make_weights(h.config("mix"), 3))
+    folder = write_folder(tmp_path, design, cfg, weights)
+    prompt = helpers.random_tokens(37, cfg["vocab"], 8)
+    e = backend(folder, dtype=dtype, graph=graph, min_bytes=0, max_tokens_per_step=64)
+    outs = e.generate([prompt], 8, samples=4, temperature=0.6, seed=2)
+    assert e.scheduler.stats["forks"] == 3 and all(len(o) == 8 for o in outs)
+    done(e)
+    if dtype == "float32":
+        assert outs == backend(folder, max_tokens_per_step=64).generate([prompt] * 4, 8, temperature=0.6, seed=2)
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graphs"])
+@pytest.mark.parametrize("min_bytes", [None, 0], ids=["apart", "shared"])
+def test_samples_with_chosen_pages(model_folders, min_bytes, graph):
+    """Layers that choose pages for others: their choices are a request's own, full layers read shared pages once."""
+    vocab = helpers.tiny_config("A")["vocab_size"]
+    prompts = [helpers.random_tokens(n, vocab, 40 + n) for n in (75, 130)]
+    sel = dict(enable_selective_cache=True, full_cache_layers=[0], subset_cache_size=4, page_size=8)
+    e = backend(model_folders["A"], graph=graph, min_bytes=min_bytes, **sel)
+    outs = e.generate(prompts, 20, temperature=0.8, seed=5, samples=3)
+    assert e.scheduler.stats["forks"] == 4
+    done(e)
+    assert outs == backend(model_folders["A"], **sel).generate([p for p in prompts for _ in range(3)], 20, temperature=0.8, seed=5)
+
+
 def test_forks_under_preemption(model_folders):
     """A pool that cannot hold all samples to their end: some are preempted and forked again or computed anew."""
     vocab = helpers.tiny_config("A")["vocab_size"]
