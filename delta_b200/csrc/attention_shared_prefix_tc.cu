@@ -145,8 +145,10 @@ __device__ __forceinline__ int list_pieces(const DkSharedPrefixParams& p, int ra
 }
 
 // What the rows' kernel needs: its pieces, and the counters cleared.  The list is published for its blocks that start before this kernel's end.
+// (A function of its own: inlined it made the other blocks' code slower. 48 rows behind 30,000 keys 52.1 and 50.7 us, 64 behind 2,048 24.8 and 24.0, the mixed
+// call 33.6 and 32.9, 8 rows behind 4,096 16.6 and 17.0.)
 template <int HD>
-__device__ void prepare_rows(const DkSharedPrefixParams& p, int* tables, int tid) {
+__device__ __noinline__ void prepare_rows(const DkSharedPrefixParams p, int* tables, int tid) {
   for (int i = tid; i < p.rows * p.KV; i += THREADS) counters(p)[i] = 0;
   Cut cut(tables, p.rows, p.groups);
   make_cut<KT, ROWS_KT, MIN_ROW_TILES, THREADS>(p, cut, tid);

@@ -72,7 +72,7 @@ __host__ __device__ __forceinline__ long long front_ints(const DkSharedPrefixPar
 // Groups of n_g rows and k_g keys have ceil(n_g / rpt) ceil(k_g / kt) tiles for a key-value head, at most (n_g / rpt + 1) (k_g / kt + 1).  Their pages are
 // distinct, or some are held by two groups (a part of all rows shares more than all do): sum k_g <= 2 pool.  So the sum is at most
 // (n / rpt + 2 pool / longest) longest / kt and a tile for every segment, which is what the working memory is made for.  Tables that ask for more are right all the
-// same: their rows read alone.  (64 rows with tables of 131,072 tokens, 32 heads on 8 of 128, a pool of 262,144 tokens: 89 MB; with 32 groups of full tables 412.)
+// same: their rows read alone.  (64 rows with tables of 131,072 tokens, 32 heads on 8 of 128, a pool of 262,144 tokens: 90 MB; with 32 groups of full tables 412.)
 struct Bounds {
   long long tiles, pieces, work_floats;
 };
@@ -163,9 +163,9 @@ __device__ __forceinline__ void scan(const int* v, int* before, int* total, int*
 }
 
 // Fills in ``c`` by a block of NT threads.  KT, ROWS_KT: p.kt, p.rows_kt; MIN_ROW_TILES: the least C.  Ends with a sync.
-// Starts of groups that are out of order or out of range could make groups overlap and pieces outnumber the work buffer: then there is no group, and every
-// row reads its keys alone.  So does a row that is shorter than its group's prefix; one whose length fits no table reads nothing.  A row that is named twice belongs
-// to its first place: every block that works the tables out finds the same pieces.
+// Starts of groups that are out of order or out of range could make groups overlap and pieces outnumber the work buffer, and groups that repeat the same pages
+// may be more tiles than it has room for: then there is no group, and every row reads its keys alone.  So does a row that is shorter than its group's
+// prefix; one whose length fits no table reads nothing.  A row that is named twice belongs to its first place: every block that works the tables out finds the same pieces.
 template <int KT, int ROWS_KT, int MIN_ROW_TILES, int NT>
 __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, int tid) {
   const auto sync = [] { __syncthreads(); };
@@ -177,6 +177,8 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     c.member[r] = NOBODY;
   }
   bool out_of_order = false;
+  if (tid == 0) c.sums[0] = 0;
+  sync();
   for (int g = tid; g <= p.groups; g += NT) {
     int a = 0, b = 0, k = 0;
     if (p.groups > 0) a = p.group_start[g];
@@ -195,9 +197,10 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
       k = k / p.ps * p.ps;
       c.declared[g] = k;
       c.prefix[g] = (long long)(b - a - 1) * k >= p.min_saved ? k : 0;      // one row shares nothing, and what saves few keys is read by each row itself
+      if (c.prefix[g] > 0) atomicAdd(&c.sums[0], few(b - a, p.rpt) * p.KV * cdiv(k, KT));
     }
   }
-  if (__syncthreads_or(out_of_order)) {
+  if (__syncthreads_or(out_of_order) || c.sums[0] > p.max_tiles) {
     for (int g = tid; g <= p.groups; g += NT) {
       c.start[g] = 0;
       if (g < p.groups) c.declared[g] = c.prefix[g] = 0;
@@ -221,42 +224,34 @@ __device__ __forceinline__ void make_cut(const DkSharedPrefixParams& p, Cut& c, 
     const int n = c.start[g + 1] - c.start[g];
     return c.prefix[g] > 0 ? few(n, p.rpt) * p.KV : 0;
   };
-  int v[4], before[4], total[4];
-#pragma unroll 1
-  for (;;) {        // (once more where the groups' tiles are too many)
-    v[0] = v[1] = v[2] = v[3] = 0;
-    for (int g = g0; g < g1; ++g) {
-      const int x = segments(g);
-      v[0] += x * cdiv(c.prefix[g], KT);
-      v[1] += x;
-    }
-    for (int r = r0; r < r1; ++r) {
-      const int m = c.member[r];
-      int len = c.len[r], own = 0, said = 0;
-      if (m != NOBODY) {
-        const int g = last_not_above(c.start, p.groups, m);
-        if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
-          own = c.prefix[g];
-          said = c.declared[g];
-        }
-      }
-      if (len < said || len > max_keys) {
-        dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
-        own = 0;
-        if (len < 0 || len > max_keys) c.len[r] = len = 0;
-      }
-      c.own[r] = own;
-      const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece
-      c.piece[r] = tiles;
-      v[2] += tiles;
-      v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
-    }
-    scan<4, NT>(v, before, total, c.sums, tid, sync);
-    if (total[0] <= p.max_tiles) break;
-    sync();                     // (the sums and prefixes were read)
-    for (int g = g0; g < g1; ++g) c.declared[g] = c.prefix[g] = 0;
-    sync();
+  int v[4] = {0, 0, 0, 0}, before[4], total[4];
+  for (int g = g0; g < g1; ++g) {
+    const int x = segments(g);
+    v[0] += x * cdiv(c.prefix[g], KT);
+    v[1] += x;
   }
+  for (int r = r0; r < r1; ++r) {
+    const int m = c.member[r];
+    int len = c.len[r], own = 0, said = 0;
+    if (m != NOBODY) {
+      const int g = last_not_above(c.start, p.groups, m);
+      if (m - c.start[g] < c.start[g + 1] - c.start[g]) {
+        own = c.prefix[g];
+        said = c.declared[g];
+      }
+    }
+    if (len < said || len > max_keys) {
+      dk_report(p.err, DK_DEV_BAD_GROUP, r, len, len < said ? said : max_keys);
+      own = 0;
+      if (len < 0 || len > max_keys) c.len[r] = len = 0;
+    }
+    c.own[r] = own;
+    const int tiles = max(1, cdiv(len - own, ROWS_KT));       // a row without a key of its own has an empty piece
+    c.piece[r] = tiles;
+    v[2] += tiles;
+    v[3] += cdiv(tiles, MIN_ROW_TILES) * p.KV;
+  }
+  scan<4, NT>(v, before, total, c.sums, tid, sync);
   c.tiles = total[0];
   c.Q = range_tiles(p, total[0], total[1]);
   c.ranges = cdiv(total[0], c.Q);
