@@ -14,8 +14,8 @@
 // keeps 32 queries; K and V of a tile of 32 keys lie in shared memory as floats, and those of the next tile are on their way while this one is
 // computed.  A thread has four queries and two keys of the scores, then four queries and eight columns of the result, two products to an instruction.
 //
-// 8 rows of 32 query heads on 4 of 128 behind 2,048 shared keys: 34.5 us.  Of these 2.7 go into the tables, 1 into the list of pieces, 5 until the first
-// keys are there, 7.5 into a tile with two or three blocks to an SM, 2 into a piece's results and 5 into the merge.  32 rows behind 4,096 keys: 132 us, a quarter of
+// 8 rows of 32 query heads on 4 of 128 behind 2,048 shared keys: 35.0 us.  Of these 2.7 go into the tables, 1 into the list of pieces, 5 until the first
+// keys are there, 7.5 into a tile with two or three blocks to an SM, 2 into a piece's results and 5 into the merge.  32 rows behind 4,096 keys and 8 behind 1,000: 134 us, a quarter of
 // the FMA units' rate: latency of shared memory between four barriers a tile, which three warps to a scheduler do not hide.  (A fourth block to an SM: 40 us for
 // the small call, since its ranges are half as long and the merge reads twice the pieces.  Weights kept twice, ready to be multiplied in pairs: 36.4.  Loops rolled
 // to two steps: 35.7 and 142.  Tiles of 64 keys with 4 x 4 scores to a thread and two blocks to an SM: 55 and 171.)

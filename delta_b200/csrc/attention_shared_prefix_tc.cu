@@ -24,8 +24,8 @@
 // SM: loops are kept rolled, and the scores are read twice from tensor memory, 32 columns at a time, instead of once into 128 registers.
 // What bounds a long line of tiles is shared memory: 224 KB a tile (128 as operands of the two products, 64 of pages coming in, 32 of weights) at 128 bytes a
 // cycle are 1,792 of the 1,918 cycles that a tile takes (48 rows behind 30,000 keys).  So neither scores fetched ahead of the exponentials (51 to 53 us),
-// chunks of 16 or 64 columns (52 to 56) nor two products to an instruction (51) help.  Weights as an operand in tensor memory would take 64 KB off, but the two
-// halves' scores and accumulators fill it.
+// chunks of 16 or 64 columns (52 to 56) nor two products to an instruction (51) help.  Weights as an operand in tensor memory would take 64 KB off: over the scores they
+// come from, since the halves' scores and accumulators fill it, so that a half's next scores wait for its product (not built).
 // The last block computes nothing: it works out the pieces of the rows' kernel, which may start as soon as they are there.
 //
 // Every wait is bounded; when one gives up the block records it, waits (bounded again) for the copies and products it has under

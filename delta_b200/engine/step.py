@@ -120,9 +120,9 @@ class ModelRunner:
         self._graphs: Dict[int, dict] = {}      # by batch size, and by (batch size, cache groups whose shared prefixes are read once)
         # A decode step reads its rows' shared pages once for all of them from so many saved bytes of a layer's keys and values on.  Steps of a
         # Yi-6B model (32 layers, bfloat16, graphs), each row on its own (the second reader finds shared pages in the L2) and shared pages
-        # once: 8 rows behind 1,024 tokens (14 MiB) 2.96 and 3.09 ms, 16 behind 2,048 (60) 3.50 and 3.58, 64 behind 512 (63) 3.69 and 3.80,
-        # 8 behind 4,096 (56) 3.28 and 3.24, 8 behind 7,000 (96) 3.57 and 3.30, 64 behind 1,024 (126) 3.97 and 3.87, 64 behind 2,048 (252) 4.53
-        # and 3.94.  In 32 bits (4 layers) 2 rows behind 64 tokens (0.3 MiB) 1.67 and 1.73, 2 behind 512 (2) 2.06 and 1.73, 64 behind 2,048 11.8 and 2.3.
+        # once: 8 rows behind 1,024 tokens (14 MiB) 3.06 and 3.22 ms, 16 behind 2,048 (60) 3.54 and 3.70, 64 behind 512 (63) 3.75 and 3.92,
+        # 8 behind 4,096 (56) 3.39 and 3.30, 8 behind 7,000 (96) 3.64 and 3.39, 64 behind 1,024 (126) 4.05 and 3.98, 64 behind 2,048 (252) 4.64
+        # and 3.97.  In 32 bits (4 layers) 2 rows behind 64 tokens (0.3 MiB) 1.71 and 1.75, 2 behind 512 (2) 2.09 and 1.74, 64 behind 2,048 11.8 and 2.3.
         self.shared_prefix_min_bytes = (1 if self.dtype == torch.float32 else 80) << 20
         self.graph_captures = 0
         self.graph_replays = 0
