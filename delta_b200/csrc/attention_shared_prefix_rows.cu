@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, Ring<HD, LOW>::BLOCKS) attention_shar
     }
   }
   asm volatile("griddepcontrol.wait;\n" ::: "memory");       // what follows this kernel follows the other one too
-  if (blockIdx.x == 0 && tid == 0) *list_of_call(p) = 0;
+  if (blockIdx.x == 0 && tid == 0) asm volatile("st.relaxed.gpu.global.u64 [%0], %1;\n" ::"l"(list_of_call(p)), "l"(0ull) : "memory");      // (others may still look)
 }
 
 bool make_map_of_pieces(CUtensorMap* m, const float* base, int pieces, int G, int hd) {
